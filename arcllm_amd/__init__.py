@@ -132,6 +132,50 @@ class Residency(C.Structure):
                 ("kv_bytes", _U64), ("working_bytes", _U64), ("total_bytes", _U64)]
 
 
+F32, F16, BF16 = 0, 1, 30  # arc_dtype (ggml type ids)
+NO_SLOT = PAGED_RELEASE = 0xFFFFFFFF
+PLAN_NO_PAGES, PLAN_TABLE, PLAN_TOKENS, PLAN_MAX_NEW, PLAN_FREE_LIST = 1, 2, 4, 8, 16
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
+
+
+class KvPages(C.Structure):
+    """arc_kv_pages: pools of K and V pages.  Built by keyword; page_stride defaults to
+    pages that lie one after the other."""
+
+    _fields_ = [("k", _P), ("v", _P), ("page_stride", _U64), ("num_pages", _U32), ("page_size", _U32),
+                ("kv_heads", _U32), ("head_dim", _U32), ("dtype", C.c_int32)]
+
+    def __init__(self, k, v, num_pages: int, page_size: int, kv_heads: int, head_dim: int = 128, dtype: int = F16,
+                 page_stride: Optional[int] = None):
+        super().__init__(_ptr(k), _ptr(v), page_size * kv_heads * head_dim if page_stride is None else page_stride,
+                         num_pages, page_size, kv_heads, head_dim, dtype)
+        self._keep = (k, v)
+
+
+class PagedBatch(C.Structure):
+    """arc_paged_batch: the requests of a step.  Arrays a call does not use may be None."""
+
+    _fields_ = [("requests", _U32), ("tokens", _U32), ("max_pages", _U32), ("max_new", _U32), ("tables", _P),
+                ("lens", _P), ("starts", _P), ("positions", _P), ("slots", _P)]
+
+    def __init__(self, requests: int, tokens: int, max_pages: int = 0, max_new: int = 0, tables=None, lens=None,
+                 starts=None, positions=None, slots=None):
+        super().__init__(requests, tokens, max_pages, max_new, _ptr(tables), _ptr(lens), _ptr(starts),
+                         _ptr(positions), _ptr(slots))
+        self._keep = (tables, lens, starts, positions, slots)
+
+
+class Rope(C.Structure):
+    """arc_rope: rotary positions with the phases on the device (see rope_phases)."""
+
+    _fields_ = [("phases", _P), ("rot_dim", _U32), ("layout", C.c_int32), ("scale", _F)]
+
+    def __init__(self, phases, rot_dim: int, layout: int = ROPE_INTERLEAVED, scale: float = 1.0):
+        super().__init__(_ptr(phases), rot_dim, layout, scale)
+        self._keep = phases
+
+
 _SIGS.update({
     "arc_model_dims_qwen25_7b": [C.POINTER(ModelDims)],
     "arc_model_tensor_info": [C.POINTER(ModelDims), C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(_U32),
@@ -155,6 +199,16 @@ _SIGS.update({
     "arc_model_tensor_device": [_P, C.c_int, C.c_int, C.POINTER(_P)],
     "arc_session_route_down": [_P, _U32, _P],
 })
+_SIGS.update({
+    "arc_paged_plan": [C.POINTER(PagedBatch), _P, _P, _U32, _P, _U32, _P, _P, _P, _P],
+    "arc_rope_phases": [_U32, C.c_double, C.c_int, C.c_double, _U32, C.c_double, C.c_double, _P, _P, _FP],
+    "arc_rope_append": [C.POINTER(KvPages), C.POINTER(PagedBatch), C.POINTER(Rope), C.c_int, _P, _U32, _P, _P, _P,
+                        _U32, _P, _U32, _P],
+    "arc_paged_attention_workspace_bytes": [C.POINTER(KvPages), C.POINTER(PagedBatch), _U32],
+    "arc_paged_attention": [C.POINTER(KvPages), C.POINTER(PagedBatch), _P, _U32, _U32, _F, _U32, _U32, _P, _U32, _P,
+                            _P],
+})
+_RESTYPE["arc_paged_attention_workspace_bytes"] = C.c_size_t
 _RESTYPE.update({"arc_model_weight_bytes": _U64, "arc_session_kernels_per_step": _U32,
                  "arc_session_prefill_kernels": _U32})
 
@@ -477,6 +531,51 @@ def prefill_qkv(wq, wk, wv, v_qtype: int, H: int, kvd: int, K: int, x, M: int, y
     """The prompt pass's q|k|v launch before bias and RoPE: y[M][H + 2 kvd] (fp32)."""
     check(lib().arc_prefill_qkv(_ptr(wq), _ptr(wk), _ptr(wv), v_qtype, H, kvd, K, _ptr(x), M, _ptr(y),
                                 _ptr(workspace), _sp(stream)))
+
+
+def paged_plan(batch: PagedBatch, old_lens, new_lens, page_size: int, free_pages, num_pages: int, free_count,
+               free_count_out, status, stream: Optional[Stream] = None) -> None:
+    """Block tables, lengths, row starts, positions and slots of a step, on the GPU (arc_paged_plan)."""
+    check(lib().arc_paged_plan(C.byref(batch), _ptr(old_lens), _ptr(new_lens), page_size, _ptr(free_pages), num_pages,
+                               _ptr(free_count), _ptr(free_count_out), _ptr(status), _sp(stream)))
+
+
+def rope_phases(rot_dim: int, theta: float, scaling: int = ROPE_PLAIN, factor: float = 1.0, original_ctx: int = 0,
+                beta_fast: float = 0.0, beta_slow: float = 0.0, freq_factors=None) -> tuple[np.ndarray, float]:
+    """(phases, scale): the angles per position of the rotated pairs, uint64 fractions of a turn, to be
+    copied to the device for a Rope, and the factor on rotated values."""
+    phases, scale = np.empty(max(1, rot_dim // 2), np.uint64), C.c_float(0.0)
+    if freq_factors is not None:
+        freq_factors = np.ascontiguousarray(freq_factors, dtype=np.float32)
+        if freq_factors.size != rot_dim // 2:
+            raise ValueError("freq_factors: one for each rotated pair")
+    check(lib().arc_rope_phases(rot_dim, theta, scaling, factor, original_ctx, beta_fast, beta_slow,
+                                None if freq_factors is None else freq_factors.ctypes.data, phases.ctypes.data,
+                                C.byref(scale)))
+    return phases, scale.value
+
+
+def rope_append(pages: KvPages, batch: PagedBatch, rope: Rope, x_dtype: int, x, ldx: int, hpk: int, q, ldq: int,
+                q_bias=None, k_bias=None, v_bias=None, stream: Optional[Stream] = None) -> None:
+    """Bias and rotary positions of the rows q|k|v of x; q to `q`, k and v into the pages (arc_rope_append)."""
+    check(lib().arc_rope_append(C.byref(pages), C.byref(batch), C.byref(rope), x_dtype, _ptr(x), ldx, _ptr(q_bias),
+                                _ptr(k_bias), _ptr(v_bias), hpk, _ptr(q), ldq, _sp(stream)))
+
+
+def paged_attention_workspace_bytes(pages: KvPages, batch: PagedBatch, hpk: int) -> int:
+    n = int(lib().arc_paged_attention_workspace_bytes(C.byref(pages), C.byref(batch), hpk))
+    if n == 0:
+        raise ArcError(2, f"no paged-attention workspace size for {pages.kv_heads} kv heads, {hpk} query heads each, "
+                          f"head_dim {pages.head_dim}")
+    return n
+
+
+def paged_attention(pages: KvPages, batch: PagedBatch, q, ldq: int, hpk: int, out, ldo: int, workspace,
+                    scale: float = 0.0, window: int = 0, sinks: int = 0, stream: Optional[Stream] = None) -> None:
+    """Attention of a step's new tokens over the pages, all positions or a sliding window and the first
+    `sinks` ones (arc_paged_attention).  scale 0: 1 / sqrt(head_dim)."""
+    check(lib().arc_paged_attention(C.byref(pages), C.byref(batch), _ptr(q), ldq, hpk, scale, window, sinks,
+                                    _ptr(out), ldo, _ptr(workspace), _sp(stream)))
 
 
 def tune_force(bs: int, rpl: int) -> None:

@@ -1,0 +1,530 @@
+// arc_paged.hip -- a serving step over a paged KV cache: the step's plan (block
+// tables, slots, positions from request lengths) and bias + rotary positions with
+// the write into the pages.  The attention over the pages is arc_paged_attn.hip.
+#include "arc_paged.hpp"
+
+#include <cmath>
+
+namespace arc {
+namespace {
+
+// -------------------------------------------------------------------- plan
+struct PlanArgs {
+    const uint32_t *old_lens, *new_lens;
+    uint32_t* free_pages;
+    const uint32_t* free_count;
+    uint32_t *free_count_out, *status;
+    uint32_t *tables, *lens, *starts, *positions, *slots;
+    uint32_t requests, rows, max_pages, max_new, num_pages, shift;  // page_size = 1 << shift
+};
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+
+// What one request contributes to the step.
+struct PlanPart {
+    uint32_t fresh, take, back;  // new tokens, pages it pops, pages it pushes
+};
+
+__device__ __forceinline__ uint32_t pages_of(uint32_t len, uint32_t shift)
+{
+    return (len >> shift) + ((len & ((1u << shift) - 1u)) != 0u);
+}
+
+__device__ __forceinline__ PlanPart plan_part(uint32_t held, uint32_t fresh, uint32_t shift)
+{
+    if (fresh == ARC_PAGED_RELEASE) return PlanPart{0u, 0u, pages_of(held, shift)};
+    return PlanPart{fresh, pages_of(held + fresh, shift) - pages_of(held, shift), 0u};
+}
+
+__device__ __forceinline__ uint32_t wave_inclusive(uint32_t v)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const uint32_t o = uint32_t(__shfl_up(int(v), d));
+        if (lane >= uint32_t(d)) v += o;
+    }
+    return v;
+}
+
+// Exclusive prefix of v over the workgroup; `total` is the sum.  `red` holds one
+// word per wave.
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* red, uint32_t& total)
+{
+    const uint32_t inc = wave_inclusive(v);
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) red[wave] = inc;
+    __syncthreads();
+    uint32_t before = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanWaves; ++i) {
+        const uint32_t r = red[i];
+        if (i < wave) before += r;
+        sum += r;
+    }
+    total = sum;
+    return before + inc - v;
+}
+
+// The last i < n with at[i] <= x, for at ascending with at[0] <= x.
+__device__ __forceinline__ uint32_t last_at_most(const uint32_t* at, uint32_t n, uint32_t x)
+{
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (at[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void plan_row(const PlanArgs& a, uint32_t n, uint32_t b, uint32_t pos)
+{
+    a.positions[n] = pos;
+    a.slots[n] = (a.tables[uint64_t(b) * a.max_pages + (pos >> a.shift)] << a.shift) | (pos & ((1u << a.shift) - 1u));
+}
+
+// The plan by one workgroup: the requests in blocks of 1024, a thread each, twice.
+// First the step's totals and every check, before anything is written; then the
+// prefix sums, from which pages, table entries and rows are dealt out evenly over
+// the threads (a binary search finds an item's request), so that one long
+// request costs no more than many short ones.  ROWS: the rows too; else
+// k_plan_rows writes them.  Bound by the latency of its dependent loads (lengths,
+// stack, table entries) and barriers.
+template <bool ROWS>
+__global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs a)
+{
+    __shared__ uint32_t red[kPlanWaves];
+    __shared__ uint32_t first[kPlanThreads];  // exclusive prefix of what is dealt out
+    __shared__ uint32_t held[kPlanThreads];
+    __shared__ unsigned long long sums[3];
+    const uint32_t tid = threadIdx.x;
+    const uint32_t blocks = (a.requests + kPlanThreads - 1) / kPlanThreads;
+    const uint32_t count = *a.free_count;
+    const uint64_t most = min(uint64_t(a.max_pages) << a.shift, uint64_t(0x7fffffffu));
+    if (tid < 3) sums[tid] = 0;
+    uint32_t bad = 0;
+    uint64_t fresh = 0, take = 0, back = 0;
+    PlanPart p{};
+    uint32_t len = 0;
+    for (uint32_t i = 0; i < blocks; ++i) {
+        const uint32_t b = i * kPlanThreads + tid;
+        p = PlanPart{};
+        if (b < a.requests) {
+            len = a.old_lens[b];
+            const uint32_t nw = a.new_lens[b];
+            const bool ended = nw == ARC_PAGED_RELEASE;
+            if (!ended && nw > a.max_new) bad |= ARC_PLAN_MAX_NEW;
+            if (uint64_t(len) + (ended ? 0u : nw) > most) bad |= ARC_PLAN_TABLE;
+            if (!bad) p = plan_part(len, nw, a.shift);
+        }
+        fresh += p.fresh;
+        take += p.take;
+        back += p.back;
+    }
+    __syncthreads();
+    // integer sums: the order does not matter
+    if (fresh) atomicAdd(&sums[0], static_cast<unsigned long long>(fresh));
+    if (take) atomicAdd(&sums[1], static_cast<unsigned long long>(take));
+    if (back) atomicAdd(&sums[2], static_cast<unsigned long long>(back));
+    bad = uint32_t(__syncthreads_or(int(bad & ARC_PLAN_MAX_NEW)) ? ARC_PLAN_MAX_NEW : 0) |
+          uint32_t(__syncthreads_or(int(bad & ARC_PLAN_TABLE)) ? ARC_PLAN_TABLE : 0);
+    fresh = sums[0];
+    take = sums[1];
+    back = sums[2];
+    uint64_t lacking = 0;
+    if (!bad) {
+        if (fresh > a.rows) bad |= ARC_PLAN_TOKENS;
+        if (uint64_t(count) + back > a.num_pages) bad |= ARC_PLAN_FREE_LIST;
+        else if (take > count + back) {
+            bad |= ARC_PLAN_NO_PAGES;
+            lacking = take - (count + back);
+        }
+    }
+    if (bad) {
+        for (uint32_t b = tid; b < a.requests; b += kPlanThreads) {
+            a.lens[b] = a.old_lens[b];
+            a.starts[b] = 0;
+        }
+        if (tid == 0) {
+            a.starts[a.requests] = 0;
+            *a.free_count_out = count;
+            a.status[0] = bad;
+            a.status[1] = uint32_t(min(lacking, uint64_t(0xffffffffu)));
+            a.status[2] = a.status[3] = 0;
+        }
+        if constexpr (ROWS)
+            for (uint32_t n = tid; n < a.rows; n += kPlanThreads) {
+                a.positions[n] = 0;
+                a.slots[n] = ARC_NO_SLOT;
+            }
+        return;
+    }
+
+    const uint32_t top = count + uint32_t(back);
+    // pages of ended requests onto the stack, before any are popped
+    if (back) {
+        uint32_t done = 0;
+        for (uint32_t i = 0; i < blocks; ++i) {
+            const uint32_t b = i * kPlanThreads + tid;
+            p = b < a.requests ? plan_part(a.old_lens[b], a.new_lens[b], a.shift) : PlanPart{};
+            uint32_t total;
+            first[tid] = block_exclusive(p.back, red, total);
+            __syncthreads();
+            for (uint32_t k = tid; k < total; k += kPlanThreads) {
+                const uint32_t j = last_at_most(first, kPlanThreads, k);
+                a.free_pages[count + done + k] = a.tables[uint64_t(i * kPlanThreads + j) * a.max_pages + (k - first[j])];
+            }
+            done += total;
+            __syncthreads();  // `first` is read no more
+        }
+    }
+    uint32_t popped = 0, row = 0;
+    for (uint32_t i = 0; i < blocks; ++i) {
+        const uint32_t b = i * kPlanThreads + tid;
+        p = PlanPart{};
+        len = 0;
+        if (b < a.requests) {
+            len = a.old_lens[b];
+            p = plan_part(len, a.new_lens[b], a.shift);
+        }
+        uint32_t total;
+        // block_exclusive's barriers come after every thread's reads above, so lens may be old_lens
+        first[tid] = block_exclusive(p.take, red, total);
+        held[tid] = len;
+        __syncthreads();
+        for (uint32_t k = tid; k < total; k += kPlanThreads) {
+            const uint32_t j = last_at_most(first, kPlanThreads, k);
+            a.tables[uint64_t(i * kPlanThreads + j) * a.max_pages + pages_of(held[j], a.shift) + (k - first[j])] =
+                a.free_pages[top - 1u - popped - k];
+        }
+        popped += total;
+        const uint32_t at = block_exclusive(p.fresh, red, total);
+        if (b < a.requests) {
+            a.lens[b] = p.back || a.new_lens[b] == ARC_PAGED_RELEASE ? 0u : len + p.fresh;
+            a.starts[b] = row + at;
+        }
+        if constexpr (ROWS) {
+            __syncthreads();  // the table entries above are written, `first` is read no more
+            first[tid] = at;
+            __syncthreads();
+            for (uint32_t k = tid; k < total; k += kPlanThreads) {
+                const uint32_t j = last_at_most(first, kPlanThreads, k);
+                plan_row(a, row + k, i * kPlanThreads + j, held[j] + (k - first[j]));
+            }
+        }
+        row += total;
+        __syncthreads();
+    }
+    if (tid == 0) {
+        a.starts[a.requests] = row;
+        *a.free_count_out = top - popped;
+        a.status[0] = a.status[1] = 0;
+        a.status[2] = row;
+        a.status[3] = popped;
+    }
+    if constexpr (ROWS)
+        for (uint32_t n = row + tid; n < a.rows; n += kPlanThreads) {
+            a.positions[n] = 0;
+            a.slots[n] = ARC_NO_SLOT;
+        }
+}
+
+// The rows of a large step, one per thread, from the starts and lengths that k_plan
+// left.
+__global__ __launch_bounds__(256) void k_plan_rows(PlanArgs a)
+{
+    const uint32_t n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= a.rows) return;
+    if (n >= a.starts[a.requests]) {
+        a.positions[n] = 0;
+        a.slots[n] = ARC_NO_SLOT;
+        return;
+    }
+    const uint32_t b = last_at_most(a.starts, a.requests, n);
+    plan_row(a, n, b, a.lens[b] - (a.starts[b + 1] - n));
+}
+
+// Rows that one workgroup writes itself; more go to a launch of their own.
+constexpr uint32_t kPlanRowsInOne = 4096;
+
+// -------------------------------------------------------------------- rope
+struct RopeArgs {
+    const void* x;
+    const float *qb, *kb, *vb;
+    const uint64_t* phases;
+    const uint32_t *positions, *slots;
+    void *q, *k, *v;
+    uint64_t page_stride;
+    uint32_t rows, ldx, ldq, heads, kv_heads, dim, rot, half, shift, num_slots;
+    float scale;
+};
+
+// cos and sin of position * phase turns, times scale: the product modulo 2^64 is
+// the angle's fraction of a turn exactly; its upper 32 bits, as a signed number, are in
+// [-1/2, 1/2) and round to fp32 with an error of at most 2^-26 turns.
+__device__ __forceinline__ void turn_of(uint32_t pos, uint64_t phase, float scale, float& c, float& s)
+{
+    const float half_turns = float(int32_t((uint64_t(pos) * phase) >> 32)) * 0x1p-31f;
+    sincospif(half_turns, &s, &c);
+    c *= scale;
+    s *= scale;
+}
+
+template <typename X>
+__device__ __forceinline__ void load4(const X* p, float* f)
+{
+    const vec4<X> v = *reinterpret_cast<const vec4<X>*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = static_cast<float>(v[i]);
+}
+
+// One lane: 8 values of one head of one row, as two groups of 4 that are loaded,
+// rotated and stored together: 8 neighbours (4 pairs of the interleaved layout,
+// values that are not rotated), or i .. i + 3 and their partners i + rot/2 .. of the
+// half layout.  Every lane computes its own 4 angles: about 150 instructions
+// against 48 bytes moved, which the memory time of a large step covers, and a
+// small one waits for no barrier.  Bound by HBM: N (heads + 2 kv_heads) dim values
+// read and written once.
+template <typename X, typename T>
+__device__ __forceinline__ void rope_unit(const RopeArgs& a, uint32_t n, uint32_t u, uint32_t slot, uint32_t pos)
+{
+    const uint32_t per = a.dim / 8, head = u / per, e = u - head * per;
+    const bool is_v = head >= a.heads + a.kv_heads;
+    const uint32_t rot = is_v ? 0u : a.rot;
+    const bool turned = 8 * e < rot;
+    const bool halves = turned && a.half;
+    const uint32_t i0 = halves ? 4 * e : 8 * e, i1 = halves ? 4 * e + rot / 2 : 8 * e + 4;
+
+    const X* src = static_cast<const X*>(a.x) + uint64_t(n) * a.ldx + head * a.dim;
+    float lo[4], hi[4];
+    load4(src + i0, lo);
+    load4(src + i1, hi);
+    T* dst;
+    const float* bias;
+    uint32_t own = head;  // the head's index among q, k or v
+    if (head < a.heads) {
+        dst = static_cast<T*>(a.q) + uint64_t(n) * a.ldq + head * a.dim;
+        bias = a.qb;
+    } else {
+        own -= is_v ? a.heads + a.kv_heads : a.heads;
+        const uint64_t at = uint64_t(slot >> a.shift) * a.page_stride +
+                            uint64_t(slot & ((1u << a.shift) - 1u)) * (a.kv_heads * a.dim) + own * a.dim;
+        dst = static_cast<T*>(is_v ? a.v : a.k) + at;
+        bias = is_v ? a.vb : a.kb;
+    }
+    if (bias) {
+        float b0[4], b1[4];
+        load4(bias + own * a.dim + i0, b0);
+        load4(bias + own * a.dim + i1, b1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lo[i] += b0[i];
+            hi[i] += b1[i];
+        }
+    }
+    if (turned) {
+        // pair i of the 4: (lo[i], hi[i]) of the half layout, neighbours of the interleaved one
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float c, s;
+            turn_of(pos, a.phases[4 * e + i], a.scale, c, s);
+            float& x = halves ? lo[i] : (i < 2 ? lo[2 * i] : hi[2 * i - 4]);
+            float& y = halves ? hi[i] : (i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]);
+            const float tx = x * c - y * s, ty = x * s + y * c;
+            x = tx;
+            y = ty;
+        }
+    }
+    vec4<T> o0, o1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        o0[i] = static_cast<T>(lo[i]);
+        o1[i] = static_cast<T>(hi[i]);
+    }
+    *reinterpret_cast<vec4<T>*>(dst + i0) = o0;
+    *reinterpret_cast<vec4<T>*>(dst + i1) = o1;
+}
+
+template <typename X, typename T>
+__global__ __launch_bounds__(256) void k_rope_append(RopeArgs a)
+{
+    const uint32_t units = (a.heads + 2 * a.kv_heads) * (a.dim / 8);
+    const uint32_t u = blockIdx.x * 256 + threadIdx.x;
+    if (u >= units) return;
+    for (uint32_t n = blockIdx.y; n < a.rows; n += gridDim.y) {
+        const uint32_t slot = a.slots[n];
+        if (slot < a.num_slots) rope_unit<X, T>(a, n, u, slot, a.positions[n]);
+    }
+}
+
+constexpr uint32_t kRopeGridRows = 32768;  // a grid's second dimension holds 65535
+
+template <typename X>
+void launch_rope_x(const RopeArgs& a, int dtype, hipStream_t st)
+{
+    const uint32_t units = (a.heads + 2 * a.kv_heads) * (a.dim / 8);
+    const dim3 grid((units + 255) / 256, a.rows < kRopeGridRows ? a.rows : kRopeGridRows);
+    if (dtype == ARC_F16) hipLaunchKernelGGL((k_rope_append<X, _Float16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_rope_append<X, bf16>), grid, dim3(256), 0, st, a);
+}
+
+}  // namespace
+}  // namespace arc
+
+using namespace arc;
+
+extern "C" {
+
+int arc_paged_plan(const arc_paged_batch* batch, const uint32_t* old_lens, const uint32_t* new_lens,
+                   uint32_t page_size, uint32_t* free_pages, uint32_t num_pages, const uint32_t* free_count,
+                   uint32_t* free_count_out, uint32_t* status, arc_stream_t stream)
+{
+    int rc = check_batch_sizes(batch);
+    if (!rc) rc = check_page_size(page_size);
+    if (!rc) rc = check_tables(batch, page_size);
+    if (rc) return rc;
+    if (!old_lens || !new_lens || !free_pages || !free_count || !free_count_out || !status ||
+        (batch->tokens && (!batch->positions || !batch->slots)))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "null argument");
+    if (num_pages == 0 || uint64_t(num_pages) * page_size >= (1ull << 32))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "num_pages %u: at least 1, num_pages * page_size below 2^32", num_pages);
+    if (batch->lens == new_lens) return set_error(ARC_ERR_INVALID_ARGUMENT, "lens may be old_lens, not new_lens");
+    PlanArgs a{};
+    a.old_lens = old_lens;
+    a.new_lens = new_lens;
+    a.free_pages = free_pages;
+    a.free_count = free_count;
+    a.free_count_out = free_count_out;
+    a.status = status;
+    a.tables = batch->tables;
+    a.lens = batch->lens;
+    a.starts = batch->starts;
+    a.positions = batch->positions;
+    a.slots = batch->slots;
+    a.requests = batch->requests;
+    a.rows = batch->tokens;
+    a.max_pages = batch->max_pages;
+    a.max_new = batch->max_new;
+    a.num_pages = num_pages;
+    a.shift = log2_of(page_size);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.rows <= kPlanRowsInOne) {
+        hipLaunchKernelGGL(k_plan<true>, dim3(1), dim3(kPlanThreads), 0, st, a);
+        return check_hip(hipGetLastError(), "step plan");
+    }
+    hipLaunchKernelGGL(k_plan<false>, dim3(1), dim3(kPlanThreads), 0, st, a);
+    if ((rc = check_hip(hipGetLastError(), "step plan"))) return rc;
+    hipLaunchKernelGGL(k_plan_rows, dim3((a.rows + 255) / 256), dim3(256), 0, st, a);
+    return check_hip(hipGetLastError(), "step rows");
+}
+
+int arc_rope_phases(uint32_t rot_dim, double theta, int scaling, double factor, uint32_t original_ctx,
+                    double beta_fast, double beta_slow, const float* freq_factors, uint64_t* phases, float* scale)
+{
+    if (!phases || !scale) return set_error(ARC_ERR_INVALID_ARGUMENT, "null phases or scale");
+    if (rot_dim == 0 || rot_dim % 8 || rot_dim > 128)
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "rot_dim %u: a multiple of 8, at most 128", rot_dim);
+    if (!(theta > 1.0) || !std::isfinite(theta)) return set_error(ARC_ERR_INVALID_ARGUMENT, "theta must be above 1");
+    if (scaling != ARC_ROPE_PLAIN && scaling != ARC_ROPE_LINEAR && scaling != ARC_ROPE_YARN)
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "scaling %d", scaling);
+    if (scaling != ARC_ROPE_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor)))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "factor must be at least 1");
+    const uint32_t n = rot_dim / 2;
+    const long double pi = 3.14159265358979323846264338L;
+    long double low = 0.0, high = 0.0;
+    if (scaling == ARC_ROPE_YARN) {
+        if (beta_fast == 0.0) beta_fast = 32.0;
+        if (beta_slow == 0.0) beta_slow = 1.0;
+        if (original_ctx == 0 || !(beta_slow > 0.0) || !(beta_fast >= beta_slow) || !std::isfinite(beta_fast))
+            return set_error(ARC_ERR_INVALID_ARGUMENT, "YaRN: original_ctx at least 1, 0 < beta_slow <= beta_fast");
+        // the pair index that turns beta times within original_ctx positions
+        auto at = [&](double beta) {
+            return rot_dim * std::log(original_ctx / (beta * 2.0L * pi)) / (2.0L * std::log((long double)(theta)));
+        };
+        low = std::fmax(std::floor(at(beta_fast)), 0.0L);
+        high = std::fmin(std::ceil(at(beta_slow)), (long double)(rot_dim) - 1.0L);
+    }
+    // in 64-bit mantissas: a double's 53 bits would cost the far positions
+    for (uint32_t i = 0; i < n; ++i) {
+        long double f = std::pow((long double)(theta), -2.0L * i / rot_dim);
+        if (scaling == ARC_ROPE_LINEAR) f /= factor;
+        if (scaling == ARC_ROPE_YARN) {
+            const long double ramp = std::fmin(std::fmax((i - low) / std::fmax(high - low, 0.001L), 0.0L), 1.0L);
+            f = f * (1.0L - ramp) + f / factor * ramp;
+        }
+        if (freq_factors) {
+            if (!(freq_factors[i] > 0.0f) || !std::isfinite(freq_factors[i]))
+                return set_error(ARC_ERR_INVALID_ARGUMENT, "freq_factors[%u] must be positive", i);
+            f /= freq_factors[i];
+        }
+        long double t = f / (2.0L * pi);
+        t = std::rint(std::ldexp(t - std::floor(t), 64));
+        phases[i] = t < 0x1p64L ? uint64_t(t) : 0u;
+    }
+    *scale = scaling == ARC_ROPE_YARN ? float(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return ARC_OK;
+}
+
+int arc_rope_append(const arc_kv_pages* pages, const arc_paged_batch* batch, const arc_rope* rope, int x_dtype,
+                    const void* x, uint32_t ldx, const float* q_bias, const float* k_bias, const float* v_bias,
+                    uint32_t hpk, void* q, uint32_t ldq, arc_stream_t stream)
+{
+    int rc = check_pages(pages);
+    if (!rc) rc = check_batch_sizes(batch);
+    if (rc) return rc;
+    if (!rope || !rope->phases || !x || !q || (batch->tokens && (!batch->positions || !batch->slots)))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "null argument");
+    if (x_dtype != ARC_F32 && x_dtype != ARC_F16 && x_dtype != ARC_BF16)
+        return set_error(ARC_ERR_UNSUPPORTED, "x is ARC_F32, ARC_F16 or ARC_BF16 (dtype %d)", x_dtype);
+    if (hpk == 0 || hpk > 64) return set_error(ARC_ERR_UNSUPPORTED, "hpk %u: 1..64 are supported", hpk);
+    if (rope->rot_dim == 0 || rope->rot_dim % 8 || rope->rot_dim > pages->head_dim)
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "rot_dim %u: a multiple of 8, at most head_dim %u", rope->rot_dim,
+                         pages->head_dim);
+    if (rope->layout != ARC_ROPE_INTERLEAVED && rope->layout != ARC_ROPE_HALF)
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "rope layout %d", rope->layout);
+    const uint32_t heads = pages->kv_heads * hpk, dim = pages->head_dim;
+    const uint32_t cols = (heads + 2 * pages->kv_heads) * dim;
+    if (ldx < cols || ldx % 8) return set_error(ARC_ERR_INVALID_ARGUMENT, "ldx %u: a multiple of 8, at least %u", ldx, cols);
+    if (ldq < heads * dim || ldq % 8)
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "ldq %u: a multiple of 8, at least %u", ldq, heads * dim);
+    if (!aligned(x, 16) || !aligned(q, 16) || !aligned(rope->phases, 8) || !aligned(q_bias, 16) || !aligned(k_bias, 16) ||
+        !aligned(v_bias, 16))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "x, q and the biases must be 16-byte aligned, the phases 8-byte");
+    const uint64_t xs = x_dtype == ARC_F32 ? 4 : 2;
+    if (rows_overlap(x, cols * xs, ldx * xs, q, uint64_t(heads) * dim * 2, uint64_t(ldq) * 2, batch->tokens))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "x and q share memory");
+    if (batch->tokens == 0) return ARC_OK;
+    RopeArgs a{};
+    a.x = x;
+    a.qb = q_bias;
+    a.kb = k_bias;
+    a.vb = v_bias;
+    a.phases = rope->phases;
+    a.positions = batch->positions;
+    a.slots = batch->slots;
+    a.q = q;
+    a.k = pages->k;
+    a.v = pages->v;
+    a.page_stride = pages->page_stride;
+    a.rows = batch->tokens;
+    a.ldx = ldx;
+    a.ldq = ldq;
+    a.heads = heads;
+    a.kv_heads = pages->kv_heads;
+    a.dim = dim;
+    a.rot = rope->rot_dim;
+    a.half = rope->layout == ARC_ROPE_HALF;
+    a.shift = log2_of(pages->page_size);
+    a.num_slots = pages->num_pages * pages->page_size;
+    a.scale = rope->scale;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (x_dtype == ARC_F32) launch_rope_x<float>(a, pages->dtype, st);
+    else if (x_dtype == ARC_F16) launch_rope_x<_Float16>(a, pages->dtype, st);
+    else launch_rope_x<bf16>(a, pages->dtype, st);
+    return check_hip(hipGetLastError(), "rope and cache write");
+}
+
+}  // extern "C"

@@ -258,6 +258,152 @@ int arc_prefill_attention(const float *q, const void *kc, const void *vc, uint32
                           uint32_t max_ctx, uint32_t pos0, uint32_t M, uint16_t *x, uint32_t ldx, int mfma,
                           arc_stream_t stream);
 
+/* ------------------------------------------------- paged cache serving */
+/* A serving step over several requests whose K and V live in pages: the plan
+ * (which page holds which position of which request), bias + rotary positions
+ * with the write into the pages, and attention of the step's new tokens.  The
+ * calls stand beside arc_prefill_qkv, whose output arc_rope_append takes, and
+ * arc_prefill_gemm, whose input arc_paged_attention writes.  No counterpart in
+ * the reference, which serves one request.  All are asynchronous on `stream`,
+ * allocate nothing, keep nothing from one call for the next, and can be
+ * captured; the structs are host memory, read during the call. */
+typedef enum arc_dtype { /* ggml type ids */
+    ARC_F32 = 0,
+    ARC_F16 = 1,
+    ARC_BF16 = 30
+} arc_dtype;
+
+#define ARC_NO_SLOT 0xffffffffu       /* slot of a row that belongs to no request */
+#define ARC_PAGED_RELEASE 0xffffffffu /* new length of a request that has ended */
+
+/* A pool of K pages and one of V pages: page p of k is
+ * [page_size][kv_heads][head_dim] elements from k + p * page_stride on, of v
+ * likewise, so one allocation can hold both, or the pages of every layer.  A
+ * session's cache of a layer (arc_session_kv) is such a pool: max_ctx /
+ * page_size pages in order.  A slot is page * page_size + place in the page. */
+typedef struct arc_kv_pages {
+    void *k, *v;          /* device, 16-byte aligned */
+    uint64_t page_stride; /* elements, >= page_size * kv_heads * head_dim, a multiple of 8 */
+    uint32_t num_pages;   /* num_pages * page_size < 2^32 */
+    uint32_t page_size;   /* positions: a power of two, 1 .. 65536 */
+    uint32_t kv_heads;    /* 1 .. 256 */
+    uint32_t head_dim;    /* 64 or 128 */
+    int32_t dtype;        /* ARC_F16 or ARC_BF16 */
+} arc_kv_pages;
+
+/* The requests of a step, device arrays.  Request b's new tokens are the rows
+ * starts[b] .. starts[b+1] - 1 of the step, at the positions lens[b] - (number of
+ * them) .. lens[b] - 1; position p of it is in page tables[b][p / page_size].  A
+ * step may have more rows (`tokens`) than the requests use: rows from
+ * starts[requests] on belong to no request and no call writes their outputs.
+ * max_pages * page_size <= 2^31. */
+typedef struct arc_paged_batch {
+    uint32_t requests;  /* <= 2^20 */
+    uint32_t tokens;    /* rows of the step, used or not, <= 2^24 */
+    uint32_t max_pages; /* entries of a table row */
+    uint32_t max_new;   /* no request has more new tokens than this */
+    uint32_t *tables;   /* [requests][max_pages] */
+    uint32_t *lens;     /* [requests] positions held, the step's new ones among them */
+    uint32_t *starts;   /* [requests + 1] */
+    uint32_t *positions; /* [tokens] */
+    uint32_t *slots;     /* [tokens] */
+} arc_paged_batch;
+
+/* status[0] of arc_paged_plan: 0, or why the step was refused. */
+#define ARC_PLAN_NO_PAGES 1   /* fewer free pages than the step needs: status[1] more are needed */
+#define ARC_PLAN_TABLE 2      /* a request would pass max_pages (or 2^31 - 1 positions) */
+#define ARC_PLAN_TOKENS 4     /* more new tokens than rows */
+#define ARC_PLAN_MAX_NEW 8    /* a request has more new tokens than max_new */
+#define ARC_PLAN_FREE_LIST 16 /* the free list would hold more than num_pages pages */
+
+/* The step's plan, on the GPU.  old_lens[b]: positions request b holds;
+ * new_lens[b]: its new tokens (0 allowed), or ARC_PAGED_RELEASE: the request has
+ * ended, its pages go back.  free_pages is a stack of *free_count page ids in an
+ * array of num_pages.  Ended requests, in order, push their pages (first to
+ * last); then the others, in order, pop the pages that they lack for their new
+ * positions.  Written: the table entries of new pages (no others), lens (old +
+ * new; 0 for ended requests), starts, for each new token its position and its
+ * slot, for rows behind the last request position 0 and ARC_NO_SLOT, the stack,
+ * *free_count_out, and status[4]: {0, 0, new tokens, pages popped}.  A step that
+ * does not fit (status[0] != 0) changes nothing: lens = old_lens, starts 0,
+ * every slot ARC_NO_SLOT, *free_count_out = *free_count, so that the step's
+ * other calls do nothing.  old_lens may be lens, and free_count free_count_out:
+ * then the plan of the next step takes up where this one ends.  Results do not
+ * depend on the order in which the GPU works. */
+int arc_paged_plan(const arc_paged_batch *batch, const uint32_t *old_lens, const uint32_t *new_lens,
+                   uint32_t page_size, uint32_t *free_pages, uint32_t num_pages, const uint32_t *free_count,
+                   uint32_t *free_count_out, uint32_t *status, arc_stream_t stream);
+
+typedef enum arc_rope_layout {
+    ARC_ROPE_INTERLEAVED = 0, /* pairs (2i, 2i + 1), the session's own layout */
+    ARC_ROPE_HALF = 1         /* pairs (i, i + rot_dim / 2) */
+} arc_rope_layout;
+
+typedef enum arc_rope_scaling {
+    ARC_ROPE_PLAIN = 0,  /* f_i = theta^(-2i / rot_dim) */
+    ARC_ROPE_LINEAR = 1, /* f_i / factor: positions interpolated */
+    ARC_ROPE_YARN = 2    /* by parts (Peng et al. 2023, YaRN): pairs of more than beta_fast turns within original_ctx
+                            positions keep f_i, of fewer than beta_slow take f_i / factor, a linear ramp over i
+                            between; rotated values times 0.1 ln(factor) + 1 */
+} arc_rope_scaling;
+
+/* Angles per position of the rotated pairs, host memory: phases[i] (rot_dim / 2
+ * of them) = f_i / (2 pi) as a fraction of a turn in units of 2^-64, rounded to
+ * nearest, so that position * phases[i] mod 2^64 is the angle at any position
+ * with an error below position * 2^-65 turns.  *scale: the factor on rotated
+ * values (1 but for YaRN).  freq_factors (host, rot_dim / 2 positive numbers, or
+ * NULL) divide f_i last: the rope_freqs tensor of a GGUF file.  beta_fast and
+ * beta_slow (32 and 1 where 0), original_ctx: YaRN only.  rot_dim: a multiple
+ * of 8, at most 128; theta > 1, factor >= 1. */
+int arc_rope_phases(uint32_t rot_dim, double theta, int scaling, double factor, uint32_t original_ctx,
+                    double beta_fast, double beta_slow, const float *freq_factors, uint64_t *phases, float *scale);
+
+typedef struct arc_rope {
+    const uint64_t *phases; /* device copy of arc_rope_phases' phases, 8-byte aligned */
+    uint32_t rot_dim;       /* the first rot_dim values of each head are rotated: a multiple of 8 <= head_dim */
+    int32_t layout;         /* arc_rope_layout */
+    float scale;            /* arc_rope_phases' scale */
+} arc_rope;
+
+/* Bias, rotary positions and cache write of a step.  Row n of x (x_dtype ARC_F32,
+ * ARC_F16 or ARC_BF16; ldx elements from row to row, a multiple of 8; 16-byte
+ * aligned) holds q | k | v: kv_heads * hpk heads, kv_heads heads, kv_heads heads of
+ * head_dim.  For every row n < batch->tokens whose slots[n] is a slot of the pool:
+ *   q[n] = rotate(x_q + q_bias), K slot = rotate(x_k + k_bias), V slot = x_v + v_bias
+ * at positions[n], where rotate turns the pair (a, b) of f_i to
+ * (a cos - b sin, a sin + b cos) * scale and leaves values from rot_dim on; computed in
+ * fp32 and rounded once to pages->dtype.  Rows with ARC_NO_SLOT (or any number
+ * past the pool) are skipped: nothing of theirs is written.  Slots of one step
+ * are distinct (two rows with one slot leave either's values there).  Biases:
+ * fp32, 16-byte aligned, or NULL.  q: ldq elements from row to row (a multiple of
+ * 8), 16-byte aligned, not sharing memory with x.  Of the batch, tokens,
+ * positions and slots are used. */
+int arc_rope_append(const arc_kv_pages *pages, const arc_paged_batch *batch, const arc_rope *rope, int x_dtype,
+                    const void *x, uint32_t ldx, const float *q_bias, const float *k_bias, const float *v_bias,
+                    uint32_t hpk, void *q, uint32_t ldq, arc_stream_t stream);
+
+/* Bytes of device workspace arc_paged_attention needs for steps of these sizes
+ * (of the batch, requests and tokens are used); 0 for sizes that it does not take. */
+size_t arc_paged_attention_workspace_bytes(const arc_kv_pages *pages, const arc_paged_batch *batch, uint32_t hpk);
+
+/* Attention of a step's new tokens over the pages.  Query head h of the row of a token
+ * at position p sees the positions j <= p of its request with p - j < window or
+ * j < sinks (every j <= p where window is 0), in kv head h / hpk:
+ *   out[n][h] = sum_j softmax_j(scale * q[n][h] . k_j) v_j
+ * q and out: pages->dtype, kv_heads * hpk heads of head_dim per row, ldq and ldo
+ * elements from row to row (multiples of 8), 16-byte aligned, sharing no memory
+ * with each other or the pages.  hpk 1..64; scale 0 means 1 / sqrt(head_dim).
+ * Scores, softmax and sums are fp32; weights enter the V product rounded to
+ * pages->dtype.  A position whose table entry is not below num_pages is not
+ * seen, and a row that sees nothing is 0; what lies in the pages at positions not seen
+ * (infinities, NaN) does not matter.  Rows behind the last request are left as they
+ * were.  workspace: arc_paged_attention_workspace_bytes() bytes, 256-byte aligned,
+ * any contents, for one call at a time (calls in order on one stream may share it).
+ * Of the batch, all but positions and slots is used. */
+int arc_paged_attention(const arc_kv_pages *pages, const arc_paged_batch *batch, const void *q, uint32_t ldq,
+                        uint32_t hpk, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
+                        void *workspace, arc_stream_t stream);
+
 /* Tuning hook: force the GEMV lane layout for later launches on this host
  * thread (bs = super-block quads per row: 1,2,4,8,16; rpl = rows per lane:
  * 1,2,4).  bs = 0 restores the automatic choice. */
