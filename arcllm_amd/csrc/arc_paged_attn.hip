@@ -63,44 +63,50 @@ struct PagedAttn {
 };
 
 // ------------------------------------------------------------------- tiles
-// One request: its new rows and positions.
+// One request: its new rows and positions, and what its tiles cost.  Costs are whole
+// numbers in doubles (the host keeps them below 2^52), exact and quicker than 64-bit
+// integers here.
 struct Request {
     uint32_t token;   // first row of the step
     uint32_t rows;    // (token, head) pairs per kv head
     int32_t base;     // position of its first new token (negative: rows without a position)
     uint32_t tiles;   // per kv head
-    uint64_t first, cap;  // cost of tile 0; no tile costs more than cap
-    uint64_t total;       // of a kv head's tiles
+    double first, cap;  // cost of tile 0; no tile costs more than cap
+    double total;       // of a kv head's tiles
 };
 
 // Cost of tiles 0 .. t-1: tile t costs min(first + t * bm, cap), in positions times
 // hpk; causal tiles grow by bm / hpk positions each.
-__device__ __forceinline__ uint64_t cost_before(const Request& r, uint32_t t, uint32_t bm)
+__device__ __forceinline__ double cost_before(const Request& r, uint32_t t, double bm)
 {
-    if (r.first + uint64_t(t) * bm <= r.cap) return t * r.first + uint64_t(bm) * (uint64_t(t) * (t - 1) / 2);  // t = 0: 0
-    const uint64_t k = r.first >= r.cap ? 0 : (r.cap - r.first + bm - 1) / bm;
-    return k * r.first + (k ? uint64_t(bm) * (k * (k - 1) / 2) : 0) + (t - k) * r.cap;
+    const double n = double(t);
+    const double k = fmin(n, r.first >= r.cap ? 0.0 : ceil((r.cap - r.first) / bm));
+    return k * r.first + bm * (k * (k - 1.0) * 0.5) + (n > k ? (n - k) * r.cap : 0.0);
 }
 
 template <bool FEW>
-__device__ __forceinline__ Request request_at(const PagedAttn& a, uint32_t b, uint32_t bm)
+__device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, uint32_t s1, uint32_t held, uint32_t bm)
 {
     Request r{};
-    const uint32_t s0 = a.starts[b], s1 = a.starts[b + 1];
     if (s1 <= s0 || s0 >= a.rows) return r;
-    const uint32_t fresh = min(s1, a.rows) - s0;
-    const uint32_t rows = fresh * a.hpk;
+    const uint32_t rows = (min(s1, a.rows) - s0) * a.hpk;
     if (FEW ? rows > a.few_rows : rows <= a.few_rows) return r;
-    const uint64_t len = min(uint64_t(a.lens[b]), uint64_t(a.max_pages) << a.shift);
+    const uint64_t len = min(uint64_t(held), uint64_t(a.max_pages) << a.shift);
     const int64_t base = int64_t(len) - int64_t(s1 - s0);
     r.token = s0;
     r.rows = rows;
     r.base = int32_t(max(base, -(int64_t(1) << 25)));
     r.tiles = (rows + bm - 1) / bm;
-    r.first = uint64_t(kTileKeys + uint32_t(max(r.base, 0))) * a.hpk + bm;
-    r.cap = a.window ? (uint64_t(kTileKeys) + a.window + a.sinks) * a.hpk + 2 * bm : ~uint64_t(0);
+    r.first = double(kTileKeys + uint32_t(max(r.base, 0))) * a.hpk + bm;
+    r.cap = a.window ? (double(kTileKeys) + a.window + a.sinks) * a.hpk + 2 * bm : 0x1p60;
     r.total = cost_before(r, r.tiles, bm);
     return r;
+}
+
+template <bool FEW>
+__device__ __forceinline__ Request request_at(const PagedAttn& a, uint32_t b, uint32_t bm)
+{
+    return request_of<FEW>(a, a.starts[b], a.starts[b + 1], a.lens[b], bm);
 }
 
 // A tile and the positions that it runs over: units of `keys` positions, first
@@ -138,137 +144,269 @@ __device__ __forceinline__ uint32_t unit_start(const Tile& x, uint32_t u, uint32
 }
 
 // ------------------------------------------------------------------ the line
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d)
-{
-    const uint32_t lo = uint32_t(__shfl_up(int(uint32_t(v)), d)), hi = uint32_t(__shfl_up(int(uint32_t(v >> 32)), d));
-    return (uint64_t(hi) << 32) | lo;
-}
-
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ uint64_t uniform(uint64_t v)
 {
     return (uint64_t(uniform(uint32_t(v >> 32))) << 32) | uniform(uint32_t(v));
 }
+__device__ __forceinline__ double of_lane(double v, int lane)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(u)), lane));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(u >> 32)), lane));
+    return __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
+}
+__device__ __forceinline__ double wave_inclusive(double v)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const double o = __shfl_up(v, d);
+        if (lane >= uint32_t(d)) v += o;
+    }
+    return v;
+}
 
-struct Line {
-    uint64_t total;     // cost of all tiles
-    uint32_t parts, w;  // parts of the line, this workgroup's (w >= parts: it has none)
-    uint64_t from, to;
-    uint32_t b;       // the request in which it begins
-    uint64_t before;  // cost of the requests before b
+// A workgroup's place in the line and the segment of it that it works on, in LDS:
+// wave 0 moves it on, the others read what they need, so that none of it is held in
+// registers while a segment is computed.
+struct Walk {
+    double total, at, to;  // cost of all tiles, what this part has done, its end
+    double before;         // cost of the requests before b
+    uint32_t parts, w, b;
+    // the segment: units [u0, u1) of a tile
+    uint32_t go;           // 0: the part is done
+    uint32_t g, u0, u1, token, complete, slot;
+    int32_t base;
+    Tile x;
 };
 
 // Boundary of part w, the same number wherever it is computed; parts <= total, so no
 // part is empty.
-__device__ __forceinline__ uint64_t part_at(uint64_t total, uint32_t w, uint32_t parts)
+__device__ __forceinline__ double part_at(double total, uint32_t w, uint32_t parts)
 {
-    return w >= parts ? total : uint64_t(double(total) * double(w) / double(parts));
+    return w >= parts ? total : floor(total * double(w) / double(parts));
 }
-
-// Every workgroup adds up all requests (two loads each; thread t takes a run of
-// them), so that no launch has to come first.  Workgroups go to the 8 XCDs in turn: an
-// XCD's workgroups take neighbouring parts, which read the same K and V.
-template <bool FEW, int NT>
-__device__ __forceinline__ Line line_of(const PagedAttn& a, uint32_t bm, uint32_t keys, uint64_t* red)
-{
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    const uint32_t each = (a.requests + NT - 1) / NT;
-    const uint32_t b0 = min(tid * each, a.requests), b1 = min(b0 + each, a.requests);
-    uint64_t sum = 0;
-    for (uint32_t b = b0; b < b1; ++b) sum += request_at<FEW>(a, b, bm).total * a.kv_heads;
-    uint64_t inc = sum;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const uint64_t o = shfl_up64(inc, d);
-        if (lane >= uint32_t(d)) inc += o;
-    }
-    if (lane == 63) red[wave] = inc;
-    __syncthreads();
-    uint64_t before = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < NT / kWave; ++i) {
-        const uint64_t r = red[i];
-        if (uint32_t(i) < wave) before += r;
-        total += r;
-    }
-    Line l;
-    l.total = uniform(total);
-    const uint64_t fit = l.total / (keys * a.hpk);
-    l.parts = uniform(uint32_t(min(uint64_t(gridDim.x), max(fit, uint64_t(l.total != 0)))));
-    l.w = blockIdx.x;
-    l.from = l.to = 0;
-    if (l.w >= l.parts) return l;
-    const uint32_t xcd = blockIdx.x & 7u, q = l.parts >> 3, rest = l.parts & 7u;
-    l.w = xcd * q + min(xcd, rest) + (blockIdx.x >> 3);
-    l.from = part_at(l.total, l.w, l.parts);
-    l.to = part_at(l.total, l.w + 1, l.parts);
-    const uint64_t lo = before + inc - sum;
-    if (lo <= l.from && l.from < lo + sum) {  // one thread, if there is any work
-        uint64_t at = lo;
-        uint32_t b = b0;
-        for (; b < b1; ++b) {
-            const uint64_t c = request_at<FEW>(a, b, bm).total * a.kv_heads;
-            if (at + c > l.from) break;
-            at += c;
-        }
-        red[NT / kWave] = b;
-        red[NT / kWave + 1] = at;
-    }
-    __syncthreads();
-    l.b = uniform(uint32_t(red[NT / kWave]));
-    l.before = uniform(red[NT / kWave + 1]);
-    return l;
-}
-
-// Part of a tile: units [u0, u1) of tile t of kv head g; where it stands in the line.
-struct Segment {
-    uint32_t g, t, u0, u1;
-    uint64_t begin, end;  // the whole tile's
-};
 
 // Which of a tile's units lie before x: monotonic in x, the same for both neighbours
 // of a cut (the same arithmetic on the same numbers).
-__device__ __forceinline__ uint32_t units_before(uint64_t x, uint64_t begin, uint64_t end, uint32_t units)
+__device__ __forceinline__ uint32_t units_before(double x, double begin, double end, uint32_t units)
 {
     if (x <= begin) return 0;
     if (x >= end) return units;
-    return min(units, uint32_t(double(x - begin) * double(units) / double(end - begin)));
+    return min(units, uint32_t((x - begin) * double(units) / (end - begin)));
 }
 
-__device__ __forceinline__ Segment segment_at(const PagedAttn& a, const Request& r, uint64_t before, uint64_t x, uint64_t to,
-                                              uint32_t bm, uint32_t keys, Tile& tile)
+// The part in which x lies.
+__device__ __forceinline__ uint32_t part_of(const Walk& l, double x)
 {
-    Segment s;
-    const uint64_t off = x - before;
-    uint32_t g = uint32_t(double(off) / double(r.total));
-    while (g && uint64_t(g) * r.total > off) --g;
-    while (uint64_t(g + 1) * r.total <= off) ++g;
-    const uint64_t in = off - uint64_t(g) * r.total;
-    uint32_t lo = 0, hi = r.tiles;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (cost_before(r, mid, bm) <= in) lo = mid;
-        else hi = mid;
-    }
-    s.g = uniform(g);
-    s.t = uniform(lo);
-    tile = tile_at(a, r, s.t, bm, keys);
-    s.begin = before + uint64_t(s.g) * r.total + cost_before(r, s.t, bm);
-    s.end = before + uint64_t(s.g) * r.total + cost_before(r, s.t + 1, bm);
-    s.u0 = units_before(x, s.begin, s.end, tile.units);
-    s.u1 = units_before(to, s.begin, s.end, tile.units);
-    s.u0 = uniform(s.u0);
-    s.u1 = uniform(s.u1);
-    return s;
-}
-
-// The workgroup in whose part x lies.
-__device__ __forceinline__ uint32_t part_of(const Line& l, uint64_t x)
-{
-    uint32_t w = min(l.parts - 1, uint32_t(double(x) * double(l.parts) / double(l.total)));
+    uint32_t w = min(l.parts - 1, uint32_t(x * double(l.parts) / l.total));
     while (w && part_at(l.total, w, l.parts) > x) --w;
     while (w + 1 < l.parts && part_at(l.total, w + 1, l.parts) <= x) ++w;
     return w;
+}
+
+// This workgroup's part, from the total.  Workgroups go to the 8 XCDs in turn: an
+// XCD's workgroups take neighbouring parts, which read the same K and V.
+__device__ __forceinline__ void take_part(const PagedAttn& a, Walk& l, double total, uint32_t keys)
+{
+    l.total = total;
+    l.parts = uint32_t(fmin(double(gridDim.x), fmax(floor(total / (double(keys) * a.hpk)), total > 0.0 ? 1.0 : 0.0)));
+    l.w = blockIdx.x;
+    l.at = l.to = 0.0;
+    if (l.w >= l.parts) return;
+    const uint32_t xcd = blockIdx.x & 7u, q = l.parts >> 3, rest = l.parts & 7u;
+    l.w = xcd * q + min(xcd, rest) + (blockIdx.x >> 3);
+    l.at = part_at(total, l.w, l.parts);
+    l.to = part_at(total, l.w + 1, l.parts);
+}
+
+// Adds up the requests, so that no launch has to come first, and finds the one in which the
+// part begins.  Up to 64 requests: wave 0 alone, one per lane; the lanes' requests are
+// returned for next_segment.  More: thread t takes a run of them.
+template <bool FEW, int NT>
+__device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, uint32_t bm, uint32_t keys, Piece* pieces, double* red)
+{
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    if (a.requests <= 64) {
+        if (wave == 0) {
+            const Request r = lane < a.requests ? request_at<FEW>(a, lane, bm) : Request{};
+            const double own = r.total * a.kv_heads, inc = wave_inclusive(own);
+            Walk m;
+            take_part(a, m, of_lane(inc, 63), keys);
+            const uint64_t behind = __ballot(inc > m.at);  // lanes from the part's first request on
+            const int b = behind ? __builtin_ctzll(behind) : 0;
+            m.b = uint32_t(b);
+            m.before = of_lane(inc - own, b);
+            if (lane == 0) l = m;
+        }
+    } else {
+        const uint32_t each = (a.requests + NT - 1) / NT;
+        const uint32_t b0 = min(tid * each, a.requests), b1 = min(b0 + each, a.requests);
+        double sum = 0.0;
+#pragma unroll 4
+        for (uint32_t b = b0; b < b1; ++b) sum += request_at<FEW>(a, b, bm).total * a.kv_heads;
+        const double inc = wave_inclusive(sum);
+        if (lane == 63) red[wave] = inc;
+        __syncthreads();
+        double before = 0.0, total = 0.0;
+#pragma unroll
+        for (int i = 0; i < NT / kWave; ++i) {
+            const double r = red[i];
+            if (uint32_t(i) < wave) before += r;
+            total += r;
+        }
+        Walk m;
+        take_part(a, m, total, keys);
+        const double lo = before + inc - sum;
+        if (tid == 0) {  // with no work, all there is
+            m.b = 0;
+            m.before = 0.0;
+            l = m;
+        }
+        __syncthreads();
+        if (lo <= m.at && m.at < lo + sum) {  // one thread, if there is any work
+            double at = lo;
+            uint32_t b = b0;
+            for (; b + 1 < b1; ++b) {
+                const double c = request_at<FEW>(a, b, bm).total * a.kv_heads;
+                if (at + c > m.at) break;
+                at += c;
+            }
+            l.b = b;
+            l.before = at;
+        }
+    }
+    __syncthreads();
+    if (tid < 2) pieces[2 * l.w + tid].n = 0;
+}
+
+// Wave 0: the part's next segment.  A cut tile gets its slot and its record for k_paged_join.
+template <bool FEW>
+__device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, uint32_t bm, uint32_t keys, Piece* pieces)
+{
+    if (threadIdx.x >= 64) return;
+    Walk m = l;
+    m.go = m.at < m.to;
+    if (m.go) {
+        Request r;
+        for (;; ++m.b) {  // the request at m.at
+            r = request_at<FEW>(a, m.b, bm);
+            if (m.at < m.before + r.total * a.kv_heads) break;
+            m.before += r.total * a.kv_heads;
+        }
+        const double off = m.at - m.before;
+        m.g = min(a.kv_heads - 1, uint32_t(off / r.total));
+        while (m.g && m.g * r.total > off) --m.g;
+        while (m.g + 1 < a.kv_heads && (m.g + 1) * r.total <= off) ++m.g;
+        const double in = off - m.g * r.total;
+        uint32_t lo = 0, hi = r.tiles;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (cost_before(r, mid, bm) <= in) lo = mid;
+            else hi = mid;
+        }
+        m.x = tile_at(a, r, lo, bm, keys);
+        const double begin = m.before + m.g * r.total + cost_before(r, lo, bm);
+        const double end = m.before + m.g * r.total + cost_before(r, lo + 1, bm);
+        m.u0 = units_before(m.at, begin, end, m.x.units);
+        m.u1 = units_before(m.to, begin, end, m.x.units);
+        m.token = r.token;
+        m.base = r.base;
+        m.complete = m.at <= begin && end <= m.to;
+        if (!m.complete) {
+            const uint32_t w0 = part_of(m, begin), w1 = part_of(m, end - 1.0);
+            const uint32_t first = 2 * w0 + (part_at(m.total, w0, m.parts) < begin ? 1u : 0u);
+            m.slot = m.w == w0 ? first : 2 * m.w;
+            if (threadIdx.x == 0)
+                pieces[m.slot] = Piece{w1 - w0 + 1, m.w - w0, w0, first, r.token, m.x.row0, m.x.rows, m.g};
+        }
+        m.at = fmin(end, m.to);
+    }
+    if (threadIdx.x == 0) l = m;
+}
+
+// What every wave needs of the segment, in scalar registers.
+struct Segment {
+    uint32_t b, g, u0, u1, token, complete, slot;
+    int32_t base;
+    Tile x;
+};
+__device__ __forceinline__ Segment read_segment(const Walk& l)
+{
+    Segment s;
+    s.b = uniform(l.b);
+    s.g = uniform(l.g);
+    s.u0 = uniform(l.u0);
+    s.u1 = uniform(l.u1);
+    s.token = uniform(l.token);
+    s.complete = uniform(l.complete);
+    s.slot = uniform(l.slot);
+    s.base = uniform(l.base);
+    s.x.row0 = uniform(l.x.row0);
+    s.x.rows = uniform(l.x.rows);
+    s.x.pos0 = uniform(l.x.pos0);
+    s.x.pos1 = uniform(l.x.pos1);
+    s.x.sink_units = uniform(l.x.sink_units);
+    s.x.low = uniform(l.x.low);
+    s.x.units = 0;
+    return s;
+}
+
+// ------------------------------------------------------------- rows of K and V
+// The element offset of a position's row: its page's and its place's.
+__device__ __forceinline__ uint64_t row_offset(const PagedAttn& a, uint32_t page, uint32_t pos, uint32_t kvd)
+{
+    return page < a.num_pages ? uint64_t(page) * a.page_stride + uint64_t(pos & ((1u << a.shift) - 1u)) * kvd : 0;
+}
+
+// A K or V row in LDS: D / 8 blocks of 16 bytes, block c of row r at place
+// c ^ swizzle(r), so that the 8 or 4 rows that a read touches at once lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t swizzle(uint32_t r)
+{
+    return D == 128 ? (r & 7u) << 1 : ((r >> 1) & 3u) << 1;
+}
+
+// N rows (N a multiple of the rows of one copy) from the pages straight into LDS, 16 bytes a lane, row i
+// at lds + i * D.  `page`: lane first + i holds the page of row i's position pos0 + i.  Which 16 bytes a lane
+// copies carries the swizzle, as LDS is written in lane order.  WIDE, pages of 16 and more: 16
+// aligned rows have one page, so the address is scalar.
+template <typename T, int D, int N, bool WIDE>
+__device__ __forceinline__ void copy_rows(const PagedAttn& a, const T* src, T* lds, uint32_t page, uint32_t first, uint32_t pos0,
+                                          uint32_t kvd, uint32_t head)
+{
+    constexpr uint32_t kAcross = D / 8, kRows = kWave / kAcross;  // lanes per row, rows per copy
+    const uint32_t lane = threadIdx.x & 63u, r0 = lane / kAcross, c = lane % kAcross;
+    typedef __attribute__((address_space(1))) const void gptr;
+    typedef __attribute__((address_space(3))) void lptr;
+    if constexpr (WIDE) {
+#pragma unroll
+        for (uint32_t i = 0; i < uint32_t(N); i += kRows) {
+            const uint32_t part = i & ~15u;  // the 16 rows that share a page
+            const uint32_t pg = uint32_t(__builtin_amdgcn_readlane(int(page), int(first + part)));
+            const T* base = src + row_offset(a, pg, pos0 + part, kvd) + head;
+            const uint32_t r = i - part + r0;
+            __builtin_amdgcn_global_load_lds((gptr*)(base + (r * kvd + ((c ^ swizzle<D>(r)) << 3))), (lptr*)(lds + i * D), 16, 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < uint32_t(N); i += kRows) {
+            const uint32_t r = i + r0;
+            const uint32_t pg = uint32_t(__shfl(int(page), int(first + r)));
+            const T* row = src + row_offset(a, pg, pos0 + r, kvd) + head;
+            __builtin_amdgcn_global_load_lds((gptr*)(row + ((c ^ swizzle<D>(r)) << 3)), (lptr*)(lds + i * D), 16, 0, 0);
+        }
+    }
+}
+
+// Waits until every load and copy of this wave has arrived.
+__device__ __forceinline__ void wait_loads()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
 }
 
 // ------------------------------------------------------------ matrix products
@@ -287,14 +425,6 @@ __device__ __forceinline__ vec8<T> narrow(const f32x16& p, int at)
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = static_cast<T>(p[at + j]);
     return r;
-}
-
-// A K or V row in LDS: D / 8 blocks of 16 bytes, block c of row r at place
-// c ^ swizzle(r), so that the 8 or 4 rows that a read touches at once lie in different banks.
-template <int D>
-__device__ __forceinline__ uint32_t swizzle(uint32_t r)
-{
-    return D == 128 ? (r & 7u) << 1 : ((r >> 1) & 3u) << 1;
 }
 
 // V^T operand: dims 32 t + (lane & 31), keys 16 s + 8 (j / 4) + 4 (lane / 32) + j % 4 of rows in
@@ -332,6 +462,28 @@ __device__ __forceinline__ bool sees(int32_t qpos, int32_t kpos, uint32_t window
     return kpos <= qpos && (window == 0 || uint32_t(qpos - kpos) < window || uint32_t(kpos) < sinks);
 }
 
+// Which of the 32 positions from k0 on a query at qpos sees, as bits.
+__device__ __forceinline__ uint32_t seen_bits(int32_t qpos, int32_t k0, uint32_t window, uint32_t sinks)
+{
+    const int32_t n = qpos - k0;  // the last of them
+    if (n < 0) return 0;
+    uint32_t bits = n >= 31 ? ~0u : (2u << n) - 1u;
+    if (window && uint32_t(n) >= window) {
+        const uint32_t first = uint32_t(n) - window + 1u, sink = sinks > uint32_t(k0) ? sinks - uint32_t(k0) : 0u;
+        bits &= (first > 31 ? 0u : ~0u << first) | (sink > 31 ? ~0u : (1u << sink) - 1u);
+    }
+    return bits;
+}
+
+// The scores of a tile of 32 positions that its query does not see become -infinity.
+__device__ __forceinline__ void hide(f32x16& sc, uint32_t bits)
+{
+    bits >>= 4u * ((threadIdx.x >> 5) & 1u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        sc[i] = int32_t(bits << (31 - 8 * (i >> 2) - (i & 3))) < 0 ? sc[i] : -INFINITY;
+}
+
 // Running softmax of one query (a lane and its partner lane ^ 32, each with half of the
 // keys): `m` is the reference that weights 2^(score - m) are relative to, `l` the lane's share of
 // their sum.  m follows the maximum only when that has grown by more than kLazy: weights then
@@ -354,38 +506,14 @@ __device__ __forceinline__ void rescale(float mx, float& m, float& l, f32x16 (&o
 // Value i of a score or output tile of 32: key, or dim, 8 (i / 4) + 4 (lane / 32) + i % 4.
 __device__ __forceinline__ uint32_t tile_index(int i) { return 8u * (i >> 2) + 4u * ((threadIdx.x >> 5) & 1u) + (i & 3); }
 
-// What infinities and NaN of V at positions that only some of a tile's rows see have to
-// add: their places in V were cleared for the product, where a weight of 0 would make NaN
-// of them; here each row that sees the position gets them.  keys: bit k set where position k0 + k
-// holds one; at: element offset of lane k's position (same for V and K).
-template <typename T, int D>
-__device__ __forceinline__ void add_nonfinite(f32x16 (&o)[D / 32], const T* v, uint64_t keys, int32_t k0, uint64_t at,
-                                           int32_t qpos, uint32_t window, uint32_t sinks)
-{
-    while (keys) {
-        const int k = __builtin_ctzll(keys);
-        keys &= keys - 1;
-        const uint64_t off = (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(at >> 32)), k))) << 32) |
-                             uint32_t(__builtin_amdgcn_readlane(int(uint32_t(at)), k));
-        if (!sees(qpos, k0 + k, window, sinks)) continue;
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = static_cast<float>(v[off + 32 * t + tile_index(i)]);
-                if (!(fabsf(x) < INFINITY)) o[t][i] += x;
-            }
-    }
-}
-
 // Query operand of 32 rows: lane -> row lane & 31, dims 16 s + 8 (lane / 32) .. + 7; zeros for
 // rows that the tile does not have.
 template <typename T, int D>
-__device__ __forceinline__ void load_q(const PagedAttn& a, const Request& r, uint32_t row, bool in, uint32_t g, vec8<T> (&q)[D / 16])
+__device__ __forceinline__ void load_q(const PagedAttn& a, uint32_t token, uint32_t row, bool in, uint32_t g, vec8<T> (&q)[D / 16])
 {
     const uint32_t h2 = (threadIdx.x >> 5) & 1u;
     const uint32_t tok = row / a.hpk, h = row - tok * a.hpk;
-    const T* p = static_cast<const T*>(a.q) + uint64_t(r.token + tok) * a.ldq + (g * a.hpk + h) * D + 8 * h2;
+    const T* p = static_cast<const T*>(a.q) + uint64_t(token + tok) * a.ldq + (g * a.hpk + h) * D + 8 * h2;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
         uint4 w = make_uint4(0, 0, 0, 0);
@@ -416,206 +544,190 @@ __device__ __forceinline__ T* out_row(const PagedAttn& a, uint32_t token, uint32
     return static_cast<T*>(a.out) + uint64_t(token + tok) * a.ldo + (g * a.hpk + h) * dim;
 }
 
-// The slot of a piece, and its record for k_paged_join.
-__device__ __forceinline__ uint32_t write_piece(Piece* pieces, const Line& l, const Segment& s, const Request& r, const Tile& x)
+// Whether every row of the tile sees all of `keys` positions from k0 on that have pages (valid).
+__device__ __forceinline__ bool all_seen(const PagedAttn& a, const Tile& x, int32_t k0, uint32_t keys, bool valid)
 {
-    const uint32_t w0 = part_of(l, s.begin), w1 = part_of(l, s.end - 1);
-    const uint32_t first = 2 * w0 + (part_at(l.total, w0, l.parts) < s.begin ? 1u : 0u);
-    const uint32_t slot = l.w == w0 ? first : 2 * l.w;
-    if (threadIdx.x == 0) pieces[slot] = Piece{w1 - w0 + 1, l.w - w0, w0, first, r.token, x.row0, x.rows, s.g};
-    return slot;
+    return valid && k0 + int32_t(keys) - 1 <= x.pos0 &&
+           (a.window == 0 || uint32_t(x.pos1 - k0) < a.window || uint32_t(k0) + keys <= a.sinks);
+}
+
+// The 16 bytes at p without infinities and NaN, or zero where the position is not in; whether there were any.
+template <typename T>
+__device__ __forceinline__ bool clean(T* p, bool in)
+{
+    uint4 w = *reinterpret_cast<const uint4*>(p);
+    if (!in) w = make_uint4(0, 0, 0, 0);
+    bool any = drop_nonfinite<T>(w.x);
+    any |= drop_nonfinite<T>(w.y);
+    any |= drop_nonfinite<T>(w.z);
+    any |= drop_nonfinite<T>(w.w);
+    *reinterpret_cast<uint4*>(p) = w;
+    return any;
+}
+
+// What infinities and NaN of V at positions that only some of a tile's rows see have to add: their
+// places in V were cleared for the product, where a weight of 0 would make NaN of them; here, after the
+// segment's units, each row that sees such a position gets them.  Units that all rows see
+// need none of it.  A slow pass over the segment's other units, for data that has any; first_of
+// and page_of as in the kernels, `span` positions of each unit.
+template <typename T, int D, typename First, typename Page>
+__device__ __forceinline__ void add_nonfinite(const PagedAttn& a, f32x16 (&o)[D / 32], const T* v, const Segment& s, uint32_t span,
+                                              int32_t qpos, uint32_t kvd, First first_of, Page page_of)
+{
+#pragma unroll 1
+    for (uint32_t u = s.u0; u < s.u1; ++u) {
+        const int32_t k0 = int32_t(first_of(u));
+        const uint32_t page = page_of(u);
+        if (all_seen(a, s.x, k0, span, true)) continue;
+#pragma unroll 1
+        for (uint32_t j = 0; j < span; ++j) {
+            const uint32_t pg = uint32_t(__builtin_amdgcn_readlane(int(page), int(j)));
+            if (pg >= a.num_pages || !sees(qpos, k0 + int32_t(j), a.window, a.sinks)) continue;
+            const T* p = v + row_offset(a, pg, uint32_t(k0) + j, kvd);
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = static_cast<float>(p[32 * t + tile_index(i)]);
+                    if (!(fabsf(x) < INFINITY)) o[t][i] += x;
+                }
+        }
+    }
+}
+
+__device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before it come before those after it
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // ------------------------------------------------------------------ few rows
 // Tiles of up to 32 rows: decode, short chunks.  Bound by reading K and V once.  4
 // waves, each on its own 32 positions of a unit with its own softmax, joined through LDS
-// at the tile's end; nothing but that join needs a barrier.  Lane -> position
-// lane & 31, half of the row's 16-byte blocks: one address serves K and V, and
-// K's registers are the score product's operand as they come (S^T = K Q^T; lane -> query).
-// V goes through LDS for its transposed operand (O^T = V^T P^T), P^T comes straight from the
-// scores' registers.  The next unit's K and V are loaded while this one is computed.
-template <typename T, int D>
-struct KvRegs {
-    uint4 k[D / 16], v[D / 16];
-};
-
-template <typename T, int D>
-__device__ __forceinline__ void load_kv(KvRegs<T, D>& r, const T* k, const T* v, uint64_t at)
-{
-    const uint32_t h2 = (threadIdx.x >> 5) & 1u;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) r.k[s] = *reinterpret_cast<const uint4*>(k + at + 16 * s + 8 * h2);
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) r.v[s] = *reinterpret_cast<const uint4*>(v + at + 16 * s + 8 * h2);
-}
-
-template <typename T, int D>
-struct FewState {
-    vec8<T> q[D / 16];
-    f32x16 o[D / 32];
-    float m, l;
-};
-
-// One wave's 32 positions from k0 on.  `in`: the lane's position has a page.
-template <typename T, int D>
-__device__ __forceinline__ void few_unit(const PagedAttn& a, FewState<T, D>& st, KvRegs<T, D>& r, T* vrows, const T* v, int32_t k0,
-                                         uint64_t at, bool in, const Tile& x, int32_t qpos)
-{
-    const uint32_t lane = threadIdx.x & 63u, l32 = lane & 31u, h2 = lane >> 5;
-    const uint64_t valid = __ballot(in);
-    const bool whole = uint32_t(valid) == 0xffffffffu && k0 + 31 <= x.pos0 &&
-                       (a.window == 0 || uint32_t(x.pos1 - k0) < a.window || uint32_t(k0) + 32u <= a.sinks);
-    uint64_t odd = 0;  // positions with infinities or NaN in V
-    if (!whole) {
-        bool any = false;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&r.v[s]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (!in) w[i] = 0;
-                any |= drop_nonfinite<T>(w[i]);
-            }
-        }
-        odd = __ballot(any);
-        odd = (odd | (odd >> 32)) & 0xffffffffu;
-    }
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s)
-        *reinterpret_cast<uint4*>(vrows + l32 * D + (((2u * s + h2) ^ swizzle<D>(l32)) << 3)) = r.v[s];
-    f32x16 sc;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) sc = mfma<T>(__builtin_bit_cast(vec8<T>, r.k[s]), st.q[s], sc);
-    float mx = -INFINITY;
-    if (whole) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint32_t j = tile_index(i);
-            const bool see = ((uint32_t(valid) >> j) & 1u) && sees(qpos, k0 + int32_t(j), a.window, a.sinks);
-            sc[i] = see ? sc[i] : -INFINITY;
-            mx = fmaxf(mx, sc[i]);
-        }
-    }
-    mx = xor_max<32>(mx) * a.scale;
-    rescale(mx, st.m, st.l, st.o);
-    const float mr = st.m == -INFINITY ? 0.0f : st.m;  // nothing seen yet: all weights 0
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.scale, -mr));
-        sum += sc[i];
-    }
-    st.l += sum;
-    // the wave's own V rows: its writes above come before these reads
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const vec8<T> p = narrow<T>(sc, 8 * s);
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t) st.o[t] = mfma<T>(load_vt<T, D>(vrows, s, t), p, st.o[t]);
-    }
-    if (odd) add_nonfinite<T, D>(st.o, v, odd, k0, at, qpos, a.window, a.sinks);
-    // the next unit's V overwrites these rows
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-template <typename T, int D>
+// at the tile's end; nothing but that join needs a barrier.  K: lane -> position
+// lane & 31, half of the row's 16-byte blocks, which is the score product's operand as it comes
+// (S^T = K Q^T; lane -> query).  V goes straight to LDS for its transposed operand (O^T = V^T
+// P^T), P^T comes from the scores' registers.  The next unit's V is on its way while
+// this one is computed, its K from the moment this one's scores are done: 16 KB a wave.
+template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
 {
-    __shared__ uint64_t red[6];
-    __shared__ __align__(16) float joined[4 * 32 * D];  // V rows of each wave, then the waves' outputs
+    __shared__ double red[4];
+    __shared__ Walk walk;
+    __shared__ __align__(16) float joined[4 * 32 * D];  // two V buffers of each wave, then the waves' outputs
     __shared__ float mw[4][32], lw[4][32];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, wave = uniform(tid >> 6);
-    const Line line = line_of<true, 256>(a, kFewRows, kFewKeys, red);
-    if (tid < 2) a.few_p[2 * line.w + tid].n = 0;
-    T* vrows = reinterpret_cast<T*>(joined) + wave * (32 * D);
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
+    start_walk<true, 256>(a, walk, kFewRows, kFewKeys, a.few_p, red);
+    T* vrows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
     const T* k = static_cast<const T*>(a.k);
     const T* v = static_cast<const T*>(a.v);
-    const uint32_t kvd = a.kv_heads * D, place = (1u << a.shift) - 1u;
-    uint32_t b = line.b;
-    uint64_t before = line.before;
-    Request r{};
-    for (uint64_t at = line.from; at < line.to;) {
-        for (;; ++b) {  // the request at `at`
-            r = request_at<true>(a, b, kFewRows);
-            if (at < before + r.total * a.kv_heads) break;
-            before += r.total * a.kv_heads;
-        }
-        Tile x;
-        const Segment s = segment_at(a, r, before, at, line.to, kFewRows, kFewKeys, x);
-        const uint32_t row = min(l32, x.rows - 1);
-        const int32_t qpos = r.base + int32_t((x.row0 + row) / a.hpk);
-        const uint32_t* table = a.tables + uint64_t(b) * a.max_pages;
-        FewState<T, D> st;
-        load_q<T, D>(a, r, x.row0 + row, l32 < x.rows, s.g, st.q);
+    const uint32_t kvd = a.kv_heads * D;
+    for (;;) {
+        next_segment<true>(a, walk, kFewRows, kFewKeys, a.few_p);
+        __syncthreads();
+        if (uniform(walk.go) == 0) break;
+        const Segment s = read_segment(walk);
+        const uint32_t head = s.g * D;
+        const uint32_t row = min(l32, s.x.rows - 1);
+        const int32_t qpos = s.base + int32_t((s.x.row0 + row) / a.hpk);
+        const uint32_t* table = a.tables + uint64_t(s.b) * a.max_pages;
+        f32x16 o[D / 32];
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) st.o[t][i] = 0.0f;
-        st.m = -INFINITY;
-        st.l = 0.0f;
+            for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+        bool odd = false;  // infinities or NaN cleared from V
 
-        // page of the lane's position in unit u: loaded a unit ahead of the K and V it points to
-        auto key_of = [&](uint32_t u) { return int32_t(unit_start(x, u, kFewKeys) + 32u * wave + l32); };
+        // the wave's first position of unit u, the page of lane l32's
+        auto first_of = [&](uint32_t u) { return unit_start(s.x, u, kFewKeys) + 32u * wave; };
         auto page_of = [&](uint32_t u) {
-            const int32_t kp = key_of(u);
-            return kp <= x.pos1 ? table[uint32_t(kp) >> a.shift] : 0xffffffffu;
+            const int32_t kp = int32_t(first_of(u) + l32);
+            return kp <= s.x.pos1 ? table[uint32_t(kp) >> a.shift] : 0xffffffffu;
         };
-        auto offset_of = [&](uint32_t page, uint32_t u) {
-            const uint32_t kp = uint32_t(key_of(u));
-            return page < a.num_pages ? uint64_t(page) * a.page_stride + uint64_t(kp & place) * kvd + s.g * D : uint64_t(0);
+        uint4 kr[D / 16];
+        auto load_k = [&](uint32_t page, uint32_t u) {
+            const T* p = k + row_offset(a, page, first_of(u) + l32, kvd) + head + 8 * h2;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) kr[i] = *reinterpret_cast<const uint4*>(p + 16 * i);
         };
         if (s.u0 < s.u1) {
-            KvRegs<T, D> cur, nxt;
             uint32_t page = page_of(s.u0);
-            uint64_t off = offset_of(page, s.u0);
-            load_kv(cur, k, v, off);
             uint32_t npage = s.u0 + 1 < s.u1 ? page_of(s.u0 + 1) : 0xffffffffu;
+            vec8<T> q[D / 16];
+            load_q<T, D>(a, s.token, s.x.row0 + row, l32 < s.x.rows, s.g, q);
+            load_k(page, s.u0);
+            copy_rows<T, D, 32, WIDE>(a, v, vrows, page, 0, first_of(s.u0), kvd, head);
+            T* vcur = vrows;
+            T* vnext = vrows + 32 * D;
             for (uint32_t u = s.u0; u < s.u1; ++u) {
-                uint64_t noff = 0;
+                const int32_t k0 = int32_t(first_of(u));
+                wait_loads();  // K, V of this unit, the next one's pages
+                const bool more = u + 1 < s.u1;
                 uint32_t far = 0xffffffffu;
-                if (u + 1 < s.u1) {
-                    noff = offset_of(npage, u + 1);
-                    load_kv(nxt, k, v, noff);
+                if (more) {
+                    copy_rows<T, D, 32, WIDE>(a, v, vnext, npage, 0, first_of(u + 1), kvd, head);
                     if (u + 2 < s.u1) far = page_of(u + 2);
                 }
-                few_unit<T, D>(a, st, cur, vrows, v, int32_t(unit_start(x, u, kFewKeys) + 32u * wave), off, page < a.num_pages, x,
-                               qpos);
-                cur = nxt;
-                off = noff;
+                f32x16 sc;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) sc = mfma<T>(__builtin_bit_cast(vec8<T>, kr[i]), q[i], sc);
+                if (more) load_k(npage, u + 1);
+
+                const bool in = page < a.num_pages;
+                const uint32_t valid = uint32_t(__ballot(in));
+                const bool whole = all_seen(a, s.x, k0, 32, valid == 0xffffffffu);
+                if (!whole) {
+                    for (uint32_t c = h2; c < D / 8; c += 2) odd |= clean(vcur + l32 * D + c * 8, in);
+                    hide(sc, valid & seen_bits(qpos, k0, a.window, a.sinks));
+                    wave_fence();
+                }
+                float mx = sc[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
+                mx = xor_max<32>(mx) * a.scale;
+                rescale(mx, m, l, o);
+                const float mr = m == -INFINITY ? 0.0f : m;  // nothing seen yet: all weights 0
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.scale, -mr));
+                    l += sc[i];
+                }
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const vec8<T> p = narrow<T>(sc, 8 * st);
+#pragma unroll
+                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vcur, st, t), p, o[t]);
+                }
+                wave_fence();  // the unit after the next is copied over these rows
+                T* const t = vcur;
+                vcur = vnext;
+                vnext = t;
                 page = npage;
                 npage = far;
             }
+            if (__ballot(odd)) add_nonfinite<T, D>(a, o, v + head, s, 32, qpos, kvd, first_of, page_of);
         }
         // the waves' states in wave order: out = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w
         __syncthreads();  // every wave is done with its V rows
-        const float l = xor_sum<32>(st.l);
-        if (l32 < x.rows) {
+        const float lsum = xor_sum<32>(l);
+        if (l32 < s.x.rows) {
 #pragma unroll
             for (int t = 0; t < D / 32; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
                     *reinterpret_cast<float4*>(&joined[(wave * 32 + l32) * D + 32 * t + tile_index(i)]) =
-                        make_float4(st.o[t][i], st.o[t][i + 1], st.o[t][i + 2], st.o[t][i + 3]);
+                        make_float4(o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]);
             if (lane < 32) {
-                mw[wave][l32] = st.m;
-                lw[wave][l32] = l;
+                mw[wave][l32] = m;
+                lw[wave][l32] = lsum;
             }
         }
         __syncthreads();
-        const bool complete = at <= s.begin && s.end <= line.to;
-        uint32_t slot = 0;
-        if (!complete) slot = write_piece(a.few_p, line, s, r, x);
-        for (uint32_t e = tid; e < x.rows * (D / 4); e += 256) {
+        for (uint32_t e = tid; e < s.x.rows * (D / 4); e += 256) {
             const uint32_t rr = e / (D / 4), d = 4 * (e % (D / 4));
             float M = -INFINITY;
 #pragma unroll
@@ -626,70 +738,57 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float f = __builtin_amdgcn_exp2f(mw[i][rr] - M0);
-                const float4 o = *reinterpret_cast<const float4*>(&joined[(i * 32 + rr) * D + d]);
+                const float4 w = *reinterpret_cast<const float4*>(&joined[(i * 32 + rr) * D + d]);
                 L = __builtin_fmaf(lw[i][rr], f, L);
-                acc.x = __builtin_fmaf(o.x, f, acc.x);
-                acc.y = __builtin_fmaf(o.y, f, acc.y);
-                acc.z = __builtin_fmaf(o.z, f, acc.z);
-                acc.w = __builtin_fmaf(o.w, f, acc.w);
+                acc.x = __builtin_fmaf(w.x, f, acc.x);
+                acc.y = __builtin_fmaf(w.y, f, acc.y);
+                acc.z = __builtin_fmaf(w.z, f, acc.z);
+                acc.w = __builtin_fmaf(w.w, f, acc.w);
             }
-            if (complete) {
+            if (s.complete) {
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // nothing seen: zeros
-                store4<T>(out_row<T>(a, r.token, x.row0 + rr, s.g, D) + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                store4<T>(out_row<T>(a, s.token, s.x.row0 + rr, s.g, D) + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             } else {
-                *reinterpret_cast<float4*>(a.few_o + (uint64_t(slot) * a.few_slot + rr) * D + d) = acc;
-                if (d == 0) a.few_ml[uint64_t(slot) * a.few_slot + rr] = make_float2(M, L);
+                *reinterpret_cast<float4*>(a.few_o + (uint64_t(s.slot) * a.few_slot + rr) * D + d) = acc;
+                if (d == 0) a.few_ml[uint64_t(s.slot) * a.few_slot + rr] = make_float2(M, L);
             }
         }
-        __syncthreads();  // the next tile's V rows overwrite `joined`
-        at = min(s.end, line.to);
+        __syncthreads();  // the next tile's V rows overwrite `joined`, its segment `walk`
     }
 }
 
 // ----------------------------------------------------------------- many rows
 // Tiles of NW * 32 rows: prompts and long chunks.  Bound by the matrix cores and the
 // softmax's vector instructions.  Each wave holds 32 rows (Q, O in registers); the
-// unit's 64 rows of K and V come through LDS, shared by the waves and double buffered:
-// while unit u is computed from one buffer, unit u + 1 is on its way to registers, and is
-// written to the other buffer at the end; one barrier per unit.  Operands as in the
+// unit's 64 rows of K and V come straight into LDS, shared by the waves and double buffered:
+// unit u + 1 is copied while unit u is computed; one barrier per unit.  Operands as in the
 // few-rows kernel, K's read from LDS.
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, bool WIDE>
 __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
 {
     constexpr int NT = NW * 64;
-    constexpr uint32_t kBm = NW * 32;
-    constexpr int kBlocks = D / 8;                       // 16-byte blocks of a row
-    constexpr int kRows = NT / kBlocks;                  // rows staged at a time
-    constexpr int kPass = kManyKeys / kRows;
-    static_assert(kPass >= 1 && kPass * kRows == int(kManyKeys), "staging covers the unit");
-    __shared__ uint64_t red[NW + 2];
+    constexpr uint32_t kBm = NW * 32, kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
     __shared__ __align__(16) T ks[2][kManyKeys * D];
     __shared__ __align__(16) T vs[2][kManyKeys * D];
-    __shared__ uint32_t odd_bits[3][2];
+    __shared__ double red[NW];
+    __shared__ Walk walk;
+    __shared__ uint32_t odd;  // infinities or NaN cleared from V in this segment
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    const Line line = line_of<false, NT>(a, kBm, kManyKeys, red);
-    if (tid < 2) a.many_p[2 * line.w + tid].n = 0;
+    start_walk<false, NT>(a, walk, kBm, kManyKeys, a.many_p, red);
     const T* k = static_cast<const T*>(a.k);
     const T* v = static_cast<const T*>(a.v);
-    const uint32_t kvd = a.kv_heads * D, place = (1u << a.shift) - 1u;
-    const uint32_t sr = tid / kBlocks, sb = tid % kBlocks;  // staged row (of a pass) and block
-    uint32_t b = line.b;
-    uint64_t before = line.before;
-    Request r{};
-    for (uint64_t at = line.from; at < line.to;) {
-        for (;; ++b) {
-            r = request_at<false>(a, b, kBm);
-            if (at < before + r.total * a.kv_heads) break;
-            before += r.total * a.kv_heads;
-        }
-        Tile x;
-        const Segment s = segment_at(a, r, before, at, line.to, kBm, kManyKeys, x);
+    const uint32_t kvd = a.kv_heads * D;
+    for (;;) {
+        next_segment<false>(a, walk, kBm, kManyKeys, a.many_p);
+        if (tid == 0) odd = 0;
+        __syncthreads();
+        if (uniform(walk.go) == 0) break;
+        const Segment s = read_segment(walk);
+        const uint32_t head = s.g * D;
         const uint32_t trow = wave * 32 + l32;
-        const uint32_t row = min(trow, x.rows - 1);
-        const int32_t qpos = r.base + int32_t((x.row0 + row) / a.hpk);
-        const uint32_t* table = a.tables + uint64_t(b) * a.max_pages;
-        vec8<T> q[D / 16];
-        load_q<T, D>(a, r, x.row0 + row, trow < x.rows, s.g, q);
+        const uint32_t row = min(trow, s.x.rows - 1);
+        const int32_t qpos = s.base + int32_t((s.x.row0 + row) / a.hpk);
+        const uint32_t* table = a.tables + uint64_t(s.b) * a.max_pages;
         f32x16 o[D / 32];
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
@@ -697,102 +796,62 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
             for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
         float m = -INFINITY, l = 0.0f;
 
-        // lane -> position lane of unit u: its page (loaded a unit ahead), then its element offset
+        // the page of the lane's position in unit u
         auto page_of = [&](uint32_t u) {
-            const int32_t kp = int32_t(unit_start(x, u, kManyKeys) + lane);
-            return kp <= x.pos1 ? table[uint32_t(kp) >> a.shift] : 0xffffffffu;
+            const int32_t kp = int32_t(unit_start(s.x, u, kManyKeys) + lane);
+            return kp <= s.x.pos1 ? table[uint32_t(kp) >> a.shift] : 0xffffffffu;
         };
-        auto offset_of = [&](uint32_t page, uint32_t u) {
-            const uint32_t kp = unit_start(x, u, kManyKeys) + lane;
-            return page < a.num_pages ? uint64_t(page) * a.page_stride + uint64_t(kp & place) * kvd + s.g * D : uint64_t(0);
+        auto copy_unit = [&](uint32_t u, uint32_t page, int buf) {
+            const uint32_t at = wave * kOwn, pos = unit_start(s.x, u, kManyKeys) + at;
+            copy_rows<T, D, kOwn, WIDE>(a, k, &ks[buf][at * D], page, at, pos, kvd, head);
+            copy_rows<T, D, kOwn, WIDE>(a, v, &vs[buf][at * D], page, at, pos, kvd, head);
         };
-        auto is_whole = [&](uint64_t valid, int32_t k0) {
-            return valid == ~uint64_t(0) && k0 + int32_t(kManyKeys) - 1 <= x.pos0 &&
-                   (a.window == 0 || uint32_t(x.pos1 - k0) < a.window || uint32_t(k0) + kManyKeys <= a.sinks);
-        };
-        uint4 sk[kPass], sv[kPass];
-        auto fetch = [&](uint64_t off) {  // this thread's blocks of the unit whose positions lie at `off` (by lane)
-#pragma unroll
-            for (int i = 0; i < kPass; ++i) {
-                const int src = int(sr + i * kRows);
-                const uint64_t row_off = (uint64_t(uint32_t(__shfl(int(uint32_t(off >> 32)), src))) << 32) |
-                                         uint32_t(__shfl(int(uint32_t(off)), src));
-                sk[i] = *reinterpret_cast<const uint4*>(k + row_off + 8 * sb);
-                sv[i] = *reinterpret_cast<const uint4*>(v + row_off + 8 * sb);
-            }
-        };
-        auto stage = [&](int buf, int bits, uint64_t valid, bool whole) {
-#pragma unroll
-            for (int i = 0; i < kPass; ++i) {
-                const uint32_t rr = sr + i * kRows;
-                if (!whole) {
-                    uint32_t* vw = reinterpret_cast<uint32_t*>(&sv[i]);
-                    const bool in = (valid >> rr) & 1u;
-                    bool any = false;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (!in) vw[j] = 0;
-                        any |= drop_nonfinite<T>(vw[j]);
-                    }
-                    if (any) atomicOr(&odd_bits[bits][rr >> 5], 1u << (rr & 31u));
-                }
-                const uint32_t to = rr * D + ((sb ^ swizzle<D>(rr)) << 3);
-                *reinterpret_cast<uint4*>(&ks[buf][to]) = sk[i];
-                *reinterpret_cast<uint4*>(&vs[buf][to]) = sv[i];
-            }
-        };
-
         if (s.u0 < s.u1) {
-            // bits of unit u in odd_bits[(u - u0) % 3]: cleared two units ahead
-            if (tid < 6) odd_bits[tid >> 1][tid & 1u] = 0;
             uint32_t page = page_of(s.u0);
-            uint64_t off = offset_of(page, s.u0);
-            uint64_t valid = __ballot(page < a.num_pages);
-            bool whole = is_whole(valid, int32_t(unit_start(x, s.u0, kManyKeys)));
-            fetch(off);
             uint32_t npage = s.u0 + 1 < s.u1 ? page_of(s.u0 + 1) : 0xffffffffu;
-            __syncthreads();
-            stage(0, 0, valid, whole);
-            __syncthreads();
-            int cur = 0, bits = 0;
+            vec8<T> q[D / 16];
+            load_q<T, D>(a, s.token, s.x.row0 + row, trow < s.x.rows, s.g, q);
+            copy_unit(s.u0, page, 0);
+            int cur = 0;
             for (uint32_t u = s.u0; u < s.u1; ++u) {
-                const int32_t k0 = int32_t(unit_start(x, u, kManyKeys));
-                uint64_t noff = 0, nvalid = 0;
-                bool nwhole = true;
-                const int nbits = bits == 2 ? 0 : bits + 1;
+                wait_loads();
+                __syncthreads();  // this unit's rows are in LDS, the other buffer is read no more
+                const int32_t k0 = int32_t(unit_start(s.x, u, kManyKeys));
+                uint32_t far = 0xffffffffu;
                 if (u + 1 < s.u1) {
-                    noff = offset_of(npage, u + 1);
-                    nvalid = __ballot(npage < a.num_pages);
-                    nwhole = is_whole(nvalid, int32_t(unit_start(x, u + 1, kManyKeys)));
-                    fetch(noff);
-                    npage = u + 2 < s.u1 ? page_of(u + 2) : 0xffffffffu;
+                    copy_unit(u + 1, npage, cur ^ 1);
+                    if (u + 2 < s.u1) far = page_of(u + 2);
                 }
-                if (tid < 2) odd_bits[nbits == 2 ? 0 : nbits + 1][tid] = 0;
+                const uint64_t valid = __ballot(page < a.num_pages);
+                const bool whole = all_seen(a, s.x, k0, kManyKeys, valid == ~uint64_t(0));
+                if (!whole) {
+                    // positions without a page, infinities and NaN out of V
+                    for (uint32_t e = tid; e < kManyKeys * (D / 8); e += NT) {
+                        const uint32_t rr = e / (D / 8);
+                        if (clean(&vs[cur][e * 8], (valid >> rr) & 1u)) odd = 1;
+                    }
+                    __syncthreads();
+                }
 
                 f32x16 sc[2];
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
+                for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sc[kt][i] = 0.0f;
 #pragma unroll
-                    for (int st = 0; st < D / 16; ++st) {
+                for (int st = 0; st < D / 16; ++st)
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) {
                         const uint32_t rr = 32u * kt + l32;
                         const vec8<T> kf =
                             *reinterpret_cast<const vec8<T>*>(&ks[cur][rr * D + (((2u * st + h2) ^ swizzle<D>(rr)) << 3)]);
                         sc[kt] = mfma<T>(kf, q[st], sc[kt]);
                     }
-                }
-                float mx = -INFINITY;
                 if (!whole) {
-#pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint32_t j = 32u * kt + tile_index(i);
-                            const bool see = ((valid >> j) & 1u) && sees(qpos, k0 + int32_t(j), a.window, a.sinks);
-                            sc[kt][i] = see ? sc[kt][i] : -INFINITY;
-                        }
+                    hide(sc[0], uint32_t(valid) & seen_bits(qpos, k0, a.window, a.sinks));
+                    hide(sc[1], uint32_t(valid >> 32) & seen_bits(qpos, k0 + 32, a.window, a.sinks));
                 }
+                float mx = sc[0][0];
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -813,27 +872,20 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
 #pragma unroll
                     for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vs[cur], st, t), p, o[t]);
                 }
-                if (!whole) {
-                    const uint64_t odd = (uint64_t(odd_bits[bits][1]) << 32) | odd_bits[bits][0];
-                    if (odd) add_nonfinite<T, D>(o, v, uniform(odd), k0, off, qpos, a.window, a.sinks);
-                }
-                if (u + 1 < s.u1) stage(cur ^ 1, nbits, nvalid, nwhole);
-                __syncthreads();
                 cur ^= 1;
-                bits = nbits;
-                off = noff;
-                valid = nvalid;
-                whole = nwhole;
+                page = npage;
+                npage = far;
             }
+            // set before the last unit's second barrier, if at all
+            if (uniform(odd))
+                add_nonfinite<T, D>(a, o, v + head, s, kManyKeys, qpos, kvd, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); },
+                                    page_of);
         }
         const float L = xor_sum<32>(l);
-        const bool complete = at <= s.begin && s.end <= line.to;
-        uint32_t slot = 0;
-        if (!complete) slot = write_piece(a.many_p, line, s, r, x);
-        if (trow < x.rows) {
-            if (complete) {
+        if (trow < s.x.rows) {
+            if (s.complete) {
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                T* dst = out_row<T>(a, r.token, x.row0 + trow, s.g, D);
+                T* dst = out_row<T>(a, s.token, s.x.row0 + trow, s.g, D);
 #pragma unroll
                 for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -841,18 +893,17 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
                         store4<T>(dst + 32 * t + tile_index(i), o[t][i] * inv, o[t][i + 1] * inv, o[t][i + 2] * inv,
                                   o[t][i + 3] * inv);
             } else {
-                float* dst = a.many_o + (uint64_t(slot) * a.many_slot + trow) * D;
+                float* dst = a.many_o + (uint64_t(s.slot) * a.many_slot + trow) * D;
 #pragma unroll
                 for (int t = 0; t < D / 32; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
                         *reinterpret_cast<float4*>(dst + 32 * t + tile_index(i)) =
                             make_float4(o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]);
-                if (h2 == 0) a.many_ml[uint64_t(slot) * a.many_slot + trow] = make_float2(m, L);
+                if (h2 == 0) a.many_ml[uint64_t(s.slot) * a.many_slot + trow] = make_float2(m, L);
             }
         }
-        at = min(s.end, line.to);
-        __syncthreads();  // the next tile's first unit overwrites LDS
+        __syncthreads();  // the next tile's first unit overwrites LDS, its segment `walk`
     }
 }
 
@@ -951,13 +1002,19 @@ Space space_of(uint32_t dim, uint32_t hpk, uint32_t tokens)
     return s;
 }
 
+template <typename T, int D, bool WIDE>
+void launch_tiles(const PagedAttn& a, hipStream_t st)
+{
+    if (a.few_wgs) hipLaunchKernelGGL((k_paged_few<T, D, WIDE>), dim3(a.few_wgs), dim3(256), 0, st, a);
+    if (a.many_wgs)
+        hipLaunchKernelGGL((k_paged_many<T, D, kManyWaves, WIDE>), dim3(a.many_wgs), dim3(kManyWaves * 64), 0, st, a);
+}
+
 template <typename T, int D>
 hipError_t launch_paged(const PagedAttn& a, hipStream_t st)
 {
-    if (a.few_wgs) hipLaunchKernelGGL((k_paged_few<T, D>), dim3(a.few_wgs), dim3(256), 0, st, a);
-    if (hipError_t e = hipGetLastError()) return e;
-    if (a.many_wgs)
-        hipLaunchKernelGGL((k_paged_many<T, D, kManyWaves>), dim3(a.many_wgs), dim3(kManyWaves * 64), 0, st, a);
+    if (a.shift >= 4) launch_tiles<T, D, true>(a, st);
+    else launch_tiles<T, D, false>(a, st);
     if (hipError_t e = hipGetLastError()) return e;
     hipLaunchKernelGGL((k_paged_join<T, D>), dim3(2 * (a.few_wgs + a.many_wgs), kJoinSplit), dim3(256), 0, st, a);
     return hipGetLastError();
