@@ -62,6 +62,16 @@ struct PagedAttn {
     uint32_t few_wgs, many_wgs;    // workgroups of this call's launches (0: not launched)
 };
 
+// The kernel's arguments (its one parameter, a PagedAttn), read again: a phase that takes its own copy keeps
+// none of it in scalar registers for the phases after it.
+__device__ __forceinline__ const PagedAttn& arguments()
+{
+    typedef __attribute__((address_space(4))) const PagedAttn Arg;
+    Arg* p = (Arg*)(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(p));
+    return *(const PagedAttn*)(p);
+}
+
 // ------------------------------------------------------------------- tiles
 // One request: its new rows and positions, and what its tiles cost.  Costs are whole
 // numbers in doubles (the host keeps them below 2^52), exact and quicker than 64-bit
@@ -226,7 +236,7 @@ __device__ __forceinline__ void take_part(const PagedAttn& a, Walk& l, double to
 // part begins.  Up to 64 requests: wave 0 alone, one per lane; the lanes' requests are
 // returned for next_segment.  More: thread t takes a run of them.
 template <bool FEW, int NT>
-__device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, uint32_t bm, uint32_t keys, Piece* pieces, double* red)
+__device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, uint32_t bm, uint32_t keys, double* red)
 {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     if (a.requests <= 64) {
@@ -279,12 +289,12 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, uint32_t
         }
     }
     __syncthreads();
-    if (tid < 2) pieces[2 * l.w + tid].n = 0;
+    if (tid < 2) (FEW ? a.few_p : a.many_p)[2 * l.w + tid].n = 0;
 }
 
 // Wave 0: the part's next segment.  A cut tile gets its slot and its record for k_paged_join.
 template <bool FEW>
-__device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, uint32_t bm, uint32_t keys, Piece* pieces)
+__device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, uint32_t bm, uint32_t keys)
 {
     if (threadIdx.x >= 64) return;
     Walk m = l;
@@ -320,7 +330,7 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, uint32
             const uint32_t first = 2 * w0 + (part_at(m.total, w0, m.parts) < begin ? 1u : 0u);
             m.slot = m.w == w0 ? first : 2 * m.w;
             if (threadIdx.x == 0)
-                pieces[m.slot] = Piece{w1 - w0 + 1, m.w - w0, w0, first, r.token, m.x.row0, m.x.rows, m.g};
+                (FEW ? a.few_p : a.many_p)[m.slot] = Piece{w1 - w0 + 1, m.w - w0, w0, first, r.token, m.x.row0, m.x.rows, m.g};
         }
         m.at = fmin(end, m.to);
     }
@@ -355,10 +365,29 @@ __device__ __forceinline__ Segment read_segment(const Walk& l)
 }
 
 // ------------------------------------------------------------- rows of K and V
-// The element offset of a position's row: its page's and its place's.
-__device__ __forceinline__ uint64_t row_offset(const PagedAttn& a, uint32_t page, uint32_t pos, uint32_t kvd)
+// What the segment's loop needs of the pool, the tables and the mask.
+template <typename T>
+struct Pool {
+    const T *k, *v;  // at the kv head
+    const uint32_t* table;
+    uint64_t page_stride;
+    uint32_t num_pages, shift, kvd, window, sinks;
+    float scale;
+};
+template <typename T, int D>
+__device__ __forceinline__ Pool<T> pool_of(const PagedAttn& a, const Segment& s)
 {
-    return page < a.num_pages ? uint64_t(page) * a.page_stride + uint64_t(pos & ((1u << a.shift) - 1u)) * kvd : 0;
+    return Pool<T>{static_cast<const T*>(a.k) + s.g * D, static_cast<const T*>(a.v) + s.g * D,
+                   a.tables + uint64_t(s.b) * a.max_pages, a.page_stride, a.num_pages, a.shift, a.kv_heads * D,
+                   a.window, a.sinks, a.scale};
+}
+
+// The element offset of a position's row: its page's and its place's; 0 for a page that is none.
+template <typename T>
+__device__ __forceinline__ uint64_t row_offset(const Pool<T>& p, uint32_t page, uint32_t pos)
+{
+    const uint64_t at = uint64_t(page) * p.page_stride + uint64_t(pos & ((1u << p.shift) - 1u)) * p.kvd;
+    return page < p.num_pages ? at : 0;
 }
 
 // A K or V row in LDS: D / 8 blocks of 16 bytes, block c of row r at place
@@ -369,34 +398,52 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r)
     return D == 128 ? (r & 7u) << 1 : ((r >> 1) & 3u) << 1;
 }
 
-// N rows (N a multiple of the rows of one copy) from the pages straight into LDS, 16 bytes a lane, row i
-// at lds + i * D.  `page`: lane first + i holds the page of row i's position pos0 + i.  Which 16 bytes a lane
-// copies carries the swizzle, as LDS is written in lane order.  WIDE, pages of 16 and more: 16
-// aligned rows have one page, so the address is scalar.
-template <typename T, int D, int N, bool WIDE>
-__device__ __forceinline__ void copy_rows(const PagedAttn& a, const T* src, T* lds, uint32_t page, uint32_t first, uint32_t pos0,
-                                          uint32_t kvd, uint32_t head)
+// 16 bytes per lane from memory straight into LDS, lane i's at lds + 16 i: from base (scalar) + off bytes, or
+// from the lane's own address.  In assembly because the compiler waits for such a copy before
+// the next read of LDS, whichever buffer that is from; there is no register for a load in
+// flight to write, and nothing else here uses m0.  wait_loads and a barrier (a wave's own rows: wait_loads) come before the rows are read.
+__device__ __forceinline__ void copy16(uint32_t lds, const void* base, uint32_t off)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t lds, const void* from)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+}
+
+// N positions' rows of K (BOTH) and V from the pages straight into LDS, row i at kl, vl + i * D.  `page`: lane
+// first + i holds the page of row i's position pos0 + i.  Which 16 bytes a lane copies carries the swizzle, as
+// LDS is written in lane order.  WIDE, pages of 16 and more: 16 aligned rows have one
+// page, so the address is scalar and the lane's part of it the same for every unit.
+template <bool BOTH, int N, bool WIDE, int D, typename T>
+__device__ __forceinline__ void copy_rows(const Pool<T>& p, T* kl, T* vl, uint32_t page, uint32_t first, uint32_t pos0)
 {
     constexpr uint32_t kAcross = D / 8, kRows = kWave / kAcross;  // lanes per row, rows per copy
+    constexpr uint32_t kGroup = N < 16 ? N : 16;
     const uint32_t lane = threadIdx.x & 63u, r0 = lane / kAcross, c = lane % kAcross;
-    typedef __attribute__((address_space(1))) const void gptr;
     typedef __attribute__((address_space(3))) void lptr;
-    if constexpr (WIDE) {
+    const uint32_t kto = uniform(uint32_t(reinterpret_cast<uintptr_t>((lptr*)(kl))));
+    const uint32_t vto = uniform(uint32_t(reinterpret_cast<uintptr_t>((lptr*)(vl))));
 #pragma unroll
-        for (uint32_t i = 0; i < uint32_t(N); i += kRows) {
-            const uint32_t part = i & ~15u;  // the 16 rows that share a page
-            const uint32_t pg = uint32_t(__builtin_amdgcn_readlane(int(page), int(first + part)));
-            const T* base = src + row_offset(a, pg, pos0 + part, kvd) + head;
-            const uint32_t r = i - part + r0;
-            __builtin_amdgcn_global_load_lds((gptr*)(base + (r * kvd + ((c ^ swizzle<D>(r)) << 3))), (lptr*)(lds + i * D), 16, 0, 0);
-        }
-    } else {
+    for (uint32_t part = 0; part < uint32_t(N); part += kGroup) {
+        if constexpr (WIDE) {
+            const uint64_t at = row_offset(p, uint32_t(__builtin_amdgcn_readlane(int(page), int(first + part))), pos0 + part);
+            const T *kb = p.k + at, *vb = p.v + at;
 #pragma unroll
-        for (uint32_t i = 0; i < uint32_t(N); i += kRows) {
-            const uint32_t r = i + r0;
-            const uint32_t pg = uint32_t(__shfl(int(page), int(first + r)));
-            const T* row = src + row_offset(a, pg, pos0 + r, kvd) + head;
-            __builtin_amdgcn_global_load_lds((gptr*)(row + ((c ^ swizzle<D>(r)) << 3)), (lptr*)(lds + i * D), 16, 0, 0);
+            for (uint32_t i = 0; i < kGroup; i += kRows) {
+                const uint32_t r = i + r0, off = (r * p.kvd + ((c ^ swizzle<D>(first + part + r)) << 3)) * 2;
+                if constexpr (BOTH) copy16(kto + (part + i) * D * 2, kb, off);
+                copy16(vto + (part + i) * D * 2, vb, off);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kGroup; i += kRows) {
+                const uint32_t r = part + i + r0;
+                const uint64_t at = row_offset(p, uint32_t(__shfl(int(page), int(first + r))), pos0 + r) +
+                                    ((c ^ swizzle<D>(first + r)) << 3);
+                if constexpr (BOTH) copy16(kto + (part + i) * D * 2, p.k + at);
+                copy16(vto + (part + i) * D * 2, p.v + at);
+            }
         }
     }
 }
@@ -545,10 +592,11 @@ __device__ __forceinline__ T* out_row(const PagedAttn& a, uint32_t token, uint32
 }
 
 // Whether every row of the tile sees all of `keys` positions from k0 on that have pages (valid).
-__device__ __forceinline__ bool all_seen(const PagedAttn& a, const Tile& x, int32_t k0, uint32_t keys, bool valid)
+template <typename T>
+__device__ __forceinline__ bool all_seen(const Pool<T>& p, const Tile& x, int32_t k0, uint32_t keys, bool valid)
 {
     return valid && k0 + int32_t(keys) - 1 <= x.pos0 &&
-           (a.window == 0 || uint32_t(x.pos1 - k0) < a.window || uint32_t(k0) + keys <= a.sinks);
+           (p.window == 0 || uint32_t(x.pos1 - k0) < p.window || uint32_t(k0) + keys <= p.sinks);
 }
 
 // The 16 bytes at p without infinities and NaN, or zero where the position is not in; whether there were any.
@@ -571,24 +619,24 @@ __device__ __forceinline__ bool clean(T* p, bool in)
 // need none of it.  A slow pass over the segment's other units, for data that has any; first_of
 // and page_of as in the kernels, `span` positions of each unit.
 template <typename T, int D, typename First, typename Page>
-__device__ __forceinline__ void add_nonfinite(const PagedAttn& a, f32x16 (&o)[D / 32], const T* v, const Segment& s, uint32_t span,
-                                              int32_t qpos, uint32_t kvd, First first_of, Page page_of)
+__device__ __forceinline__ void add_nonfinite(const Pool<T>& p, f32x16 (&o)[D / 32], const Segment& s, uint32_t span,
+                                              int32_t qpos, First first_of, Page page_of)
 {
 #pragma unroll 1
     for (uint32_t u = s.u0; u < s.u1; ++u) {
         const int32_t k0 = int32_t(first_of(u));
         const uint32_t page = page_of(u);
-        if (all_seen(a, s.x, k0, span, true)) continue;
+        if (all_seen(p, s.x, k0, span, true)) continue;
 #pragma unroll 1
         for (uint32_t j = 0; j < span; ++j) {
             const uint32_t pg = uint32_t(__builtin_amdgcn_readlane(int(page), int(j)));
-            if (pg >= a.num_pages || !sees(qpos, k0 + int32_t(j), a.window, a.sinks)) continue;
-            const T* p = v + row_offset(a, pg, uint32_t(k0) + j, kvd);
+            if (pg >= p.num_pages || !sees(qpos, k0 + int32_t(j), p.window, p.sinks)) continue;
+            const T* row = p.v + row_offset(p, pg, uint32_t(k0) + j);
 #pragma unroll
             for (int t = 0; t < D / 32; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float x = static_cast<float>(p[32 * t + tile_index(i)]);
+                    const float x = static_cast<float>(row[32 * t + tile_index(i)]);
                     if (!(fabsf(x) < INFINITY)) o[t][i] += x;
                 }
         }
@@ -611,27 +659,23 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 // P^T), P^T comes from the scores' registers.  The next unit's V is on its way while
 // this one is computed, its K from the moment this one's scores are done: 16 KB a wave.
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
+__global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 {
     __shared__ double red[4];
     __shared__ Walk walk;
     __shared__ __align__(16) float joined[4 * 32 * D];  // two V buffers of each wave, then the waves' outputs
     __shared__ float mw[4][32], lw[4][32];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<true, 256>(a, walk, kFewRows, kFewKeys, a.few_p, red);
+    start_walk<true, 256>(arguments(), walk, kFewRows, kFewKeys, red);
     T* vrows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
-    const T* k = static_cast<const T*>(a.k);
-    const T* v = static_cast<const T*>(a.v);
-    const uint32_t kvd = a.kv_heads * D;
     for (;;) {
-        next_segment<true>(a, walk, kFewRows, kFewKeys, a.few_p);
+        next_segment<true>(arguments(), walk, kFewRows, kFewKeys);
         __syncthreads();
         if (uniform(walk.go) == 0) break;
         const Segment s = read_segment(walk);
-        const uint32_t head = s.g * D;
+        const Pool<T> p = pool_of<T, D>(arguments(), s);
         const uint32_t row = min(l32, s.x.rows - 1);
-        const int32_t qpos = s.base + int32_t((s.x.row0 + row) / a.hpk);
-        const uint32_t* table = a.tables + uint64_t(s.b) * a.max_pages;
+        const int32_t qpos = s.base + int32_t((s.x.row0 + row) / arguments().hpk);
         f32x16 o[D / 32];
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
@@ -644,21 +688,21 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
         auto first_of = [&](uint32_t u) { return unit_start(s.x, u, kFewKeys) + 32u * wave; };
         auto page_of = [&](uint32_t u) {
             const int32_t kp = int32_t(first_of(u) + l32);
-            return kp <= s.x.pos1 ? table[uint32_t(kp) >> a.shift] : 0xffffffffu;
+            return kp <= s.x.pos1 ? p.table[uint32_t(kp) >> p.shift] : 0xffffffffu;
         };
         uint4 kr[D / 16];
         auto load_k = [&](uint32_t page, uint32_t u) {
-            const T* p = k + row_offset(a, page, first_of(u) + l32, kvd) + head + 8 * h2;
+            const T* at = p.k + row_offset(p, page, first_of(u) + l32) + 8 * h2;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) kr[i] = *reinterpret_cast<const uint4*>(p + 16 * i);
+            for (int i = 0; i < D / 16; ++i) kr[i] = *reinterpret_cast<const uint4*>(at + 16 * i);
         };
         if (s.u0 < s.u1) {
             uint32_t page = page_of(s.u0);
             uint32_t npage = s.u0 + 1 < s.u1 ? page_of(s.u0 + 1) : 0xffffffffu;
             vec8<T> q[D / 16];
-            load_q<T, D>(a, s.token, s.x.row0 + row, l32 < s.x.rows, s.g, q);
+            load_q<T, D>(arguments(), s.token, s.x.row0 + row, l32 < s.x.rows, s.g, q);
             load_k(page, s.u0);
-            copy_rows<T, D, 32, WIDE>(a, v, vrows, page, 0, first_of(s.u0), kvd, head);
+            copy_rows<false, 32, WIDE, D>(p, vrows, vrows, page, 0, first_of(s.u0));
             T* vcur = vrows;
             T* vnext = vrows + 32 * D;
             for (uint32_t u = s.u0; u < s.u1; ++u) {
@@ -667,7 +711,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
                 const bool more = u + 1 < s.u1;
                 uint32_t far = 0xffffffffu;
                 if (more) {
-                    copy_rows<T, D, 32, WIDE>(a, v, vnext, npage, 0, first_of(u + 1), kvd, head);
+                    copy_rows<false, 32, WIDE, D>(p, vnext, vnext, npage, 0, first_of(u + 1));
                     if (u + 2 < s.u1) far = page_of(u + 2);
                 }
                 f32x16 sc;
@@ -677,30 +721,30 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
                 for (int i = 0; i < D / 16; ++i) sc = mfma<T>(__builtin_bit_cast(vec8<T>, kr[i]), q[i], sc);
                 if (more) load_k(npage, u + 1);
 
-                const bool in = page < a.num_pages;
+                const bool in = page < p.num_pages;
                 const uint32_t valid = uint32_t(__ballot(in));
-                const bool whole = all_seen(a, s.x, k0, 32, valid == 0xffffffffu);
+                const bool whole = all_seen(p, s.x, k0, 32, valid == 0xffffffffu);
                 if (!whole) {
                     for (uint32_t c = h2; c < D / 8; c += 2) odd |= clean(vcur + l32 * D + c * 8, in);
-                    hide(sc, valid & seen_bits(qpos, k0, a.window, a.sinks));
+                    hide(sc, valid & seen_bits(qpos, k0, p.window, p.sinks));
                     wave_fence();
                 }
                 float mx = sc[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-                mx = xor_max<32>(mx) * a.scale;
+                mx = xor_max<32>(mx) * p.scale;
                 rescale(mx, m, l, o);
                 const float mr = m == -INFINITY ? 0.0f : m;  // nothing seen yet: all weights 0
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.scale, -mr));
+                    sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale, -mr));
                     l += sc[i];
                 }
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
-                    const vec8<T> p = narrow<T>(sc, 8 * st);
+                    const vec8<T> w = narrow<T>(sc, 8 * st);
 #pragma unroll
-                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vcur, st, t), p, o[t]);
+                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vcur, st, t), w, o[t]);
                 }
                 wave_fence();  // the unit after the next is copied over these rows
                 T* const t = vcur;
@@ -709,7 +753,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
                 page = npage;
                 npage = far;
             }
-            if (__ballot(odd)) add_nonfinite<T, D>(a, o, v + head, s, 32, qpos, kvd, first_of, page_of);
+            if (__ballot(odd)) add_nonfinite<T, D>(p, o, s, 32, qpos, first_of, page_of);
         }
         // the waves' states in wave order: out = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w
         __syncthreads();  // every wave is done with its V rows
@@ -727,6 +771,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
             }
         }
         __syncthreads();
+        const PagedAttn& e_ = arguments();
         for (uint32_t e = tid; e < s.x.rows * (D / 4); e += 256) {
             const uint32_t rr = e / (D / 4), d = 4 * (e % (D / 4));
             float M = -INFINITY;
@@ -747,10 +792,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
             }
             if (s.complete) {
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // nothing seen: zeros
-                store4<T>(out_row<T>(a, s.token, s.x.row0 + rr, s.g, D) + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                store4<T>(out_row<T>(e_, s.token, s.x.row0 + rr, s.g, D) + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             } else {
-                *reinterpret_cast<float4*>(a.few_o + (uint64_t(s.slot) * a.few_slot + rr) * D + d) = acc;
-                if (d == 0) a.few_ml[uint64_t(s.slot) * a.few_slot + rr] = make_float2(M, L);
+                *reinterpret_cast<float4*>(e_.few_o + (uint64_t(s.slot) * e_.few_slot + rr) * D + d) = acc;
+                if (d == 0) e_.few_ml[uint64_t(s.slot) * e_.few_slot + rr] = make_float2(M, L);
             }
         }
         __syncthreads();  // the next tile's V rows overwrite `joined`, its segment `walk`
@@ -764,7 +809,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a)
 // unit u + 1 is copied while unit u is computed; one barrier per unit.  Operands as in the
 // few-rows kernel, K's read from LDS.
 template <typename T, int D, int NW, bool WIDE>
-__global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
+__global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 {
     constexpr int NT = NW * 64;
     constexpr uint32_t kBm = NW * 32, kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
@@ -774,21 +819,17 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
     __shared__ Walk walk;
     __shared__ uint32_t odd;  // infinities or NaN cleared from V in this segment
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<false, NT>(a, walk, kBm, kManyKeys, a.many_p, red);
-    const T* k = static_cast<const T*>(a.k);
-    const T* v = static_cast<const T*>(a.v);
-    const uint32_t kvd = a.kv_heads * D;
+    start_walk<false, NT>(arguments(), walk, kBm, kManyKeys, red);
     for (;;) {
-        next_segment<false>(a, walk, kBm, kManyKeys, a.many_p);
+        next_segment<false>(arguments(), walk, kBm, kManyKeys);
         if (tid == 0) odd = 0;
         __syncthreads();
         if (uniform(walk.go) == 0) break;
         const Segment s = read_segment(walk);
-        const uint32_t head = s.g * D;
+        const Pool<T> p = pool_of<T, D>(arguments(), s);
         const uint32_t trow = wave * 32 + l32;
         const uint32_t row = min(trow, s.x.rows - 1);
-        const int32_t qpos = s.base + int32_t((s.x.row0 + row) / a.hpk);
-        const uint32_t* table = a.tables + uint64_t(s.b) * a.max_pages;
+        const int32_t qpos = s.base + int32_t((s.x.row0 + row) / arguments().hpk);
         f32x16 o[D / 32];
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
@@ -799,18 +840,17 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
         // the page of the lane's position in unit u
         auto page_of = [&](uint32_t u) {
             const int32_t kp = int32_t(unit_start(s.x, u, kManyKeys) + lane);
-            return kp <= s.x.pos1 ? table[uint32_t(kp) >> a.shift] : 0xffffffffu;
+            return kp <= s.x.pos1 ? p.table[uint32_t(kp) >> p.shift] : 0xffffffffu;
         };
         auto copy_unit = [&](uint32_t u, uint32_t page, int buf) {
             const uint32_t at = wave * kOwn, pos = unit_start(s.x, u, kManyKeys) + at;
-            copy_rows<T, D, kOwn, WIDE>(a, k, &ks[buf][at * D], page, at, pos, kvd, head);
-            copy_rows<T, D, kOwn, WIDE>(a, v, &vs[buf][at * D], page, at, pos, kvd, head);
+            copy_rows<true, kOwn, WIDE, D>(p, &ks[buf][at * D], &vs[buf][at * D], page, at, pos);
         };
         if (s.u0 < s.u1) {
             uint32_t page = page_of(s.u0);
             uint32_t npage = s.u0 + 1 < s.u1 ? page_of(s.u0 + 1) : 0xffffffffu;
             vec8<T> q[D / 16];
-            load_q<T, D>(a, s.token, s.x.row0 + row, trow < s.x.rows, s.g, q);
+            load_q<T, D>(arguments(), s.token, s.x.row0 + row, trow < s.x.rows, s.g, q);
             copy_unit(s.u0, page, 0);
             int cur = 0;
             for (uint32_t u = s.u0; u < s.u1; ++u) {
@@ -822,8 +862,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
                     copy_unit(u + 1, npage, cur ^ 1);
                     if (u + 2 < s.u1) far = page_of(u + 2);
                 }
-                const uint64_t valid = __ballot(page < a.num_pages);
-                const bool whole = all_seen(a, s.x, k0, kManyKeys, valid == ~uint64_t(0));
+                const uint64_t valid = __ballot(page < p.num_pages);
+                const bool whole = all_seen(p, s.x, k0, kManyKeys, valid == ~uint64_t(0));
                 if (!whole) {
                     // positions without a page, infinities and NaN out of V
                     for (uint32_t e = tid; e < kManyKeys * (D / 8); e += NT) {
@@ -848,29 +888,29 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
                         sc[kt] = mfma<T>(kf, q[st], sc[kt]);
                     }
                 if (!whole) {
-                    hide(sc[0], uint32_t(valid) & seen_bits(qpos, k0, a.window, a.sinks));
-                    hide(sc[1], uint32_t(valid >> 32) & seen_bits(qpos, k0 + 32, a.window, a.sinks));
+                    hide(sc[0], uint32_t(valid) & seen_bits(qpos, k0, p.window, p.sinks));
+                    hide(sc[1], uint32_t(valid >> 32) & seen_bits(qpos, k0 + 32, p.window, p.sinks));
                 }
                 float mx = sc[0][0];
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
-                mx = xor_max<32>(mx) * a.scale;
+                mx = xor_max<32>(mx) * p.scale;
                 rescale(mx, m, l, o);
                 const float mr = m == -INFINITY ? 0.0f : m;
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        sc[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], a.scale, -mr));
+                        sc[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], p.scale, -mr));
                         l += sc[kt][i];
                     }
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
-                    const vec8<T> p = narrow<T>(sc[st >> 1], 8 * (st & 1));
+                    const vec8<T> w = narrow<T>(sc[st >> 1], 8 * (st & 1));
 #pragma unroll
-                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vs[cur], st, t), p, o[t]);
+                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vs[cur], st, t), w, o[t]);
                 }
                 cur ^= 1;
                 page = npage;
@@ -878,14 +918,14 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
             }
             // set before the last unit's second barrier, if at all
             if (uniform(odd))
-                add_nonfinite<T, D>(a, o, v + head, s, kManyKeys, qpos, kvd, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); },
-                                    page_of);
+                add_nonfinite<T, D>(p, o, s, kManyKeys, qpos, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); }, page_of);
         }
         const float L = xor_sum<32>(l);
+        const PagedAttn& e_ = arguments();
         if (trow < s.x.rows) {
             if (s.complete) {
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                T* dst = out_row<T>(a, s.token, s.x.row0 + trow, s.g, D);
+                T* dst = out_row<T>(e_, s.token, s.x.row0 + trow, s.g, D);
 #pragma unroll
                 for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -893,14 +933,14 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn a)
                         store4<T>(dst + 32 * t + tile_index(i), o[t][i] * inv, o[t][i + 1] * inv, o[t][i + 2] * inv,
                                   o[t][i + 3] * inv);
             } else {
-                float* dst = a.many_o + (uint64_t(s.slot) * a.many_slot + trow) * D;
+                float* dst = e_.many_o + (uint64_t(s.slot) * e_.many_slot + trow) * D;
 #pragma unroll
                 for (int t = 0; t < D / 32; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
                         *reinterpret_cast<float4*>(dst + 32 * t + tile_index(i)) =
                             make_float4(o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]);
-                if (h2 == 0) a.many_ml[uint64_t(s.slot) * a.many_slot + trow] = make_float2(m, L);
+                if (h2 == 0) e_.many_ml[uint64_t(s.slot) * e_.many_slot + trow] = make_float2(m, L);
             }
         }
         __syncthreads();  // the next tile's first unit overwrites LDS, its segment `walk`
