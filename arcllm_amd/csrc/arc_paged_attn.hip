@@ -33,6 +33,7 @@ constexpr uint32_t kManyKeys = 64;     // positions of a many-rows tile's unit
 constexpr uint32_t kFewWgs = 512;      // most parts of the line
 constexpr uint32_t kManyWgs = 512;
 constexpr int kManyWaves = 4;
+constexpr uint32_t kManyRows = kManyWaves * 32;
 constexpr uint32_t kTileKeys = 64;     // a tile's start and end cost about this many positions
 constexpr float kLazy = 8.0f;          // see rescale
 
@@ -83,6 +84,7 @@ struct Request {
     uint32_t tiles;   // per kv head
     double first, cap;  // cost of tile 0; no tile costs more than cap
     double total;       // of a kv head's tiles
+    float units;        // no fewer than its tiles have for a kv head, about as many
 };
 
 // Cost of tiles 0 .. t-1: tile t costs min(first + t * bm, cap), in positions times
@@ -90,13 +92,14 @@ struct Request {
 __device__ __forceinline__ double cost_before(const Request& r, uint32_t t, double bm)
 {
     const double n = double(t);
-    const double k = fmin(n, r.first >= r.cap ? 0.0 : ceil((r.cap - r.first) / bm));
+    const double k = fmin(n, r.first >= r.cap ? 0.0 : ceil((r.cap - r.first) * (1.0 / bm)));
     return k * r.first + bm * (k * (k - 1.0) * 0.5) + (n > k ? (n - k) * r.cap : 0.0);
 }
 
 template <bool FEW>
-__device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, uint32_t s1, uint32_t held, uint32_t bm)
+__device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, uint32_t s1, uint32_t held)
 {
+    constexpr uint32_t bm = FEW ? kFewRows : kManyRows, keys = FEW ? kFewKeys : kManyKeys;
     Request r{};
     if (s1 <= s0 || s0 >= a.rows) return r;
     const uint32_t rows = (min(s1, a.rows) - s0) * a.hpk;
@@ -110,13 +113,10 @@ __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, u
     r.first = double(kTileKeys + uint32_t(max(r.base, 0))) * a.hpk + bm;
     r.cap = a.window ? (double(kTileKeys) + a.window + a.sinks) * a.hpk + 2 * bm : 0x1p60;
     r.total = cost_before(r, r.tiles, bm);
+    const float spans = float(r.tiles) * ceilf(float(len) * (1.0f / keys));
+    r.units = a.window ? fminf(spans, float(r.tiles) * (ceilf((float(a.window) + float(a.sinks)) * (1.0f / keys)) + 2.0f)) : spans;
+    r.units = fmaxf(r.units, 1.0f);
     return r;
-}
-
-template <bool FEW>
-__device__ __forceinline__ Request request_at(const PagedAttn& a, uint32_t b, uint32_t bm)
-{
-    return request_of<FEW>(a, a.starts[b], a.starts[b + 1], a.lens[b], bm);
 }
 
 // A tile and the positions that it runs over: units of `keys` positions, first
@@ -182,7 +182,8 @@ __device__ __forceinline__ double wave_inclusive(double v)
 // wave 0 moves it on, the others read what they need, so that none of it is held in
 // registers while a segment is computed.
 struct Walk {
-    double total, at, to;  // cost of all tiles, what this part has done, its end
+    double total, step;    // cost of all tiles, of a part
+    double at, to;         // how far this part has come, its end
     double before;         // cost of the requests before b
     uint32_t parts, w, b;
     // the segment: units [u0, u1) of a tile
@@ -192,122 +193,156 @@ struct Walk {
     Tile x;
 };
 
-// Boundary of part w, the same number wherever it is computed; parts <= total, so no
+// Boundary of part w, the same number wherever it is computed; steps are at least 1, so no
 // part is empty.
-__device__ __forceinline__ double part_at(double total, uint32_t w, uint32_t parts)
+__device__ __forceinline__ double part_at(const Walk& l, uint32_t w)
 {
-    return w >= parts ? total : floor(total * double(w) / double(parts));
+    return w >= l.parts ? l.total : floor(l.step * double(w));
 }
 
+// Quotients that only have to be near, or the same in every workgroup.
+__device__ __forceinline__ float near_ratio(double x, double y) { return float(x) * __builtin_amdgcn_rcpf(float(y)); }
+
 // Which of a tile's units lie before x: monotonic in x, the same for both neighbours
-// of a cut (the same arithmetic on the same numbers).
+// of a cut (the same arithmetic on the same numbers).  The added 2^-8 keeps cuts that
+// should fall on a unit's border on it.
 __device__ __forceinline__ uint32_t units_before(double x, double begin, double end, uint32_t units)
 {
     if (x <= begin) return 0;
     if (x >= end) return units;
-    return min(units, uint32_t((x - begin) * double(units) / (end - begin)));
+    return min(units, uint32_t((x - begin) * double(near_ratio(units, end - begin)) + 0x1p-8));
 }
 
 // The part in which x lies.
 __device__ __forceinline__ uint32_t part_of(const Walk& l, double x)
 {
-    uint32_t w = min(l.parts - 1, uint32_t(x * double(l.parts) / l.total));
-    while (w && part_at(l.total, w, l.parts) > x) --w;
-    while (w + 1 < l.parts && part_at(l.total, w + 1, l.parts) <= x) ++w;
+    uint32_t w = min(l.parts - 1, uint32_t(near_ratio(x, l.step)));
+    while (w && part_at(l, w) > x) --w;
+    while (w + 1 < l.parts && part_at(l, w + 1) <= x) ++w;
     return w;
 }
 
-// This workgroup's part, from the total.  Workgroups go to the 8 XCDs in turn: an
-// XCD's workgroups take neighbouring parts, which read the same K and V.
-__device__ __forceinline__ void take_part(const PagedAttn& a, Walk& l, double total, uint32_t keys)
+// This workgroup's part, from the total: parts of a unit or more.  Workgroups go to the 8 XCDs
+// in turn: an XCD's workgroups take neighbouring parts, which read the same K and V.
+__device__ __forceinline__ void take_part(Walk& l, double total, float units)
 {
     l.total = total;
-    l.parts = uint32_t(fmin(double(gridDim.x), fmax(floor(total / (double(keys) * a.hpk)), total > 0.0 ? 1.0 : 0.0)));
+    l.parts = total > 0.0 ? min(uint32_t(gridDim.x), uint32_t(fminf(units, 65536.0f))) : 0u;
+    l.step = total / double(max(l.parts, 1u));
     l.w = blockIdx.x;
     l.at = l.to = 0.0;
     if (l.w >= l.parts) return;
     const uint32_t xcd = blockIdx.x & 7u, q = l.parts >> 3, rest = l.parts & 7u;
     l.w = xcd * q + min(xcd, rest) + (blockIdx.x >> 3);
-    l.at = part_at(total, l.w, l.parts);
-    l.to = part_at(total, l.w + 1, l.parts);
+    l.at = part_at(l, l.w);
+    l.to = part_at(l, l.w + 1);
+}
+
+// The first 64 requests, read once.
+struct Heads {
+    uint32_t s0[64], s1[64], len[64];
+};
+template <bool FEW>
+__device__ __forceinline__ Request request_at(const PagedAttn& a, const Heads& h, uint32_t b)
+{
+    if (a.requests <= 64) return request_of<FEW>(a, h.s0[b], h.s1[b], h.len[b]);
+    return request_of<FEW>(a, a.starts[b], a.starts[b + 1], a.lens[b]);
 }
 
 // Adds up the requests, so that no launch has to come first, and finds the one in which the
-// part begins.  Up to 64 requests: wave 0 alone, one per lane; the lanes' requests are
-// returned for next_segment.  More: thread t takes a run of them.
+// part begins.  Up to 64 requests: wave 0 alone, one per lane.  More: thread t takes a run
+// of them.  For next_segment, which wave 0 runs too, no barrier is needed.
 template <bool FEW, int NT>
-__device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, uint32_t bm, uint32_t keys, double* red)
+__device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h, double* red)
 {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     if (a.requests <= 64) {
-        if (wave == 0) {
-            const Request r = lane < a.requests ? request_at<FEW>(a, lane, bm) : Request{};
-            const double own = r.total * a.kv_heads, inc = wave_inclusive(own);
-            Walk m;
-            take_part(a, m, of_lane(inc, 63), keys);
-            const uint64_t behind = __ballot(inc > m.at);  // lanes from the part's first request on
-            const int b = behind ? __builtin_ctzll(behind) : 0;
-            m.b = uint32_t(b);
-            m.before = of_lane(inc - own, b);
-            if (lane == 0) l = m;
+        if (wave) return;
+        Request r{};
+        if (lane < a.requests) {
+            const uint32_t s0 = a.starts[lane], s1 = a.starts[lane + 1], len = a.lens[lane];
+            h.s0[lane] = s0;
+            h.s1[lane] = s1;
+            h.len[lane] = len;
+            r = request_of<FEW>(a, s0, s1, len);
         }
-    } else {
-        const uint32_t each = (a.requests + NT - 1) / NT;
-        const uint32_t b0 = min(tid * each, a.requests), b1 = min(b0 + each, a.requests);
-        double sum = 0.0;
-#pragma unroll 4
-        for (uint32_t b = b0; b < b1; ++b) sum += request_at<FEW>(a, b, bm).total * a.kv_heads;
-        const double inc = wave_inclusive(sum);
-        if (lane == 63) red[wave] = inc;
-        __syncthreads();
-        double before = 0.0, total = 0.0;
-#pragma unroll
-        for (int i = 0; i < NT / kWave; ++i) {
-            const double r = red[i];
-            if (uint32_t(i) < wave) before += r;
-            total += r;
-        }
+        const double own = r.total * a.kv_heads, inc = wave_inclusive(own);
         Walk m;
-        take_part(a, m, total, keys);
-        const double lo = before + inc - sum;
-        if (tid == 0) {  // with no work, all there is
-            m.b = 0;
-            m.before = 0.0;
-            l = m;
-        }
-        __syncthreads();
-        if (lo <= m.at && m.at < lo + sum) {  // one thread, if there is any work
-            double at = lo;
-            uint32_t b = b0;
-            for (; b + 1 < b1; ++b) {
-                const double c = request_at<FEW>(a, b, bm).total * a.kv_heads;
-                if (at + c > m.at) break;
-                at += c;
-            }
-            l.b = b;
-            l.before = at;
-        }
+        take_part(m, of_lane(inc, 63), group_sum<kWave>(r.units) * a.kv_heads);
+        const uint64_t behind = __ballot(inc > m.at);  // lanes from the part's first request on
+        const int b = behind ? __builtin_ctzll(behind) : 0;
+        m.b = uint32_t(b);
+        m.before = of_lane(inc - own, b);
+        if (lane == 0) l = m;
+        if (lane < 2) (FEW ? a.few_p : a.many_p)[2 * m.w + lane].n = 0;
+        return;
+    }
+    const uint32_t each = (a.requests + NT - 1) / NT;
+    const uint32_t b0 = min(tid * each, a.requests), b1 = min(b0 + each, a.requests);
+    double sum = 0.0;
+    float units = 0.0f;
+#pragma unroll 4
+    for (uint32_t b = b0; b < b1; ++b) {
+        const Request r = request_at<FEW>(a, h, b);
+        sum += r.total * a.kv_heads;
+        units += r.units;
+    }
+    const double inc = wave_inclusive(sum);
+    units = group_sum<kWave>(units);
+    if (lane == 63) {
+        red[wave] = inc;
+        red[NT / kWave + wave] = double(units);
     }
     __syncthreads();
-    if (tid < 2) (FEW ? a.few_p : a.many_p)[2 * l.w + tid].n = 0;
+    double before = 0.0, total = 0.0, all = 0.0;
+#pragma unroll
+    for (int i = 0; i < NT / kWave; ++i) {
+        const double r = red[i];
+        if (uint32_t(i) < wave) before += r;
+        total += r;
+        all += red[NT / kWave + i];
+    }
+    Walk m;
+    take_part(m, total, float(all) * a.kv_heads);
+    const double lo = before + inc - sum;
+    if (tid == 0) {  // with no work, all there is
+        m.b = 0;
+        m.before = 0.0;
+        l = m;
+    }
+    __syncthreads();
+    if (lo <= m.at && m.at < lo + sum) {  // one thread, if there is any work
+        double at = lo;
+        uint32_t b = b0;
+        for (; b + 1 < b1; ++b) {
+            const double c = request_at<FEW>(a, h, b).total * a.kv_heads;
+            if (at + c > m.at) break;
+            at += c;
+        }
+        l.b = b;
+        l.before = at;
+    }
+    __syncthreads();
+    if (tid < 2) (FEW ? a.few_p : a.many_p)[2 * m.w + tid].n = 0;
 }
 
 // Wave 0: the part's next segment.  A cut tile gets its slot and its record for k_paged_join.
 template <bool FEW>
-__device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, uint32_t bm, uint32_t keys)
+__device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, const Heads& h)
 {
+    constexpr uint32_t bm = FEW ? kFewRows : kManyRows, keys = FEW ? kFewKeys : kManyKeys;
     if (threadIdx.x >= 64) return;
     Walk m = l;
     m.go = m.at < m.to;
     if (m.go) {
         Request r;
         for (;; ++m.b) {  // the request at m.at
-            r = request_at<FEW>(a, m.b, bm);
+            r = request_at<FEW>(a, h, m.b);
             if (m.at < m.before + r.total * a.kv_heads) break;
             m.before += r.total * a.kv_heads;
         }
         const double off = m.at - m.before;
-        m.g = min(a.kv_heads - 1, uint32_t(off / r.total));
+        m.g = min(a.kv_heads - 1, uint32_t(near_ratio(off, r.total)));
         while (m.g && m.g * r.total > off) --m.g;
         while (m.g + 1 < a.kv_heads && (m.g + 1) * r.total <= off) ++m.g;
         const double in = off - m.g * r.total;
@@ -327,7 +362,7 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, uint32
         m.complete = m.at <= begin && end <= m.to;
         if (!m.complete) {
             const uint32_t w0 = part_of(m, begin), w1 = part_of(m, end - 1.0);
-            const uint32_t first = 2 * w0 + (part_at(m.total, w0, m.parts) < begin ? 1u : 0u);
+            const uint32_t first = 2 * w0 + (part_at(m, w0) < begin ? 1u : 0u);
             m.slot = m.w == w0 ? first : 2 * m.w;
             if (threadIdx.x == 0)
                 (FEW ? a.few_p : a.many_p)[m.slot] = Piece{w1 - w0 + 1, m.w - w0, w0, first, r.token, m.x.row0, m.x.rows, m.g};
@@ -661,15 +696,16 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 {
-    __shared__ double red[4];
+    __shared__ double red[8];
     __shared__ Walk walk;
+    __shared__ Heads heads;
     __shared__ __align__(16) float joined[4 * 32 * D];  // two V buffers of each wave, then the waves' outputs
     __shared__ float mw[4][32], lw[4][32];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<true, 256>(arguments(), walk, kFewRows, kFewKeys, red);
+    start_walk<true, 256>(arguments(), walk, heads, red);
     T* vrows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
     for (;;) {
-        next_segment<true>(arguments(), walk, kFewRows, kFewKeys);
+        next_segment<true>(arguments(), walk, heads);
         __syncthreads();
         if (uniform(walk.go) == 0) break;
         const Segment s = read_segment(walk);
@@ -812,16 +848,18 @@ template <typename T, int D, int NW, bool WIDE>
 __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 {
     constexpr int NT = NW * 64;
-    constexpr uint32_t kBm = NW * 32, kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
+    static_assert(NW == kManyWaves, "the walk's tiles");
+    constexpr uint32_t kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
     __shared__ __align__(16) T ks[2][kManyKeys * D];
     __shared__ __align__(16) T vs[2][kManyKeys * D];
-    __shared__ double red[NW];
+    __shared__ double red[2 * NW];
     __shared__ Walk walk;
+    __shared__ Heads heads;
     __shared__ uint32_t odd;  // infinities or NaN cleared from V in this segment
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<false, NT>(arguments(), walk, kBm, kManyKeys, red);
+    start_walk<false, NT>(arguments(), walk, heads, red);
     for (;;) {
-        next_segment<false>(arguments(), walk, kBm, kManyKeys);
+        next_segment<false>(arguments(), walk, heads);
         if (tid == 0) odd = 0;
         __syncthreads();
         if (uniform(walk.go) == 0) break;
@@ -949,65 +987,90 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 
 // ---------------------------------------------------------------------- join
 // Adds the pieces of the tiles that were cut, in order: out = sum_i 2^(m_i - M) o_i /
-// sum_i 2^(m_i - M) l_i.  One group of workgroups per slot; the n workgroup groups of a tile's
-// n pieces share its rows, a row at a time: D / 4 lanes across, 256 / (D / 4) pieces
-// at once.
-constexpr uint32_t kJoinSplit = 4;
+// sum_i 2^(m_i - M) l_i.  A workgroup for the two slots of each part (kManySplit of them where tiles
+// have many rows); the workgroups of a tile's n pieces share its rows.  D / 4 lanes span a row; few
+// pieces (long rows of tiles cut once or twice): 256 / (D / 4) rows at once, each by its lanes
+// alone; many (one long context): a row at a time, its pieces dealt out over the groups of lanes.
+constexpr uint32_t kManySplit = 4;
+constexpr uint32_t kManyPieces = 8;
+
+struct JoinRow {
+    float L;
+    float4 acc;
+};
+__device__ __forceinline__ void add_piece(JoinRow& r, float f, float l, const float4& o)
+{
+    r.L = __builtin_fmaf(l, f, r.L);
+    r.acc.x = __builtin_fmaf(o.x, f, r.acc.x);
+    r.acc.y = __builtin_fmaf(o.y, f, r.acc.y);
+    r.acc.z = __builtin_fmaf(o.z, f, r.acc.z);
+    r.acc.w = __builtin_fmaf(o.w, f, r.acc.w);
+}
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, const JoinRow& r)
+{
+    const float inv = r.L == 0.0f ? 0.0f : 1.0f / r.L;
+    store4<T>(p, r.acc.x * inv, r.acc.y * inv, r.acc.z * inv, r.acc.w * inv);
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
 {
     constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes;
     __shared__ __align__(16) float4 part[kGroups][kLanes];
     __shared__ float part_l[kGroups];
-    const uint32_t few = 2 * a.few_wgs;
-    const bool is_few = blockIdx.x < few;
-    const uint32_t own = is_few ? blockIdx.x : blockIdx.x - few;
-    const Piece p = (is_few ? a.few_p : a.many_p)[own];
-    if (p.n == 0) return;
+    const bool is_few = blockIdx.x < a.few_wgs;
+    if (is_few && blockIdx.y) return;
+    const uint32_t own = is_few ? blockIdx.x : blockIdx.x - a.few_wgs, split = is_few ? 1 : kManySplit;
     const float* po = is_few ? a.few_o : a.many_o;
     const float2* pml = is_few ? a.few_ml : a.many_ml;
     const uint32_t srows = is_few ? a.few_slot : a.many_slot;
     const uint32_t tid = threadIdx.x, grp = tid / kLanes, d = tid % kLanes;
-    auto slot_of = [&](uint32_t i) { return uint64_t(i ? 2 * (p.wg + i) : p.slot); };
-    for (uint32_t row = p.idx * kJoinSplit + blockIdx.y; row < p.rows; row += p.n * kJoinSplit) {
-        float M = -INFINITY;
-        for (uint32_t i = grp; i < p.n; i += kGroups) M = fmaxf(M, pml[slot_of(i) * srows + row].x);
-        __syncthreads();  // the row before is done with part
-        if (d == 0) part_l[grp] = M;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t j = 0; j < kGroups; ++j) M = fmaxf(M, part_l[j]);
-        const float M0 = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f;
-        float4 acc = make_float4(0, 0, 0, 0);
-        for (uint32_t i = grp; i < p.n; i += kGroups) {
-            const float2 ml = pml[slot_of(i) * srows + row];
-            const float f = __builtin_amdgcn_exp2f(ml.x - M0);
-            const float4 o = *reinterpret_cast<const float4*>(po + (slot_of(i) * srows + row) * D + 4 * d);
-            L = __builtin_fmaf(ml.y, f, L);
-            acc.x = __builtin_fmaf(o.x, f, acc.x);
-            acc.y = __builtin_fmaf(o.y, f, acc.y);
-            acc.z = __builtin_fmaf(o.z, f, acc.z);
-            acc.w = __builtin_fmaf(o.w, f, acc.w);
-        }
-        __syncthreads();  // part_l is read
-        part[grp][d] = acc;
-        if (d == 0) part_l[grp] = L;
-        __syncthreads();
-        if (grp == 0) {
-            L = 0.0f;
-            acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (uint32_t j = 0; j < kGroups; ++j) {
-                const float4 o = part[j][d];
-                L += part_l[j];
-                acc.x += o.x;
-                acc.y += o.y;
-                acc.z += o.z;
-                acc.w += o.w;
+    for (uint32_t second = 0; second < 2; ++second) {
+        const Piece p = (is_few ? a.few_p : a.many_p)[2 * own + second];
+        if (p.n == 0) continue;
+        auto at = [&](uint32_t i, uint32_t row) { return uint64_t(i ? 2 * (p.wg + i) : p.slot) * srows + row; };
+        const uint32_t turn = p.idx * split + blockIdx.y, turns = p.n * split;
+        if (p.n <= kManyPieces) {
+            for (uint32_t row = turn * kGroups + grp; row < p.rows; row += turns * kGroups) {
+                float M = -INFINITY;
+                for (uint32_t i = 0; i < p.n; ++i) M = fmaxf(M, pml[at(i, row)].x);
+                const float M0 = M == -INFINITY ? 0.0f : M;
+                JoinRow r{0.0f, make_float4(0, 0, 0, 0)};
+#pragma unroll 2
+                for (uint32_t i = 0; i < p.n; ++i) {
+                    const float2 ml = pml[at(i, row)];
+                    add_piece(r, __builtin_amdgcn_exp2f(ml.x - M0), ml.y, *reinterpret_cast<const float4*>(po + at(i, row) * D + 4 * d));
+                }
+                store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, r);
             }
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            store4<T>(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            continue;
+        }
+        for (uint32_t row = turn; row < p.rows; row += turns) {
+            float M = -INFINITY;
+            for (uint32_t i = grp; i < p.n; i += kGroups) M = fmaxf(M, pml[at(i, row)].x);
+            __syncthreads();  // the row before is done with part and part_l
+            if (d == 0) part_l[grp] = M;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t j = 0; j < kGroups; ++j) M = fmaxf(M, part_l[j]);
+            const float M0 = M == -INFINITY ? 0.0f : M;
+            JoinRow r{0.0f, make_float4(0, 0, 0, 0)};
+#pragma unroll 4
+            for (uint32_t i = grp; i < p.n; i += kGroups) {
+                const float2 ml = pml[at(i, row)];
+                add_piece(r, __builtin_amdgcn_exp2f(ml.x - M0), ml.y, *reinterpret_cast<const float4*>(po + at(i, row) * D + 4 * d));
+            }
+            __syncthreads();  // part_l is read
+            part[grp][d] = r.acc;
+            if (d == 0) part_l[grp] = r.L;
+            __syncthreads();
+            if (grp == 0) {
+                r = JoinRow{0.0f, make_float4(0, 0, 0, 0)};
+#pragma unroll
+                for (uint32_t j = 0; j < kGroups; ++j) add_piece(r, 1.0f, part_l[j], part[j][d]);
+                store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, r);
+            }
         }
     }
 }
@@ -1056,7 +1119,7 @@ hipError_t launch_paged(const PagedAttn& a, hipStream_t st)
     if (a.shift >= 4) launch_tiles<T, D, true>(a, st);
     else launch_tiles<T, D, false>(a, st);
     if (hipError_t e = hipGetLastError()) return e;
-    hipLaunchKernelGGL((k_paged_join<T, D>), dim3(2 * (a.few_wgs + a.many_wgs), kJoinSplit), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_paged_join<T, D>), dim3(a.few_wgs + a.many_wgs, a.many_wgs ? kManySplit : 1), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
