@@ -437,20 +437,30 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r)
 // from the lane's own address.  In assembly because the compiler waits for such a copy before
 // the next read of LDS, whichever buffer that is from; there is no register for a load in
 // flight to write, and nothing else here uses m0.  wait_loads and a barrier (a wave's own rows: wait_loads) come before the rows are read.
+// ONCE: data that no other workgroup reads goes past the caches' keeping (nt): 2 contexts of 131071, 8 kv
+// heads (727 MB) 139 -> 121 us.
+template <bool ONCE>
 __device__ __forceinline__ void copy16(uint32_t lds, const void* base, uint32_t off)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
+template <bool ONCE>
 __device__ __forceinline__ void copy16(uint32_t lds, const void* from)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(from) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
 }
 
-// N positions' rows of K (BOTH) and V from the pages straight into LDS, row i at kl, vl + i * D.  `page`: lane
+// N positions' rows of K and V, or one of them, from the pages straight into LDS, row i at kl, vl + i * D.  `page`: lane
 // first + i holds the page of row i's position pos0 + i.  Which 16 bytes a lane copies carries the swizzle, as
 // LDS is written in lane order.  WIDE, pages of 16 and more: 16 aligned rows have one
 // page, so the address is scalar and the lane's part of it the same for every unit.
-template <bool BOTH, int N, bool WIDE, int D, typename T>
+template <bool K, bool V, bool ONCE, int N, bool WIDE, int D, typename T>
 __device__ __forceinline__ void copy_rows(const Pool<T>& p, T* kl, T* vl, uint32_t page, uint32_t first, uint32_t pos0)
 {
     constexpr uint32_t kAcross = D / 8, kRows = kWave / kAcross;  // lanes per row, rows per copy
@@ -467,8 +477,8 @@ __device__ __forceinline__ void copy_rows(const Pool<T>& p, T* kl, T* vl, uint32
 #pragma unroll
             for (uint32_t i = 0; i < kGroup; i += kRows) {
                 const uint32_t r = i + r0, off = (r * p.kvd + ((c ^ swizzle<D>(first + part + r)) << 3)) * 2;
-                if constexpr (BOTH) copy16(kto + (part + i) * D * 2, kb, off);
-                copy16(vto + (part + i) * D * 2, vb, off);
+                if constexpr (K) copy16<ONCE>(kto + (part + i) * D * 2, kb, off);
+                if constexpr (V) copy16<ONCE>(vto + (part + i) * D * 2, vb, off);
             }
         } else {
 #pragma unroll
@@ -476,8 +486,8 @@ __device__ __forceinline__ void copy_rows(const Pool<T>& p, T* kl, T* vl, uint32
                 const uint32_t r = part + i + r0;
                 const uint64_t at = row_offset(p, uint32_t(__shfl(int(page), int(first + r))), pos0 + r) +
                                     ((c ^ swizzle<D>(first + r)) << 3);
-                if constexpr (BOTH) copy16(kto + (part + i) * D * 2, p.k + at);
-                copy16(vto + (part + i) * D * 2, p.v + at);
+                if constexpr (K) copy16<ONCE>(kto + (part + i) * D * 2, p.k + at);
+                if constexpr (V) copy16<ONCE>(vto + (part + i) * D * 2, p.v + at);
             }
         }
     }
@@ -488,6 +498,14 @@ __device__ __forceinline__ void wait_loads()
 {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
+// Waits until this wave's reads of LDS are done: a copy may then overwrite what they read.
+__device__ __forceinline__ void wait_lds()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     asm volatile("" ::: "memory");
 }
 
@@ -688,22 +706,22 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 // ------------------------------------------------------------------ few rows
 // Tiles of up to 32 rows: decode, short chunks.  Bound by reading K and V once.  4
 // waves, each on its own 32 positions of a unit with its own softmax, joined through LDS
-// at the tile's end; nothing but that join needs a barrier.  K: lane -> position
-// lane & 31, half of the row's 16-byte blocks, which is the score product's operand as it comes
-// (S^T = K Q^T; lane -> query).  V goes straight to LDS for its transposed operand (O^T = V^T
-// P^T), P^T comes from the scores' registers.  The next unit's V is on its way while
-// this one is computed, its K from the moment this one's scores are done: 16 KB a wave.
+// at the tile's end; nothing but that join needs a barrier.  K and V come straight into
+// the wave's own LDS rows, in whole rows.  S^T = K Q^T (lane -> query), O^T = V^T P^T, P^T from the
+// scores' registers.  The next unit's K is on its way as soon as this one's scores are done, its V
+// after the output: with 8 waves a CU some 110 KB of 128 are in flight.
 template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 {
     __shared__ double red[8];
     __shared__ Walk walk;
     __shared__ Heads heads;
-    __shared__ __align__(16) float joined[4 * 32 * D];  // two V buffers of each wave, then the waves' outputs
+    __shared__ __align__(16) float joined[4 * 32 * D];  // K and V rows of each wave, then the waves' outputs
     __shared__ float mw[4][32], lw[4][32];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
     start_walk<true, 256>(arguments(), walk, heads, red);
-    T* vrows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
+    T* krows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
+    T* vrows = krows + 32 * D;
     for (;;) {
         next_segment<true>(arguments(), walk, heads);
         __syncthreads();
@@ -726,42 +744,36 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
             const int32_t kp = int32_t(first_of(u) + l32);
             return kp <= s.x.pos1 ? p.table[uint32_t(kp) >> p.shift] : 0xffffffffu;
         };
-        uint4 kr[D / 16];
-        auto load_k = [&](uint32_t page, uint32_t u) {
-            const T* at = p.k + row_offset(p, page, first_of(u) + l32) + 8 * h2;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) kr[i] = *reinterpret_cast<const uint4*>(at + 16 * i);
-        };
         if (s.u0 < s.u1) {
             uint32_t page = page_of(s.u0);
             uint32_t npage = s.u0 + 1 < s.u1 ? page_of(s.u0 + 1) : 0xffffffffu;
             vec8<T> q[D / 16];
             load_q<T, D>(arguments(), s.token, s.x.row0 + row, l32 < s.x.rows, s.g, q);
-            load_k(page, s.u0);
-            copy_rows<false, 32, WIDE, D>(p, vrows, vrows, page, 0, first_of(s.u0));
-            T* vcur = vrows;
-            T* vnext = vrows + 32 * D;
+            copy_rows<true, true, true, 32, WIDE, D>(p, krows, vrows, page, 0, first_of(s.u0));
             for (uint32_t u = s.u0; u < s.u1; ++u) {
                 const int32_t k0 = int32_t(first_of(u));
                 wait_loads();  // K, V of this unit, the next one's pages
                 const bool more = u + 1 < s.u1;
-                uint32_t far = 0xffffffffu;
-                if (more) {
-                    copy_rows<false, 32, WIDE, D>(p, vnext, vnext, npage, 0, first_of(u + 1));
-                    if (u + 2 < s.u1) far = page_of(u + 2);
-                }
                 f32x16 sc;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) sc = mfma<T>(__builtin_bit_cast(vec8<T>, kr[i]), q[i], sc);
-                if (more) load_k(npage, u + 1);
+                for (int i = 0; i < D / 16; ++i) {
+                    const vec8<T> kf = *reinterpret_cast<const vec8<T>*>(&krows[l32 * D + (((2u * i + h2) ^ swizzle<D>(l32)) << 3)]);
+                    sc = mfma<T>(kf, q[i], sc);
+                }
+                uint32_t far = 0xffffffffu;
+                if (more) {
+                    wait_lds();
+                    copy_rows<true, false, true, 32, WIDE, D>(p, krows, krows, npage, 0, first_of(u + 1));
+                    if (u + 2 < s.u1) far = page_of(u + 2);
+                }
 
                 const bool in = page < p.num_pages;
                 const uint32_t valid = uint32_t(__ballot(in));
                 const bool whole = all_seen(p, s.x, k0, 32, valid == 0xffffffffu);
                 if (!whole) {
-                    for (uint32_t c = h2; c < D / 8; c += 2) odd |= clean(vcur + l32 * D + c * 8, in);
+                    for (uint32_t c = h2; c < D / 8; c += 2) odd |= clean(vrows + l32 * D + c * 8, in);
                     hide(sc, valid & seen_bits(qpos, k0, p.window, p.sinks));
                     wave_fence();
                 }
@@ -780,12 +792,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 for (int st = 0; st < 2; ++st) {
                     const vec8<T> w = narrow<T>(sc, 8 * st);
 #pragma unroll
-                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vcur, st, t), w, o[t]);
+                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vrows, st, t), w, o[t]);
                 }
-                wave_fence();  // the unit after the next is copied over these rows
-                T* const t = vcur;
-                vcur = vnext;
-                vnext = t;
+                if (more) {
+                    wait_lds();
+                    copy_rows<false, true, true, 32, WIDE, D>(p, vrows, vrows, npage, 0, first_of(u + 1));
+                }
                 page = npage;
                 npage = far;
             }
@@ -882,7 +894,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
         };
         auto copy_unit = [&](uint32_t u, uint32_t page, int buf) {
             const uint32_t at = wave * kOwn, pos = unit_start(s.x, u, kManyKeys) + at;
-            copy_rows<true, kOwn, WIDE, D>(p, &ks[buf][at * D], &vs[buf][at * D], page, at, pos);
+            copy_rows<true, true, false, kOwn, WIDE, D>(p, &ks[buf][at * D], &vs[buf][at * D], page, at, pos);
         };
         if (s.u0 < s.u1) {
             uint32_t page = page_of(s.u0);
