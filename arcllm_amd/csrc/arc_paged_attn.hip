@@ -425,12 +425,18 @@ __device__ __forceinline__ uint64_t row_offset(const Pool<T>& p, uint32_t page, 
     return page < p.num_pages ? at : 0;
 }
 
-// A K or V row in LDS: D / 8 blocks of 16 bytes, block c of row r at place
-// c ^ swizzle(r), so that the 8 or 4 rows that a read touches at once lie in different banks.
+// A K or V row in LDS: D / 8 blocks of 16 bytes, block c of row r at place c ^ swizzle(r).  LDS serves 256
+// bytes at a time from 64 banks: a read of K's 16-byte blocks takes 16 lanes, whose rows differ modulo 16; a
+// transposing read of V takes 32 lanes, 4 rows of 4 blocks.  Each set falls on all 64 banks.
 template <int D>
-__device__ __forceinline__ uint32_t swizzle(uint32_t r)
+__device__ __forceinline__ uint32_t k_swizzle(uint32_t r)
 {
-    return D == 128 ? (r & 7u) << 1 : ((r >> 1) & 3u) << 1;
+    return D == 128 ? r & 15u : (r >> 1) & 7u;  // D = 64: two rows to 256 bytes
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_swizzle(uint32_t r)
+{
+    return D == 128 ? (r & 3u) << 2 : ((r >> 1) & 1u) << 2;
 }
 
 // 16 bytes per lane from memory straight into LDS, lane i's at lds + 16 i: from base (scalar) + off bytes, or
@@ -476,18 +482,17 @@ __device__ __forceinline__ void copy_rows(const Pool<T>& p, T* kl, T* vl, uint32
             const T *kb = p.k + at, *vb = p.v + at;
 #pragma unroll
             for (uint32_t i = 0; i < kGroup; i += kRows) {
-                const uint32_t r = i + r0, off = (r * p.kvd + ((c ^ swizzle<D>(first + part + r)) << 3)) * 2;
-                if constexpr (K) copy16<ONCE>(kto + (part + i) * D * 2, kb, off);
-                if constexpr (V) copy16<ONCE>(vto + (part + i) * D * 2, vb, off);
+                const uint32_t r = i + r0, row = first + part + r;
+                if constexpr (K) copy16<ONCE>(kto + (part + i) * D * 2, kb, (r * p.kvd + ((c ^ k_swizzle<D>(row)) << 3)) * 2);
+                if constexpr (V) copy16<ONCE>(vto + (part + i) * D * 2, vb, (r * p.kvd + ((c ^ v_swizzle<D>(row)) << 3)) * 2);
             }
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < kGroup; i += kRows) {
                 const uint32_t r = part + i + r0;
-                const uint64_t at = row_offset(p, uint32_t(__shfl(int(page), int(first + r))), pos0 + r) +
-                                    ((c ^ swizzle<D>(first + r)) << 3);
-                if constexpr (K) copy16<ONCE>(kto + (part + i) * D * 2, p.k + at);
-                if constexpr (V) copy16<ONCE>(vto + (part + i) * D * 2, p.v + at);
+                const uint64_t at = row_offset(p, uint32_t(__shfl(int(page), int(first + r))), pos0 + r);
+                if constexpr (K) copy16<ONCE>(kto + (part + i) * D * 2, p.k + at + ((c ^ k_swizzle<D>(first + r)) << 3));
+                if constexpr (V) copy16<ONCE>(vto + (part + i) * D * 2, p.v + at + ((c ^ v_swizzle<D>(first + r)) << 3));
             }
         }
     }
@@ -538,7 +543,7 @@ __device__ __forceinline__ vec8<T> load_vt(const T* rows, int s, int t)
     for (int j = 0; j < 2; ++j) {
         const uint32_t r = 16u * s + 8u * j + 4u * (lane >> 5) + (i >> 2);
         const uint32_t block = 4u * t + 2u * ((lane >> 4) & 1u) + ((i >> 1) & 1u);
-        const T* p = rows + r * D + ((block ^ swizzle<D>(r)) << 3) + 4u * (i & 1u);
+        const T* p = rows + r * D + ((block ^ v_swizzle<D>(r)) << 3) + 4u * (i & 1u);
         part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
     }
     typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -759,7 +764,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
-                    const vec8<T> kf = *reinterpret_cast<const vec8<T>*>(&krows[l32 * D + (((2u * i + h2) ^ swizzle<D>(l32)) << 3)]);
+                    const vec8<T> kf = *reinterpret_cast<const vec8<T>*>(&krows[l32 * D + (((2u * i + h2) ^ k_swizzle<D>(l32)) << 3)]);
                     sc = mfma<T>(kf, q[i], sc);
                 }
                 uint32_t far = 0xffffffffu;
@@ -934,7 +939,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                     for (int kt = 0; kt < 2; ++kt) {
                         const uint32_t rr = 32u * kt + l32;
                         const vec8<T> kf =
-                            *reinterpret_cast<const vec8<T>*>(&ks[cur][rr * D + (((2u * st + h2) ^ swizzle<D>(rr)) << 3)]);
+                            *reinterpret_cast<const vec8<T>*>(&ks[cur][rr * D + (((2u * st + h2) ^ k_swizzle<D>(rr)) << 3)]);
                         sc[kt] = mfma<T>(kf, q[st], sc[kt]);
                     }
                 if (!whole) {
