@@ -326,9 +326,9 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
     if (tid < 2) (FEW ? a.few_p : a.many_p)[2 * m.w + tid].n = 0;
 }
 
-// Wave 0: the part's next segment.  A cut tile gets its slot and its record for k_paged_join.
+// Wave 0: the part's next segment after l's.  A cut tile gets its slot and its record for k_paged_join.
 template <bool FEW>
-__device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, const Heads& h)
+__device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, Walk& to, const Heads& h)
 {
     constexpr uint32_t bm = FEW ? kFewRows : kManyRows, keys = FEW ? kFewKeys : kManyKeys;
     if (threadIdx.x >= 64) return;
@@ -369,7 +369,7 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, Walk& l, const 
         }
         m.at = fmin(end, m.to);
     }
-    if (threadIdx.x == 0) l = m;
+    if (threadIdx.x == 0) to = m;
 }
 
 // What every wave needs of the segment, in scalar registers.
@@ -522,6 +522,9 @@ __device__ __forceinline__ f32x16 mfma(vec8<T> x, vec8<T> y, f32x16 c)
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
 }
 
+// Kinds of instructions for the scheduler, and how many LDS reads go ahead of the first product.
+constexpr int kMfma = 0x008, kDsRead = 0x100, kAhead = 8;
+
 // 8 consecutive values to 16 bits, round to nearest even.
 template <typename T>
 __device__ __forceinline__ vec8<T> narrow(const f32x16& p, int at)
@@ -551,15 +554,21 @@ __device__ __forceinline__ vec8<T> load_vt(const T* rows, int s, int t)
     return __builtin_bit_cast(vec8<T>, both);
 }
 
-// Whether any of the two 16-bit values of w is infinite or NaN, and w without them.
+// Nonzero where one of the two 16-bit values of w is infinite or NaN.
 template <typename T>
-__device__ __forceinline__ bool drop_nonfinite(uint32_t& w)
+__device__ __forceinline__ uint32_t nonfinite(uint32_t w)
+{
+    constexpr uint32_t kExp = __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
+    const uint32_t x = ~w & kExp;  // a half that is zero here
+    return (x - 0x00010001u) & ~x & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t without_nonfinite(uint32_t w)
 {
     constexpr uint32_t kExp = __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
-    const bool lo = (w & kExp) == kExp, hi = ((w >> 16) & kExp) == kExp;
-    if (lo) w &= 0xffff0000u;
-    if (hi) w &= 0x0000ffffu;
-    return lo || hi;
+    if ((w & kExp) == kExp) w &= 0xffff0000u;
+    if (((w >> 16) & kExp) == kExp) w &= 0x0000ffffu;
+    return w;
 }
 
 __device__ __forceinline__ bool sees(int32_t qpos, int32_t kpos, uint32_t window, uint32_t sinks)
@@ -657,18 +666,18 @@ __device__ __forceinline__ bool all_seen(const Pool<T>& p, const Tile& x, int32_
            (p.window == 0 || uint32_t(x.pos1 - k0) < p.window || uint32_t(k0) + keys <= p.sinks);
 }
 
-// The 16 bytes at p without infinities and NaN, or zero where the position is not in; whether there were any.
+// Clears infinities and NaN of the 16 bytes at p, or all of them where the position is not in; whether there were
+// infinities or NaN of one that is.
 template <typename T>
 __device__ __forceinline__ bool clean(T* p, bool in)
 {
     uint4 w = *reinterpret_cast<const uint4*>(p);
-    if (!in) w = make_uint4(0, 0, 0, 0);
-    bool any = drop_nonfinite<T>(w.x);
-    any |= drop_nonfinite<T>(w.y);
-    any |= drop_nonfinite<T>(w.z);
-    any |= drop_nonfinite<T>(w.w);
+    const bool any = (nonfinite<T>(w.x) | nonfinite<T>(w.y) | nonfinite<T>(w.z) | nonfinite<T>(w.w)) != 0;
+    if (in && !any) return false;
+    w = in ? make_uint4(without_nonfinite<T>(w.x), without_nonfinite<T>(w.y), without_nonfinite<T>(w.z), without_nonfinite<T>(w.w))
+           : make_uint4(0, 0, 0, 0);
     *reinterpret_cast<uint4*>(p) = w;
-    return any;
+    return in && any;
 }
 
 // What infinities and NaN of V at positions that only some of a tile's rows see have to add: their
@@ -694,8 +703,10 @@ __device__ __forceinline__ void add_nonfinite(const Pool<T>& p, f32x16 (&o)[D / 
             for (int t = 0; t < D / 32; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float x = static_cast<float>(row[32 * t + tile_index(i)]);
-                    if (!(fabsf(x) < INFINITY)) o[t][i] += x;
+                    // all exponent bits set: the sum carries into the sign, which becomes a mask
+                    const int32_t x = __builtin_bit_cast(int32_t, static_cast<float>(row[32 * t + tile_index(i)]));
+                    const int32_t keep = int32_t((uint32_t(x) & 0x7f800000u) + 0x00800000u) >> 31;
+                    o[t][i] += __builtin_bit_cast(float, x & keep);
                 }
         }
     }
@@ -719,19 +730,19 @@ template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 {
     __shared__ double red[8];
-    __shared__ Walk walk;
+    __shared__ Walk walk[2];  // this segment and the next
     __shared__ Heads heads;
     __shared__ __align__(16) float joined[4 * 32 * D];  // K and V rows of each wave, then the waves' outputs
     __shared__ float mw[4][32], lw[4][32];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<true, 256>(arguments(), walk, heads, red);
+    start_walk<true, 256>(arguments(), walk[1], heads, red);
+    next_segment<true>(arguments(), walk[1], walk[0], heads);
     T* krows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
     T* vrows = krows + 32 * D;
-    for (;;) {
-        next_segment<true>(arguments(), walk, heads);
+    for (uint32_t turn = 0;; turn ^= 1u) {
         __syncthreads();
-        if (uniform(walk.go) == 0) break;
-        const Segment s = read_segment(walk);
+        if (uniform(walk[turn].go) == 0) break;
+        const Segment s = read_segment(walk[turn]);
         const Pool<T> p = pool_of<T, D>(arguments(), s);
         const uint32_t row = min(l32, s.x.rows - 1);
         const int32_t qpos = s.base + int32_t((s.x.row0 + row) / arguments().hpk);
@@ -755,6 +766,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
             vec8<T> q[D / 16];
             load_q<T, D>(arguments(), s.token, s.x.row0 + row, l32 < s.x.rows, s.g, q);
             copy_rows<true, true, true, 32, WIDE, D>(p, krows, vrows, page, 0, first_of(s.u0));
+            next_segment<true>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while those are on their way
             for (uint32_t u = s.u0; u < s.u1; ++u) {
                 const int32_t k0 = int32_t(first_of(u));
                 wait_loads();  // K, V of this unit, the next one's pages
@@ -807,6 +819,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 npage = far;
             }
             if (__ballot(odd)) add_nonfinite<T, D>(p, o, s, 32, qpos, first_of, page_of);
+        } else {
+            next_segment<true>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
         // the waves' states in wave order: out = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w
         __syncthreads();  // every wave is done with its V rows
@@ -851,7 +865,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 if (d == 0) e_.few_ml[uint64_t(s.slot) * e_.few_slot + rr] = make_float2(M, L);
             }
         }
-        __syncthreads();  // the next tile's V rows overwrite `joined`, its segment `walk`
     }
 }
 
@@ -870,17 +883,17 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
     __shared__ __align__(16) T ks[2][kManyKeys * D];
     __shared__ __align__(16) T vs[2][kManyKeys * D];
     __shared__ double red[2 * NW];
-    __shared__ Walk walk;
+    __shared__ Walk walk[2];  // this segment and the next
     __shared__ Heads heads;
     __shared__ uint32_t odd;  // infinities or NaN cleared from V in this segment
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<false, NT>(arguments(), walk, heads, red);
-    for (;;) {
-        next_segment<false>(arguments(), walk, heads);
-        if (tid == 0) odd = 0;
-        __syncthreads();
-        if (uniform(walk.go) == 0) break;
-        const Segment s = read_segment(walk);
+    start_walk<false, NT>(arguments(), walk[1], heads, red);
+    next_segment<false>(arguments(), walk[1], walk[0], heads);
+    for (uint32_t turn = 0;; turn ^= 1u) {
+        __syncthreads();  // the tile before is done with LDS
+        if (uniform(walk[turn].go) == 0) break;
+        if (tid == 0) odd = 0;  // set after the first unit's barrier at the earliest
+        const Segment s = read_segment(walk[turn]);
         const Pool<T> p = pool_of<T, D>(arguments(), s);
         const uint32_t trow = wave * 32 + l32;
         const uint32_t row = min(trow, s.x.rows - 1);
@@ -907,6 +920,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
             vec8<T> q[D / 16];
             load_q<T, D>(arguments(), s.token, s.x.row0 + row, trow < s.x.rows, s.g, q);
             copy_unit(s.u0, page, 0);
+            next_segment<false>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while that is on its way
             int cur = 0;
             for (uint32_t u = s.u0; u < s.u1; ++u) {
                 wait_loads();
@@ -933,6 +947,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sc[kt][i] = 0.0f;
+                // K's operands 4 steps ahead of their products: LDS answers in some 200 cycles
 #pragma unroll
                 for (int st = 0; st < D / 16; ++st)
 #pragma unroll
@@ -942,6 +957,18 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                             *reinterpret_cast<const vec8<T>*>(&ks[cur][rr * D + (((2u * st + h2) ^ k_swizzle<D>(rr)) << 3)]);
                         sc[kt] = mfma<T>(kf, q[st], sc[kt]);
                     }
+                __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+#pragma unroll
+                for (int i = 0; i < D / 8 - kAhead; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                // V's operands a step ahead of theirs
+                vec8<T> vt[2][D / 32];
+#pragma unroll
+                for (int t = 0; t < D / 32; ++t) vt[0][t] = load_vt<T, D>(vs[cur], 0, t);
                 if (!whole) {
                     hide(sc[0], uint32_t(valid) & seen_bits(qpos, k0, p.window, p.sinks));
                     hide(sc[1], uint32_t(valid >> 32) & seen_bits(qpos, k0 + 32, p.window, p.sinks));
@@ -954,18 +981,25 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                 mx = xor_max<32>(mx) * p.scale;
                 rescale(mx, m, l, o);
                 const float mr = m == -INFINITY ? 0.0f : m;
+                auto weights = [&](int st) {  // the 16 positions of step st: their weights, rounded; l adds the unrounded
+                    f32x16& x = sc[st >> 1];
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        sc[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], p.scale, -mr));
-                        l += sc[kt][i];
+                    for (int i = 8 * (st & 1); i < 8 * (st & 1) + 8; ++i) {
+                        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], p.scale, -mr));
+                        l += x[i];
                     }
+                    return narrow<T>(x, 8 * (st & 1));
+                };
+                vec8<T> w = weights(0);
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
-                    const vec8<T> w = narrow<T>(sc[st >> 1], 8 * (st & 1));
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (st < 3)
 #pragma unroll
-                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(load_vt<T, D>(vs[cur], st, t), w, o[t]);
+                        for (int t = 0; t < D / 32; ++t) vt[(st + 1) & 1][t] = load_vt<T, D>(vs[cur], st + 1, t);
+#pragma unroll
+                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(vt[st & 1][t], w, o[t]);
+                    if (st < 3) w = weights(st + 1);
                 }
                 cur ^= 1;
                 page = npage;
@@ -974,6 +1008,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
             // set before the last unit's second barrier, if at all
             if (uniform(odd))
                 add_nonfinite<T, D>(p, o, s, kManyKeys, qpos, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); }, page_of);
+        } else {
+            next_segment<false>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
         const float L = xor_sum<32>(l);
         const PagedAttn& e_ = arguments();
@@ -998,7 +1034,6 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                 if (h2 == 0) e_.many_ml[uint64_t(s.slot) * e_.many_slot + trow] = make_float2(m, L);
             }
         }
-        __syncthreads();  // the next tile's first unit overwrites LDS, its segment `walk`
     }
 }
 
