@@ -4,7 +4,7 @@
 //
 // Rows.  The hpk query heads of a kv head read the same K and V, so the rows of a
 // request and kv head g are its (token, head) pairs, token-major: row r is token
-// r / hpk, head g * hpk + r % hpk.  A tile is up to kFewRows (few) or NW * 32 (many) of
+// r / hpk, head g * hpk + r % hpk.  A tile is up to 32 (few) or 32 for each wave (many) of
 // them; it runs over the positions that any of them sees, a unit at a time.
 //
 // Work.  Requests differ in length by orders of magnitude, and the host does not know
@@ -31,9 +31,12 @@ constexpr uint32_t kFewRows = 32;      // rows of a few-rows tile
 constexpr uint32_t kFewKeys = 128;     // positions of its unit, 32 for each wave
 constexpr uint32_t kManyKeys = 64;     // positions of a many-rows tile's unit
 constexpr uint32_t kFewWgs = 512;      // most parts of the line
-constexpr uint32_t kManyWgs = 512;
-constexpr int kManyWaves = 4;
-constexpr uint32_t kManyRows = kManyWaves * 32;
+// Waves of a many-rows workgroup, 32 rows each, and workgroups that fill the card.  Heads of 128: 8 waves on a CU
+// share each unit's copy, where two workgroups of 4 copied it twice: a chunk of 4096 tokens at 12288, 28 heads,
+// 880 instead of 950 us (and 1.55 instead of 1.88 million cycles: the rest is the clock, which the matrix
+// cores' power holds down).  Heads of 64 leave registers for 3 workgroups of 4 waves.
+constexpr int many_waves(uint32_t dim) { return dim == 128 ? 8 : 4; }
+constexpr uint32_t many_wgs(uint32_t dim) { return dim == 128 ? 256 : 768; }
 constexpr uint32_t kTileKeys = 64;     // a tile's start and end cost about this many positions
 constexpr float kLazy = 8.0f;          // see rescale
 
@@ -96,10 +99,10 @@ __device__ __forceinline__ double cost_before(const Request& r, uint32_t t, doub
     return k * r.first + bm * (k * (k - 1.0) * 0.5) + (n > k ? (n - k) * r.cap : 0.0);
 }
 
-template <bool FEW>
+template <bool FEW, uint32_t bm>
 __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, uint32_t s1, uint32_t held)
 {
-    constexpr uint32_t bm = FEW ? kFewRows : kManyRows, keys = FEW ? kFewKeys : kManyKeys;
+    constexpr uint32_t keys = FEW ? kFewKeys : kManyKeys;
     Request r{};
     if (s1 <= s0 || s0 >= a.rows) return r;
     const uint32_t rows = (min(s1, a.rows) - s0) * a.hpk;
@@ -242,17 +245,17 @@ __device__ __forceinline__ void take_part(Walk& l, double total, float units)
 struct Heads {
     uint32_t s0[64], s1[64], len[64];
 };
-template <bool FEW>
+template <bool FEW, uint32_t bm>
 __device__ __forceinline__ Request request_at(const PagedAttn& a, const Heads& h, uint32_t b)
 {
-    if (a.requests <= 64) return request_of<FEW>(a, h.s0[b], h.s1[b], h.len[b]);
-    return request_of<FEW>(a, a.starts[b], a.starts[b + 1], a.lens[b]);
+    if (a.requests <= 64) return request_of<FEW, bm>(a, h.s0[b], h.s1[b], h.len[b]);
+    return request_of<FEW, bm>(a, a.starts[b], a.starts[b + 1], a.lens[b]);
 }
 
 // Adds up the requests, so that no launch has to come first, and finds the one in which the
 // part begins.  Up to 64 requests: wave 0 alone, one per lane.  More: thread t takes a run
 // of them.  For next_segment, which wave 0 runs too, no barrier is needed.
-template <bool FEW, int NT>
+template <bool FEW, uint32_t bm, int NT>
 __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h, double* red)
 {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
@@ -264,7 +267,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
             h.s0[lane] = s0;
             h.s1[lane] = s1;
             h.len[lane] = len;
-            r = request_of<FEW>(a, s0, s1, len);
+            r = request_of<FEW, bm>(a, s0, s1, len);
         }
         const double own = r.total * a.kv_heads, inc = wave_inclusive(own);
         Walk m;
@@ -283,7 +286,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
     float units = 0.0f;
 #pragma unroll 4
     for (uint32_t b = b0; b < b1; ++b) {
-        const Request r = request_at<FEW>(a, h, b);
+        const Request r = request_at<FEW, bm>(a, h, b);
         sum += r.total * a.kv_heads;
         units += r.units;
     }
@@ -315,7 +318,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
         double at = lo;
         uint32_t b = b0;
         for (; b + 1 < b1; ++b) {
-            const double c = request_at<FEW>(a, h, b).total * a.kv_heads;
+            const double c = request_at<FEW, bm>(a, h, b).total * a.kv_heads;
             if (at + c > m.at) break;
             at += c;
         }
@@ -327,17 +330,17 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
 }
 
 // Wave 0: the part's next segment after l's.  A cut tile gets its slot and its record for k_paged_join.
-template <bool FEW>
+template <bool FEW, uint32_t bm>
 __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, Walk& to, const Heads& h)
 {
-    constexpr uint32_t bm = FEW ? kFewRows : kManyRows, keys = FEW ? kFewKeys : kManyKeys;
+    constexpr uint32_t keys = FEW ? kFewKeys : kManyKeys;
     if (threadIdx.x >= 64) return;
     Walk m = l;
     m.go = m.at < m.to;
     if (m.go) {
         Request r;
         for (;; ++m.b) {  // the request at m.at
-            r = request_at<FEW>(a, h, m.b);
+            r = request_at<FEW, bm>(a, h, m.b);
             if (m.at < m.before + r.total * a.kv_heads) break;
             m.before += r.total * a.kv_heads;
         }
@@ -735,8 +738,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
     __shared__ __align__(16) float joined[4 * 32 * D];  // K and V rows of each wave, then the waves' outputs
     __shared__ float mw[4][32], lw[4][32];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<true, 256>(arguments(), walk[1], heads, red);
-    next_segment<true>(arguments(), walk[1], walk[0], heads);
+    start_walk<true, kFewRows, 256>(arguments(), walk[1], heads, red);
+    next_segment<true, kFewRows>(arguments(), walk[1], walk[0], heads);
     T* krows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
     T* vrows = krows + 32 * D;
     for (uint32_t turn = 0;; turn ^= 1u) {
@@ -766,7 +769,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
             vec8<T> q[D / 16];
             load_q<T, D>(arguments(), s.token, s.x.row0 + row, l32 < s.x.rows, s.g, q);
             copy_rows<true, true, true, 32, WIDE, D>(p, krows, vrows, page, 0, first_of(s.u0));
-            next_segment<true>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while those are on their way
+            next_segment<true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while those are on their way
             for (uint32_t u = s.u0; u < s.u1; ++u) {
                 const int32_t k0 = int32_t(first_of(u));
                 wait_loads();  // K, V of this unit, the next one's pages
@@ -820,7 +823,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
             }
             if (__ballot(odd)) add_nonfinite<T, D>(p, o, s, 32, qpos, first_of, page_of);
         } else {
-            next_segment<true>(arguments(), walk[turn], walk[turn ^ 1u], heads);
+            next_segment<true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
         // the waves' states in wave order: out = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w
         __syncthreads();  // every wave is done with its V rows
@@ -878,8 +881,7 @@ template <typename T, int D, int NW, bool WIDE>
 __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 {
     constexpr int NT = NW * 64;
-    static_assert(NW == kManyWaves, "the walk's tiles");
-    constexpr uint32_t kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
+    constexpr uint32_t kBm = NW * 32, kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
     __shared__ __align__(16) T ks[2][kManyKeys * D];
     __shared__ __align__(16) T vs[2][kManyKeys * D];
     __shared__ double red[2 * NW];
@@ -887,8 +889,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
     __shared__ Heads heads;
     __shared__ uint32_t odd;  // infinities or NaN cleared from V in this segment
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<false, NT>(arguments(), walk[1], heads, red);
-    next_segment<false>(arguments(), walk[1], walk[0], heads);
+    start_walk<false, kBm, NT>(arguments(), walk[1], heads, red);
+    next_segment<false, kBm>(arguments(), walk[1], walk[0], heads);
     for (uint32_t turn = 0;; turn ^= 1u) {
         __syncthreads();  // the tile before is done with LDS
         if (uniform(walk[turn].go) == 0) break;
@@ -920,7 +922,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
             vec8<T> q[D / 16];
             load_q<T, D>(arguments(), s.token, s.x.row0 + row, trow < s.x.rows, s.g, q);
             copy_unit(s.u0, page, 0);
-            next_segment<false>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while that is on its way
+            next_segment<false, kBm>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while that is on its way
             int cur = 0;
             for (uint32_t u = s.u0; u < s.u1; ++u) {
                 wait_loads();
@@ -1009,7 +1011,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
             if (uniform(odd))
                 add_nonfinite<T, D>(p, o, s, kManyKeys, qpos, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); }, page_of);
         } else {
-            next_segment<false>(arguments(), walk[turn], walk[turn ^ 1u], heads);
+            next_segment<false, kBm>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
         const float L = xor_sum<32>(l);
         const PagedAttn& e_ = arguments();
@@ -1140,7 +1142,8 @@ Space space_of(uint32_t dim, uint32_t hpk, uint32_t tokens)
     const uint64_t rows = uint64_t(tokens ? tokens : 1) * hpk;
     Space s{};
     s.few_slot = uint32_t(rows < kFewRows ? rows : kFewRows);
-    s.many_slot = uint32_t(rows <= kFewRows ? 0 : rows < kManyWaves * 32 ? rows : kManyWaves * 32);
+    const uint32_t bm = 32u * uint32_t(many_waves(dim)), wgs = many_wgs(dim);
+    s.many_slot = uint32_t(rows <= kFewRows ? 0 : rows < bm ? rows : bm);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -1148,11 +1151,11 @@ Space space_of(uint32_t dim, uint32_t hpk, uint32_t tokens)
         return here;
     };
     s.few_p = take(2 * kFewWgs * sizeof(Piece));
-    s.many_p = take(2 * kManyWgs * sizeof(Piece));
+    s.many_p = take(2 * wgs * sizeof(Piece));
     s.few_ml = take(2 * kFewWgs * size_t(s.few_slot) * sizeof(float2));
-    s.many_ml = take(2 * kManyWgs * size_t(s.many_slot) * sizeof(float2));
+    s.many_ml = take(2 * wgs * size_t(s.many_slot) * sizeof(float2));
     s.few_o = take(2 * kFewWgs * size_t(s.few_slot) * dim * sizeof(float));
-    s.many_o = take(2 * kManyWgs * size_t(s.many_slot) * dim * sizeof(float));
+    s.many_o = take(2 * wgs * size_t(s.many_slot) * dim * sizeof(float));
     s.bytes = at;
     return s;
 }
@@ -1162,7 +1165,7 @@ void launch_tiles(const PagedAttn& a, hipStream_t st)
 {
     if (a.few_wgs) hipLaunchKernelGGL((k_paged_few<T, D, WIDE>), dim3(a.few_wgs), dim3(256), 0, st, a);
     if (a.many_wgs)
-        hipLaunchKernelGGL((k_paged_many<T, D, kManyWaves, WIDE>), dim3(a.many_wgs), dim3(kManyWaves * 64), 0, st, a);
+        hipLaunchKernelGGL((k_paged_many<T, D, many_waves(D), WIDE>), dim3(a.many_wgs), dim3(many_waves(D) * 64), 0, st, a);
 }
 
 template <typename T, int D>
@@ -1257,7 +1260,7 @@ int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch,
     const bool many = most_rows > kFewRows, few = !many || batch->requests > 1;
     a.few_rows = !many ? ~0u : few ? kFewRows : 0u;
     a.few_wgs = few ? kFewWgs : 0;
-    a.many_wgs = many ? kManyWgs : 0;
+    a.many_wgs = many ? many_wgs(pages->head_dim) : 0;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool f16 = pages->dtype == ARC_F16;
     const hipError_t e = pages->head_dim == 64 ? (f16 ? launch_paged<_Float16, 64>(a, st) : launch_paged<bf16, 64>(a, st))
