@@ -28,7 +28,8 @@ template <typename T>
 using vec2 = T __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kFewRows = 32;      // rows of a few-rows tile
-constexpr uint32_t kFewKeys = 128;     // positions of its unit, 32 for each wave
+constexpr uint32_t kFewKeys = 32;      // positions of its unit, one wave's
+constexpr uint32_t kFewWaves = 4;
 constexpr uint32_t kManyKeys = 64;     // positions of a many-rows tile's unit
 constexpr uint32_t kFewWgs = 512;      // most parts of the line
 // Waves of a many-rows workgroup, 32 rows each, and workgroups that fill the card.  Heads of 128: 8 waves on a CU
@@ -115,7 +116,7 @@ __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, u
     r.tiles = (rows + bm - 1) / bm;
     r.first = double(kTileKeys + uint32_t(max(r.base, 0))) * a.hpk + bm;
     r.cap = a.window ? (double(kTileKeys) + a.window + a.sinks) * a.hpk + 2 * bm : 0x1p60;
-    r.total = cost_before(r, r.tiles, bm);
+    r.total = r.tiles == 1 ? fmin(r.first, r.cap) : cost_before(r, r.tiles, bm);
     const float spans = float(r.tiles) * ceilf(float(len) * (1.0f / keys));
     r.units = a.window ? fminf(spans, float(r.tiles) * (ceilf((float(a.window) + float(a.sinks)) * (1.0f / keys)) + 2.0f)) : spans;
     r.units = fmaxf(r.units, 1.0f);
@@ -170,14 +171,25 @@ __device__ __forceinline__ double of_lane(double v, int lane)
     const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(u >> 32)), lane));
     return __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
 }
+// v of the lane that a DPP row operation names, 0 where that is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u)), CTRL, ROWS, 0xf, false));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), CTRL, ROWS, 0xf, false));
+    return __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
+}
+// Inclusive prefix sums over the wave: in each row of 16 lanes, then row 0's and 2's totals into rows 1
+// and 3, then the lower half's into the upper.
 __device__ __forceinline__ double wave_inclusive(double v)
 {
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const double o = __shfl_up(v, d);
-        if (lane >= uint32_t(d)) v += o;
-    }
+    v += dpp_f64<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_f64<0x112, 0xf>(v);
+    v += dpp_f64<0x114, 0xf>(v);
+    v += dpp_f64<0x118, 0xf>(v);
+    v += dpp_f64<0x142, 0xa>(v);  // row_bcast 15
+    v += dpp_f64<0x143, 0xc>(v);  // row_bcast 31
     return v;
 }
 
@@ -225,12 +237,12 @@ __device__ __forceinline__ uint32_t part_of(const Walk& l, double x)
     return w;
 }
 
-// This workgroup's part, from the total: parts of a unit or more.  Workgroups go to the 8 XCDs
+// This workgroup's part, from the total: parts of a unit (few rows: one for each wave) or more.  Workgroups go to the 8 XCDs
 // in turn: an XCD's workgroups take neighbouring parts, which read the same K and V.
 __device__ __forceinline__ void take_part(Walk& l, double total, float units)
 {
     l.total = total;
-    l.parts = total > 0.0 ? min(uint32_t(gridDim.x), uint32_t(fminf(units, 65536.0f))) : 0u;
+    l.parts = total > 0.0 ? min(uint32_t(gridDim.x), uint32_t(fminf(fmaxf(units, 1.0f), 65536.0f))) : 0u;
     l.step = total / double(max(l.parts, 1u));
     l.w = blockIdx.x;
     l.at = l.to = 0.0;
@@ -271,7 +283,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
         }
         const double own = r.total * a.kv_heads, inc = wave_inclusive(own);
         Walk m;
-        take_part(m, of_lane(inc, 63), group_sum<kWave>(r.units) * a.kv_heads);
+        take_part(m, of_lane(inc, 63), group_sum<kWave>(r.units) * a.kv_heads * (FEW ? 1.0f / kFewWaves : 1.0f));
         const uint64_t behind = __ballot(inc > m.at);  // lanes from the part's first request on
         const int b = behind ? __builtin_ctzll(behind) : 0;
         m.b = uint32_t(b);
@@ -306,7 +318,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
         all += red[NT / kWave + i];
     }
     Walk m;
-    take_part(m, total, float(all) * a.kv_heads);
+    take_part(m, total, float(all) * a.kv_heads * (FEW ? 1.0f / kFewWaves : 1.0f));
     const double lo = before + inc - sum;
     if (tid == 0) {  // with no work, all there is
         m.b = 0;
@@ -349,15 +361,19 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, 
         while (m.g && m.g * r.total > off) --m.g;
         while (m.g + 1 < a.kv_heads && (m.g + 1) * r.total <= off) ++m.g;
         const double in = off - m.g * r.total;
-        uint32_t lo = 0, hi = r.tiles;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (cost_before(r, mid, bm) <= in) lo = mid;
-            else hi = mid;
+        uint32_t lo = 0;
+        double begin = m.before + m.g * r.total, end = begin + r.total;
+        if (r.tiles > 1) {
+            uint32_t hi = r.tiles;
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (cost_before(r, mid, bm) <= in) lo = mid;
+                else hi = mid;
+            }
+            end = begin + cost_before(r, lo + 1, bm);
+            begin += cost_before(r, lo, bm);
         }
         m.x = tile_at(a, r, lo, bm, keys);
-        const double begin = m.before + m.g * r.total + cost_before(r, lo, bm);
-        const double end = m.before + m.g * r.total + cost_before(r, lo + 1, bm);
         m.u0 = units_before(m.at, begin, end, m.x.units);
         m.u1 = units_before(m.to, begin, end, m.x.units);
         m.token = r.token;
@@ -686,14 +702,14 @@ __device__ __forceinline__ bool clean(T* p, bool in)
 // What infinities and NaN of V at positions that only some of a tile's rows see have to add: their
 // places in V were cleared for the product, where a weight of 0 would make NaN of them; here, after the
 // segment's units, each row that sees such a position gets them.  Units that all rows see
-// need none of it.  A slow pass over the segment's other units, for data that has any; first_of
-// and page_of as in the kernels, `span` positions of each unit.
+// need none of it.  A slow pass over the wave's other units (from, from + step ..), for data that has any;
+// first_of and page_of as in the kernels, `span` positions of each unit.
 template <typename T, int D, typename First, typename Page>
-__device__ __forceinline__ void add_nonfinite(const Pool<T>& p, f32x16 (&o)[D / 32], const Segment& s, uint32_t span,
-                                              int32_t qpos, First first_of, Page page_of)
+__device__ __forceinline__ void add_nonfinite(const Pool<T>& p, f32x16 (&o)[D / 32], const Segment& s, uint32_t from, uint32_t step,
+                                              uint32_t span, int32_t qpos, First first_of, Page page_of)
 {
 #pragma unroll 1
-    for (uint32_t u = s.u0; u < s.u1; ++u) {
+    for (uint32_t u = from; u < s.u1; u += step) {
         const int32_t k0 = int32_t(first_of(u));
         const uint32_t page = page_of(u);
         if (all_seen(p, s.x, k0, span, true)) continue;
@@ -724,7 +740,7 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 
 // ------------------------------------------------------------------ few rows
 // Tiles of up to 32 rows: decode, short chunks.  Bound by reading K and V once.  4
-// waves, each on its own 32 positions of a unit with its own softmax, joined through LDS
+// waves, each on units of 32 positions with its own softmax, joined through LDS
 // at the tile's end; nothing but that join needs a barrier.  K and V come straight into
 // the wave's own LDS rows, in whole rows.  S^T = K Q^T (lane -> query), O^T = V^T P^T, P^T from the
 // scores' registers.  The next unit's K is on its way as soon as this one's scores are done, its V
@@ -757,23 +773,24 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
         float m = -INFINITY, l = 0.0f;
         bool odd = false;  // infinities or NaN cleared from V
 
-        // the wave's first position of unit u, the page of lane l32's
-        auto first_of = [&](uint32_t u) { return unit_start(s.x, u, kFewKeys) + 32u * wave; };
+        // the first position of unit u, the page of lane l32's
+        auto first_of = [&](uint32_t u) { return unit_start(s.x, u, kFewKeys); };
         auto page_of = [&](uint32_t u) {
             const int32_t kp = int32_t(first_of(u) + l32);
             return kp <= s.x.pos1 ? p.table[uint32_t(kp) >> p.shift] : 0xffffffffu;
         };
-        if (s.u0 < s.u1) {
-            uint32_t page = page_of(s.u0);
-            uint32_t npage = s.u0 + 1 < s.u1 ? page_of(s.u0 + 1) : 0xffffffffu;
+        const uint32_t mine = s.u0 + wave;  // the waves take the units in turn
+        if (mine < s.u1) {
+            uint32_t page = page_of(mine);
+            uint32_t npage = mine + kFewWaves < s.u1 ? page_of(mine + kFewWaves) : 0xffffffffu;
             vec8<T> q[D / 16];
             load_q<T, D>(arguments(), s.token, s.x.row0 + row, l32 < s.x.rows, s.g, q);
-            copy_rows<true, true, true, 32, WIDE, D>(p, krows, vrows, page, 0, first_of(s.u0));
+            copy_rows<true, true, true, 32, WIDE, D>(p, krows, vrows, page, 0, first_of(mine));
             next_segment<true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while those are on their way
-            for (uint32_t u = s.u0; u < s.u1; ++u) {
+            for (uint32_t u = mine; u < s.u1; u += kFewWaves) {
                 const int32_t k0 = int32_t(first_of(u));
                 wait_loads();  // K, V of this unit, the next one's pages
-                const bool more = u + 1 < s.u1;
+                const bool more = u + kFewWaves < s.u1;
                 f32x16 sc;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
@@ -785,8 +802,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 uint32_t far = 0xffffffffu;
                 if (more) {
                     wait_lds();
-                    copy_rows<true, false, true, 32, WIDE, D>(p, krows, krows, npage, 0, first_of(u + 1));
-                    if (u + 2 < s.u1) far = page_of(u + 2);
+                    copy_rows<true, false, true, 32, WIDE, D>(p, krows, krows, npage, 0, first_of(u + kFewWaves));
+                    if (u + 2 * kFewWaves < s.u1) far = page_of(u + 2 * kFewWaves);
                 }
 
                 const bool in = page < p.num_pages;
@@ -816,12 +833,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 }
                 if (more) {
                     wait_lds();
-                    copy_rows<false, true, true, 32, WIDE, D>(p, vrows, vrows, npage, 0, first_of(u + 1));
+                    copy_rows<false, true, true, 32, WIDE, D>(p, vrows, vrows, npage, 0, first_of(u + kFewWaves));
                 }
                 page = npage;
                 npage = far;
             }
-            if (__ballot(odd)) add_nonfinite<T, D>(p, o, s, 32, qpos, first_of, page_of);
+            if (__ballot(odd)) add_nonfinite<T, D>(p, o, s, mine, kFewWaves, 32, qpos, first_of, page_of);
         } else {
             next_segment<true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
@@ -1009,7 +1026,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
             }
             // set before the last unit's second barrier, if at all
             if (uniform(odd))
-                add_nonfinite<T, D>(p, o, s, kManyKeys, qpos, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); }, page_of);
+                add_nonfinite<T, D>(p, o, s, s.u0, 1, kManyKeys, qpos, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); }, page_of);
         } else {
             next_segment<false, kBm>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
@@ -1254,10 +1271,13 @@ int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch,
     a.many_o = reinterpret_cast<float*>(ws + sp.many_o);
     a.few_slot = sp.few_slot;
     a.many_slot = sp.many_slot;
-    // which kernels can have work: no request has more rows than max_new says, and then the few-rows
-    // kernel takes them all; a single request with more goes to the many-rows kernel whatever it holds
+    // which kernels can have work: with no request of more rows than a few-rows tile has, as max_new says, the
+    // few-rows kernel takes them all; where tokens, if all are used, leave each request more, the many-rows
+    // kernel does (either is right for any request)
     const uint64_t most_rows = uint64_t(batch->max_new < batch->tokens ? batch->max_new : batch->tokens) * hpk;
-    const bool many = most_rows > kFewRows, few = !many || batch->requests > 1;
+    const uint64_t others = uint64_t(batch->requests - 1) * batch->max_new;
+    const bool many = most_rows > kFewRows;
+    const bool few = !many || batch->tokens <= others || (batch->tokens - others) * hpk <= kFewRows;
     a.few_rows = !many ? ~0u : few ? kFewRows : 0u;
     a.few_wgs = few ? kFewWgs : 0;
     a.many_wgs = many ? many_wgs(pages->head_dim) : 0;
