@@ -1058,8 +1058,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 
 // ---------------------------------------------------------------------- join
 // Adds the pieces of the tiles that were cut, in order: out = sum_i 2^(m_i - M) o_i /
-// sum_i 2^(m_i - M) l_i.  A workgroup for the two slots of each part (kManySplit of them where tiles
-// have many rows); the workgroups of a tile's n pieces share its rows.  D / 4 lanes span a row; few
+// sum_i 2^(m_i - M) l_i.  A workgroup for each slot (kManySplit of them where tiles have many
+// rows); the workgroups of a tile's n pieces share its rows.  D / 4 lanes span a row; few
 // pieces (long rows of tiles cut once or twice): 256 / (D / 4) rows at once, each by its lanes
 // alone; many (one long context): a row at a time, its pieces dealt out over the groups of lanes.
 constexpr uint32_t kManySplit = 4;
@@ -1090,58 +1090,65 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
     constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes;
     __shared__ __align__(16) float4 part[kGroups][kLanes];
     __shared__ float part_l[kGroups];
-    const bool is_few = blockIdx.x < a.few_wgs;
+    const bool is_few = blockIdx.x < 2 * a.few_wgs;
     if (is_few && blockIdx.y) return;
-    const uint32_t own = is_few ? blockIdx.x : blockIdx.x - a.few_wgs, split = is_few ? 1 : kManySplit;
+    const Piece p = is_few ? a.few_p[blockIdx.x] : a.many_p[blockIdx.x - 2 * a.few_wgs];
+    if (p.n == 0) return;
+    const uint32_t split = is_few ? 1 : kManySplit;
     const float* po = is_few ? a.few_o : a.many_o;
     const float2* pml = is_few ? a.few_ml : a.many_ml;
     const uint32_t srows = is_few ? a.few_slot : a.many_slot;
     const uint32_t tid = threadIdx.x, grp = tid / kLanes, d = tid % kLanes;
-    for (uint32_t second = 0; second < 2; ++second) {
-        const Piece p = (is_few ? a.few_p : a.many_p)[2 * own + second];
-        if (p.n == 0) continue;
-        auto at = [&](uint32_t i, uint32_t row) { return uint64_t(i ? 2 * (p.wg + i) : p.slot) * srows + row; };
-        const uint32_t turn = p.idx * split + blockIdx.y, turns = p.n * split;
-        if (p.n <= kManyPieces) {
-            for (uint32_t row = turn * kGroups + grp; row < p.rows; row += turns * kGroups) {
-                float M = -INFINITY;
-                for (uint32_t i = 0; i < p.n; ++i) M = fmaxf(M, pml[at(i, row)].x);
-                const float M0 = M == -INFINITY ? 0.0f : M;
-                JoinRow r{0.0f, make_float4(0, 0, 0, 0)};
-#pragma unroll 2
-                for (uint32_t i = 0; i < p.n; ++i) {
-                    const float2 ml = pml[at(i, row)];
-                    add_piece(r, __builtin_amdgcn_exp2f(ml.x - M0), ml.y, *reinterpret_cast<const float4*>(po + at(i, row) * D + 4 * d));
-                }
-                store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, r);
-            }
-            continue;
-        }
-        for (uint32_t row = turn; row < p.rows; row += turns) {
-            float M = -INFINITY;
-            for (uint32_t i = grp; i < p.n; i += kGroups) M = fmaxf(M, pml[at(i, row)].x);
-            __syncthreads();  // the row before is done with part and part_l
-            if (d == 0) part_l[grp] = M;
-            __syncthreads();
+    auto at = [&](uint32_t i, uint32_t row) { return uint64_t(i ? 2 * (p.wg + i) : p.slot) * srows + row; };
+    const uint32_t turn = p.idx * split + blockIdx.y, turns = p.n * split;
+    if (p.n <= kManyPieces) {
+        for (uint32_t row = turn * kGroups + grp; row < p.rows; row += turns * kGroups) {
+            float2 ml[kManyPieces];
+            float4 o[kManyPieces];
 #pragma unroll
-            for (uint32_t j = 0; j < kGroups; ++j) M = fmaxf(M, part_l[j]);
+            for (uint32_t i = 0; i < kManyPieces; ++i)  // all of them on their way at once
+                if (i < p.n) {
+                    ml[i] = pml[at(i, row)];
+                    o[i] = *reinterpret_cast<const float4*>(po + at(i, row) * D + 4 * d);
+                }
+            float M = -INFINITY;
+#pragma unroll
+            for (uint32_t i = 0; i < kManyPieces; ++i)
+                if (i < p.n) M = fmaxf(M, ml[i].x);
             const float M0 = M == -INFINITY ? 0.0f : M;
             JoinRow r{0.0f, make_float4(0, 0, 0, 0)};
-#pragma unroll 4
-            for (uint32_t i = grp; i < p.n; i += kGroups) {
-                const float2 ml = pml[at(i, row)];
-                add_piece(r, __builtin_amdgcn_exp2f(ml.x - M0), ml.y, *reinterpret_cast<const float4*>(po + at(i, row) * D + 4 * d));
-            }
-            __syncthreads();  // part_l is read
-            part[grp][d] = r.acc;
-            if (d == 0) part_l[grp] = r.L;
-            __syncthreads();
-            if (grp == 0) {
-                r = JoinRow{0.0f, make_float4(0, 0, 0, 0)};
 #pragma unroll
-                for (uint32_t j = 0; j < kGroups; ++j) add_piece(r, 1.0f, part_l[j], part[j][d]);
-                store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, r);
-            }
+            for (uint32_t i = 0; i < kManyPieces; ++i)
+                if (i < p.n) add_piece(r, __builtin_amdgcn_exp2f(ml[i].x - M0), ml[i].y, o[i]);
+            store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, r);
+        }
+        return;
+    }
+    for (uint32_t row = turn; row < p.rows; row += turns) {
+        float M = -INFINITY;
+#pragma unroll 4
+        for (uint32_t i = grp; i < p.n; i += kGroups) M = fmaxf(M, pml[at(i, row)].x);
+        __syncthreads();  // the row before is done with part and part_l
+        if (d == 0) part_l[grp] = M;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < kGroups; ++j) M = fmaxf(M, part_l[j]);
+        const float M0 = M == -INFINITY ? 0.0f : M;
+        JoinRow r{0.0f, make_float4(0, 0, 0, 0)};
+#pragma unroll 4
+        for (uint32_t i = grp; i < p.n; i += kGroups) {
+            const float2 ml = pml[at(i, row)];
+            add_piece(r, __builtin_amdgcn_exp2f(ml.x - M0), ml.y, *reinterpret_cast<const float4*>(po + at(i, row) * D + 4 * d));
+        }
+        __syncthreads();  // part_l is read
+        part[grp][d] = r.acc;
+        if (d == 0) part_l[grp] = r.L;
+        __syncthreads();
+        if (grp == 0) {
+            r = JoinRow{0.0f, make_float4(0, 0, 0, 0)};
+#pragma unroll
+            for (uint32_t j = 0; j < kGroups; ++j) add_piece(r, 1.0f, part_l[j], part[j][d]);
+            store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, r);
         }
     }
 }
@@ -1191,7 +1198,7 @@ hipError_t launch_paged(const PagedAttn& a, hipStream_t st)
     if (a.shift >= 4) launch_tiles<T, D, true>(a, st);
     else launch_tiles<T, D, false>(a, st);
     if (hipError_t e = hipGetLastError()) return e;
-    hipLaunchKernelGGL((k_paged_join<T, D>), dim3(a.few_wgs + a.many_wgs, a.many_wgs ? kManySplit : 1), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_paged_join<T, D>), dim3(2 * (a.few_wgs + a.many_wgs), a.many_wgs ? kManySplit : 1), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
