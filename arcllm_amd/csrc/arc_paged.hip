@@ -18,12 +18,10 @@ struct PlanArgs {
     uint32_t requests, rows, max_pages, max_new, num_pages, shift;  // page_size = 1 << shift
 };
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = kPlanThreads / kWave;
-
-// What one request contributes to the step.
+// What one request contributes to the step: new tokens, pages it pops, pages it pushes.
+// Whole numbers in doubles, which add up exactly where 32 bits would wrap.
 struct PlanPart {
-    uint32_t fresh, take, back;  // new tokens, pages it pops, pages it pushes
+    double fresh, take, back;
 };
 
 __device__ __forceinline__ uint32_t pages_of(uint32_t len, uint32_t shift)
@@ -33,39 +31,8 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t len, uint32_t shift)
 
 __device__ __forceinline__ PlanPart plan_part(uint32_t held, uint32_t fresh, uint32_t shift)
 {
-    if (fresh == ARC_PAGED_RELEASE) return PlanPart{0u, 0u, pages_of(held, shift)};
-    return PlanPart{fresh, pages_of(held + fresh, shift) - pages_of(held, shift), 0u};
-}
-
-__device__ __forceinline__ uint32_t wave_inclusive(uint32_t v)
-{
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const uint32_t o = uint32_t(__shfl_up(int(v), d));
-        if (lane >= uint32_t(d)) v += o;
-    }
-    return v;
-}
-
-// Exclusive prefix of v over the workgroup; `total` is the sum.  `red` holds one
-// word per wave.
-__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* red, uint32_t& total)
-{
-    const uint32_t inc = wave_inclusive(v);
-    const int wave = threadIdx.x >> 6;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) red[wave] = inc;
-    __syncthreads();
-    uint32_t before = 0, sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPlanWaves; ++i) {
-        const uint32_t r = red[i];
-        if (i < wave) before += r;
-        sum += r;
-    }
-    total = sum;
-    return before + inc - v;
+    if (fresh == ARC_PAGED_RELEASE) return PlanPart{0.0, 0.0, double(pages_of(held, shift))};
+    return PlanPart{double(fresh), double(pages_of(held + fresh, shift) - pages_of(held, shift)), 0.0};
 }
 
 // The last i < n with at[i] <= x, for at ascending with at[0] <= x.
@@ -80,71 +47,119 @@ __device__ __forceinline__ uint32_t last_at_most(const uint32_t* at, uint32_t n,
     return lo;
 }
 
-__device__ __forceinline__ void plan_row(const PlanArgs& a, uint32_t n, uint32_t b, uint32_t pos)
+// The same over N entries in LDS, without branches: searches for several items run side by side.
+template <uint32_t N>
+__device__ __forceinline__ uint32_t last_at_most(const uint32_t (&at)[N], uint32_t x)
 {
-    a.positions[n] = pos;
-    a.slots[n] = (a.tables[uint64_t(b) * a.max_pages + (pos >> a.shift)] << a.shift) | (pos & ((1u << a.shift) - 1u));
+    static_assert((N & (N - 1)) == 0, "a power of two");
+    uint32_t lo = 0;
+#pragma unroll
+    for (uint32_t step = N / 2; step; step >>= 1) lo += at[lo + step] <= x ? step : 0u;
+    return lo;
 }
 
-// The plan by one workgroup: the requests in blocks of 1024, a thread each, twice.
-// First the step's totals and every check, before anything is written; then the
-// prefix sums, from which pages, table entries and rows are dealt out evenly over
-// the threads (a binary search finds an item's request), so that one long
-// request costs no more than many short ones.  ROWS: the rows too; else
-// k_plan_rows writes them.  Bound by the latency of its dependent loads (lengths,
-// stack, table entries) and barriers.
-template <bool ROWS>
-__global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs a)
+// A block of NT requests, thread by thread: exclusive prefix sums of their parts.
+template <int NT>
+struct PlanBlock {
+    double sums[3][NT / kWave];
+    uint32_t bad[NT / kWave];
+    uint32_t held[NT], fresh[NT], take[NT], back[NT];
+};
+
+// Prefix sums of p over the workgroup; `all` gets the sums, bad what any thread had.
+template <int NT>
+__device__ __forceinline__ PlanPart block_prefix(const PlanPart& p, PlanBlock<NT>& s, PlanPart& all, uint32_t& bad)
 {
-    __shared__ uint32_t red[kPlanWaves];
-    __shared__ uint32_t first[kPlanThreads];  // exclusive prefix of what is dealt out
-    __shared__ uint32_t held[kPlanThreads];
-    __shared__ unsigned long long sums[3];
-    const uint32_t tid = threadIdx.x;
-    const uint32_t blocks = (a.requests + kPlanThreads - 1) / kPlanThreads;
-    const uint32_t count = *a.free_count;
-    const uint64_t most = min(uint64_t(a.max_pages) << a.shift, uint64_t(0x7fffffffu));
-    if (tid < 3) sums[tid] = 0;
-    uint32_t bad = 0;
-    uint64_t fresh = 0, take = 0, back = 0;
-    PlanPart p{};
-    uint32_t len = 0;
-    for (uint32_t i = 0; i < blocks; ++i) {
-        const uint32_t b = i * kPlanThreads + tid;
-        p = PlanPart{};
-        if (b < a.requests) {
-            len = a.old_lens[b];
-            const uint32_t nw = a.new_lens[b];
-            const bool ended = nw == ARC_PAGED_RELEASE;
-            if (!ended && nw > a.max_new) bad |= ARC_PLAN_MAX_NEW;
-            if (uint64_t(len) + (ended ? 0u : nw) > most) bad |= ARC_PLAN_TABLE;
-            if (!bad) p = plan_part(len, nw, a.shift);
-        }
-        fresh += p.fresh;
-        take += p.take;
-        back += p.back;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const PlanPart inc{wave_inclusive(p.fresh), wave_inclusive(p.take), wave_inclusive(p.back)};
+    const uint32_t any = (__ballot(bad & ARC_PLAN_MAX_NEW) ? ARC_PLAN_MAX_NEW : 0u) | (__ballot(bad & ARC_PLAN_TABLE) ? ARC_PLAN_TABLE : 0u);
+    __syncthreads();  // the sums and prefixes before are read no more
+    if (lane == 63) {
+        s.sums[0][wave] = inc.fresh;
+        s.sums[1][wave] = inc.take;
+        s.sums[2][wave] = inc.back;
+        s.bad[wave] = any;
     }
     __syncthreads();
-    // integer sums: the order does not matter
-    if (fresh) atomicAdd(&sums[0], static_cast<unsigned long long>(fresh));
-    if (take) atomicAdd(&sums[1], static_cast<unsigned long long>(take));
-    if (back) atomicAdd(&sums[2], static_cast<unsigned long long>(back));
-    bad = uint32_t(__syncthreads_or(int(bad & ARC_PLAN_MAX_NEW)) ? ARC_PLAN_MAX_NEW : 0) |
-          uint32_t(__syncthreads_or(int(bad & ARC_PLAN_TABLE)) ? ARC_PLAN_TABLE : 0);
-    fresh = sums[0];
-    take = sums[1];
-    back = sums[2];
-    uint64_t lacking = 0;
+    PlanPart before{inc.fresh - p.fresh, inc.take - p.take, inc.back - p.back};
+    all = PlanPart{0.0, 0.0, 0.0};
+#pragma unroll
+    for (uint32_t i = 0; i < NT / kWave; ++i) {
+        if (i < wave) {
+            before.fresh += s.sums[0][i];
+            before.take += s.sums[1][i];
+            before.back += s.sums[2][i];
+        }
+        all.fresh += s.sums[0][i];
+        all.take += s.sums[1][i];
+        all.back += s.sums[2][i];
+        bad |= s.bad[i];
+    }
+    return before;
+}
+
+// n items over the workgroup's threads, 4 at a time each: the loads of all four before the first store, so
+// that their latencies are one.  get(k) reads item k, put(k, x) stores it.
+template <int NT, typename Get, typename Put>
+__device__ __forceinline__ void deal(uint32_t n, Get get, Put put)
+{
+    for (uint32_t k0 = threadIdx.x; k0 < n; k0 += 4 * NT) {
+        uint2 x[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (k0 + i * NT < n) x[i] = get(k0 + i * NT);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (k0 + i * NT < n) put(k0 + i * NT, x[i]);
+    }
+}
+
+// The plan by one workgroup: the requests in blocks of NT, a thread each.  First the step's totals and every
+// check, before anything is written; then pages, table entries and rows are dealt out evenly over the
+// threads from the prefix sums (a binary search in LDS finds an item's request), so that one long request costs
+// no more than many short ones.  A row whose page is new takes it from the stack itself, as the table entry's
+// writer does, so no row waits for a table entry.  ROWS: the rows too; else k_plan_rows writes them.
+// Bound by the latency of three dependent loads (lengths, an ended request's entries, the stack) and
+// the barriers: 24 requests 5 us, 700 with 2500 pages 8 us, and as many again in k_plan_rows for 30000 rows.
+template <int NT, bool ROWS>
+__global__ __launch_bounds__(NT) void k_plan(PlanArgs a)
+{
+    __shared__ PlanBlock<NT> s;
+    const uint32_t tid = threadIdx.x;
+    const uint32_t blocks = (a.requests + NT - 1) / NT;
+    const uint32_t count = *a.free_count;
+    const uint64_t most = min(uint64_t(a.max_pages) << a.shift, uint64_t(0x7fffffffu));
+    uint32_t bad = 0, len = 0, fresh = 0;
+    PlanPart p{}, before{}, total{};
+    auto read = [&](uint32_t block) {
+        const uint32_t b = block * NT + tid;
+        len = b < a.requests ? a.old_lens[b] : 0u;
+        fresh = b < a.requests ? a.new_lens[b] : 0u;
+    };
+    for (uint32_t i = 0; i < blocks; ++i) {
+        read(i);
+        const bool ended = fresh == ARC_PAGED_RELEASE;
+        const uint32_t bad_before = bad;
+        if (!ended && fresh > a.max_new) bad |= ARC_PLAN_MAX_NEW;
+        if (uint64_t(len) + (ended ? 0u : fresh) > most) bad |= ARC_PLAN_TABLE;
+        p = bad == bad_before ? plan_part(len, fresh, a.shift) : PlanPart{};
+        PlanPart all;
+        before = block_prefix<NT>(p, s, all, bad);
+        total.fresh += all.fresh;
+        total.take += all.take;
+        total.back += all.back;
+    }
+    double lacking = 0.0;
     if (!bad) {
-        if (fresh > a.rows) bad |= ARC_PLAN_TOKENS;
-        if (uint64_t(count) + back > a.num_pages) bad |= ARC_PLAN_FREE_LIST;
-        else if (take > count + back) {
+        if (total.fresh > double(a.rows)) bad |= ARC_PLAN_TOKENS;
+        if (count + total.back > double(a.num_pages)) bad |= ARC_PLAN_FREE_LIST;
+        else if (total.take > count + total.back) {
             bad |= ARC_PLAN_NO_PAGES;
-            lacking = take - (count + back);
+            lacking = total.take - (count + total.back);
         }
     }
     if (bad) {
-        for (uint32_t b = tid; b < a.requests; b += kPlanThreads) {
+        for (uint32_t b = tid; b < a.requests; b += NT) {
             a.lens[b] = a.old_lens[b];
             a.starts[b] = 0;
         }
@@ -152,71 +167,83 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs a)
             a.starts[a.requests] = 0;
             *a.free_count_out = count;
             a.status[0] = bad;
-            a.status[1] = uint32_t(min(lacking, uint64_t(0xffffffffu)));
+            a.status[1] = uint32_t(fmin(lacking, 4294967295.0));
             a.status[2] = a.status[3] = 0;
         }
         if constexpr (ROWS)
-            for (uint32_t n = tid; n < a.rows; n += kPlanThreads) {
+            for (uint32_t n = tid; n < a.rows; n += NT) {
                 a.positions[n] = 0;
                 a.slots[n] = ARC_NO_SLOT;
             }
         return;
     }
 
-    const uint32_t top = count + uint32_t(back);
+    // every total fits 32 bits from here on
+    const uint32_t top = count + uint32_t(total.back);
+    auto publish = [&]() {  // this block's prefixes, for the searches
+        s.held[tid] = len;
+        s.fresh[tid] = uint32_t(before.fresh);
+        s.take[tid] = uint32_t(before.take);
+        s.back[tid] = uint32_t(before.back);
+        __syncthreads();
+    };
+    auto block_of = [&](uint32_t i) {  // reads block i again, where there is more than one
+        if (blocks == 1) return PlanPart{total.fresh, total.take, total.back};
+        read(i);
+        p = plan_part(len, fresh, a.shift);
+        PlanPart all;
+        uint32_t none = 0;
+        before = block_prefix<NT>(p, s, all, none);
+        return all;
+    };
+    if (blocks == 1) publish();
     // pages of ended requests onto the stack, before any are popped
-    if (back) {
+    if (total.back > 0.0) {
         uint32_t done = 0;
         for (uint32_t i = 0; i < blocks; ++i) {
-            const uint32_t b = i * kPlanThreads + tid;
-            p = b < a.requests ? plan_part(a.old_lens[b], a.new_lens[b], a.shift) : PlanPart{};
-            uint32_t total;
-            first[tid] = block_exclusive(p.back, red, total);
-            __syncthreads();
-            for (uint32_t k = tid; k < total; k += kPlanThreads) {
-                const uint32_t j = last_at_most(first, kPlanThreads, k);
-                a.free_pages[count + done + k] = a.tables[uint64_t(i * kPlanThreads + j) * a.max_pages + (k - first[j])];
-            }
-            done += total;
-            __syncthreads();  // `first` is read no more
+            const uint32_t pages = uint32_t(block_of(i).back);
+            if (blocks > 1) publish();
+            deal<NT>(
+                pages,
+                [&](uint32_t k) {
+                    const uint32_t j = last_at_most(s.back, k);
+                    return make_uint2(a.tables[uint64_t(i * NT + j) * a.max_pages + (k - s.back[j])], 0u);
+                },
+                [&](uint32_t k, uint2 x) { a.free_pages[count + done + k] = x.x; });
+            done += pages;
         }
+        __syncthreads();
     }
     uint32_t popped = 0, row = 0;
     for (uint32_t i = 0; i < blocks; ++i) {
-        const uint32_t b = i * kPlanThreads + tid;
-        p = PlanPart{};
-        len = 0;
-        if (b < a.requests) {
-            len = a.old_lens[b];
-            p = plan_part(len, a.new_lens[b], a.shift);
+        const PlanPart all = block_of(i);
+        if (blocks > 1) publish();
+        const uint32_t b = i * NT + tid, pages = uint32_t(all.take), rows = uint32_t(all.fresh);
+        deal<NT>(
+            pages, [&](uint32_t k) { return make_uint2(a.free_pages[top - 1u - popped - k], last_at_most(s.take, k)); },
+            [&](uint32_t k, uint2 x) {
+                a.tables[uint64_t(i * NT + x.y) * a.max_pages + pages_of(s.held[x.y], a.shift) + (k - s.take[x.y])] = x.x;
+            });
+        if (b < a.requests) {  // every read of old_lens is done: lens may be the same
+            a.lens[b] = fresh == ARC_PAGED_RELEASE ? 0u : len + fresh;
+            a.starts[b] = row + uint32_t(before.fresh);
         }
-        uint32_t total;
-        // block_exclusive's barriers come after every thread's reads above, so lens may be old_lens
-        first[tid] = block_exclusive(p.take, red, total);
-        held[tid] = len;
-        __syncthreads();
-        for (uint32_t k = tid; k < total; k += kPlanThreads) {
-            const uint32_t j = last_at_most(first, kPlanThreads, k);
-            a.tables[uint64_t(i * kPlanThreads + j) * a.max_pages + pages_of(held[j], a.shift) + (k - first[j])] =
-                a.free_pages[top - 1u - popped - k];
-        }
-        popped += total;
-        const uint32_t at = block_exclusive(p.fresh, red, total);
-        if (b < a.requests) {
-            a.lens[b] = p.back || a.new_lens[b] == ARC_PAGED_RELEASE ? 0u : len + p.fresh;
-            a.starts[b] = row + at;
-        }
-        if constexpr (ROWS) {
-            __syncthreads();  // the table entries above are written, `first` is read no more
-            first[tid] = at;
-            __syncthreads();
-            for (uint32_t k = tid; k < total; k += kPlanThreads) {
-                const uint32_t j = last_at_most(first, kPlanThreads, k);
-                plan_row(a, row + k, i * kPlanThreads + j, held[j] + (k - first[j]));
-            }
-        }
-        row += total;
-        __syncthreads();
+        if constexpr (ROWS)
+            deal<NT>(
+                rows,
+                [&](uint32_t k) {
+                    const uint32_t j = last_at_most(s.fresh, k), pos = s.held[j] + (k - s.fresh[j]);
+                    const uint32_t entry = pos >> a.shift, had = pages_of(s.held[j], a.shift);
+                    const uint32_t page = entry < had ? a.tables[uint64_t(i * NT + j) * a.max_pages + entry]
+                                                      : a.free_pages[top - 1u - popped - s.take[j] - (entry - had)];
+                    return make_uint2(page, pos);
+                },
+                [&](uint32_t k, uint2 x) {
+                    a.positions[row + k] = x.y;
+                    a.slots[row + k] = (x.x << a.shift) | (x.y & ((1u << a.shift) - 1u));
+                });
+        popped += pages;
+        row += rows;
     }
     if (tid == 0) {
         a.starts[a.requests] = row;
@@ -226,29 +253,46 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(PlanArgs a)
         a.status[3] = popped;
     }
     if constexpr (ROWS)
-        for (uint32_t n = row + tid; n < a.rows; n += kPlanThreads) {
+        for (uint32_t n = row + tid; n < a.rows; n += NT) {
             a.positions[n] = 0;
             a.slots[n] = ARC_NO_SLOT;
         }
 }
 
-// The rows of a large step, one per thread, from the starts and lengths that k_plan
-// left.
+// The rows of a large step, one per thread, from the starts, lengths and tables that k_plan left.  IN_LDS: all
+// starts, for the search.
+constexpr uint32_t kStartsInLds = 4096;
+template <bool IN_LDS>
 __global__ __launch_bounds__(256) void k_plan_rows(PlanArgs a)
 {
+    __shared__ uint32_t own[IN_LDS ? kStartsInLds : 1];
     const uint32_t n = blockIdx.x * 256 + threadIdx.x;
+    if constexpr (IN_LDS) {
+        for (uint32_t b = threadIdx.x; b <= a.requests; b += 256) own[b] = a.starts[b];
+        __syncthreads();
+    }
+    const uint32_t* starts = IN_LDS ? own : a.starts;
     if (n >= a.rows) return;
-    if (n >= a.starts[a.requests]) {
+    if (n >= starts[a.requests]) {
         a.positions[n] = 0;
         a.slots[n] = ARC_NO_SLOT;
         return;
     }
-    const uint32_t b = last_at_most(a.starts, a.requests, n);
-    plan_row(a, n, b, a.lens[b] - (a.starts[b + 1] - n));
+    const uint32_t b = last_at_most(starts, a.requests, n), pos = a.lens[b] - (starts[b + 1] - n);
+    a.positions[n] = pos;
+    a.slots[n] = (a.tables[uint64_t(b) * a.max_pages + (pos >> a.shift)] << a.shift) | (pos & ((1u << a.shift) - 1u));
 }
 
 // Rows that one workgroup writes itself; more go to a launch of their own.
 constexpr uint32_t kPlanRowsInOne = 4096;
+
+template <bool ROWS>
+void launch_plan(const PlanArgs& a, hipStream_t st)
+{
+    // a small step: 4 waves, whose barriers cost less than 16 waves'
+    if (a.requests <= 256 && a.rows <= 1024) hipLaunchKernelGGL((k_plan<256, ROWS>), dim3(1), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_plan<1024, ROWS>), dim3(1), dim3(1024), 0, st, a);
+}
 
 // -------------------------------------------------------------------- rope
 struct RopeArgs {
@@ -412,12 +456,14 @@ int arc_paged_plan(const arc_paged_batch* batch, const uint32_t* old_lens, const
     a.shift = log2_of(page_size);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a.rows <= kPlanRowsInOne) {
-        hipLaunchKernelGGL(k_plan<true>, dim3(1), dim3(kPlanThreads), 0, st, a);
+        launch_plan<true>(a, st);
         return check_hip(hipGetLastError(), "step plan");
     }
-    hipLaunchKernelGGL(k_plan<false>, dim3(1), dim3(kPlanThreads), 0, st, a);
+    launch_plan<false>(a, st);
     if ((rc = check_hip(hipGetLastError(), "step plan"))) return rc;
-    hipLaunchKernelGGL(k_plan_rows, dim3((a.rows + 255) / 256), dim3(256), 0, st, a);
+    const dim3 grid((a.rows + 255) / 256);
+    if (a.requests < kStartsInLds) hipLaunchKernelGGL(k_plan_rows<true>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_plan_rows<false>, grid, dim3(256), 0, st, a);
     return check_hip(hipGetLastError(), "step rows");
 }
 

@@ -17,6 +17,28 @@ using vec8 = T __attribute__((ext_vector_type(8)));
 template <typename T>
 using vec4 = T __attribute__((ext_vector_type(4)));
 
+// v of the lane that a DPP row operation names, 0 where that is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u)), CTRL, ROWS, 0xf, false));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), CTRL, ROWS, 0xf, false));
+    return __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
+}
+// Inclusive prefix sums over the wave: in each row of 16 lanes, then row 0's and 2's totals into rows 1
+// and 3, then the lower half's into the upper.
+__device__ __forceinline__ double wave_inclusive(double v)
+{
+    v += dpp_f64<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_f64<0x112, 0xf>(v);
+    v += dpp_f64<0x114, 0xf>(v);
+    v += dpp_f64<0x118, 0xf>(v);
+    v += dpp_f64<0x142, 0xa>(v);  // row_bcast 15
+    v += dpp_f64<0x143, 0xc>(v);  // row_bcast 31
+    return v;
+}
+
 inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 // Whether `rows` rows of `width` bytes, `stride` apart, at a and at b share memory:

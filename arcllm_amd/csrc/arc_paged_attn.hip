@@ -171,28 +171,6 @@ __device__ __forceinline__ double of_lane(double v, int lane)
     const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(u >> 32)), lane));
     return __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
 }
-// v of the lane that a DPP row operation names, 0 where that is none.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp_f64(double v)
-{
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u)), CTRL, ROWS, 0xf, false));
-    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), CTRL, ROWS, 0xf, false));
-    return __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
-}
-// Inclusive prefix sums over the wave: in each row of 16 lanes, then row 0's and 2's totals into rows 1
-// and 3, then the lower half's into the upper.
-__device__ __forceinline__ double wave_inclusive(double v)
-{
-    v += dpp_f64<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
-    v += dpp_f64<0x112, 0xf>(v);
-    v += dpp_f64<0x114, 0xf>(v);
-    v += dpp_f64<0x118, 0xf>(v);
-    v += dpp_f64<0x142, 0xa>(v);  // row_bcast 15
-    v += dpp_f64<0x143, 0xc>(v);  // row_bcast 31
-    return v;
-}
-
 // A workgroup's place in the line and the segment of it that it works on, in LDS:
 // wave 0 moves it on, the others read what they need, so that none of it is held in
 // registers while a segment is computed.
