@@ -306,15 +306,19 @@ struct RopeArgs {
     float scale;
 };
 
-// cos and sin of position * phase turns, times scale: the product modulo 2^64 is
-// the angle's fraction of a turn exactly; its upper 32 bits, as a signed number, are in
-// [-1/2, 1/2) and round to fp32 with an error of at most 2^-26 turns.
-__device__ __forceinline__ void turn_of(uint32_t pos, uint64_t phase, float scale, float& c, float& s)
+// The pair (x, y) turned by position * phase turns, times scale: the product modulo 2^64 is the angle's
+// fraction of a turn exactly; its upper 32 bits, as a signed number, are in [-1/2, 1/2) and round to
+// fp32 with an error of at most 2^-26 turns.
+__device__ __forceinline__ void rotate(uint32_t pos, uint64_t phase, float scale, float& x, float& y)
 {
     const float half_turns = float(int32_t((uint64_t(pos) * phase) >> 32)) * 0x1p-31f;
+    float s, c;
     sincospif(half_turns, &s, &c);
     c *= scale;
     s *= scale;
+    const float tx = x * c - y * s, ty = x * s + y * c;
+    x = tx;
+    y = ty;
 }
 
 template <typename X>
@@ -325,22 +329,22 @@ __device__ __forceinline__ void load4(const X* p, float* f)
     for (int i = 0; i < 4; ++i) f[i] = static_cast<float>(v[i]);
 }
 
-// One lane: 8 values of one head of one row, as two groups of 4 that are loaded,
-// rotated and stored together: 8 neighbours (4 pairs of the interleaved layout,
-// values that are not rotated), or i .. i + 3 and their partners i + rot/2 .. of the
-// half layout.  Every lane computes its own 4 angles: about 150 instructions
-// against 48 bytes moved, which the memory time of a large step covers, and a
-// small one waits for no barrier.  Bound by HBM: N (heads + 2 kv_heads) dim values
-// read and written once.
+// One lane: 8 values of one head of one row, as two groups of 4 that are loaded, rotated and stored together.
+// Half layout: i .. i + 3 and their partners i + rot / 2 ..; values that are not rotated, and
+// the interleaved layout, whose groups are 2 pairs each: a group of the head's first half and one of its
+// second (of what is left of them), so that neighbouring lanes load neighbouring 16 bytes.  Every lane computes
+// its own 4 angles: about 150 instructions against 48 bytes moved, which the memory time of a large
+// step covers, and a small one waits for no barrier.  Bound by HBM: N (heads + 2 kv_heads) dim
+// values read and written once.
 template <typename X, typename T>
 __device__ __forceinline__ void rope_unit(const RopeArgs& a, uint32_t n, uint32_t u, uint32_t slot, uint32_t pos)
 {
     const uint32_t per = a.dim / 8, head = u / per, e = u - head * per;
     const bool is_v = head >= a.heads + a.kv_heads;
     const uint32_t rot = is_v ? 0u : a.rot;
-    const bool turned = 8 * e < rot;
-    const bool halves = turned && a.half;
-    const uint32_t i0 = halves ? 4 * e : 8 * e, i1 = halves ? 4 * e + rot / 2 : 8 * e + 4;
+    const bool halves = a.half && 8 * e < rot;
+    const uint32_t skip = a.half && !halves ? rot : 0u;  // the half layout's rotated part, before the others
+    const uint32_t i0 = skip + 4 * (e - skip / 8), i1 = i0 + (halves ? rot : a.dim - skip) / 2;
 
     const X* src = static_cast<const X*>(a.x) + uint64_t(n) * a.ldx + head * a.dim;
     float lo[4], hi[4];
@@ -369,17 +373,17 @@ __device__ __forceinline__ void rope_unit(const RopeArgs& a, uint32_t n, uint32_
             hi[i] += b1[i];
         }
     }
-    if (turned) {
-        // pair i of the 4: (lo[i], hi[i]) of the half layout, neighbours of the interleaved one
+    if (halves) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float c, s;
-            turn_of(pos, a.phases[4 * e + i], a.scale, c, s);
-            float& x = halves ? lo[i] : (i < 2 ? lo[2 * i] : hi[2 * i - 4]);
-            float& y = halves ? hi[i] : (i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]);
-            const float tx = x * c - y * s, ty = x * s + y * c;
-            x = tx;
-            y = ty;
+        for (int i = 0; i < 4; ++i) rotate(pos, a.phases[i0 + i], a.scale, lo[i], hi[i]);
+    } else if (!a.half) {
+        if (i0 < rot) {
+            rotate(pos, a.phases[i0 / 2], a.scale, lo[0], lo[1]);
+            rotate(pos, a.phases[i0 / 2 + 1], a.scale, lo[2], lo[3]);
+        }
+        if (i1 < rot) {
+            rotate(pos, a.phases[i1 / 2], a.scale, hi[0], hi[1]);
+            rotate(pos, a.phases[i1 / 2 + 1], a.scale, hi[2], hi[3]);
         }
     }
     vec4<T> o0, o1;
