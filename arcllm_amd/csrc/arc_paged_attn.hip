@@ -108,7 +108,7 @@ __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, u
     if (s1 <= s0 || s0 >= a.rows) return r;
     const uint32_t rows = (min(s1, a.rows) - s0) * a.hpk;
     if (FEW ? rows > a.few_rows : rows <= a.few_rows) return r;
-    const uint64_t len = min(uint64_t(held), uint64_t(a.max_pages) << a.shift);
+    const uint64_t len = min(uint64_t(held), min(uint64_t(a.max_pages) << a.shift, uint64_t(0x7fffffffu)));
     const int64_t base = int64_t(len) - int64_t(s1 - s0);
     r.token = s0;
     r.rows = rows;
@@ -215,8 +215,9 @@ __device__ __forceinline__ uint32_t part_of(const Walk& l, double x)
     return w;
 }
 
-// This workgroup's part, from the total: parts of a unit (few rows: one for each wave) or more.  Workgroups go to the 8 XCDs
-// in turn: an XCD's workgroups take neighbouring parts, which read the same K and V.
+// This workgroup's part, from the total: parts of a unit (few rows: one for each wave) or more.
+// Workgroups go to the 8 XCDs in turn: an XCD's workgroups take neighbouring parts, which read the
+// same K and V.
 __device__ __forceinline__ void take_part(Walk& l, double total, float units)
 {
     l.total = total;
@@ -267,7 +268,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
         m.b = uint32_t(b);
         m.before = of_lane(inc - own, b);
         if (lane == 0) l = m;
-        if (lane < 2) (FEW ? a.few_p : a.many_p)[2 * m.w + lane].n = 0;
+        if (lane == 0) (FEW ? a.few_p : a.many_p)[2 * m.w].n = (FEW ? a.few_p : a.many_p)[2 * m.w + 1].n = 0;
         return;
     }
     const uint32_t each = (a.requests + NT - 1) / NT;
@@ -316,7 +317,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
         l.before = at;
     }
     __syncthreads();
-    if (tid < 2) (FEW ? a.few_p : a.many_p)[2 * m.w + tid].n = 0;
+    if (tid == 0) (FEW ? a.few_p : a.many_p)[2 * m.w].n = (FEW ? a.few_p : a.many_p)[2 * m.w + 1].n = 0;
 }
 
 // Wave 0: the part's next segment after l's.  A cut tile gets its slot and its record for k_paged_join.
@@ -328,11 +329,16 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, 
     Walk m = l;
     m.go = m.at < m.to;
     if (m.go) {
-        Request r;
-        for (;; ++m.b) {  // the request at m.at
+        Request r{};
+        for (; m.b < a.requests; ++m.b) {  // the request at m.at
             r = request_at<FEW, bm>(a, h, m.b);
             if (m.at < m.before + r.total * a.kv_heads) break;
             m.before += r.total * a.kv_heads;
+        }
+        if (m.b >= a.requests) {  // starts or lens changed during the call
+            m.go = 0;
+            if (threadIdx.x == 0) to = m;
+            return;
         }
         const double off = m.at - m.before;
         m.g = min(a.kv_heads - 1, uint32_t(near_ratio(off, r.total)));
@@ -439,7 +445,8 @@ __device__ __forceinline__ uint32_t v_swizzle(uint32_t r)
 // 16 bytes per lane from memory straight into LDS, lane i's at lds + 16 i: from base (scalar) + off bytes, or
 // from the lane's own address.  In assembly because the compiler waits for such a copy before
 // the next read of LDS, whichever buffer that is from; there is no register for a load in
-// flight to write, and nothing else here uses m0.  wait_loads and a barrier (a wave's own rows: wait_loads) come before the rows are read.
+// flight to write, and nothing else here uses m0.  wait_loads and a barrier (a wave's own rows: wait_loads)
+// come before the rows are read.
 // ONCE: data that no other workgroup reads goes past the caches' keeping (nt): 2 contexts of 131071, 8 kv
 // heads (727 MB) 139 -> 121 us.
 template <bool ONCE>
@@ -459,8 +466,8 @@ __device__ __forceinline__ void copy16(uint32_t lds, const void* from)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
 }
 
-// N positions' rows of K and V, or one of them, from the pages straight into LDS, row i at kl, vl + i * D.  `page`: lane
-// first + i holds the page of row i's position pos0 + i.  Which 16 bytes a lane copies carries the swizzle, as
+// N positions' rows of K and V, or one of them, from the pages straight into LDS, row i at kl, vl + i * D.
+// `page`: lane first + i holds the page of row i's position pos0 + i.  Which 16 bytes a lane copies carries the swizzle, as
 // LDS is written in lane order.  WIDE, pages of 16 and more: 16 aligned rows have one
 // page, so the address is scalar and the lane's part of it the same for every unit.
 template <bool K, bool V, bool ONCE, int N, bool WIDE, int D, typename T>
@@ -690,7 +697,7 @@ __device__ __forceinline__ void add_nonfinite(const Pool<T>& p, f32x16 (&o)[D / 
     for (uint32_t u = from; u < s.u1; u += step) {
         const int32_t k0 = int32_t(first_of(u));
         const uint32_t page = page_of(u);
-        if (all_seen(p, s.x, k0, span, true)) continue;
+        if (all_seen(p, s.x, k0, span, __ballot(page < p.num_pages) == ~uint64_t(0))) continue;  // lanes beyond span repeat
 #pragma unroll 1
         for (uint32_t j = 0; j < span; ++j) {
             const uint32_t pg = uint32_t(__builtin_amdgcn_readlane(int(page), int(j)));
@@ -726,11 +733,19 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 {
-    __shared__ double red[8];
-    __shared__ Walk walk[2];  // this segment and the next
-    __shared__ Heads heads;
-    __shared__ __align__(16) float joined[4 * 32 * D];  // K and V rows of each wave, then the waves' outputs
-    __shared__ float mw[4][32], lw[4][32];
+    __shared__ struct {  // rows first: m0, which says where a copy goes, is used below 2^16 only
+        __align__(16) float joined[4 * 32 * D];  // K and V rows of each wave, then the waves' outputs
+        float mw[4][32], lw[4][32];
+        double red[8];
+        Walk walk[2];  // this segment and the next
+        Heads heads;
+    } lds;
+    static_assert(sizeof(lds.joined) <= 65536, "rows below 2^16");
+    auto& joined = lds.joined;
+    auto &mw = lds.mw, &lw = lds.lw;
+    auto& walk = lds.walk;
+    Heads& heads = lds.heads;
+    double* red = lds.red;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
     start_walk<true, kFewRows, 256>(arguments(), walk[1], heads, red);
     next_segment<true, kFewRows>(arguments(), walk[1], walk[0], heads);
@@ -877,12 +892,20 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 {
     constexpr int NT = NW * 64;
     constexpr uint32_t kBm = NW * 32, kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
-    __shared__ __align__(16) T ks[2][kManyKeys * D];
-    __shared__ __align__(16) T vs[2][kManyKeys * D];
-    __shared__ double red[2 * NW];
-    __shared__ Walk walk[2];  // this segment and the next
-    __shared__ Heads heads;
-    __shared__ uint32_t odd;  // infinities or NaN cleared from V in this segment
+    __shared__ struct {  // rows first: m0, which says where a copy goes, is used below 2^16 only
+        __align__(16) T ks[2][kManyKeys * D];
+        __align__(16) T vs[2][kManyKeys * D];
+        double red[2 * NW];
+        Walk walk[2];  // this segment and the next
+        Heads heads;
+        uint32_t odd;  // infinities or NaN cleared from V in this segment
+    } lds;
+    static_assert(sizeof(lds.ks) + sizeof(lds.vs) <= 65536, "rows below 2^16");
+    auto &ks = lds.ks, &vs = lds.vs;
+    auto& walk = lds.walk;
+    Heads& heads = lds.heads;
+    double* red = lds.red;
+    uint32_t& odd = lds.odd;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
     start_walk<false, kBm, NT>(arguments(), walk[1], heads, red);
     next_segment<false, kBm>(arguments(), walk[1], walk[0], heads);
@@ -1220,7 +1243,7 @@ int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch,
     // the line's costs (positions times hpk, over tiles and kv heads) stay below 2^52: times 1024 parts and
     // as doubles they are exact
     const unsigned __int128 most = (unsigned __int128)(uint64_t(batch->tokens) * hpk / kFewRows + batch->requests) *
-                                   pages->kv_heads * hpk * (uint64_t(batch->max_pages) * pages->page_size + 1024);
+                                   pages->kv_heads * hpk * (uint64_t(batch->max_pages) * pages->page_size + batch->tokens + 1024);
     if (most >> 52) return set_error(ARC_ERR_UNSUPPORTED, "tokens, heads and max_pages: more work than one call takes");
     if (batch->tokens == 0 || batch->requests == 0) return ARC_OK;
     const Space sp = space_of(pages->head_dim, hpk, batch->tokens);
