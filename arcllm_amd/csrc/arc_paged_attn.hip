@@ -38,8 +38,11 @@ constexpr uint32_t kFewWgs = 512;      // most parts of the line
 // cores' power holds down).  Heads of 64 leave registers for 3 workgroups of 4 waves.
 constexpr int many_waves(uint32_t dim) { return dim == 128 ? 8 : 4; }
 constexpr uint32_t many_wgs(uint32_t dim) { return dim == 128 ? 256 : 768; }
-constexpr uint32_t kTileKeys = 64;     // a tile's start and end cost about this many positions
+// A tile's start and end, in positions: few rows 2.5 us, where a part's 128 take 4.6; many rows (bm of them) 7 us
+// (pages, first copy, stores), where 64 take 1.9 and, with 4 waves, other workgroups of the CU have the time.
+constexpr uint32_t tile_ends(bool few, uint32_t bm) { return few ? 64 : bm; }
 constexpr float kLazy = 8.0f;          // see rescale
+constexpr uint32_t kManyPieces = 8;    // a tile in more pieces is joined in another way
 
 // What a part of a tile left in the workspace, one per slot; two slots per
 // workgroup (its part may end one tile and begin another).
@@ -103,7 +106,7 @@ __device__ __forceinline__ double cost_before(const Request& r, uint32_t t, doub
 template <bool FEW, uint32_t bm>
 __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, uint32_t s1, uint32_t held)
 {
-    constexpr uint32_t keys = FEW ? kFewKeys : kManyKeys;
+    constexpr uint32_t keys = FEW ? kFewKeys : kManyKeys, ends = tile_ends(FEW, bm);
     Request r{};
     if (s1 <= s0 || s0 >= a.rows) return r;
     const uint32_t rows = (min(s1, a.rows) - s0) * a.hpk;
@@ -114,8 +117,8 @@ __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, u
     r.rows = rows;
     r.base = int32_t(max(base, -(int64_t(1) << 25)));
     r.tiles = (rows + bm - 1) / bm;
-    r.first = double(kTileKeys + uint32_t(max(r.base, 0))) * a.hpk + bm;
-    r.cap = a.window ? (double(kTileKeys) + a.window + a.sinks) * a.hpk + 2 * bm : 0x1p60;
+    r.first = double(ends + uint32_t(max(r.base, 0))) * a.hpk + bm;
+    r.cap = a.window ? (double(ends) + a.window + a.sinks) * a.hpk + 2 * bm : 0x1p60;
     r.total = r.tiles == 1 ? fmin(r.first, r.cap) : cost_before(r, r.tiles, bm);
     const float spans = float(r.tiles) * ceilf(float(len) * (1.0f / keys));
     r.units = a.window ? fminf(spans, float(r.tiles) * (ceilf((float(a.window) + float(a.sinks)) * (1.0f / keys)) + 2.0f)) : spans;
@@ -181,7 +184,8 @@ struct Walk {
     uint32_t parts, w, b;
     // the segment: units [u0, u1) of a tile
     uint32_t go;           // 0: the part is done
-    uint32_t g, u0, u1, token, complete, slot;
+    uint32_t g, u0, u1, token, slot;
+    uint32_t pieces;       // of the tile, 0: the segment is all of it
     int32_t base;
     Tile x;
 };
@@ -362,13 +366,14 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, 
         m.u1 = units_before(m.to, begin, end, m.x.units);
         m.token = r.token;
         m.base = r.base;
-        m.complete = m.at <= begin && end <= m.to;
-        if (!m.complete) {
+        m.pieces = 0;
+        if (m.at > begin || end > m.to) {
             const uint32_t w0 = part_of(m, begin), w1 = part_of(m, end - 1.0);
             const uint32_t first = 2 * w0 + (part_at(m, w0) < begin ? 1u : 0u);
             m.slot = m.w == w0 ? first : 2 * m.w;
+            m.pieces = w1 - w0 + 1;
             if (threadIdx.x == 0)
-                (FEW ? a.few_p : a.many_p)[m.slot] = Piece{w1 - w0 + 1, m.w - w0, w0, first, r.token, m.x.row0, m.x.rows, m.g};
+                (FEW ? a.few_p : a.many_p)[m.slot] = Piece{m.pieces, m.w - w0, w0, first, r.token, m.x.row0, m.x.rows, m.g};
         }
         m.at = fmin(end, m.to);
     }
@@ -377,7 +382,7 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, 
 
 // What every wave needs of the segment, in scalar registers.
 struct Segment {
-    uint32_t b, g, u0, u1, token, complete, slot;
+    uint32_t b, g, u0, u1, token, slot, pieces;
     int32_t base;
     Tile x;
 };
@@ -389,8 +394,8 @@ __device__ __forceinline__ Segment read_segment(const Walk& l)
     s.u0 = uniform(l.u0);
     s.u1 = uniform(l.u1);
     s.token = uniform(l.token);
-    s.complete = uniform(l.complete);
     s.slot = uniform(l.slot);
+    s.pieces = uniform(l.pieces);
     s.base = uniform(l.base);
     s.x.row0 = uniform(l.x.row0);
     s.x.rows = uniform(l.x.rows);
@@ -623,6 +628,13 @@ __device__ __forceinline__ void rescale(float mx, float& m, float& l, f32x16 (&o
 
 // Value i of a score or output tile of 32: key, or dim, 8 (i / 4) + 4 (lane / 32) + i % 4.
 __device__ __forceinline__ uint32_t tile_index(int i) { return 8u * (i >> 2) + 4u * ((threadIdx.x >> 5) & 1u) + (i & 3); }
+
+// Where a slot holds 4 values of a row from dim d on.  Row by row, or, in blocks: 32 rows' same 8 dims side by
+// side, as a wave of the many-rows kernel has them, so that its stores cover whole lines.
+__device__ __forceinline__ uint32_t piece_place(bool blocks, uint32_t row, uint32_t dim, uint32_t d)
+{
+    return blocks ? (row & ~31u) * dim + (d & ~7u) * 32 + (row & 31u) * 8 + (d & 7u) : row * dim + d;
+}
 
 // Query operand of 32 rows: lane -> row lane & 31, dims 16 s + 8 (lane / 32) .. + 7; zeros for
 // rows that the tile does not have.
@@ -870,7 +882,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 acc.z = __builtin_fmaf(w.z, f, acc.z);
                 acc.w = __builtin_fmaf(w.w, f, acc.w);
             }
-            if (s.complete) {
+            if (s.pieces == 0) {
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // nothing seen: zeros
                 store4<T>(out_row<T>(e_, s.token, s.x.row0 + rr, s.g, D) + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             } else {
@@ -1034,7 +1046,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
         const float L = xor_sum<32>(l);
         const PagedAttn& e_ = arguments();
         if (trow < s.x.rows) {
-            if (s.complete) {
+            if (s.pieces == 0) {
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
                 T* dst = out_row<T>(e_, s.token, s.x.row0 + trow, s.g, D);
 #pragma unroll
@@ -1044,12 +1056,13 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                         store4<T>(dst + 32 * t + tile_index(i), o[t][i] * inv, o[t][i + 1] * inv, o[t][i + 2] * inv,
                                   o[t][i + 3] * inv);
             } else {
-                float* dst = e_.many_o + (uint64_t(s.slot) * e_.many_slot + trow) * D;
+                float* dst = e_.many_o + uint64_t(s.slot) * e_.many_slot * D;
+                const bool blocks = s.pieces <= kManyPieces;
 #pragma unroll
                 for (int t = 0; t < D / 32; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<float4*>(dst + 32 * t + tile_index(i)) =
+                        *reinterpret_cast<float4*>(dst + piece_place(blocks, trow, D, 32 * t + tile_index(i))) =
                             make_float4(o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]);
                 if (h2 == 0) e_.many_ml[uint64_t(s.slot) * e_.many_slot + trow] = make_float2(m, L);
             }
@@ -1064,7 +1077,6 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 // pieces (long rows of tiles cut once or twice): 256 / (D / 4) rows at once, each by its lanes
 // alone; many (one long context): a row at a time, its pieces dealt out over the groups of lanes.
 constexpr uint32_t kManySplit = 4;
-constexpr uint32_t kManyPieces = 8;
 
 struct JoinRow {
     float L;
@@ -1099,8 +1111,15 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
     const float* po = is_few ? a.few_o : a.many_o;
     const float2* pml = is_few ? a.few_ml : a.many_ml;
     const uint32_t srows = is_few ? a.few_slot : a.many_slot;
-    const uint32_t tid = threadIdx.x, grp = tid / kLanes, d = tid % kLanes;
-    auto at = [&](uint32_t i, uint32_t row) { return uint64_t(i ? 2 * (p.wg + i) : p.slot) * srows + row; };
+    const uint32_t tid = threadIdx.x;
+    const bool blocks = !is_few && p.n <= kManyPieces;
+    const uint32_t grp = blocks ? (tid >> 1) % kGroups : tid / kLanes;  // its row of kGroups
+    const uint32_t d = 4 * (blocks ? 2 * (tid / (2 * kGroups)) + (tid & 1u) : tid % kLanes);
+    auto slot = [&](uint32_t i) { return uint64_t(i ? 2 * (p.wg + i) : p.slot) * srows; };
+    auto ml_at = [&](uint32_t i, uint32_t row) { return pml[slot(i) + row]; };
+    auto o_at = [&](uint32_t i, uint32_t row) {
+        return *reinterpret_cast<const float4*>(po + slot(i) * D + piece_place(blocks, row, D, d));
+    };
     const uint32_t turn = p.idx * split + blockIdx.y, turns = p.n * split;
     if (p.n <= kManyPieces) {
         for (uint32_t row = turn * kGroups + grp; row < p.rows; row += turns * kGroups) {
@@ -1109,8 +1128,8 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
 #pragma unroll
             for (uint32_t i = 0; i < kManyPieces; ++i)  // all of them on their way at once
                 if (i < p.n) {
-                    ml[i] = pml[at(i, row)];
-                    o[i] = *reinterpret_cast<const float4*>(po + at(i, row) * D + 4 * d);
+                    ml[i] = ml_at(i, row);
+                    o[i] = o_at(i, row);
                 }
             float M = -INFINITY;
 #pragma unroll
@@ -1121,14 +1140,14 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
 #pragma unroll
             for (uint32_t i = 0; i < kManyPieces; ++i)
                 if (i < p.n) add_piece(r, __builtin_amdgcn_exp2f(ml[i].x - M0), ml[i].y, o[i]);
-            store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, r);
+            store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + d, r);
         }
         return;
     }
     for (uint32_t row = turn; row < p.rows; row += turns) {
         float M = -INFINITY;
 #pragma unroll 4
-        for (uint32_t i = grp; i < p.n; i += kGroups) M = fmaxf(M, pml[at(i, row)].x);
+        for (uint32_t i = grp; i < p.n; i += kGroups) M = fmaxf(M, ml_at(i, row).x);
         __syncthreads();  // the row before is done with part and part_l
         if (d == 0) part_l[grp] = M;
         __syncthreads();
@@ -1138,18 +1157,18 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
         JoinRow r{0.0f, make_float4(0, 0, 0, 0)};
 #pragma unroll 4
         for (uint32_t i = grp; i < p.n; i += kGroups) {
-            const float2 ml = pml[at(i, row)];
-            add_piece(r, __builtin_amdgcn_exp2f(ml.x - M0), ml.y, *reinterpret_cast<const float4*>(po + at(i, row) * D + 4 * d));
+            const float2 ml = ml_at(i, row);
+            add_piece(r, __builtin_amdgcn_exp2f(ml.x - M0), ml.y, o_at(i, row));
         }
         __syncthreads();  // part_l is read
-        part[grp][d] = r.acc;
+        part[grp][d / 4] = r.acc;
         if (d == 0) part_l[grp] = r.L;
         __syncthreads();
         if (grp == 0) {
             r = JoinRow{0.0f, make_float4(0, 0, 0, 0)};
 #pragma unroll
-            for (uint32_t j = 0; j < kGroups; ++j) add_piece(r, 1.0f, part_l[j], part[j][d]);
-            store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + 4 * d, r);
+            for (uint32_t j = 0; j < kGroups; ++j) add_piece(r, 1.0f, part_l[j], part[j][d / 4]);
+            store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + d, r);
         }
     }
 }
@@ -1168,7 +1187,7 @@ Space space_of(uint32_t dim, uint32_t hpk, uint32_t tokens)
     Space s{};
     s.few_slot = uint32_t(rows < kFewRows ? rows : kFewRows);
     const uint32_t bm = 32u * uint32_t(many_waves(dim)), wgs = many_wgs(dim);
-    s.many_slot = uint32_t(rows <= kFewRows ? 0 : rows < bm ? rows : bm);
+    s.many_slot = uint32_t(rows <= kFewRows ? 0 : rows < bm ? (rows + 31) / 32 * 32 : bm);  // see piece_place
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
