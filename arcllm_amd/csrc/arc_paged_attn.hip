@@ -36,7 +36,7 @@ constexpr uint32_t kFewWgs = 512;      // most parts of the line
 // share each unit's copy, where two workgroups of 4 copied it twice: a chunk of 4096 tokens at 12288, 28 heads,
 // 880 instead of 950 us (and 1.55 instead of 1.88 million cycles: the rest is the clock, which the matrix
 // cores' power holds down).  Heads of 64 leave registers for 3 workgroups of 4 waves.
-constexpr int many_waves(uint32_t dim) { return dim == 128 ? 8 : 4; }
+constexpr int many_waves(uint32_t dim) { return dim == 128 ? 8 : 2; }
 constexpr uint32_t many_wgs(uint32_t dim) { return dim == 128 ? 256 : 768; }
 // A tile's start and end, in positions: few rows 2.5 us, where a part's 128 take 4.6; many rows (bm of them) 7 us
 // (pages, first copy, stores), where 64 take 1.9 and, with 4 waves, other workgroups of the CU have the time.
@@ -1072,11 +1072,14 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 
 // ---------------------------------------------------------------------- join
 // Adds the pieces of the tiles that were cut, in order: out = sum_i 2^(m_i - M) o_i /
-// sum_i 2^(m_i - M) l_i.  A workgroup for each slot (kManySplit of them where tiles have many
+// sum_i 2^(m_i - M) l_i.  A workgroup for each slot (many_split of them where tiles have many
 // rows); the workgroups of a tile's n pieces share its rows.  D / 4 lanes span a row; few
 // pieces (long rows of tiles cut once or twice): 256 / (D / 4) rows at once, each by its lanes
 // alone; many (one long context): a row at a time, its pieces dealt out over the groups of lanes.
-constexpr uint32_t kManySplit = 4;
+// What bounds it is the way to memory and back: the record, the sums, all of a row's pieces at once, and as few
+// turns after that as the card has workgroups for.  Heads of 128, a chunk of 500 at 2500: 42.4 us the call with 8
+// workgroups a slot, 45.3 with 4, 42.7 with 16; of 64, three chunks of 700: 52 with 2 or 4, 58 with 8.
+constexpr uint32_t many_split(uint32_t dim) { return dim == 128 ? 8 : 2; }
 
 struct JoinRow {
     float L;
@@ -1100,14 +1103,14 @@ __device__ __forceinline__ void store_row(T* p, const JoinRow& r)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
 {
-    constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes;
+    constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes, kSplit = many_split(D);
     __shared__ __align__(16) float4 part[kGroups][kLanes];
     __shared__ float part_l[kGroups];
     const bool is_few = blockIdx.x < 2 * a.few_wgs;
-    if (is_few && blockIdx.y) return;
-    const Piece p = is_few ? a.few_p[blockIdx.x] : a.many_p[blockIdx.x - 2 * a.few_wgs];
+    const uint32_t many = blockIdx.x - 2 * a.few_wgs;
+    const Piece p = is_few ? a.few_p[blockIdx.x] : a.many_p[many / kSplit];
     if (p.n == 0) return;
-    const uint32_t split = is_few ? 1 : kManySplit;
+    const uint32_t split = is_few ? 1 : kSplit, part_of_slot = is_few ? 0 : many % kSplit;
     const float* po = is_few ? a.few_o : a.many_o;
     const float2* pml = is_few ? a.few_ml : a.many_ml;
     const uint32_t srows = is_few ? a.few_slot : a.many_slot;
@@ -1120,7 +1123,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
     auto o_at = [&](uint32_t i, uint32_t row) {
         return *reinterpret_cast<const float4*>(po + slot(i) * D + piece_place(blocks, row, D, d));
     };
-    const uint32_t turn = p.idx * split + blockIdx.y, turns = p.n * split;
+    const uint32_t turn = p.idx * split + part_of_slot, turns = p.n * split;
     if (p.n <= kManyPieces) {
         for (uint32_t row = turn * kGroups + grp; row < p.rows; row += turns * kGroups) {
             float2 ml[kManyPieces];
@@ -1218,7 +1221,7 @@ hipError_t launch_paged(const PagedAttn& a, hipStream_t st)
     if (a.shift >= 4) launch_tiles<T, D, true>(a, st);
     else launch_tiles<T, D, false>(a, st);
     if (hipError_t e = hipGetLastError()) return e;
-    hipLaunchKernelGGL((k_paged_join<T, D>), dim3(2 * (a.few_wgs + a.many_wgs), a.many_wgs ? kManySplit : 1), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_paged_join<T, D>), dim3(2 * (a.few_wgs + many_split(D) * a.many_wgs)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
