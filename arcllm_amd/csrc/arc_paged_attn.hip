@@ -24,8 +24,6 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-template <typename T>
-using vec2 = T __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kFewRows = 32;      // rows of a few-rows tile
 constexpr uint32_t kFewKeys = 32;      // positions of its unit, one wave's
@@ -333,16 +331,22 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, 
     Walk m = l;
     m.go = m.at < m.to;
     if (m.go) {
-        Request r{};
-        for (; m.b < a.requests; ++m.b) {  // the request at m.at
-            r = request_at<FEW, bm>(a, h, m.b);
-            if (m.at < m.before + r.total * a.kv_heads) break;
+        Request r = request_at<FEW, bm>(a, h, m.b);  // the request at m.at: this one, or one of those behind it
+        while (m.at >= m.before + r.total * a.kv_heads) {
             m.before += r.total * a.kv_heads;
-        }
-        if (m.b >= a.requests) {  // starts or lens changed during the call
-            m.go = 0;
-            if (threadIdx.x == 0) to = m;
-            return;
+            const uint32_t next = ++m.b + threadIdx.x;
+            if (next < a.requests) r = request_at<FEW, bm>(a, h, next);
+            const double own = next < a.requests ? r.total * a.kv_heads : 0.0, inc = wave_inclusive(own);
+            const uint64_t behind = __ballot(m.before + inc > m.at);
+            if (behind == 0 && m.b + 64 >= a.requests) {  // starts or lens changed during the call
+                m.go = 0;
+                if (threadIdx.x == 0) to = m;
+                return;
+            }
+            const int i = behind ? __builtin_ctzll(behind) : 63;
+            m.b += uint32_t(i);
+            m.before += of_lane(inc - own, i);
+            r = request_at<FEW, bm>(a, h, m.b);
         }
         const double off = m.at - m.before;
         m.g = min(a.kv_heads - 1, uint32_t(near_ratio(off, r.total)));
