@@ -34,7 +34,7 @@ constexpr uint32_t kFewWgs = 512;      // most parts of the line
 // share each unit's copy, where two workgroups of 4 copied it twice: a chunk of 4096 tokens at 12288, 28 heads,
 // 880 instead of 950 us (and 1.55 instead of 1.88 million cycles: the rest is the clock, which the matrix
 // cores' power holds down).  Heads of 64 leave registers for 3 workgroups of 4 waves.
-constexpr int many_waves(uint32_t dim) { return dim == 128 ? 8 : 2; }
+constexpr int many_waves(uint32_t dim) { return dim == 128 ? 8 : 4; }
 constexpr uint32_t many_wgs(uint32_t dim) { return dim == 128 ? 256 : 768; }
 // A tile's start and end, in positions: few rows 2.5 us, where a part's 128 take 4.6; many rows (bm of them) 7 us
 // (pages, first copy, stores), where 64 take 1.9 and, with 4 waves, other workgroups of the CU have the time.
