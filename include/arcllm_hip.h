@@ -296,7 +296,9 @@ typedef struct arc_kv_pages {
  * them) .. lens[b] - 1; position p of it is in page tables[b][p / page_size].  A
  * step may have more rows (`tokens`) than the requests use: rows from
  * starts[requests] on belong to no request and no call writes their outputs.
- * max_pages * page_size <= 2^31. */
+ * max_pages * page_size <= 2^31; attention takes a len beyond that, or beyond
+ * 2^31 - 1, as that.  A captured call keeps the numbers here and reads the arrays
+ * at each replay. */
 typedef struct arc_paged_batch {
     uint32_t requests;  /* <= 2^20 */
     uint32_t tokens;    /* rows of the step, used or not, <= 2^24 */
@@ -311,7 +313,7 @@ typedef struct arc_paged_batch {
 
 /* status[0] of arc_paged_plan: 0, or why the step was refused. */
 #define ARC_PLAN_NO_PAGES 1   /* fewer free pages than the step needs: status[1] more are needed */
-#define ARC_PLAN_TABLE 2      /* a request would pass max_pages (or 2^31 - 1 positions) */
+#define ARC_PLAN_TABLE 2      /* a request would pass max_pages, or 2^31 - 1 positions */
 #define ARC_PLAN_TOKENS 4     /* more new tokens than rows */
 #define ARC_PLAN_MAX_NEW 8    /* a request has more new tokens than max_new */
 #define ARC_PLAN_FREE_LIST 16 /* the free list would hold more than num_pages pages */
@@ -376,8 +378,8 @@ typedef struct arc_rope {
  * past the pool) are skipped: nothing of theirs is written.  Slots of one step
  * are distinct (two rows with one slot leave either's values there).  Biases:
  * fp32, 16-byte aligned, or NULL.  q: ldq elements from row to row (a multiple of
- * 8), 16-byte aligned, not sharing memory with x.  Of the batch, tokens,
- * positions and slots are used. */
+ * 8), 16-byte aligned, not sharing memory with x (nor x and q with the pages:
+ * not checked).  Of the batch, tokens, positions and slots are used. */
 int arc_rope_append(const arc_kv_pages *pages, const arc_paged_batch *batch, const arc_rope *rope, int x_dtype,
                     const void *x, uint32_t ldx, const float *q_bias, const float *k_bias, const float *v_bias,
                     uint32_t hpk, void *q, uint32_t ldq, arc_stream_t stream);
@@ -392,14 +394,18 @@ size_t arc_paged_attention_workspace_bytes(const arc_kv_pages *pages, const arc_
  *   out[n][h] = sum_j softmax_j(scale * q[n][h] . k_j) v_j
  * q and out: pages->dtype, kv_heads * hpk heads of head_dim per row, ldq and ldo
  * elements from row to row (multiples of 8), 16-byte aligned, sharing no memory
- * with each other or the pages.  hpk 1..64; scale 0 means 1 / sqrt(head_dim).
+ * with each other (refused) or the pages (not checked).  hpk 1..64; scale 0 means
+ * 1 / sqrt(head_dim).
  * Scores, softmax and sums are fp32; weights enter the V product rounded to
  * pages->dtype.  A position whose table entry is not below num_pages is not
- * seen, and a row that sees nothing is 0; what lies in the pages at positions not seen
- * (infinities, NaN) does not matter.  Rows behind the last request are left as they
+ * seen, and a row that sees nothing, or whose scores are all -infinity, is 0; what lies in
+ * the pages at positions not seen (infinities, NaN) does not matter.  Rows behind the last request are left as they
  * were.  workspace: arc_paged_attention_workspace_bytes() bytes, 256-byte aligned,
- * any contents, for one call at a time (calls in order on one stream may share it).
- * Of the batch, all but positions and slots is used. */
+ * any contents, for one call at a time (calls in order on one stream may share it; two
+ * graphs that may run at once, or two streams, need one each).  Of the batch, all but
+ * positions and slots is used; max_new decides speed only.  Refused
+ * (ARC_ERR_UNSUPPORTED): (tokens * hpk / 32 + requests) * kv_heads * hpk * (max_pages *
+ * page_size + tokens + 1024) >= 2^52. */
 int arc_paged_attention(const arc_kv_pages *pages, const arc_paged_batch *batch, const void *q, uint32_t ldq,
                         uint32_t hpk, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
                         void *workspace, arc_stream_t stream);

@@ -66,6 +66,18 @@ def test_attention_refusals(call):
     refused(call)
 
 
+def test_attention_refuses_more_work_than_its_costs_can_hold():
+    # (tokens * hpk / 32 + requests) * kv_heads * hpk * (max_pages * page_size + tokens + 1024) < 2^52, also where
+    # there is nothing to do, so that the sizes alone decide
+    p = pages(kv_heads=256, head_dim=128, page_size=16, page_stride=16 * 256 * 128)
+    width = 256 * 64 * 128
+    def of(requests, max_pages):
+        attention(p, batch(requests=requests, tokens=0, max_pages=max_pages), ldq=width, ldo=width, hpk=64)
+    of(128, (1 << 27) - 65)  # 2^7 * 2^14 * (2^31 - 16)
+    refused(lambda: of(128, (1 << 27) - 64))  # 2^52
+    refused(lambda: of(1 << 20, 1 << 27))
+
+
 def test_attention_of_nothing_is_done():
     attention(b=batch(tokens=0))
     attention(b=batch(requests=0))
