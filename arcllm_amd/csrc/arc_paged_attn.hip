@@ -188,8 +188,7 @@ struct Walk {
     Tile x;
 };
 
-// Boundary of part w, the same number wherever it is computed; steps are at least 1, so no
-// part is empty.
+// Boundary of part w, the same number wherever it is computed; a part has a unit's cost or more, so none is empty.
 __device__ __forceinline__ double part_at(const Walk& l, uint32_t w)
 {
     return w >= l.parts ? l.total : floor(l.step * double(w));
@@ -208,13 +207,15 @@ __device__ __forceinline__ uint32_t units_before(double x, double begin, double 
     return min(units, uint32_t((x - begin) * double(near_ratio(units, end - begin)) + 0x1p-8));
 }
 
-// The part in which x lies.
-__device__ __forceinline__ uint32_t part_of(const Walk& l, double x)
+// The part in which x lies, of the lower lanes' x and of the upper lanes', by the whole wave: near_ratio is off by
+// one at most and the boundaries' rounding adds another, so 8 candidates hold it.
+__device__ __forceinline__ void parts_of(const Walk& l, double x, uint32_t& lower, uint32_t& upper)
 {
-    uint32_t w = min(l.parts - 1, uint32_t(near_ratio(x, l.step)));
-    while (w && part_at(l, w) > x) --w;
-    while (w + 1 < l.parts && part_at(l, w + 1) <= x) ++w;
-    return w;
+    const int32_t w0 = int32_t(min(l.parts - 1, uint32_t(near_ratio(x, l.step)))) - 4;
+    const int32_t w = w0 + int32_t(threadIdx.x & 7u);
+    const uint64_t from = __ballot(w <= 0 || (uint32_t(w) < l.parts && floor(l.step * double(w)) <= x));
+    lower = uint32_t(__builtin_amdgcn_readlane(w0, 0) + __builtin_popcount(uint32_t(from) & 255u) - 1);
+    upper = uint32_t(__builtin_amdgcn_readlane(w0, 32) + __builtin_popcount(uint32_t(from >> 32) & 255u) - 1);
 }
 
 // This workgroup's part, from the total: parts of a unit (few rows: one for each wave) or more.
@@ -224,7 +225,7 @@ __device__ __forceinline__ void take_part(Walk& l, double total, float units)
 {
     l.total = total;
     l.parts = total > 0.0 ? min(uint32_t(gridDim.x), uint32_t(fminf(fmaxf(units, 1.0f), 65536.0f))) : 0u;
-    l.step = total / double(max(l.parts, 1u));
+    l.step = total * double(__builtin_amdgcn_rcpf(float(max(l.parts, 1u))));  // the last part has what that leaves
     l.w = blockIdx.x;
     l.at = l.to = 0.0;
     if (l.w >= l.parts) return;
@@ -245,11 +246,88 @@ __device__ __forceinline__ Request request_at(const PagedAttn& a, const Heads& h
     return request_of<FEW, bm>(a, a.starts[b], a.starts[b + 1], a.lens[b]);
 }
 
+// Wave 0: the segment of request r, b of the step, that lies at m.at, and the part's way on.  A cut tile gets its slot
+// and its record for k_paged_join.  One wave's work that all others wait for, a chain of dependent steps: so
+// searches are by 64 lanes at once, and what is needed twice (of a tile's ends, a part's ends) is computed in the lower
+// and the upper lanes.
+template <bool FEW, uint32_t bm>
+__device__ __forceinline__ void cut_segment(const PagedAttn& a, Walk& m, const Request& r)
+{
+    constexpr uint32_t keys = FEW ? kFewKeys : kManyKeys;
+    const uint32_t lane = threadIdx.x & 63u;
+    const bool upper = lane >= 32;
+    const double off = m.at - m.before;
+    const int32_t g0 = int32_t(min(a.kv_heads - 1, uint32_t(near_ratio(off, r.total)))) - 2, gl = g0 + int32_t(lane & 3u);
+    m.g = uint32_t(uniform(g0) + __builtin_popcount(uint32_t(__ballot(gl <= 0 || (uint32_t(gl) < a.kv_heads && gl * r.total <= off))) & 15u) - 1);
+    const double start = m.before + m.g * r.total, in = m.at - start;
+    uint32_t t = 0;
+    double begin = start, end = start + r.total;
+    if (r.tiles > 1) {
+#pragma unroll 1
+        for (uint32_t n = r.tiles; n > 1;) {  // the tile is one of n from t on
+            const uint32_t each = (n + 63) / 64, c = lane * each;
+            const uint32_t i = uint32_t(__builtin_popcountll(__ballot(c < n && cost_before(r, t + c, bm) <= in))) - 1;
+            t += i * each;
+            n = min(each, n - i * each);
+        }
+        const double ends = start + cost_before(r, t + (upper ? 1 : 0), bm);
+        begin = of_lane(ends, 0);
+        end = of_lane(ends, 32);
+    }
+    m.x = tile_at(a, r, t, bm, keys);
+    const uint32_t units = units_before(upper ? m.to : m.at, begin, end, m.x.units);
+    m.u0 = uint32_t(__builtin_amdgcn_readlane(int(units), 0));
+    m.u1 = uint32_t(__builtin_amdgcn_readlane(int(units), 32));
+    m.token = r.token;
+    m.base = r.base;
+    m.pieces = 0;
+    if (m.at > begin || end > m.to) {
+        uint32_t w0, w1;
+        parts_of(m, upper ? end - 1.0 : begin, w0, w1);
+        const uint32_t first = 2 * w0 + (part_at(m, w0) < begin ? 1u : 0u);
+        m.slot = m.w == w0 ? first : 2 * m.w;
+        m.pieces = w1 - w0 + 1;
+        if (lane == 0)
+            (FEW ? a.few_p : a.many_p)[m.slot] = Piece{m.pieces, m.w - w0, w0, first, r.token, m.x.row0, m.x.rows, m.g};
+    }
+    m.at = fmin(end, m.to);
+}
+
+// Wave 0: the part's next segment after l's.
+template <bool FEW, uint32_t bm>
+__device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, Walk& to, const Heads& h)
+{
+    if (threadIdx.x >= 64) return;
+    Walk m = l;
+    m.go = m.at < m.to;
+    if (m.go) {
+        Request r = request_at<FEW, bm>(a, h, m.b);  // the request at m.at: this one, or one of those behind it
+        while (m.at >= m.before + r.total * a.kv_heads) {
+            m.before += r.total * a.kv_heads;
+            const uint32_t next = ++m.b + threadIdx.x;
+            if (next < a.requests) r = request_at<FEW, bm>(a, h, next);
+            const double own = next < a.requests ? r.total * a.kv_heads : 0.0, inc = wave_inclusive(own);
+            const uint64_t behind = __ballot(m.before + inc > m.at);
+            if (behind == 0 && m.b + 64 >= a.requests) {  // starts or lens changed during the call
+                m.go = 0;
+                if (threadIdx.x == 0) to = m;
+                return;
+            }
+            const int i = behind ? __builtin_ctzll(behind) : 63;
+            m.b += uint32_t(i);
+            m.before += of_lane(inc - own, i);
+            r = request_at<FEW, bm>(a, h, m.b);
+        }
+        cut_segment<FEW, bm>(a, m, r);
+    }
+    if (threadIdx.x == 0) to = m;
+}
+
 // Adds up the requests, so that no launch has to come first, and finds the one in which the
-// part begins.  Up to 64 requests: wave 0 alone, one per lane.  More: thread t takes a run
-// of them.  For next_segment, which wave 0 runs too, no barrier is needed.
+// part begins and its first segment, `to`.  Up to 64 requests: wave 0 alone, one per lane.  More: thread t takes a run
+// of them, l says where the part begins and next_segment, which wave 0 runs too, goes on from there.
 template <bool FEW, uint32_t bm, int NT>
-__device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h, double* red)
+__device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Walk& to, Heads& h, double* red)
 {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     if (a.requests <= 64) {
@@ -265,12 +343,19 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
         const double own = r.total * a.kv_heads, inc = wave_inclusive(own);
         Walk m;
         take_part(m, of_lane(inc, 63), group_sum<kWave>(r.units) * a.kv_heads * (FEW ? 1.0f / kFewWaves : 1.0f));
-        const uint64_t behind = __ballot(inc > m.at);  // lanes from the part's first request on
-        const int b = behind ? __builtin_ctzll(behind) : 0;
-        m.b = uint32_t(b);
-        m.before = of_lane(inc - own, b);
-        if (lane == 0) l = m;
         if (lane == 0) (FEW ? a.few_p : a.many_p)[2 * m.w].n = (FEW ? a.few_p : a.many_p)[2 * m.w + 1].n = 0;
+        m.go = m.at < m.to;
+        if (m.go) {
+            const uint64_t behind = __ballot(inc > m.at);  // lanes from the part's first request on
+            const int b = behind ? __builtin_ctzll(behind) : 0;
+            m.b = uint32_t(b);
+            m.before = of_lane(inc - own, b);
+            const Request rb{uint32_t(__builtin_amdgcn_readlane(int(r.token), b)), uint32_t(__builtin_amdgcn_readlane(int(r.rows), b)),
+                             __builtin_amdgcn_readlane(r.base, b), uint32_t(__builtin_amdgcn_readlane(int(r.tiles), b)),
+                             of_lane(r.first, b), of_lane(r.cap, b), of_lane(r.total, b), 0.0f};
+            cut_segment<FEW, bm>(a, m, rb);
+        }
+        if (lane == 0) to = m;
         return;
     }
     const uint32_t each = (a.requests + NT - 1) / NT;
@@ -320,68 +405,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Heads& h
     }
     __syncthreads();
     if (tid == 0) (FEW ? a.few_p : a.many_p)[2 * m.w].n = (FEW ? a.few_p : a.many_p)[2 * m.w + 1].n = 0;
-}
-
-// Wave 0: the part's next segment after l's.  A cut tile gets its slot and its record for k_paged_join.
-template <bool FEW, uint32_t bm>
-__device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, Walk& to, const Heads& h)
-{
-    constexpr uint32_t keys = FEW ? kFewKeys : kManyKeys;
-    if (threadIdx.x >= 64) return;
-    Walk m = l;
-    m.go = m.at < m.to;
-    if (m.go) {
-        Request r = request_at<FEW, bm>(a, h, m.b);  // the request at m.at: this one, or one of those behind it
-        while (m.at >= m.before + r.total * a.kv_heads) {
-            m.before += r.total * a.kv_heads;
-            const uint32_t next = ++m.b + threadIdx.x;
-            if (next < a.requests) r = request_at<FEW, bm>(a, h, next);
-            const double own = next < a.requests ? r.total * a.kv_heads : 0.0, inc = wave_inclusive(own);
-            const uint64_t behind = __ballot(m.before + inc > m.at);
-            if (behind == 0 && m.b + 64 >= a.requests) {  // starts or lens changed during the call
-                m.go = 0;
-                if (threadIdx.x == 0) to = m;
-                return;
-            }
-            const int i = behind ? __builtin_ctzll(behind) : 63;
-            m.b += uint32_t(i);
-            m.before += of_lane(inc - own, i);
-            r = request_at<FEW, bm>(a, h, m.b);
-        }
-        const double off = m.at - m.before;
-        m.g = min(a.kv_heads - 1, uint32_t(near_ratio(off, r.total)));
-        while (m.g && m.g * r.total > off) --m.g;
-        while (m.g + 1 < a.kv_heads && (m.g + 1) * r.total <= off) ++m.g;
-        const double in = off - m.g * r.total;
-        uint32_t lo = 0;
-        double begin = m.before + m.g * r.total, end = begin + r.total;
-        if (r.tiles > 1) {
-            uint32_t hi = r.tiles;
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (cost_before(r, mid, bm) <= in) lo = mid;
-                else hi = mid;
-            }
-            end = begin + cost_before(r, lo + 1, bm);
-            begin += cost_before(r, lo, bm);
-        }
-        m.x = tile_at(a, r, lo, bm, keys);
-        m.u0 = units_before(m.at, begin, end, m.x.units);
-        m.u1 = units_before(m.to, begin, end, m.x.units);
-        m.token = r.token;
-        m.base = r.base;
-        m.pieces = 0;
-        if (m.at > begin || end > m.to) {
-            const uint32_t w0 = part_of(m, begin), w1 = part_of(m, end - 1.0);
-            const uint32_t first = 2 * w0 + (part_at(m, w0) < begin ? 1u : 0u);
-            m.slot = m.w == w0 ? first : 2 * m.w;
-            m.pieces = w1 - w0 + 1;
-            if (threadIdx.x == 0)
-                (FEW ? a.few_p : a.many_p)[m.slot] = Piece{m.pieces, m.w - w0, w0, first, r.token, m.x.row0, m.x.rows, m.g};
-        }
-        m.at = fmin(end, m.to);
-    }
-    if (threadIdx.x == 0) to = m;
+    next_segment<FEW, bm>(a, l, to, h);
 }
 
 // What every wave needs of the segment, in scalar registers.
@@ -767,8 +791,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
     Heads& heads = lds.heads;
     double* red = lds.red;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<true, kFewRows, 256>(arguments(), walk[1], heads, red);
-    next_segment<true, kFewRows>(arguments(), walk[1], walk[0], heads);
+    start_walk<true, kFewRows, 256>(arguments(), walk[1], walk[0], heads, red);
     T* krows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
     T* vrows = krows + 32 * D;
     for (uint32_t turn = 0;; turn ^= 1u) {
@@ -931,8 +954,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
     double* red = lds.red;
     uint32_t& odd = lds.odd;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<false, kBm, NT>(arguments(), walk[1], heads, red);
-    next_segment<false, kBm>(arguments(), walk[1], walk[0], heads);
+    start_walk<false, kBm, NT>(arguments(), walk[1], walk[0], heads, red);
     for (uint32_t turn = 0;; turn ^= 1u) {
         __syncthreads();  // the tile before is done with LDS
         if (uniform(walk[turn].go) == 0) break;
