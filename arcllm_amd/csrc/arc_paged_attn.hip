@@ -36,9 +36,10 @@ constexpr uint32_t kFewWgs = 512;      // most parts of the line
 // cores' power holds down).  Heads of 64 leave registers for 3 workgroups of 4 waves.
 constexpr int many_waves(uint32_t dim) { return dim == 128 ? 8 : 4; }
 constexpr uint32_t many_wgs(uint32_t dim) { return dim == 128 ? 256 : 768; }
-// A tile's start and end, in positions: few rows 2.5 us, where a part's 128 take 4.6; many rows (bm of them) 7 us
-// (pages, first copy, stores), where 64 take 1.9 and, with 4 waves, other workgroups of the CU have the time.
-constexpr uint32_t tile_ends(bool few, uint32_t bm) { return few ? 64 : bm; }
+// A tile's start and end (pages, first copy, stores), in positions: few rows 3 us, where a part's 32 take 0.5 (300
+// requests of up to 1500, 28 heads: 72 us with 64 here, 64 with 192, 60 with 256 to 448; 64 of up to 8000: 57.6, 54.3,
+// 54.6); many rows (bm of them) 7 us, where 64 take 1.9 and, with 4 waves, other workgroups of the CU have the time.
+constexpr uint32_t tile_ends(bool few, uint32_t bm) { return few ? 256 : bm; }
 constexpr float kLazy = 8.0f;          // see rescale
 constexpr uint32_t kManyPieces = 8;    // a tile in more pieces is joined in another way
 
