@@ -120,7 +120,7 @@ __device__ __forceinline__ void deal(uint32_t n, Get get, Put put)
 // no more than many short ones.  A row whose page is new takes it from the stack itself, as the table entry's
 // writer does, so no row waits for a table entry.  ROWS: the rows too; else k_plan_rows writes them.
 // Bound by the latency of three dependent loads (lengths, an ended request's entries, the stack) and
-// the barriers: 24 requests 4.0 us, 700 with 60 prompts and 43000 rows 9.8 us and 3.9 us in
+// the barriers: 24 requests 4.0 us, 700 with 60 prompts and 43000 rows 9.6 us and 3.9 us in
 // k_plan_rows, of which an empty launch is 2.2.
 template <int NT, bool ROWS>
 __global__ __launch_bounds__(NT) void k_plan(PlanArgs a)

@@ -482,7 +482,7 @@ __device__ __forceinline__ uint32_t v_swizzle(uint32_t r)
 // flight to write, and nothing else here uses m0.  wait_loads and a barrier (a wave's own rows: wait_loads)
 // come before the rows are read.
 // ONCE: data that no other workgroup reads goes past the caches' keeping (nt): 2 contexts of 131071, 8 kv
-// heads (727 MB) 139 -> 121 us.
+// heads (732 MB): 13 % less time.
 template <bool ONCE>
 __device__ __forceinline__ void copy16(uint32_t lds, const void* base, uint32_t off)
 {
@@ -773,8 +773,8 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 // the wave's own LDS rows, in whole rows.  S^T = K Q^T (lane -> query), O^T = V^T P^T, P^T from the
 // scores' registers.  The next unit's K is on its way as soon as this one's scores are done, its V
 // after the output: with 8 waves a CU some 110 KB of 128 are in flight.  Measured, the call with its join: 64
-// requests of up to 8000, 28 heads on 4 (271 MB) 58 us, 4.7 TB/s, of which 4 are the walk and 4 the join; 2 of
-// 131071, 64 on 8 (732 MB) 126 us, 5.8 TB/s; plain reads of as much reach 6.2.
+// requests of up to 8000, 28 heads on 4 (271 MB) 56 us, 4.8 TB/s, of which 3 are the walk and 4 the join; 2 of
+// 131071, 64 on 8 (732 MB) 125 us, 5.9 TB/s; plain reads of as much reach 6.2.
 template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 {
@@ -931,7 +931,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 // unit's 64 rows of K and V come straight into LDS, shared by the waves and double buffered:
 // unit u + 1 is copied while unit u is computed; one barrier per unit.  Operands as in the
 // few-rows kernel, K's read from LDS.  Measured: 4096 tokens at 12288, 28 heads of 128 on 4, 842 GFLOP that are
-// seen: 836 us, 1.0 PFLOP/s of the 1.23 that a large fp16 product reaches; with zeros for data 650 us, so the
+// seen: 830 to 900 us, 1.0 PFLOP/s of the 1.23 that a large fp16 product reaches; with zeros for data 650 us, so the
 // clock under the matrix cores' power is what is left.  3 x 2000 tokens in a window of 1024, heads of 64: 130 us,
 // 0.54 PFLOP/s, bound by the softmax's vector instructions, as many per score as heads of 128 have for twice the
 // products.
@@ -1112,8 +1112,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 // pieces (long rows of tiles cut once or twice): 256 / (D / 4) rows at once, each by its lanes
 // alone; many (one long context): a row at a time, its pieces dealt out over the groups of lanes.
 // What bounds it is the way to memory and back: the record, the sums, all of a row's pieces at once, and as few
-// turns after that as the card has workgroups for.  Heads of 128, a chunk of 500 at 2500: 42.4 us the call with 8
-// workgroups a slot, 45.3 with 4, 42.7 with 16; of 64, three chunks of 700: 52 with 2 or 4, 58 with 8.
+// turns after that as the card has workgroups for.  Heads of 128, a chunk of 500 at 2500, 40 us the call with 8
+// workgroups a slot: 3 more with 4, as long with 16; of 64, three chunks of 700, 49 us with 2: as long with 4, 6
+// more with 8.
 constexpr uint32_t many_split(uint32_t dim) { return dim == 128 ? 8 : 2; }
 
 struct JoinRow {
