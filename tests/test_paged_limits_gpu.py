@@ -137,3 +137,22 @@ def test_nothing_is_written_behind_the_workspace(hpk, new, dim):
     bits = s.attention(workspace=ws)
     s.check(bits, rows={0, new // 2, new - 1, new})
     assert np.all(ws.download(np.uint8)[n:] == 0x5A)
+
+
+@pytest.mark.parametrize("kv_heads,dim,old,new", [(256, 64, [70, 0, 33], [1, 2, 40]), (97, 128, [40, 9], [1, 35]),
+                                                  (255, 64, [0], [1])])
+def test_many_kv_heads(kv_heads, dim, old, new):
+    """Parts that begin and end at any of them."""
+    s = pl.Step(old, new, 16, kv_heads, 1, dim, arc.F16, SEED + kv_heads).upload()
+    s.check(s.attention())
+
+
+@pytest.mark.parametrize("new,hpk,dim,window,max_new", [(1300, 64, 64, 0, None), (1300, 64, 64, 100, None),
+                                                        (5000, 16, 128, 0, None), (5000, 16, 128, 700, None),
+                                                        (200, 64, 64, 0, 0), (200, 64, 128, 9, 0)])
+def test_more_tiles_than_a_wave_has_lanes(new, hpk, dim, window, max_new):
+    """Of 128, 256 and 32 rows: each row is some tile's, wherever the parts are cut."""
+    s = pl.Step([150, 3], [new, 2], 32, 2, hpk, dim, arc.BF16, SEED + new, max_new=max_new).upload()
+    bits = s.attention(window=window)
+    assert not np.any(np.all(bits[: s.used, : s.width].reshape(s.used, -1, dim) == 0xABCD, axis=2))
+    s.check(bits, window=window, rows={0, 1, 2, 3, 63, 64, 65, 127, new // 2, new - 2, new - 1, new, new + 1})
