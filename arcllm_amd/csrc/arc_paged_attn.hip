@@ -63,7 +63,7 @@ struct PagedAttn {
     float scale;         // |scale| * log2(e)
     uint32_t neg;        // 0x80008000 where scale < 0: q's signs are flipped
     float *few_o, *many_o;    // [2 * workgroups][slot rows][D] sums of pieces
-    float2 *few_ml, *many_ml; // [2 * workgroups][slot rows] running maximum (times scale) and sum
+    float2 *few_ml, *many_ml; // [2 * workgroups][slot rows] reference score and sum
     Piece *few_p, *many_p;
     uint32_t few_slot, many_slot;  // rows of a slot
     uint32_t few_wgs, many_wgs;    // workgroups of this call's launches (0: not launched)
@@ -638,17 +638,60 @@ __device__ __forceinline__ void hide(f32x16& sc, uint32_t bits)
         sc[i] = int32_t(bits << (31 - 8 * (i >> 2) - (i & 3))) < 0 ? sc[i] : -INFINITY;
 }
 
-// Running softmax of one query (a lane and its partner lane ^ 32, each with half of the
-// keys): `m` is the reference that weights 2^(score - m) are relative to, `l` the lane's share of
-// their sum.  m follows the maximum only when that has grown by more than kLazy: weights then
-// reach 2^kLazy instead of 1, which costs no accuracy (relative rounding) and saves nearly
-// every rescaling of the output.
-template <int NO>
-__device__ __forceinline__ void rescale(float mx, float& m, float& l, f32x16 (&o)[NO])
+// Weights.  A score's weight is 2^(score * scale - R) with R = m * scale for a reference score m, about the largest
+// so far.  Up to kLarge R is -c, rounded, and the exponent one fused multiply and add: what c's rounding adds to
+// every exponent is in R too, so only the size of the weights knows of it (by 2^-13 powers of two at kLarge, 16 at 2^28,
+// which no 16-bit weight survives).  Beyond, R is m * scale itself and the exponent (score - m) * scale, exact where it
+// counts, for one instruction more a score: a branch that scores of models do not take, and whose test costs 0.5 to 2 % (64
+// requests of up to 8000 56.3 -> 56.6 us, 3 x 2000 in a window 136.8 -> 137.5).  The form of large scores for all of
+// them would add an instruction to the seven that each score has.
+constexpr float kLarge = 4096.0f;
+__device__ __forceinline__ float offset_of(float m, float scale)
 {
-    if (__ballot(mx > m + kLazy) == 0) return;  // m = -inf: any score that is one
+#pragma clang fp contract(off)  // the rounded product, wherever it goes
+    return -(m * scale);
+}
+__device__ __forceinline__ bool is_large(float c) { return !(fabsf(c) <= kLarge); }
+
+// The factor 2^(R - R') that takes sums with the reference m to the reference `to`, which is not -infinity; 0 for m =
+// -infinity, sums of nothing.  R is m * scale and what its rounding adds, if it is rounded.
+__device__ __forceinline__ float moved(float m, float to, float scale)
+{
+#pragma clang fp contract(off)
+    auto rounding = [&](float r) {
+        const float c = offset_of(r, scale);
+        return is_large(c) ? 0.0f : -__builtin_fmaf(r, scale, c);
+    };
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(m - to, scale, rounding(m) - rounding(to)));
+}
+
+// For the reference m: the k and c with which fma(score, k, c) is a score's exponent; large ones are exponents afterwards
+// (k = 1, c = 0).  m = -infinity, nothing seen yet: as 0, all weights 0.
+template <typename... Scores>
+__device__ __forceinline__ void exponents(float m, float& k, float& c, Scores&... sc)
+{
+    const float r = m == -INFINITY ? 0.0f : m;
+    c = offset_of(r, k);
+    if (__builtin_expect(__ballot(is_large(c)) == 0, 1)) return;
+    auto each = [&](f32x16& x) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = is_large(c) ? (x[i] - r) * k : __builtin_fmaf(x[i], k, c);
+    };
+    (each(sc), ...);
+    c = 0.0f;
+    k = 1.0f;
+}
+
+// Running softmax of one query (a lane and its partner lane ^ 32, each with half of the
+// keys): `m` is the reference score, `l` the lane's share of the sum of weights.  m follows the maximum only when that has
+// grown by more than kLazy powers of two: weights then reach 2^kLazy instead of 1, which costs no accuracy (relative
+// rounding) and saves nearly every rescaling of the output.
+template <int NO>
+__device__ __forceinline__ void rescale(float mx, float scale, float& m, float& l, f32x16 (&o)[NO])
+{
+    if (__ballot((mx - m) * scale > kLazy) == 0) return;  // m = -inf: any score that is one
     const float to = fmaxf(m, mx);
-    const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    const float f = to == -INFINITY ? 1.0f : moved(m, to, scale);
     m = to;
     l *= f;
 #pragma unroll
@@ -854,12 +897,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 float mx = sc[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-                mx = xor_max<32>(mx) * p.scale;
-                rescale(mx, m, l, o);
-                const float mr = m == -INFINITY ? 0.0f : m;  // nothing seen yet: all weights 0
+                rescale(xor_max<32>(mx), p.scale, m, l, o);
+                float k = p.scale, c;
+                exponents(m, k, c, sc);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale, -mr));
+                    sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], k, c));
                     l += sc[i];
                 }
 #pragma unroll
@@ -879,7 +922,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
         } else {
             next_segment<true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
-        // the waves' states in wave order: out = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w
+        // the waves' states in wave order: out = sum_w f_w o_w / sum_w f_w l_w, f_w to the largest reference M
         __syncthreads();  // every wave is done with its V rows
         const float lsum = xor_sum<32>(l);
         if (l32 < s.x.rows) {
@@ -906,7 +949,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
             float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float f = __builtin_amdgcn_exp2f(mw[i][rr] - M0);
+                const float f = moved(mw[i][rr], M0, e_.scale);
                 const float4 w = *reinterpret_cast<const float4*>(&joined[(i * 32 + rr) * D + d]);
                 L = __builtin_fmaf(lw[i][rr], f, L);
                 acc.x = __builtin_fmaf(w.x, f, acc.x);
@@ -1045,14 +1088,14 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
-                mx = xor_max<32>(mx) * p.scale;
-                rescale(mx, m, l, o);
-                const float mr = m == -INFINITY ? 0.0f : m;
+                rescale(xor_max<32>(mx), p.scale, m, l, o);
+                float k = p.scale, c;
+                exponents(m, k, c, sc[0], sc[1]);
                 auto weights = [&](int st) {  // the 16 positions of step st: their weights, rounded; l adds the unrounded
                     f32x16& x = sc[st >> 1];
 #pragma unroll
                     for (int i = 8 * (st & 1); i < 8 * (st & 1) + 8; ++i) {
-                        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], p.scale, -mr));
+                        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], k, c));
                         l += x[i];
                     }
                     return narrow<T>(x, 8 * (st & 1));
@@ -1106,8 +1149,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
 }
 
 // ---------------------------------------------------------------------- join
-// Adds the pieces of the tiles that were cut, in order: out = sum_i 2^(m_i - M) o_i /
-// sum_i 2^(m_i - M) l_i.  A workgroup for each slot (many_split of them where tiles have many
+// Adds the pieces of the tiles that were cut, in order: out = sum_i f_i o_i / sum_i f_i l_i with f_i = 2^(R_i - R), to
+// the largest reference.  A workgroup for each slot (many_split of them where tiles have many
 // rows); the workgroups of a tile's n pieces share its rows.  D / 4 lanes span a row; few
 // pieces (long rows of tiles cut once or twice): 256 / (D / 4) rows at once, each by its lanes
 // alone; many (one long context): a row at a time, its pieces dealt out over the groups of lanes.
@@ -1178,7 +1221,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
             JoinRow r{0.0f, make_float4(0, 0, 0, 0)};
 #pragma unroll
             for (uint32_t i = 0; i < kManyPieces; ++i)
-                if (i < p.n) add_piece(r, __builtin_amdgcn_exp2f(ml[i].x - M0), ml[i].y, o[i]);
+                if (i < p.n) add_piece(r, moved(ml[i].x, M0, a.scale), ml[i].y, o[i]);
             store_row(out_row<T>(a, p.token, p.row0 + row, p.g, D) + d, r);
         }
         return;
@@ -1197,7 +1240,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a)
 #pragma unroll 4
         for (uint32_t i = grp; i < p.n; i += kGroups) {
             const float2 ml = ml_at(i, row);
-            add_piece(r, __builtin_amdgcn_exp2f(ml.x - M0), ml.y, o_at(i, row));
+            add_piece(r, moved(ml.x, M0, a.scale), ml.y, o_at(i, row));
         }
         __syncthreads();  // part_l is read
         part[grp][d / 4] = r.acc;
