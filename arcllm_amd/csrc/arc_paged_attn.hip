@@ -41,6 +41,8 @@ constexpr uint32_t many_wgs(uint32_t dim) { return dim == 128 ? 256 : 768; }
 // 54.6); many rows (bm of them) 7 us, where 64 take 1.9 and, with 4 waves, other workgroups of the CU have the time.
 constexpr uint32_t tile_ends(bool few, uint32_t bm) { return few ? 256 : bm; }
 constexpr float kLazy = 8.0f;          // see rescale
+template <typename T>
+constexpr float kLift = __is_same(T, _Float16) ? 7.0f : 0.0f;
 constexpr uint32_t kManyPieces = 8;    // a tile in more pieces is joined in another way
 
 // What a part of a tile left in the workspace, one per slot; two slots per
@@ -564,8 +566,9 @@ __device__ __forceinline__ f32x16 mfma(vec8<T> x, vec8<T> y, f32x16 c)
 constexpr int kMfma = 0x008, kDsRead = 0x100, kAhead = 8;
 
 // 8 consecutive values to 16 bits, round to nearest even.  The weights' one rounding, which the second product's
-// 16-bit operands ask for; their sum l takes them unrounded.  The roundings of many keys average out: the outputs'
-// distance from 64 bits is a fifth to a third above the final rounding's own (2.0e-4 -> 2.6e-4 in fp16).
+// 16-bit operands ask for; their sum l takes them unrounded.  Roundings of keys with different weights average out: the
+// outputs' distance from 64 bits is a fifth to a third above the final rounding's own (2.0e-4 -> 2.6e-4 in fp16).  Many
+// keys of one weight are all rounded alike, by half a step at most, as much as the output's own rounding.
 template <typename T>
 __device__ __forceinline__ vec8<T> narrow(const f32x16& p, int at)
 {
@@ -684,13 +687,17 @@ __device__ __forceinline__ void exponents(float m, float& k, float& c, Scores&..
 
 // Running softmax of one query (a lane and its partner lane ^ 32, each with half of the
 // keys): `m` is the reference score, `l` the lane's share of the sum of weights.  m follows the maximum only when that has
-// grown by more than kLazy powers of two: weights then reach 2^kLazy instead of 1, which costs no accuracy (relative
-// rounding) and saves nearly every rescaling of the output.
-template <int NO>
+// grown by more than kLazy powers of two, which saves nearly every rescaling of the output and costs no accuracy
+// (relative rounding).  In fp16 it stays kLift powers of two below: the largest weight is 2^7 to 2^15, the upper part of the
+// type's range, and weights keep all their bits down to 2^-21 of the largest and count down to 2^-32.  With the largest at 1 a
+// context of 2^17 keys of 2^-25 each, one sharp key before them, lost 0.4 %.  bf16 has fp32's range.
+template <typename T, int NO>
 __device__ __forceinline__ void rescale(float mx, float scale, float& m, float& l, f32x16 (&o)[NO])
 {
-    if (__ballot((mx - m) * scale > kLazy) == 0) return;  // m = -inf: any score that is one
-    const float to = fmaxf(m, mx);
+    if (__ballot((mx - m) * scale > kLift<T> + kLazy) == 0) return;  // m = -inf: any score that is one
+    // a scale so small that the lift is beyond 2^100 in scores takes less of it
+    const float lift = kLift<T> > 0.0f ? fminf(kLift<T> * __builtin_amdgcn_rcpf(scale), 0x1p100f) : 0.0f;
+    const float to = fmaxf(m, mx - lift);
     const float f = to == -INFINITY ? 1.0f : moved(m, to, scale);
     m = to;
     l *= f;
@@ -897,14 +904,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 float mx = sc[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-                rescale(xor_max<32>(mx), p.scale, m, l, o);
+                rescale<T>(xor_max<32>(mx), p.scale, m, l, o);
                 float k = p.scale, c;
                 exponents(m, k, c, sc);
+                float sum = 0.0f;  // the unit's: a weight that would vanish beside l counts among its like
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], k, c));
-                    l += sc[i];
+                    sum += sc[i];
                 }
+                l += sum;
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     const vec8<T> w = narrow<T>(sc, 8 * st);
@@ -979,7 +988,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 // 0.54 PFLOP/s, bound by the softmax's vector instructions, as many per score as heads of 128 have for twice the
 // products.
 template <typename T, int D, int NW, bool WIDE>
-__global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
+__global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAttn)
 {
     constexpr int NT = NW * 64;
     constexpr uint32_t kBm = NW * 32, kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
@@ -1088,15 +1097,16 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
-                rescale(xor_max<32>(mx), p.scale, m, l, o);
+                rescale<T>(xor_max<32>(mx), p.scale, m, l, o);
                 float k = p.scale, c;
                 exponents(m, k, c, sc[0], sc[1]);
-                auto weights = [&](int st) {  // the 16 positions of step st: their weights, rounded; l adds the unrounded
+                float sum = 0.0f;  // as in the few-rows kernel
+                auto weights = [&](int st) {  // the 16 positions of step st: their weights, rounded; sum adds the unrounded
                     f32x16& x = sc[st >> 1];
 #pragma unroll
                     for (int i = 8 * (st & 1); i < 8 * (st & 1) + 8; ++i) {
                         x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], k, c));
-                        l += x[i];
+                        sum += x[i];
                     }
                     return narrow<T>(x, 8 * (st & 1));
                 };
@@ -1111,6 +1121,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_paged_many(PagedAttn)
                     for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(vt[st & 1][t], w, o[t]);
                     if (st < 3) w = weights(st + 1);
                 }
+                l += sum;
                 cur ^= 1;
                 page = npage;
                 npage = far;

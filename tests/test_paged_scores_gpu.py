@@ -69,3 +69,31 @@ def test_scores_as_large_as_fp32_holds(new, sign):
     s.give(0, np.full((300 + new, 1, 128), 2.0 ** 60))
     for scale in (2.0 ** -60, 1.0, 2.0 ** 60):
         s.check_exact(s.upload().attention(scale=scale), scale, 400)
+
+
+@pytest.mark.parametrize("new,requests,dim", [(1, 1, 64), (1, 64, 64), (40, 1, 128), (40, 96, 64), (40, 32, 128)])
+@pytest.mark.parametrize("below", [14.5, 18.7, 20.35, 23.6, 24.6, 25.01, 28.7])
+@pytest.mark.parametrize("dtype", [arc.F16, arc.BF16])
+def test_one_sharp_key_before_a_long_context(dtype, below, new, requests, dim):
+    """131071 positions, one of them `below` powers of two above all others, V = 1: rows are 1.  The faint keys all
+    round alike, so theirs is one rounding 131070 times.  Many requests share the pages, one of faint keys over
+    and over and one with the sharp one: a tile is one part then and its sums go over the whole context, one addition for
+    16 positions at most."""
+    n, page, kv = 131071, 64, 8
+    s = px.GivenStep([2 * page - new] + [0] * (requests - 1), [new] * requests, page, kv, 1, dim, dtype, SEED + 2)
+    s.give_q(1.0)
+    k = np.zeros((2 * page, kv, dim))
+    k[page + 9] = 1.0
+    s.give(0, k, np.ones(k.shape))
+    faint, sharp = s.tables[0, :2]
+    s.max_pages, s.lens[:] = 2048, n
+    s.tables = np.full((requests, 2048), faint, np.uint32)
+    s.tables[:, 12] = sharp
+    scale = float(np.float32(below / (dim * px.LOG2E)))
+    bits = s.upload().attention(scale=scale)
+    x = np.zeros((n, dim))
+    x[12 * page + 9] = 1.0
+    ref, tol = px.exact_row(np.ones((1, dim)), x, np.ones((n, dim)), scale, n // 16, dtype)
+    assert np.abs(ref - 1).max() < 1e-9
+    err = np.abs(px.pl.from_bits(bits, dtype) - 1.0).max()
+    assert err <= tol.max(), (err, tol.max())
