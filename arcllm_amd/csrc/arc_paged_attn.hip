@@ -1349,7 +1349,9 @@ int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch,
         return set_error(ARC_ERR_INVALID_ARGUMENT, "ldq %u, ldo %u: multiples of 8, at least %u", ldq, ldo, width);
     if (!aligned(q, 16) || !aligned(out, 16)) return set_error(ARC_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
     if (!aligned(workspace, 256)) return set_error(ARC_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
-    if (!std::isfinite(scale)) return set_error(ARC_ERR_INVALID_ARGUMENT, "scale must be finite");
+    const float s = scale == 0.0f ? 1.0f / std::sqrt(float(pages->head_dim)) : scale;
+    const float s2 = std::fabs(s) * 1.44269504088896f;  // of powers of two
+    if (!std::isfinite(s2)) return set_error(ARC_ERR_INVALID_ARGUMENT, "scale %g: finite, at most 2^127", double(scale));
     if (rows_overlap(q, uint64_t(width) * 2, uint64_t(ldq) * 2, out, uint64_t(width) * 2, uint64_t(ldo) * 2, batch->tokens))
         return set_error(ARC_ERR_INVALID_ARGUMENT, "q and out share memory");
     // the line's costs (positions times hpk, over tiles and kv heads) stay below 2^52: times 1024 parts and
@@ -1380,8 +1382,7 @@ int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch,
     a.hpk = hpk;
     a.window = window;
     a.sinks = sinks;
-    const float s = scale == 0.0f ? 1.0f / std::sqrt(float(pages->head_dim)) : scale;
-    a.scale = std::fabs(s) * 1.44269504088896f;
+    a.scale = s2;
     a.neg = s < 0.0f ? 0x80008000u : 0u;
     a.few_p = reinterpret_cast<Piece*>(ws + sp.few_p);
     a.many_p = reinterpret_cast<Piece*>(ws + sp.many_p);

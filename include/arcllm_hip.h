@@ -395,7 +395,7 @@ size_t arc_paged_attention_workspace_bytes(const arc_kv_pages *pages, const arc_
  * q and out: pages->dtype, kv_heads * hpk heads of head_dim per row, ldq and ldo
  * elements from row to row (multiples of 8), 16-byte aligned, sharing no memory
  * with each other (refused) or the pages (not checked).  hpk 1..64; scale 0 means
- * 1 / sqrt(head_dim).
+ * 1 / sqrt(head_dim), else |scale| is at most 2^127.
  * Scores, softmax and sums are fp32, right for finite scores of any size; weights enter the V product rounded to
  * pages->dtype.  A position whose table entry is not below num_pages is not
  * seen, and a row that sees nothing, or whose scores are all -infinity, is 0; what lies in
