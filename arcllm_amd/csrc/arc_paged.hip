@@ -287,12 +287,12 @@ __global__ __launch_bounds__(256) void k_plan_rows(PlanArgs a)
 // Rows that one workgroup writes itself; more go to a launch of their own.
 constexpr uint32_t kPlanRowsInOne = 4096;
 
-template <bool ROWS>
 void launch_plan(const PlanArgs& a, hipStream_t st)
 {
+    if (a.rows > kPlanRowsInOne) hipLaunchKernelGGL((k_plan<1024, false>), dim3(1), dim3(1024), 0, st, a);
     // a small step: 4 waves, whose barriers cost less than 16 waves'
-    if (a.requests <= 256 && a.rows <= 1024) hipLaunchKernelGGL((k_plan<256, ROWS>), dim3(1), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_plan<1024, ROWS>), dim3(1), dim3(1024), 0, st, a);
+    else if (a.requests <= 256 && a.rows <= 1024) hipLaunchKernelGGL((k_plan<256, true>), dim3(1), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_plan<1024, true>), dim3(1), dim3(1024), 0, st, a);
 }
 
 // -------------------------------------------------------------------- rope
@@ -471,12 +471,8 @@ int arc_paged_plan(const arc_paged_batch* batch, const uint32_t* old_lens, const
     a.num_pages = num_pages;
     a.shift = log2_of(page_size);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a.rows <= kPlanRowsInOne) {
-        launch_plan<true>(a, st);
-        return check_hip(hipGetLastError(), "step plan");
-    }
-    launch_plan<false>(a, st);
-    if ((rc = check_hip(hipGetLastError(), "step plan"))) return rc;
+    launch_plan(a, st);
+    if ((rc = check_hip(hipGetLastError(), "step plan")) || a.rows <= kPlanRowsInOne) return rc;
     const dim3 grid((a.rows + 255) / 256);
     if (a.requests < kStartsInLds) hipLaunchKernelGGL(k_plan_rows<true>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(k_plan_rows<false>, grid, dim3(256), 0, st, a);
