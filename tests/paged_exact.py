@@ -76,3 +76,31 @@ def exact_row(q, k, v, scale, depth, dtype):
     mass = w @ size / total
     tol = (step + rel) @ size / total + np.abs(ref) * rel.sum(1, keepdims=True) / total
     return ref, tol + (2 * depth * 2.0 ** -24 + 2.0 ** -22) * mass + 1.01 * u * np.abs(ref) + 2.0 ** -24
+
+
+# ------------------------------------------------------------ position codes
+def coded_rows(n, kv_heads, dim, course):
+    """K and V, [n, kv_heads, dim], for q = 1: V is 1 in one dim, that of a block of 32 positions in even kv heads, of the
+    position itself in odd ones, so that an output is the weight of the positions with its code and one that is
+    left out or taken twice shows.  Scores are whole numbers: equal, or 0 .. 7 along the context, rising or falling."""
+    pos = np.arange(n)
+    level = {"equal": pos * 0, "rising": pos * 8 // n, "falling": 7 - pos * 8 // n}[course]
+    K, V = np.zeros((n, kv_heads, dim)), np.zeros((n, kv_heads, dim))
+    K[:, :, 0] = level[:, None]
+    for g in range(kv_heads):
+        V[pos, g, (pos if g % 2 else pos // 32) % dim] = 1.0
+    return K, V
+
+
+def coded_step(old, new, kv_heads, hpk, dim, dtype, course, page=16):
+    s = GivenStep(old, new, page, kv_heads, hpk, dim, dtype, 1)
+    s.give_q(1.0)
+    for b, n in enumerate(s.lens):
+        s.give(b, *coded_rows(int(n), kv_heads, dim, course))
+    return s
+
+
+# long contexts that are cut into many parts: old, new, kv_heads, hpk, dim, window, sinks
+CODED = [([131070], [1], 1, 2, 64, 0, 0), ([40000, 12345, 70], [1, 1, 1], 2, 4, 128, 0, 0), ([20000, 333], [1, 3], 2, 8, 64, 0, 0),
+         ([50000, 9000], [1, 5], 2, 4, 128, 7000, 100), ([12000], [200], 2, 4, 128, 0, 0), ([9000, 2000], [70, 130], 2, 2, 64, 0, 0),
+         ([15000], [300], 2, 2, 64, 3000, 70), ([0, 4000], [600, 1], 2, 4, 128, 0, 0)]
