@@ -645,9 +645,9 @@ __device__ __forceinline__ void hide(f32x16& sc, uint32_t bits)
 // so far.  Up to kLarge R is -c, rounded, and the exponent one fused multiply and add: what c's rounding adds to
 // every exponent is in R too, so only the size of the weights knows of it (by 2^-13 powers of two at kLarge, 16 at 2^28,
 // which no 16-bit weight survives).  Beyond, R is m * scale itself and the exponent (score - m) * scale, exact where it
-// counts, for one instruction more a score: a branch that scores of models do not take, and whose test costs 0.5 to 2 % (64
-// requests of up to 8000 56.3 -> 56.6 us, 3 x 2000 in a window 136.8 -> 137.5).  The form of large scores for all of
-// them would add an instruction to the seven that each score has.
+// counts, for one instruction more a score: a branch that scores of models do not take, on a flag that changes with m.  It
+// costs up to 1 % (64 requests of up to 8000 56.8 -> 57.0 us, a chunk of 4096 at 12288 897 -> 900); decided again in each unit
+// 1.4 % (909).  The form of large scores for all would add an instruction to the seven that each score has.
 constexpr float kLarge = 4096.0f;
 __device__ __forceinline__ float offset_of(float m, float scale)
 {
@@ -668,43 +668,49 @@ __device__ __forceinline__ float moved(float m, float to, float scale)
     return __builtin_amdgcn_exp2f(__builtin_fmaf(m - to, scale, rounding(m) - rounding(to)));
 }
 
-// For the reference m: the k and c with which fma(score, k, c) is a score's exponent; large ones are exponents afterwards
-// (k = 1, c = 0).  m = -infinity, nothing seen yet: as 0, all weights 0.
-template <typename... Scores>
-__device__ __forceinline__ void exponents(float m, float& k, float& c, Scores&... sc)
-{
-    const float r = m == -INFINITY ? 0.0f : m;
-    c = offset_of(r, k);
-    if (__builtin_expect(__ballot(is_large(c)) == 0, 1)) return;
-    auto each = [&](f32x16& x) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = is_large(c) ? (x[i] - r) * k : __builtin_fmaf(x[i], k, c);
-    };
-    (each(sc), ...);
-    c = 0.0f;
-    k = 1.0f;
-}
-
 // Running softmax of one query (a lane and its partner lane ^ 32, each with half of the
-// keys): `m` is the reference score, `l` the lane's share of the sum of weights.  m follows the maximum only when that has
+// keys): `m` is the reference score, `l` the lane's share of the sum of weights.
+struct Running {
+    float m = -INFINITY, l = 0.0f;
+    float c = 0.0f;      // offset_of(m), of 0 while nothing is seen: all weights are 0 then
+    bool large = false;  // is_large(c) in any lane
+};
+// m follows the maximum only when that has
 // grown by more than kLazy powers of two, which saves nearly every rescaling of the output and costs no accuracy
 // (relative rounding).  In fp16 it stays kLift powers of two below: the largest weight is 2^7 to 2^15, the upper part of the
 // type's range, and weights keep all their bits down to 2^-21 of the largest and count down to 2^-32.  With the largest at 1 a
-// context of 2^17 keys of 2^-25 each, one sharp key before them, lost 0.4 %.  bf16 has fp32's range.
+// context of 2^17 keys of 2^-24 each, one sharp key before them, was 0.5 % off.  bf16 has fp32's range.
 template <typename T, int NO>
-__device__ __forceinline__ void rescale(float mx, float scale, float& m, float& l, f32x16 (&o)[NO])
+__device__ __forceinline__ void rescale(float mx, float scale, Running& s, f32x16 (&o)[NO])
 {
-    if (__ballot((mx - m) * scale > kLift<T> + kLazy) == 0) return;  // m = -inf: any score that is one
+    if (__ballot((mx - s.m) * scale > kLift<T> + kLazy) == 0) return;  // m = -inf: any score that is one
     // a scale so small that the lift is beyond 2^100 in scores takes less of it
     const float lift = kLift<T> > 0.0f ? fminf(kLift<T> * __builtin_amdgcn_rcpf(scale), 0x1p100f) : 0.0f;
-    const float to = fmaxf(m, mx - lift);
-    const float f = to == -INFINITY ? 1.0f : moved(m, to, scale);
-    m = to;
-    l *= f;
+    const float to = fmaxf(s.m, mx - lift);
+    const float f = to == -INFINITY ? 1.0f : moved(s.m, to, scale);
+    s.m = to;
+    s.l *= f;
+    s.c = to == -INFINITY ? 0.0f : offset_of(to, scale);
+    s.large = __ballot(is_large(s.c)) != 0;
 #pragma unroll
     for (int t = 0; t < NO; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] *= f;
+}
+
+// The k and c with which fma(score, k, c) is a score's exponent; large ones are exponents afterwards (k = 1, c = 0).
+template <typename... Scores>
+__device__ __forceinline__ void exponents(const Running& s, float& k, float& c, Scores&... sc)
+{
+    c = s.c;
+    if (__builtin_expect(!s.large, 1)) return;
+    auto each = [&](f32x16& x) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = is_large(s.c) ? (x[i] - s.m) * k : __builtin_fmaf(x[i], k, s.c);
+    };
+    (each(sc), ...);
+    c = 0.0f;
+    k = 1.0f;
 }
 
 // Value i of a score or output tile of 32: key, or dim, 8 (i / 4) + 4 (lane / 32) + i % 4.
@@ -857,7 +863,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
         for (int t = 0; t < D / 32; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-        float m = -INFINITY, l = 0.0f;
+        Running run;
         bool odd = false;  // infinities or NaN cleared from V
 
         // the first position of unit u, the page of lane l32's
@@ -904,16 +910,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 float mx = sc[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-                rescale<T>(xor_max<32>(mx), p.scale, m, l, o);
+                rescale<T>(xor_max<32>(mx), p.scale, run, o);
                 float k = p.scale, c;
-                exponents(m, k, c, sc);
+                exponents(run, k, c, sc);
                 float sum = 0.0f;  // the unit's: a weight that would vanish beside l counts among its like
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], k, c));
                     sum += sc[i];
                 }
-                l += sum;
+                run.l += sum;
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     const vec8<T> w = narrow<T>(sc, 8 * st);
@@ -933,7 +939,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
         }
         // the waves' states in wave order: out = sum_w f_w o_w / sum_w f_w l_w, f_w to the largest reference M
         __syncthreads();  // every wave is done with its V rows
-        const float lsum = xor_sum<32>(l);
+        const float lsum = xor_sum<32>(run.l);
         if (l32 < s.x.rows) {
 #pragma unroll
             for (int t = 0; t < D / 32; ++t)
@@ -942,7 +948,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                     *reinterpret_cast<float4*>(&joined[(wave * 32 + l32) * D + 32 * t + tile_index(i)]) =
                         make_float4(o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]);
             if (lane < 32) {
-                mw[wave][l32] = m;
+                mw[wave][l32] = run.m;
                 lw[wave][l32] = lsum;
             }
         }
@@ -1022,7 +1028,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
         for (int t = 0; t < D / 32; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-        float m = -INFINITY, l = 0.0f;
+        Running run;
 
         // the page of the lane's position in unit u
         auto page_of = [&](uint32_t u) {
@@ -1097,9 +1103,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
-                rescale<T>(xor_max<32>(mx), p.scale, m, l, o);
+                rescale<T>(xor_max<32>(mx), p.scale, run, o);
                 float k = p.scale, c;
-                exponents(m, k, c, sc[0], sc[1]);
+                exponents(run, k, c, sc[0], sc[1]);
                 float sum = 0.0f;  // as in the few-rows kernel
                 auto weights = [&](int st) {  // the 16 positions of step st: their weights, rounded; sum adds the unrounded
                     f32x16& x = sc[st >> 1];
@@ -1121,7 +1127,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
                     for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(vt[st & 1][t], w, o[t]);
                     if (st < 3) w = weights(st + 1);
                 }
-                l += sum;
+                run.l += sum;
                 cur ^= 1;
                 page = npage;
                 npage = far;
@@ -1132,7 +1138,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
         } else {
             next_segment<false, kBm>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
-        const float L = xor_sum<32>(l);
+        const float L = xor_sum<32>(run.l);
         const PagedAttn& e_ = arguments();
         if (trow < s.x.rows) {
             if (s.pieces == 0) {
@@ -1153,7 +1159,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
                     for (int i = 0; i < 16; i += 4)
                         *reinterpret_cast<float4*>(dst + piece_place(blocks, trow, D, 32 * t + tile_index(i))) =
                             make_float4(o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]);
-                if (h2 == 0) e_.many_ml[uint64_t(s.slot) * e_.many_slot + trow] = make_float2(m, L);
+                if (h2 == 0) e_.many_ml[uint64_t(s.slot) * e_.many_slot + trow] = make_float2(run.m, L);
             }
         }
     }
