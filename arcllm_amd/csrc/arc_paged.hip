@@ -261,7 +261,8 @@ __global__ __launch_bounds__(NT) void k_plan(PlanArgs a)
 }
 
 // The rows of a large step, one per thread, from the starts, lengths and tables that k_plan left.  IN_LDS: all
-// starts, for the search.
+// starts, for the search, while they fit 16 KB: 700 requests, the call 11.2 us instead of 12.1; 1500, 19.0 and 19.4; at the
+// limit their copy costs what it saves (4000: 30.8, from memory 29.1), and beyond more (8000: 54.4 and 49.0).
 constexpr uint32_t kStartsInLds = 4096;
 template <bool IN_LDS>
 __global__ __launch_bounds__(256) void k_plan_rows(PlanArgs a)
@@ -284,13 +285,15 @@ __global__ __launch_bounds__(256) void k_plan_rows(PlanArgs a)
     a.slots[n] = (a.tables[uint64_t(b) * a.max_pages + (pos >> a.shift)] << a.shift) | (pos & ((1u << a.shift) - 1u));
 }
 
-// Rows that one workgroup writes itself; more go to a launch of their own.
+// Rows that one workgroup writes itself; more go to a launch of their own.  24 requests, 1000, 4000 and 8000 rows: 7.3, 8.7
+// and 10.2 us in one launch, 9.3 to 9.4 in two; one row a request: 3000 in 20.9 and 25.1, 6000 in 40.8 and 39.2.
 constexpr uint32_t kPlanRowsInOne = 4096;
 
 void launch_plan(const PlanArgs& a, hipStream_t st)
 {
     if (a.rows > kPlanRowsInOne) hipLaunchKernelGGL((k_plan<1024, false>), dim3(1), dim3(1024), 0, st, a);
-    // a small step: 4 waves, whose barriers cost less than 16 waves'
+    // a small step: 4 waves, whose barriers cost less than 16 waves': 24 requests 4.7 us instead of 7.3, 256 5.0 instead
+    // of 7.4, 900 rows 4.8 instead of 7.2; 512 requests are more than a thread's each (6.7 and 7.3), 1000 11.4 and 7.5
     else if (a.requests <= 256 && a.rows <= 1024) hipLaunchKernelGGL((k_plan<256, true>), dim3(1), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_plan<1024, true>), dim3(1), dim3(1024), 0, st, a);
 }
@@ -336,8 +339,8 @@ __device__ __forceinline__ void load4(const X* p, float* f)
 // second (of what is left of them), so that neighbouring lanes load neighbouring 16 bytes.  Every lane computes
 // its own 4 angles: about 150 instructions against 48 bytes moved, which the memory time of a large
 // step covers, and a small one waits for no barrier.  Bound by HBM: N (heads + 2 kv_heads) dim
-// values read and written once; 8192 rows of 36 heads of 128, fp32 to fp16 (201 MB): 46 us, 4.4 TB/s, where a copy
-// reaches 4.7.
+// values read and written once; 8192 rows of 36 heads of 128, fp32 to fp16 (201 MB): 46 us with other inputs in each call,
+// 4.4 TB/s, where a copy reaches 4.7 (35.6 us with one input over and over, part of which the last cache then holds).
 template <typename X, typename T>
 __device__ __forceinline__ void rope_unit(const RopeArgs& a, uint32_t n, uint32_t u, uint32_t slot, uint32_t pos)
 {

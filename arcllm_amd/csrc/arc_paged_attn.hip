@@ -43,7 +43,9 @@ constexpr uint32_t tile_ends(bool few, uint32_t bm) { return few ? 256 : bm; }
 constexpr float kLazy = 8.0f;          // see rescale
 template <typename T>
 constexpr float kLift = __is_same(T, _Float16) ? 7.0f : 0.0f;
-constexpr uint32_t kManyPieces = 8;    // a tile in more pieces is joined in another way
+// A tile in more pieces is joined in another way.  8 (16, 4): a chunk of 500 at 2500, 28 heads of 128, 40 us (42, 56); 700
+// at 700, 64 of 64, 28 (30, 44); 100 at 8000, 28 of 128, 47 (51, 45); but 256 at 2000 50 (33, 45), 256 at 8000 70 (52, 65).
+constexpr uint32_t kManyPieces = 8;
 
 // What a part of a tile left in the workspace, one per slot; two slots per
 // workgroup (its part may end one tile and begin another).
@@ -646,7 +648,7 @@ __device__ __forceinline__ void hide(f32x16& sc, uint32_t bits)
 // every exponent is in R too, so only the size of the weights knows of it (by 2^-13 powers of two at kLarge, 16 at 2^28,
 // which no 16-bit weight survives).  Beyond, R is m * scale itself and the exponent (score - m) * scale, exact where it
 // counts, for one instruction more a score: a branch that scores of models do not take, on a flag that changes with m.  It
-// costs up to 1 % (64 requests of up to 8000 56.8 -> 57.0 us, a chunk of 4096 at 12288 897 -> 900); decided again in each unit
+// costs 0 to 2 % (64 requests of up to 8000 56.8 -> 57.0 us, a chunk of 4096 at 12288 897 -> 900); decided again in each unit
 // 1.4 % (909).  The form of large scores for all would add an instruction to the seven that each score has.
 constexpr float kLarge = 4096.0f;
 __device__ __forceinline__ float offset_of(float m, float scale)
@@ -829,8 +831,8 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 // the wave's own LDS rows, in whole rows.  S^T = K Q^T (lane -> query), O^T = V^T P^T, P^T from the
 // scores' registers.  The next unit's K is on its way as soon as this one's scores are done, its V
 // after the output: with 8 waves a CU some 110 KB of 128 are in flight.  Measured, the call with its join: 64
-// requests of up to 8000, 28 heads on 4 (271 MB) 56 us, 4.8 TB/s, of which 3 are the walk and 4 the join; 2 of
-// 131071, 64 on 8 (732 MB) 125 us, 5.9 TB/s; plain reads of as much reach 6.2.
+// requests of up to 8000, 28 heads on 4 (271 MB) 57 us, 4.8 TB/s, of which 3 are the walk and 4 the join; 2 of
+// 131071, 64 on 8 (732 MB) 123 us, 5.9 TB/s; plain reads of as much reach 6.2.  Pages of 1 to 8 positions: as long.
 template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 {
@@ -989,9 +991,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 // unit's 64 rows of K and V come straight into LDS, shared by the waves and double buffered:
 // unit u + 1 is copied while unit u is computed; one barrier per unit.  Operands as in the
 // few-rows kernel, K's read from LDS.  Measured: 4096 tokens at 12288, 28 heads of 128 on 4, 842 GFLOP that are
-// seen: 830 to 900 us, 1.0 PFLOP/s of the 1.23 that a large fp16 product reaches; with zeros for data 650 us, so the
-// clock under the matrix cores' power is what is left.  3 x 2000 tokens in a window of 1024, heads of 64: 130 us,
-// 0.54 PFLOP/s, bound by the softmax's vector instructions, as many per score as heads of 128 have for twice the
+// seen: 850 to 910 us by the card, 0.93 to 0.99 PFLOP/s of the 1.23 that a large fp16 product reaches; with zeros for data 650 us, so the
+// clock under the matrix cores' power is what is left.  3 x 2000 tokens in a window of 1024, heads of 64: 137 to
+// 146 us, 0.5 PFLOP/s, bound by the softmax's vector instructions, as many per score as heads of 128 have for twice the
 // products.
 template <typename T, int D, int NW, bool WIDE>
 __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAttn)

@@ -396,10 +396,12 @@ size_t arc_paged_attention_workspace_bytes(const arc_kv_pages *pages, const arc_
  * elements from row to row (multiples of 8), 16-byte aligned, sharing no memory
  * with each other (refused) or the pages (not checked).  hpk 1..64; scale 0 means
  * 1 / sqrt(head_dim), else |scale| is at most 2^127.
- * Scores, softmax and sums are fp32, right for finite scores of any size; weights enter the V product rounded to
- * pages->dtype.  A position whose table entry is not below num_pages is not
- * seen, and a row that sees nothing, or whose scores are all -infinity, is 0; what lies in
- * the pages at positions not seen (infinities, NaN) does not matter.  Rows behind the last request are left as they
+ * Scores, softmax and sums are fp32, for finite scores of any size; weights enter the V product rounded to
+ * pages->dtype (in fp16 those below 2^-32 of the largest are 0), which puts a row a fifth to a third further from
+ * the exact one than its own rounding does.  A position whose table entry is not below num_pages is not
+ * seen, and a row that sees nothing, or whose scores are all -infinity beside finite values, is 0; what lies in
+ * the pages at positions not seen (infinities, NaN) does not matter.  An infinity of V seen at a weight that
+ * rounds to 0 gives itself or NaN.  Rows behind the last request are left as they
  * were.  workspace: arc_paged_attention_workspace_bytes() bytes, 256-byte aligned,
  * any contents, for one call at a time (calls in order on one stream may share it; two
  * graphs that may run at once, or two streams, need one each).  Of the batch, all but
