@@ -97,3 +97,17 @@ def test_one_sharp_key_before_a_long_context(dtype, below, new, requests, dim):
     assert np.abs(ref - 1).max() < 1e-9
     err = np.abs(px.pl.from_bits(bits, dtype) - 1.0).max()
     assert err <= tol.max(), (err, tol.max())
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("scale", [1e-45, 1e-38, 2.0 ** -100, 2.0 ** -30, 2.0 ** 100, 2.0 ** 127])
+@pytest.mark.parametrize("dtype", [arc.F16, arc.BF16])
+def test_scales_of_any_size(dtype, scale, new):
+    """Whole scores 0 .. 3: means of V where the scale leaves them equal, of V at the largest score where it does not."""
+    s = px.GivenStep([500, 20], [new, 1], 16, 2, 2, 64, dtype, SEED + 3)
+    s.give_q(1.0)
+    for b, n in enumerate(s.lens):
+        k = np.zeros((int(n), 2, 64))
+        k[:, :, 7] = np.random.default_rng(b).integers(0, 4, (int(n), 2))
+        s.give(b, k)
+    s.check_exact(s.upload().attention(scale=scale), scale, 600)
