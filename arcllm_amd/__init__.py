@@ -135,6 +135,9 @@ class Residency(C.Structure):
 F32, F16, BF16 = 0, 1, 30  # arc_dtype (ggml type ids)
 NO_SLOT = PAGED_RELEASE = 0xFFFFFFFF
 PLAN_NO_PAGES, PLAN_TABLE, PLAN_TOKENS, PLAN_MAX_NEW, PLAN_FREE_LIST = 1, 2, 4, 8, 16
+NO_PARENT = NO_TOKEN = 0xFFFFFFFF
+TREE_MAX_WORDS = 32
+FP8_BLOCK = 128
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
 
@@ -176,6 +179,37 @@ class Rope(C.Structure):
         self._keep = phases
 
 
+class Tree(C.Structure):
+    """arc_tree: trees of drafted tokens in a step, by each row's parent, and the masks made from them."""
+
+    _fields_ = [("parents", _P), ("masks", _P), ("mask_words", _U32)]
+
+    def __init__(self, parents, masks, mask_words: int):
+        super().__init__(_ptr(parents), _ptr(masks), mask_words)
+        self._keep = (parents, masks)
+
+
+class Fp8Rows(C.Structure):
+    """arc_fp8_rows: activations in e4m3, scales [blocks of 128 columns][lds].  ldq defaults to cols, lds to rows."""
+
+    _fields_ = [("q", _P), ("scales", _P), ("rows", _U32), ("cols", _U32), ("ldq", _U32), ("lds", _U32)]
+
+    def __init__(self, q, scales, rows: int, cols: int, ldq: Optional[int] = None, lds: Optional[int] = None):
+        super().__init__(_ptr(q), _ptr(scales), rows, cols, cols if ldq is None else ldq, rows if lds is None else lds)
+        self._keep = (q, scales)
+
+
+class Fp8Weights(C.Structure):
+    """arc_fp8_weights: e4m3 weights, scales [blocks of 128 rows][lds].  ldw defaults to cols, lds to its blocks."""
+
+    _fields_ = [("w", _P), ("scales", _P), ("rows", _U32), ("cols", _U32), ("ldw", _U32), ("lds", _U32)]
+
+    def __init__(self, w, scales, rows: int, cols: int, ldw: Optional[int] = None, lds: Optional[int] = None):
+        super().__init__(_ptr(w), _ptr(scales), rows, cols, cols if ldw is None else ldw,
+                         (cols + FP8_BLOCK - 1) // FP8_BLOCK if lds is None else lds)
+        self._keep = (w, scales)
+
+
 _SIGS.update({
     "arc_model_dims_qwen25_7b": [C.POINTER(ModelDims)],
     "arc_model_tensor_info": [C.POINTER(ModelDims), C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(_U32),
@@ -208,7 +242,22 @@ _SIGS.update({
     "arc_paged_attention": [C.POINTER(KvPages), C.POINTER(PagedBatch), _P, _U32, _U32, _F, _U32, _U32, _P, _U32, _P,
                             _P],
 })
-_RESTYPE["arc_paged_attention_workspace_bytes"] = C.c_size_t
+_SIGS.update({
+    "arc_tree_plan": [C.POINTER(PagedBatch), C.POINTER(Tree), _P],
+    "arc_tree_attention_workspace_bytes": [C.POINTER(KvPages), C.POINTER(PagedBatch), _U32],
+    "arc_tree_attention": [C.POINTER(KvPages), C.POINTER(PagedBatch), C.POINTER(Tree), _P, _U32, _U32, _F, _U32, _U32, _P,
+                           _U32, _P, _P],
+    "arc_tree_commit_workspace_bytes": [C.POINTER(PagedBatch)],
+    "arc_tree_commit": [C.POINTER(KvPages), _U32, C.POINTER(PagedBatch), C.POINTER(Tree), C.c_int, _P, _U64, _U32, _P, _P,
+                        _P, _P, _P, _P, _U32, _P, _P, _P, _P],
+    "arc_fp8_quantize": [C.c_int, _P, _U32, C.POINTER(Fp8Rows), _P],
+    "arc_fp8_gemm_workspace_bytes": [_U32, _U32, _U32, C.c_int],
+    "arc_fp8_gemm": [C.POINTER(Fp8Weights), C.POINTER(Fp8Rows), C.c_int, _P, _U32, _P, _U32, _P, _P],
+    "arc_fp8_gateup": [C.POINTER(Fp8Weights), C.POINTER(Fp8Weights), C.POINTER(Fp8Rows), C.c_int, _P, _U32, _P, _P],
+})
+_RESTYPE.update({name: C.c_size_t for name in
+                 ("arc_paged_attention_workspace_bytes", "arc_tree_attention_workspace_bytes",
+                  "arc_tree_commit_workspace_bytes", "arc_fp8_gemm_workspace_bytes")})
 _RESTYPE.update({"arc_model_weight_bytes": _U64, "arc_session_kernels_per_step": _U32,
                  "arc_session_prefill_kernels": _U32})
 
@@ -576,6 +625,72 @@ def paged_attention(pages: KvPages, batch: PagedBatch, q, ldq: int, hpk: int, ou
     `sinks` ones (arc_paged_attention).  scale 0: 1 / sqrt(head_dim)."""
     check(lib().arc_paged_attention(C.byref(pages), C.byref(batch), _ptr(q), ldq, hpk, scale, window, sinks,
                                     _ptr(out), ldo, _ptr(workspace), _sp(stream)))
+
+
+def tree_plan(batch: PagedBatch, tree: Tree, stream: Optional[Stream] = None) -> None:
+    """Masks and positions of a step's rows from their parents (arc_tree_plan)."""
+    check(lib().arc_tree_plan(C.byref(batch), C.byref(tree), _sp(stream)))
+
+
+def tree_attention_workspace_bytes(pages: KvPages, batch: PagedBatch, hpk: int) -> int:
+    n = int(lib().arc_tree_attention_workspace_bytes(C.byref(pages), C.byref(batch), hpk))
+    if n == 0:
+        raise ArcError(2, f"no tree-attention workspace size for {pages.kv_heads} kv heads, {hpk} query heads each, "
+                          f"head_dim {pages.head_dim}")
+    return n
+
+
+def tree_attention(pages: KvPages, batch: PagedBatch, tree: Tree, q, ldq: int, hpk: int, out, ldo: int, workspace,
+                   scale: float = 0.0, window: int = 0, sinks: int = 0, stream: Optional[Stream] = None) -> None:
+    """Attention of trees of drafted tokens (and of prompts' chunks) over the pages: the context and, of the
+    step's own rows, those that a row's mask names (arc_tree_attention)."""
+    check(lib().arc_tree_attention(C.byref(pages), C.byref(batch), C.byref(tree), _ptr(q), ldq, hpk, scale, window,
+                                   sinks, _ptr(out), ldo, _ptr(workspace), _sp(stream)))
+
+
+def tree_commit_workspace_bytes(batch: PagedBatch) -> int:
+    n = int(lib().arc_tree_commit_workspace_bytes(C.byref(batch)))
+    if n == 0:
+        raise ArcError(2, f"no tree-commit workspace size for {batch.requests} requests, {batch.tokens} rows")
+    return n
+
+
+def tree_commit(layers, batch: PagedBatch, tree: Tree, drafts, targets, lens_out, counts, tokens_out, workspace,
+                free_pages=None, num_pages: int = 0, free_count=None, free_count_out=None, logits=None,
+                logits_dtype: int = F32, ldl: int = 0, vocab: int = 0, stream: Optional[Stream] = None) -> None:
+    """The walk down each tree, the accepted rows' move in the pages of every layer (`layers`: KvPages), lengths
+    and the pages that go back (arc_tree_commit).  With logits, `targets` is written, else read."""
+    pools = (KvPages * len(layers))(*layers)
+    check(lib().arc_tree_commit(pools, len(layers), C.byref(batch), C.byref(tree), logits_dtype, _ptr(logits), ldl, vocab,
+                                _ptr(drafts), _ptr(targets), _ptr(lens_out), _ptr(counts), _ptr(tokens_out),
+                                _ptr(free_pages), num_pages, _ptr(free_count), _ptr(free_count_out), _ptr(workspace),
+                                _sp(stream)))
+
+
+def fp8_quantize(x_dtype: int, x, ldx: int, rows: Fp8Rows, stream: Optional[Stream] = None) -> None:
+    """Rows of x to e4m3 with a scale for each block of 128 columns (arc_fp8_quantize)."""
+    check(lib().arc_fp8_quantize(x_dtype, _ptr(x), ldx, C.byref(rows), _sp(stream)))
+
+
+def fp8_gemm_workspace_bytes(n: int, k: int, rows: int, gated: bool = False) -> int:
+    size = int(lib().arc_fp8_gemm_workspace_bytes(n, k, rows, 1 if gated else 0))
+    if size == 0:
+        raise ArcError(2, f"no fp8 product workspace size for {rows} rows, {n} x {k} weights")
+    return size
+
+
+def fp8_gemm(w: Fp8Weights, rows: Fp8Rows, y_dtype: int, y, ldy: int, workspace, residual=None, ldr: int = 0,
+             stream: Optional[Stream] = None) -> None:
+    """y = rows . w^T (+ residual) in e4m3 with scales by blocks of 128 (arc_fp8_gemm)."""
+    check(lib().arc_fp8_gemm(C.byref(w), C.byref(rows), y_dtype, _ptr(y), ldy, _ptr(residual), ldr, _ptr(workspace),
+                             _sp(stream)))
+
+
+def fp8_gateup(gate: Fp8Weights, up: Fp8Weights, rows: Fp8Rows, y_dtype: int, y, ldy: int, workspace,
+               stream: Optional[Stream] = None) -> None:
+    """y = silu(rows . gate^T) * (rows . up^T) (arc_fp8_gateup)."""
+    check(lib().arc_fp8_gateup(C.byref(gate), C.byref(up), C.byref(rows), y_dtype, _ptr(y), ldy, _ptr(workspace),
+                               _sp(stream)))
 
 
 def tune_force(bs: int, rpl: int) -> None:

@@ -14,6 +14,10 @@
 // tile in one part is written out; a part of one leaves its sums in the workspace
 // (Piece) and k_paged_join adds the pieces of a tile in order, so results do not
 // depend on timing.
+//
+// Trees (TREE).  A request's rows may be the nodes of a tree of drafted tokens: node i lies at place i behind the
+// context, sees all of that (its window's part) and the nodes that its mask names, none of them behind itself.  So a
+// tile runs over the same units as a causal one, and only those that reach behind the context look at masks.
 #include "arc_paged.hpp"
 
 #include <cmath>
@@ -71,6 +75,8 @@ struct PagedAttn {
     Piece *few_p, *many_p;
     uint32_t few_slot, many_slot;  // rows of a slot
     uint32_t few_wgs, many_wgs;    // workgroups of this call's launches (0: not launched)
+    const uint32_t *masks, *positions;  // of trees
+    uint32_t words;
 };
 
 // The kernel's arguments (its one parameter, a PagedAttn), read again: a phase that takes its own copy keeps
@@ -106,7 +112,10 @@ __device__ __forceinline__ double cost_before(const Request& r, uint32_t t, doub
     return k * r.first + bm * (k * (k - 1.0) * 0.5) + (n > k ? (n - k) * r.cap : 0.0);
 }
 
-template <bool FEW, uint32_t bm>
+// Whether a request's rows are a tree, not a chunk.
+__device__ __forceinline__ bool is_tree(const PagedAttn& a, const Request& r) { return r.rows <= 32 * a.words * a.hpk; }
+
+template <bool TREE, bool FEW, uint32_t bm>
 __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, uint32_t s1, uint32_t held)
 {
     constexpr uint32_t keys = FEW ? kFewKeys : kManyKeys, ends = tile_ends(FEW, bm);
@@ -121,10 +130,11 @@ __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, u
     r.base = int32_t(max(base, -(int64_t(1) << 25)));
     r.tiles = (rows + bm - 1) / bm;
     r.first = double(ends + uint32_t(max(r.base, 0))) * a.hpk + bm;
-    r.cap = a.window ? (double(ends) + a.window + a.sinks) * a.hpk + 2 * bm : 0x1p60;
+    const uint32_t nodes = TREE && is_tree(a, r) ? rows : 0;  // the tree lies behind the first node's window
+    r.cap = a.window ? (double(ends) + a.window + a.sinks) * a.hpk + nodes + 2 * bm : 0x1p60;
     r.total = r.tiles == 1 ? fmin(r.first, r.cap) : cost_before(r, r.tiles, bm);
     const float spans = float(r.tiles) * ceilf(float(len) * (1.0f / keys));
-    r.units = a.window ? fminf(spans, float(r.tiles) * (ceilf((float(a.window) + float(a.sinks)) * (1.0f / keys)) + 2.0f)) : spans;
+    r.units = a.window ? fminf(spans, float(r.tiles) * (ceilf((float(a.window) + float(a.sinks) + float(nodes / a.hpk)) * (1.0f / keys)) + 2.0f)) : spans;
     r.units = fmaxf(r.units, 1.0f);
     return r;
 }
@@ -138,12 +148,14 @@ struct Tile {
     uint32_t units;
 };
 
+template <bool TREE>
 __device__ __forceinline__ Tile tile_at(const PagedAttn& a, const Request& r, uint32_t t, uint32_t bm, uint32_t keys)
 {
     Tile x;
     x.row0 = t * bm;
     x.rows = min(bm, r.rows - x.row0);
     x.pos0 = r.base + int32_t(x.row0 / a.hpk);
+    if (TREE && is_tree(a, r)) x.pos0 = r.base - 1;  // what all rows see ends with the context, as do their windows
     x.pos1 = r.base + int32_t((x.row0 + x.rows - 1) / a.hpk);
     const uint32_t end = uint32_t(max(x.pos1 + 1, 0));
     const uint32_t all = (end + keys - 1) / keys;
@@ -244,18 +256,18 @@ __device__ __forceinline__ void take_part(Walk& l, double total, float units)
 struct Heads {
     uint32_t s0[64], s1[64], len[64];
 };
-template <bool FEW, uint32_t bm>
+template <bool TREE, bool FEW, uint32_t bm>
 __device__ __forceinline__ Request request_at(const PagedAttn& a, const Heads& h, uint32_t b)
 {
-    if (a.requests <= 64) return request_of<FEW, bm>(a, h.s0[b], h.s1[b], h.len[b]);
-    return request_of<FEW, bm>(a, a.starts[b], a.starts[b + 1], a.lens[b]);
+    if (a.requests <= 64) return request_of<TREE, FEW, bm>(a, h.s0[b], h.s1[b], h.len[b]);
+    return request_of<TREE, FEW, bm>(a, a.starts[b], a.starts[b + 1], a.lens[b]);
 }
 
 // Wave 0: the segment of request r, b of the step, that lies at m.at, and the part's way on.  A cut tile gets its slot
 // and its record for k_paged_join.  One wave's work that all others wait for, a chain of dependent steps: so
 // searches are by 64 lanes at once, and what is needed twice (of a tile's ends, a part's ends) is computed in the lower
 // and the upper lanes.
-template <bool FEW, uint32_t bm>
+template <bool TREE, bool FEW, uint32_t bm>
 __device__ __forceinline__ void cut_segment(const PagedAttn& a, Walk& m, const Request& r)
 {
     constexpr uint32_t keys = FEW ? kFewKeys : kManyKeys;
@@ -279,7 +291,7 @@ __device__ __forceinline__ void cut_segment(const PagedAttn& a, Walk& m, const R
         begin = of_lane(ends, 0);
         end = of_lane(ends, 32);
     }
-    m.x = tile_at(a, r, t, bm, keys);
+    m.x = tile_at<TREE>(a, r, t, bm, keys);
     const uint32_t units = units_before(upper ? m.to : m.at, begin, end, m.x.units);
     m.u0 = uint32_t(__builtin_amdgcn_readlane(int(units), 0));
     m.u1 = uint32_t(__builtin_amdgcn_readlane(int(units), 32));
@@ -299,18 +311,18 @@ __device__ __forceinline__ void cut_segment(const PagedAttn& a, Walk& m, const R
 }
 
 // Wave 0: the part's next segment after l's.
-template <bool FEW, uint32_t bm>
+template <bool TREE, bool FEW, uint32_t bm>
 __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, Walk& to, const Heads& h)
 {
     if (threadIdx.x >= 64) return;
     Walk m = l;
     m.go = m.at < m.to;
     if (m.go) {
-        Request r = request_at<FEW, bm>(a, h, m.b);  // the request at m.at: this one, or one of those behind it
+        Request r = request_at<TREE, FEW, bm>(a, h, m.b);  // the request at m.at: this one, or one of those behind it
         while (m.at >= m.before + r.total * a.kv_heads) {
             m.before += r.total * a.kv_heads;
             const uint32_t next = ++m.b + threadIdx.x;
-            if (next < a.requests) r = request_at<FEW, bm>(a, h, next);
+            if (next < a.requests) r = request_at<TREE, FEW, bm>(a, h, next);
             const double own = next < a.requests ? r.total * a.kv_heads : 0.0, inc = wave_inclusive(own);
             const uint64_t behind = __ballot(m.before + inc > m.at);
             if (behind == 0 && m.b + 64 >= a.requests) {  // starts or lens changed during the call
@@ -321,9 +333,9 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, 
             const int i = behind ? __builtin_ctzll(behind) : 63;
             m.b += uint32_t(i);
             m.before += of_lane(inc - own, i);
-            r = request_at<FEW, bm>(a, h, m.b);
+            r = request_at<TREE, FEW, bm>(a, h, m.b);
         }
-        cut_segment<FEW, bm>(a, m, r);
+        cut_segment<TREE, FEW, bm>(a, m, r);
     }
     if (threadIdx.x == 0) to = m;
 }
@@ -331,7 +343,7 @@ __device__ __forceinline__ void next_segment(const PagedAttn& a, const Walk& l, 
 // Adds up the requests, so that no launch has to come first, and finds the one in which the
 // part begins and its first segment, `to`.  Up to 64 requests: wave 0 alone, one per lane.  More: thread t takes a run
 // of them, l says where the part begins and next_segment, which wave 0 runs too, goes on from there.
-template <bool FEW, uint32_t bm, int NT>
+template <bool TREE, bool FEW, uint32_t bm, int NT>
 __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Walk& to, Heads& h, double* red)
 {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
@@ -343,7 +355,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Walk& to
             h.s0[lane] = s0;
             h.s1[lane] = s1;
             h.len[lane] = len;
-            r = request_of<FEW, bm>(a, s0, s1, len);
+            r = request_of<TREE, FEW, bm>(a, s0, s1, len);
         }
         const double own = r.total * a.kv_heads, inc = wave_inclusive(own);
         Walk m;
@@ -358,7 +370,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Walk& to
             const Request rb{uint32_t(__builtin_amdgcn_readlane(int(r.token), b)), uint32_t(__builtin_amdgcn_readlane(int(r.rows), b)),
                              __builtin_amdgcn_readlane(r.base, b), uint32_t(__builtin_amdgcn_readlane(int(r.tiles), b)),
                              of_lane(r.first, b), of_lane(r.cap, b), of_lane(r.total, b), 0.0f};
-            cut_segment<FEW, bm>(a, m, rb);
+            cut_segment<TREE, FEW, bm>(a, m, rb);
         }
         if (lane == 0) to = m;
         return;
@@ -369,7 +381,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Walk& to
     float units = 0.0f;
 #pragma unroll 4
     for (uint32_t b = b0; b < b1; ++b) {
-        const Request r = request_at<FEW, bm>(a, h, b);
+        const Request r = request_at<TREE, FEW, bm>(a, h, b);
         sum += r.total * a.kv_heads;
         units += r.units;
     }
@@ -401,7 +413,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Walk& to
         double at = lo;
         uint32_t b = b0;
         for (; b + 1 < b1; ++b) {
-            const double c = request_at<FEW, bm>(a, h, b).total * a.kv_heads;
+            const double c = request_at<TREE, FEW, bm>(a, h, b).total * a.kv_heads;
             if (at + c > m.at) break;
             at += c;
         }
@@ -410,7 +422,7 @@ __device__ __forceinline__ void start_walk(const PagedAttn& a, Walk& l, Walk& to
     }
     __syncthreads();
     if (tid == 0) (FEW ? a.few_p : a.many_p)[2 * m.w].n = (FEW ? a.few_p : a.many_p)[2 * m.w + 1].n = 0;
-    next_segment<FEW, bm>(a, l, to, h);
+    next_segment<TREE, FEW, bm>(a, l, to, h);
 }
 
 // What every wave needs of the segment, in scalar registers.
@@ -634,6 +646,72 @@ __device__ __forceinline__ uint32_t seen_bits(int32_t qpos, int32_t k0, uint32_t
     return bits;
 }
 
+// What a lane's query sees: its position in the cache, and, where its request's rows are a tree, its mask.
+template <bool TREE>
+struct Sight {
+    int32_t qpos;
+    __device__ __forceinline__ uint32_t bits(int32_t k0, uint32_t window, uint32_t sinks) const
+    {
+        return seen_bits(qpos, k0, window, sinks);
+    }
+    __device__ __forceinline__ bool at(int32_t kpos, uint32_t window, uint32_t sinks) const { return sees(qpos, kpos, window, sinks); }
+};
+template <>
+struct Sight<true> {
+    int32_t qpos;
+    int32_t base;          // place of node 0
+    int32_t depth;         // of the row's node
+    uint32_t words;        // of its mask; 0: a chunk's row
+    const uint32_t* mask;
+    __device__ __forceinline__ uint32_t word(int32_t w) const { return uint32_t(w) < words ? mask[w] : 0; }
+    // Of the nodes in `nodes`, from node `first` on, those that a window leaves: node j is as deep as the mask has
+    // bits below j.
+    __device__ __forceinline__ uint32_t in_window(uint32_t nodes, int32_t first, uint32_t window, uint32_t sinks) const
+    {
+        uint32_t left = 0;
+        for (; nodes; nodes &= nodes - 1) {
+            const uint32_t t = uint32_t(__builtin_ctz(nodes)), j = uint32_t(first + int32_t(t));
+            int32_t d = __builtin_popcount(word(int32_t(j >> 5)) & ((1u << (j & 31u)) - 1u));
+            for (uint32_t w = 0; w < (j >> 5); ++w) d += __builtin_popcount(word(int32_t(w)));
+            if (uint32_t(max(depth - d, 0)) < window || uint32_t(max(base + d, 0)) < sinks) left |= 1u << t;
+        }
+        return left;
+    }
+    __device__ __forceinline__ uint32_t bits(int32_t k0, uint32_t window, uint32_t sinks) const
+    {
+        if (words == 0) return seen_bits(qpos, k0, window, sinks);
+        const int32_t first = k0 - base;  // the node at k0
+        const uint32_t context = first >= 0 ? 0u : first <= -32 ? ~0u : (1u << -first) - 1u;
+        uint32_t seen = context ? context & seen_bits(base + depth, k0, window, sinks) : 0u;
+        if (context != ~0u) {
+            const int32_t w = first >> 5;
+            uint32_t nodes = uint32_t(((uint64_t(word(w + 1)) << 32) | word(w)) >> (uint32_t(first) & 31u));
+            nodes &= seen_bits(qpos, k0, 0, 0);
+            if (window && uint32_t(depth) >= window) nodes = in_window(nodes, first, window, sinks);
+            seen |= nodes;
+        }
+        return seen;
+    }
+    __device__ __forceinline__ bool at(int32_t kpos, uint32_t window, uint32_t sinks) const
+    {
+        return bits(kpos & ~31, window, sinks) >> (uint32_t(kpos) & 31u) & 1u;
+    }
+};
+template <bool TREE>
+__device__ __forceinline__ Sight<TREE> sight_of(const PagedAttn& a, const Segment& s, uint32_t row)
+{
+    const uint32_t i = (s.x.row0 + row) / a.hpk;
+    Sight<TREE> v;
+    v.qpos = s.base + int32_t(i);
+    if constexpr (TREE) {
+        v.base = s.base;
+        v.words = s.x.pos0 < s.base ? a.words : 0u;  // see tile_at
+        v.mask = a.masks + uint64_t(s.token + i) * a.words;
+        v.depth = a.window && v.words ? int32_t(a.positions[s.token + i]) - s.base : 0;
+    }
+    return v;
+}
+
 // The scores of a tile of 32 positions that its query does not see become -infinity.
 __device__ __forceinline__ void hide(f32x16& sc, uint32_t bits)
 {
@@ -790,9 +868,9 @@ __device__ __forceinline__ bool clean(T* p, bool in)
 // segment's units, each row that sees such a position gets them.  Units that all rows see
 // need none of it.  A slow pass over the wave's other units (from, from + step ..), for data that has any;
 // first_of and page_of as in the kernels, `span` positions of each unit.
-template <typename T, int D, typename First, typename Page>
+template <typename T, int D, bool TREE, typename First, typename Page>
 __device__ __forceinline__ void add_nonfinite(const Pool<T>& p, f32x16 (&o)[D / 32], const Segment& s, uint32_t from, uint32_t step,
-                                              uint32_t span, int32_t qpos, First first_of, Page page_of)
+                                              uint32_t span, const Sight<TREE>& sight, First first_of, Page page_of)
 {
 #pragma unroll 1
     for (uint32_t u = from; u < s.u1; u += step) {
@@ -802,7 +880,7 @@ __device__ __forceinline__ void add_nonfinite(const Pool<T>& p, f32x16 (&o)[D / 
 #pragma unroll 1
         for (uint32_t j = 0; j < span; ++j) {
             const uint32_t pg = uint32_t(__builtin_amdgcn_readlane(int(page), int(j)));
-            if (pg >= p.num_pages || !sees(qpos, k0 + int32_t(j), p.window, p.sinks)) continue;
+            if (pg >= p.num_pages || !sight.at(k0 + int32_t(j), p.window, p.sinks)) continue;
             const T* row = p.v + row_offset(p, pg, uint32_t(k0) + j);
 #pragma unroll
             for (int t = 0; t < D / 32; ++t)
@@ -833,7 +911,7 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 // after the output: with 8 waves a CU some 110 KB of 128 are in flight.  Measured, the call with its join: 64
 // requests of up to 8000, 28 heads on 4 (271 MB) 57 us, 4.8 TB/s, of which 3 are the walk and 4 the join; 2 of
 // 131071, 64 on 8 (732 MB) 123 us, 5.9 TB/s; plain reads of as much reach 6.2.  Pages of 1 to 8 positions: as long.
-template <typename T, int D, bool WIDE>
+template <typename T, int D, bool WIDE, bool TREE>
 __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 {
     __shared__ struct {  // rows first: m0, which says where a copy goes, is used below 2^16 only
@@ -850,7 +928,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
     Heads& heads = lds.heads;
     double* red = lds.red;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<true, kFewRows, 256>(arguments(), walk[1], walk[0], heads, red);
+    start_walk<TREE, true, kFewRows, 256>(arguments(), walk[1], walk[0], heads, red);
     T* krows = reinterpret_cast<T*>(joined) + wave * (2 * 32 * D);
     T* vrows = krows + 32 * D;
     for (uint32_t turn = 0;; turn ^= 1u) {
@@ -859,7 +937,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
         const Segment s = read_segment(walk[turn]);
         const Pool<T> p = pool_of<T, D>(arguments(), s);
         const uint32_t row = min(l32, s.x.rows - 1);
-        const int32_t qpos = s.base + int32_t((s.x.row0 + row) / arguments().hpk);
+        const Sight<TREE> sight = sight_of<TREE>(arguments(), s, row);
         f32x16 o[D / 32];
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
@@ -881,7 +959,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
             vec8<T> q[D / 16];
             load_q<T, D>(arguments(), s.token, s.x.row0 + row, l32 < s.x.rows, s.g, q);
             copy_rows<true, true, true, 32, WIDE, D>(p, krows, vrows, page, 0, first_of(mine));
-            next_segment<true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while those are on their way
+            next_segment<TREE, true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while those are on their way
             for (uint32_t u = mine; u < s.u1; u += kFewWaves) {
                 const int32_t k0 = int32_t(first_of(u));
                 wait_loads();  // K, V of this unit, the next one's pages
@@ -906,7 +984,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 const bool whole = all_seen(p, s.x, k0, 32, valid == 0xffffffffu);
                 if (!whole) {
                     for (uint32_t c = h2; c < D / 8; c += 2) odd |= clean(vrows + l32 * D + c * 8, in);
-                    hide(sc, valid & seen_bits(qpos, k0, p.window, p.sinks));
+                    hide(sc, valid & sight.bits(k0, p.window, p.sinks));
                     wave_fence();
                 }
                 float mx = sc[0];
@@ -935,9 +1013,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
                 page = npage;
                 npage = far;
             }
-            if (__ballot(odd)) add_nonfinite<T, D>(p, o, s, mine, kFewWaves, 32, qpos, first_of, page_of);
+            if (__ballot(odd)) add_nonfinite<T, D, TREE>(p, o, s, mine, kFewWaves, 32, sight, first_of, page_of);
         } else {
-            next_segment<true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);
+            next_segment<TREE, true, kFewRows>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
         // the waves' states in wave order: out = sum_w f_w o_w / sum_w f_w l_w, f_w to the largest reference M
         __syncthreads();  // every wave is done with its V rows
@@ -995,7 +1073,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 // clock under the matrix cores' power is what is left.  3 x 2000 tokens in a window of 1024, heads of 64: 137 to
 // 146 us, 0.5 PFLOP/s, bound by the softmax's vector instructions, as many per score as heads of 128 have for twice the
 // products.
-template <typename T, int D, int NW, bool WIDE>
+template <typename T, int D, int NW, bool WIDE, bool TREE>
 __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAttn)
 {
     constexpr int NT = NW * 64;
@@ -1015,7 +1093,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
     double* red = lds.red;
     uint32_t& odd = lds.odd;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l32 = lane & 31u, h2 = lane >> 5, wave = uniform(tid >> 6);
-    start_walk<false, kBm, NT>(arguments(), walk[1], walk[0], heads, red);
+    start_walk<TREE, false, kBm, NT>(arguments(), walk[1], walk[0], heads, red);
     for (uint32_t turn = 0;; turn ^= 1u) {
         __syncthreads();  // the tile before is done with LDS
         if (uniform(walk[turn].go) == 0) break;
@@ -1024,7 +1102,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
         const Pool<T> p = pool_of<T, D>(arguments(), s);
         const uint32_t trow = wave * 32 + l32;
         const uint32_t row = min(trow, s.x.rows - 1);
-        const int32_t qpos = s.base + int32_t((s.x.row0 + row) / arguments().hpk);
+        const Sight<TREE> sight = sight_of<TREE>(arguments(), s, row);
         f32x16 o[D / 32];
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
@@ -1047,7 +1125,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
             vec8<T> q[D / 16];
             load_q<T, D>(arguments(), s.token, s.x.row0 + row, trow < s.x.rows, s.g, q);
             copy_unit(s.u0, page, 0);
-            next_segment<false, kBm>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while that is on its way
+            next_segment<TREE, false, kBm>(arguments(), walk[turn], walk[turn ^ 1u], heads);  // while that is on its way
             int cur = 0;
             for (uint32_t u = s.u0; u < s.u1; ++u) {
                 wait_loads();
@@ -1097,8 +1175,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
 #pragma unroll
                 for (int t = 0; t < D / 32; ++t) vt[0][t] = load_vt<T, D>(vs[cur], 0, t);
                 if (!whole) {
-                    hide(sc[0], uint32_t(valid) & seen_bits(qpos, k0, p.window, p.sinks));
-                    hide(sc[1], uint32_t(valid >> 32) & seen_bits(qpos, k0 + 32, p.window, p.sinks));
+                    hide(sc[0], uint32_t(valid) & sight.bits(k0, p.window, p.sinks));
+                    hide(sc[1], uint32_t(valid >> 32) & sight.bits(k0 + 32, p.window, p.sinks));
                 }
                 float mx = sc[0][0];
 #pragma unroll
@@ -1136,9 +1214,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
             }
             // set before the last unit's second barrier, if at all
             if (uniform(odd))
-                add_nonfinite<T, D>(p, o, s, s.u0, 1, kManyKeys, qpos, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); }, page_of);
+                add_nonfinite<T, D, TREE>(p, o, s, s.u0, 1, kManyKeys, sight, [&](uint32_t u) { return unit_start(s.x, u, kManyKeys); }, page_of);
         } else {
-            next_segment<false, kBm>(arguments(), walk[turn], walk[turn ^ 1u], heads);
+            next_segment<TREE, false, kBm>(arguments(), walk[turn], walk[turn ^ 1u], heads);
         }
         const float L = xor_sum<32>(run.l);
         const PagedAttn& e_ = arguments();
@@ -1305,19 +1383,19 @@ Space space_of(uint32_t dim, uint32_t hpk, uint32_t tokens)
     return s;
 }
 
-template <typename T, int D, bool WIDE>
+template <typename T, int D, bool WIDE, bool TREE>
 void launch_tiles(const PagedAttn& a, hipStream_t st)
 {
-    if (a.few_wgs) hipLaunchKernelGGL((k_paged_few<T, D, WIDE>), dim3(a.few_wgs), dim3(256), 0, st, a);
+    if (a.few_wgs) hipLaunchKernelGGL((k_paged_few<T, D, WIDE, TREE>), dim3(a.few_wgs), dim3(256), 0, st, a);
     if (a.many_wgs)
-        hipLaunchKernelGGL((k_paged_many<T, D, many_waves(D), WIDE>), dim3(a.many_wgs), dim3(many_waves(D) * 64), 0, st, a);
+        hipLaunchKernelGGL((k_paged_many<T, D, many_waves(D), WIDE, TREE>), dim3(a.many_wgs), dim3(many_waves(D) * 64), 0, st, a);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TREE>
 hipError_t launch_paged(const PagedAttn& a, hipStream_t st)
 {
-    if (a.shift >= 4) launch_tiles<T, D, true>(a, st);
-    else launch_tiles<T, D, false>(a, st);
+    if (a.shift >= 4) launch_tiles<T, D, true, TREE>(a, st);
+    else launch_tiles<T, D, false, TREE>(a, st);
     if (hipError_t e = hipGetLastError()) return e;
     hipLaunchKernelGGL((k_paged_join<T, D>), dim3(2 * (a.few_wgs + many_split(D) * a.many_wgs)), dim3(256), 0, st, a);
     return hipGetLastError();
@@ -1332,25 +1410,24 @@ int check_sizes(const arc_kv_pages* pages, const arc_paged_batch* batch, uint32_
     return ARC_OK;
 }
 
-}  // namespace
-}  // namespace arc
-
-using namespace arc;
-
-extern "C" {
-
-size_t arc_paged_attention_workspace_bytes(const arc_kv_pages* pages, const arc_paged_batch* batch, uint32_t hpk)
+template <bool TREE>
+hipError_t launch_type(const PagedAttn& a, const arc_kv_pages* pages, hipStream_t st)
 {
-    return check_sizes(pages, batch, hpk) ? 0 : space_of(pages->head_dim, hpk, batch->tokens).bytes;
+    const bool f16 = pages->dtype == ARC_F16;
+    if (pages->head_dim == 64) return f16 ? launch_paged<_Float16, 64, TREE>(a, st) : launch_paged<bf16, 64, TREE>(a, st);
+    return f16 ? launch_paged<_Float16, 128, TREE>(a, st) : launch_paged<bf16, 128, TREE>(a, st);
 }
 
-int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch, const void* q, uint32_t ldq,
-                        uint32_t hpk, float scale, uint32_t window, uint32_t sinks, void* out, uint32_t ldo,
-                        void* workspace, arc_stream_t stream)
+int attention(const arc_kv_pages* pages, const arc_paged_batch* batch, const arc_tree* tree, const void* q, uint32_t ldq, uint32_t hpk,
+              float scale, uint32_t window, uint32_t sinks, void* out, uint32_t ldo, void* workspace, hipStream_t st)
 {
     int rc = check_sizes(pages, batch, hpk);
     if (!rc) rc = check_tables(batch, pages->page_size);
     if (rc) return rc;
+    if (tree && (!tree->masks || (window && !batch->positions)))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "null masks, or positions with a window");
+    if (tree && (tree->mask_words == 0 || tree->mask_words > ARC_TREE_MAX_WORDS))
+        return set_error(ARC_ERR_UNSUPPORTED, "mask_words %u: 1..%u are supported", tree->mask_words, uint32_t(ARC_TREE_MAX_WORDS));
     if (!q || !out || !workspace) return set_error(ARC_ERR_INVALID_ARGUMENT, "null argument");
     const uint32_t width = pages->kv_heads * hpk * pages->head_dim;
     if (ldq < width || ldq % 8 || ldo < width || ldo % 8)
@@ -1392,6 +1469,11 @@ int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch,
     a.sinks = sinks;
     a.scale = s2;
     a.neg = s < 0.0f ? 0x80008000u : 0u;
+    if (tree) {
+        a.masks = tree->masks;
+        a.positions = batch->positions;
+        a.words = tree->mask_words;
+    }
     a.few_p = reinterpret_cast<Piece*>(ws + sp.few_p);
     a.many_p = reinterpret_cast<Piece*>(ws + sp.many_p);
     a.few_ml = reinterpret_cast<float2*>(ws + sp.few_ml);
@@ -1410,11 +1492,40 @@ int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch,
     a.few_rows = !many ? ~0u : few ? kFewRows : 0u;
     a.few_wgs = few ? kFewWgs : 0;
     a.many_wgs = many ? many_wgs(pages->head_dim) : 0;
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool f16 = pages->dtype == ARC_F16;
-    const hipError_t e = pages->head_dim == 64 ? (f16 ? launch_paged<_Float16, 64>(a, st) : launch_paged<bf16, 64>(a, st))
-                                               : (f16 ? launch_paged<_Float16, 128>(a, st) : launch_paged<bf16, 128>(a, st));
-    return check_hip(e, "paged attention");
+    const hipError_t e = tree ? launch_type<true>(a, pages, st) : launch_type<false>(a, pages, st);
+    return check_hip(e, tree ? "tree attention" : "paged attention");
+}
+
+}  // namespace
+}  // namespace arc
+
+using namespace arc;
+
+extern "C" {
+
+size_t arc_paged_attention_workspace_bytes(const arc_kv_pages* pages, const arc_paged_batch* batch, uint32_t hpk)
+{
+    return check_sizes(pages, batch, hpk) ? 0 : space_of(pages->head_dim, hpk, batch->tokens).bytes;
+}
+
+int arc_paged_attention(const arc_kv_pages* pages, const arc_paged_batch* batch, const void* q, uint32_t ldq,
+                        uint32_t hpk, float scale, uint32_t window, uint32_t sinks, void* out, uint32_t ldo,
+                        void* workspace, arc_stream_t stream)
+{
+    return attention(pages, batch, nullptr, q, ldq, hpk, scale, window, sinks, out, ldo, workspace, static_cast<hipStream_t>(stream));
+}
+
+size_t arc_tree_attention_workspace_bytes(const arc_kv_pages* pages, const arc_paged_batch* batch, uint32_t hpk)
+{
+    return check_sizes(pages, batch, hpk) ? 0 : space_of(pages->head_dim, hpk, batch->tokens).bytes;
+}
+
+int arc_tree_attention(const arc_kv_pages* pages, const arc_paged_batch* batch, const arc_tree* tree, const void* q, uint32_t ldq,
+                       uint32_t hpk, float scale, uint32_t window, uint32_t sinks, void* out, uint32_t ldo, void* workspace,
+                       arc_stream_t stream)
+{
+    if (!tree) return set_error(ARC_ERR_INVALID_ARGUMENT, "null tree");
+    return attention(pages, batch, tree, q, ldq, hpk, scale, window, sinks, out, ldo, workspace, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

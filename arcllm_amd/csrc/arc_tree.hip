@@ -1,0 +1,386 @@
+// arc_tree.hip -- a step that verifies trees of drafted tokens: masks and positions from
+// the parents, and the step's end (the target's tokens, the walk down each tree, the
+// accepted rows' move in every layer's pages, the pages that go back).
+//
+// A request's rows are a tree if they are no more than 32 * mask_words, else a prompt's
+// chunk.  Node i's parent is a node before it.
+#include "arc_paged.hpp"
+
+namespace arc {
+namespace {
+
+constexpr uint32_t kMaxLogitRows = 1u << 20;
+constexpr uint32_t kMaxNodes = 32 * ARC_TREE_MAX_WORDS;
+
+// The rows of request b that the step has, and how many starts says; the context's length.
+struct Rows {
+    uint32_t first, n, all;
+};
+__device__ __forceinline__ Rows rows_of(const uint32_t* starts, uint32_t tokens, uint32_t b)
+{
+    const uint32_t s0 = starts[b], s1 = starts[b + 1], end = min(s1, tokens);
+    return Rows{s0, s0 < end ? end - s0 : 0u, s1 > s0 ? s1 - s0 : 0u};
+}
+__device__ __forceinline__ uint32_t base_of(uint32_t len, const Rows& r) { return len > r.all ? len - r.all : 0u; }
+
+// -------------------------------------------------------------------- plan
+struct TreePlan {
+    const uint32_t *lens, *starts, *parents;
+    uint32_t *masks, *positions;
+    uint32_t requests, tokens, words;
+};
+
+// A workgroup to a request, a lane to a node: it climbs from its node to the root, in LDS, and writes each word of its
+// mask when it has left it behind.  A climb is a chain of LDS reads (some 60 ns each): the tree's depth bounds it.
+__global__ __launch_bounds__(256) void k_tree_plan(TreePlan a)
+{
+    __shared__ uint32_t parent[kMaxNodes];
+    const uint32_t b = blockIdx.x, tid = threadIdx.x;
+    const Rows r = rows_of(a.starts, a.tokens, b);
+    if (r.n == 0) return;
+    const uint32_t base = base_of(a.lens[b], r);
+    if (r.n > 32 * a.words) {  // a chunk
+        for (uint32_t i = tid; i < r.n; i += 256) a.positions[r.first + i] = base + i;
+        return;
+    }
+    for (uint32_t i = tid; i < r.n; i += 256) parent[i] = a.parents[r.first + i];
+    __syncthreads();
+    for (uint32_t i = tid; i < r.n; i += 256) {
+        uint32_t* out = a.masks + uint64_t(r.first + i) * a.words;
+        uint32_t word = i >> 5, bits = 0, depth = 0, at = i;
+        for (uint32_t w = word + 1; w < a.words; ++w) out[w] = 0;
+        for (;;) {
+            bits |= 1u << (at & 31u);
+            const uint32_t up = parent[at];
+            if (up >= at) break;  // none, or not a node before this one
+            ++depth;
+            if ((up >> 5) != word) {
+                out[word] = bits;
+                bits = 0;
+                while (--word != (up >> 5)) out[word] = 0;
+            }
+            at = up;
+        }
+        out[word] = bits;
+        while (word) out[--word] = 0;
+        a.positions[r.first + i] = base + depth;
+    }
+}
+
+// ------------------------------------------------------------ target tokens
+struct Best {
+    float val;
+    uint32_t idx;
+};
+// The larger value, the lower index of equals; NaN is below all numbers.
+__device__ __forceinline__ Best better(const Best& a, const Best& b)
+{
+    return b.val > a.val || (b.val == a.val && b.idx < a.idx) ? b : a;
+}
+template <typename T>
+__device__ __forceinline__ void take(Best& best, T v, uint32_t i)
+{
+    const float f = static_cast<float>(v);
+    if (f > best.val || (f == best.val && i < best.idx)) best = Best{f, i};
+}
+constexpr uint32_t kNoToken = 0xffffffffu;
+
+struct Argmax {
+    const void* logits;
+    const uint32_t* starts;
+    Best* parts;  // [tokens][splits]
+    uint64_t ldl;
+    uint32_t requests, tokens, vocab, splits;
+};
+// A workgroup to a part of a row; rows behind the last request are not read.
+template <typename T>
+__global__ __launch_bounds__(256) void k_tree_argmax(Argmax a)
+{
+    __shared__ Best waves[4];
+    const uint32_t row = blockIdx.x / a.splits, split = blockIdx.x % a.splits, tid = threadIdx.x;
+    if (row >= a.starts[a.requests]) return;
+    const uint32_t each = ((a.vocab + a.splits - 1) / a.splits + 7) & ~7u;
+    const uint32_t c0 = min(split * each, a.vocab), c1 = min(c0 + each, a.vocab);
+    const T* p = static_cast<const T*>(a.logits) + uint64_t(row) * a.ldl;
+    Best best{-INFINITY, kNoToken};
+    for (uint32_t c = c0 + tid; c < c1; c += 256) take(best, p[c], c);
+    for (int d = 32; d; d >>= 1) best = better(best, Best{__shfl_xor(best.val, d), uint32_t(__shfl_xor(int(best.idx), d))});
+    if ((tid & 63u) == 0) waves[tid >> 6] = best;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < 4; ++i) best = better(best, waves[i]);
+        a.parts[uint64_t(row) * a.splits + split] = best;
+    }
+}
+
+// --------------------------------------------------------------------- walk
+struct Walk {
+    const uint32_t *lens, *starts, *parents, *drafts;
+    uint32_t *targets, *lens_out, *counts, *tokens_out;
+    uint32_t *path, *held;  // [tokens] the walk's rows; [requests] lens, which lens_out may take the place of
+    const Best* parts;
+    uint32_t requests, tokens, words, splits;
+};
+
+// A workgroup to a request: the target's token of each row, from the parts of its logits if there are any, then wave 0
+// walks from node 0 to the first child that holds the target's token, as long as there is one.
+__global__ __launch_bounds__(256) void k_tree_walk(Walk a)
+{
+    __shared__ uint32_t parent[kMaxNodes], draft[kMaxNodes], said[kMaxNodes], path[kMaxNodes];
+    __shared__ uint32_t kept;
+    const uint32_t b = blockIdx.x, tid = threadIdx.x;
+    const Rows r = rows_of(a.starts, a.tokens, b);
+    const uint32_t len = a.lens[b];
+    if (a.splits)
+        for (uint32_t i = tid; i < r.n; i += 256) {
+            Best best{-INFINITY, kNoToken};
+            for (uint32_t s = 0; s < a.splits; ++s) best = better(best, a.parts[uint64_t(r.first + i) * a.splits + s]);
+            a.targets[r.first + i] = best.idx == kNoToken ? 0u : best.idx;
+        }
+    __syncthreads();
+    const bool tree = r.n <= 32 * a.words;
+    if (!tree || r.n == 0) {
+        for (uint32_t i = tid; i < r.n; i += 256) a.tokens_out[r.first + i] = i ? kNoToken : a.targets[r.first + r.n - 1];
+        if (tid == 0) {
+            a.counts[b] = r.n ? 1 : 0;
+            a.held[b] = len;
+            a.lens_out[b] = len;
+        }
+        return;
+    }
+    for (uint32_t i = tid; i < r.n; i += 256) {
+        parent[i] = a.parents[r.first + i];
+        draft[i] = a.drafts[r.first + i];
+        said[i] = a.targets[r.first + i];
+    }
+    __syncthreads();
+    if (tid < 64) {
+        uint32_t node = 0, n = 0;
+        for (;;) {
+            if (tid == 0) path[n] = node;
+            ++n;
+            const uint32_t want = said[node];
+            uint32_t next = kNoToken;
+            for (uint32_t i = (node + 1) & ~63u; i < r.n; i += 64) {
+                const uint32_t c = i + tid;
+                const uint64_t fits = __ballot(c > node && c < r.n && parent[c] == node && draft[c] == want);
+                if (fits) {
+                    next = i + uint32_t(__builtin_ctzll(fits));
+                    break;
+                }
+            }
+            if (next == kNoToken) break;
+            node = next;
+        }
+        if (tid == 0) kept = n;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < r.n; i += 256) {
+        a.tokens_out[r.first + i] = i < kept ? said[path[i]] : kNoToken;
+        if (i < kept) a.path[r.first + i] = path[i];
+    }
+    if (tid == 0) {
+        a.counts[b] = kept;
+        a.held[b] = len;
+        a.lens_out[b] = base_of(len, r) + kept;
+    }
+}
+
+// --------------------------------------------------------------------- move
+struct Layers {
+    void *k[ARC_MAX_LAYERS], *v[ARC_MAX_LAYERS];
+};
+struct Move {
+    const uint32_t *tables, *held, *starts, *counts, *path;
+    uint32_t *free_pages, *free_count_out;
+    const uint32_t* free_count;
+    uint64_t page_bytes;  // from page to page
+    uint32_t requests, tokens, words, max_pages, num_pages, list_pages, shift, row_bytes, layers;
+};
+
+// The row of position pos in a pool, or none: a page that is none, a position past the table.
+__device__ __forceinline__ bool place_of(const Move& a, uint32_t b, uint32_t pos, uint64_t& at)
+{
+    if ((pos >> a.shift) >= a.max_pages) return false;
+    const uint32_t page = a.tables[uint64_t(b) * a.max_pages + (pos >> a.shift)];
+    at = uint64_t(page) * a.page_bytes + uint64_t(pos & ((1u << a.shift) - 1u)) * a.row_bytes;
+    return page < a.num_pages;
+}
+
+// A workgroup to a request and layer: row path[i] of the walk to place i, each thread the same 16 bytes of every row, so
+// that a row is read before its place is written (path[i] >= i, in rising order).  The workgroups of one more layer
+// number return the pages.
+__global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
+{
+    const uint32_t tid = threadIdx.x, layer = blockIdx.y;
+    if (layer < a.layers) {
+        const uint32_t b = blockIdx.x;
+        if (b >= a.requests) return;
+        const Rows r = rows_of(a.starts, a.tokens, b);
+        if (r.n == 0 || r.n > 32 * a.words || a.held[b] < r.all) return;
+        const uint32_t base = a.held[b] - r.all, kept = a.counts[b], width = a.row_bytes / 16;
+        for (uint32_t c = tid; c < 2 * width; c += 256) {
+            uint8_t* pool = static_cast<uint8_t*>(c < width ? layers.k[layer] : layers.v[layer]) + (c < width ? c : c - width) * 16;
+            for (uint32_t i = 1; i < kept; ++i) {
+                const uint32_t from = a.path[r.first + i];
+                uint64_t to_at, from_at;
+                if (from == i || !place_of(a, b, base + i, to_at) || !place_of(a, b, base + from, from_at)) continue;
+                *reinterpret_cast<uint4*>(pool + to_at) = *reinterpret_cast<const uint4*>(pool + from_at);
+            }
+        }
+        return;
+    }
+    if (blockIdx.x || !a.free_pages) return;
+    __shared__ uint32_t sums[4];
+    uint32_t count = *a.free_count;
+    for (uint32_t b0 = 0; b0 < a.requests; b0 += 256) {
+        const uint32_t b = b0 + tid;
+        uint32_t low = 0, back = 0;
+        if (b < a.requests) {
+            const Rows r = rows_of(a.starts, a.tokens, b);
+            const uint32_t len = a.held[b], size = 1u << a.shift;
+            if (r.n && r.n <= 32 * a.words && len >= r.all) {
+                low = uint32_t((uint64_t(len - r.all + a.counts[b]) + size - 1) >> a.shift);
+                back = min(uint32_t((uint64_t(len) + size - 1) >> a.shift), a.max_pages);
+                back = back > low ? back - low : 0;
+            }
+        }
+        uint32_t inc = back;  // sums of the requests up to this one
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t v = uint32_t(__shfl_up(int(inc), d));
+            if (int(tid & 63u) >= d) inc += v;
+        }
+        if ((tid & 63u) == 63) sums[tid >> 6] = inc;
+        __syncthreads();
+        uint32_t before = count + inc - back;
+        for (uint32_t w = 0; w < 4; ++w) {
+            if (w < (tid >> 6)) before += sums[w];
+            count += sums[w];
+        }
+        for (uint32_t i = 0; i < back; ++i)
+            if (before + i < a.list_pages) a.free_pages[before + i] = a.tables[uint64_t(b) * a.max_pages + low + i];
+        __syncthreads();
+    }
+    if (tid == 0) *a.free_count_out = min(count, a.list_pages);
+}
+
+// ---------------------------------------------------------------------- host
+int check_tree(const arc_tree* t)
+{
+    if (!t || !t->parents) return set_error(ARC_ERR_INVALID_ARGUMENT, "null tree or parents");
+    if (t->mask_words == 0 || t->mask_words > ARC_TREE_MAX_WORDS)
+        return set_error(ARC_ERR_UNSUPPORTED, "mask_words %u: 1..%u are supported", t->mask_words, uint32_t(ARC_TREE_MAX_WORDS));
+    return ARC_OK;
+}
+
+// Parts of a row of logits: enough workgroups to fill the card.
+uint32_t splits_of(uint32_t tokens)
+{
+    uint32_t s = 1;
+    while (s < 64 && uint64_t(tokens) * s < 2048) s *= 2;
+    return s;
+}
+
+// Where a commit's workspace holds what.
+struct Space {
+    size_t held, parts, bytes;
+};
+Space space_of(const arc_paged_batch* b)
+{
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    Space s;
+    s.held = up(b->tokens * sizeof(uint32_t));
+    s.parts = s.held + up(b->requests * sizeof(uint32_t));
+    s.bytes = s.parts + up((size_t(b->tokens) * splits_of(b->tokens) + 1) * sizeof(Best));
+    return s;
+}
+
+}  // namespace
+}  // namespace arc
+
+using namespace arc;
+
+extern "C" {
+
+int arc_tree_plan(const arc_paged_batch* batch, const arc_tree* tree, arc_stream_t stream)
+{
+    int rc = check_batch_sizes(batch);
+    if (!rc) rc = check_tree(tree);
+    if (rc) return rc;
+    if (!batch->lens || !batch->starts || !batch->positions || !tree->masks)
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "null lens, starts, positions or masks");
+    if (batch->requests == 0 || batch->tokens == 0) return ARC_OK;
+    const TreePlan a{batch->lens, batch->starts, tree->parents, tree->masks, batch->positions, batch->requests, batch->tokens, tree->mask_words};
+    hipLaunchKernelGGL(k_tree_plan, dim3(batch->requests), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    return check_hip(hipGetLastError(), "tree plan");
+}
+
+size_t arc_tree_commit_workspace_bytes(const arc_paged_batch* batch)
+{
+    return check_batch_sizes(batch) ? 0 : space_of(batch).bytes;
+}
+
+int arc_tree_commit(const arc_kv_pages* layers, uint32_t num_layers, const arc_paged_batch* batch, const arc_tree* tree, int logits_dtype,
+                    const void* logits, uint64_t ldl, uint32_t vocab, const uint32_t* drafts, uint32_t* targets, uint32_t* lens_out,
+                    uint32_t* counts, uint32_t* tokens_out, uint32_t* free_pages, uint32_t num_pages, const uint32_t* free_count,
+                    uint32_t* free_count_out, void* workspace, arc_stream_t stream)
+{
+    if (num_layers == 0 || num_layers > ARC_MAX_LAYERS)
+        return set_error(ARC_ERR_UNSUPPORTED, "%u layers: 1..%u are supported", num_layers, uint32_t(ARC_MAX_LAYERS));
+    if (!layers) return set_error(ARC_ERR_INVALID_ARGUMENT, "null pages");
+    for (uint32_t i = 0; i < num_layers; ++i) {
+        if (int rc = check_pages(layers + i)) return rc;
+        const arc_kv_pages &p = layers[i], &q = layers[0];
+        if (p.page_size != q.page_size || p.page_stride != q.page_stride || p.num_pages != q.num_pages || p.kv_heads != q.kv_heads ||
+            p.head_dim != q.head_dim || p.dtype != q.dtype)
+            return set_error(ARC_ERR_INVALID_ARGUMENT, "layer %u: pages of another shape than layer 0's", i);
+    }
+    int rc = check_batch_sizes(batch);
+    if (!rc) rc = check_tables(batch, layers->page_size);
+    if (!rc) rc = check_tree(tree);
+    if (rc) return rc;
+    if (!drafts || !targets || !lens_out || !counts || !tokens_out || !workspace)
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "null argument");
+    if (!aligned(workspace, 256)) return set_error(ARC_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    if (free_pages && (!free_count || !free_count_out || num_pages == 0))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "a free list needs its counts and num_pages");
+    if (logits) {
+        const uint32_t size = logits_dtype == ARC_F32 ? 4 : logits_dtype == ARC_F16 || logits_dtype == ARC_BF16 ? 2 : 0;
+        if (size == 0) return set_error(ARC_ERR_UNSUPPORTED, "logits are ARC_F32, ARC_F16 or ARC_BF16 (dtype %d)", logits_dtype);
+        if (vocab == 0 || vocab > (1u << 24) || ldl < vocab)
+            return set_error(ARC_ERR_INVALID_ARGUMENT, "vocab %u, ldl %llu: 1 .. 2^24, ldl at least vocab", vocab, static_cast<unsigned long long>(ldl));
+        if (!aligned(logits, size)) return set_error(ARC_ERR_INVALID_ARGUMENT, "logits must be aligned to their type");
+        if (batch->tokens > kMaxLogitRows) return set_error(ARC_ERR_UNSUPPORTED, "%u rows of logits: at most 2^20", batch->tokens);
+    }
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const Space sp = space_of(batch);
+    uint32_t *path = reinterpret_cast<uint32_t*>(ws), *held = reinterpret_cast<uint32_t*>(ws + sp.held);
+    Best* parts = reinterpret_cast<Best*>(ws + sp.parts);
+    const uint32_t splits = logits ? splits_of(batch->tokens) : 0;
+    if (splits && batch->requests && batch->tokens) {
+        const Argmax a{logits, batch->starts, parts, ldl, batch->requests, batch->tokens, vocab, splits};
+        const dim3 grid(batch->tokens * splits), block(256);
+        if (logits_dtype == ARC_F32) hipLaunchKernelGGL(k_tree_argmax<float>, grid, block, 0, st, a);
+        else if (logits_dtype == ARC_F16) hipLaunchKernelGGL(k_tree_argmax<_Float16>, grid, block, 0, st, a);
+        else hipLaunchKernelGGL(k_tree_argmax<bf16>, grid, block, 0, st, a);
+        if (hipError_t e = hipGetLastError()) return check_hip(e, "tree commit");
+    }
+    const Walk w{batch->lens, batch->starts, tree->parents, drafts, targets, lens_out, counts, tokens_out, path, held, parts,
+                 batch->requests, batch->tokens, tree->mask_words, splits};
+    if (batch->requests) hipLaunchKernelGGL(k_tree_walk, dim3(batch->requests), dim3(256), 0, st, w);
+    if (hipError_t e = hipGetLastError()) return check_hip(e, "tree commit");
+    const uint32_t row_bytes = layers->kv_heads * layers->head_dim * 2;
+    const Move m{batch->tables, held, batch->starts, counts, path, free_pages, free_count_out, free_count,
+                 layers->page_stride * 2, batch->requests, batch->tokens, tree->mask_words, batch->max_pages, layers->num_pages,
+                 num_pages, log2_of(layers->page_size), row_bytes, num_layers};
+    Layers l{};
+    for (uint32_t i = 0; i < num_layers; ++i) {
+        l.k[i] = layers[i].k;
+        l.v[i] = layers[i].v;
+    }
+    hipLaunchKernelGGL(k_tree_move, dim3(batch->requests ? batch->requests : 1, num_layers + (free_pages ? 1 : 0)), dim3(256), 0, st, m, l);
+    return check_hip(hipGetLastError(), "tree commit");
+}
+
+}  // extern "C"

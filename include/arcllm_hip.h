@@ -412,6 +412,106 @@ int arc_paged_attention(const arc_kv_pages *pages, const arc_paged_batch *batch,
                         uint32_t hpk, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
                         void *workspace, arc_stream_t stream);
 
+/* A step that verifies trees of drafted tokens, over the same pages: arc_paged_plan
+ * for as many new tokens as each request's tree has, arc_tree_plan, per layer
+ * arc_rope_append and arc_tree_attention, and arc_tree_commit.  Node 0 of a
+ * request is its last token, whose K and V are not in the cache yet; every other
+ * node is a drafted token that continues one of the nodes before it.  A request of
+ * one row has drafted nothing; one of more rows than 32 * mask_words is a prompt's
+ * chunk, causal.  No counterpart in the reference, which decodes one token at a time. */
+#define ARC_MAX_LAYERS 64             /* of a model */
+#define ARC_TREE_MAX_WORDS 32         /* trees of up to 1024 nodes */
+#define ARC_NO_PARENT 0xffffffffu
+#define ARC_NO_TOKEN 0xffffffffu
+
+typedef struct arc_tree { /* device arrays, in the order of the step's rows */
+    const uint32_t *parents; /* [tokens] the node, counted from the request's first row, that a row continues;
+                                ARC_NO_PARENT, or any number not below its own: none.  A chunk's are not read */
+    uint32_t *masks;         /* [tokens][mask_words] bit j of a row: it sees node j of its request */
+    uint32_t mask_words;     /* 1 .. ARC_TREE_MAX_WORDS */
+} arc_tree;
+
+/* Masks and positions of the step's rows: of a tree's node, the nodes from which it
+ * descends and itself, and the context's length (lens - rows) plus its depth; of a chunk's
+ * row its place, with no mask.  After arc_paged_plan, whose positions of trees count
+ * rows and not depths (its slots stay: node i lies in slot i behind the context).  Rows
+ * behind the last request are left as they were.  Of the batch, requests, tokens, lens,
+ * starts and positions (written) are used. */
+int arc_tree_plan(const arc_paged_batch *batch, const arc_tree *tree, arc_stream_t stream);
+
+/* Bytes of device workspace arc_tree_attention needs, as arc_paged_attention_workspace_bytes. */
+size_t arc_tree_attention_workspace_bytes(const arc_kv_pages *pages, const arc_paged_batch *batch, uint32_t hpk);
+
+/* arc_paged_attention, in all that it says of arguments, numbers and workspace, for trees: the row of
+ * node i sees every position before its tree and those nodes j <= i whose bit is set in
+ * its mask (bits above i do not count; a row without any sees the context alone).  With a window, two
+ * positions' distance is that of positions[]: the context's length plus depth, as is the position that
+ * sinks are compared with.  A chunk is causal.  masks need not come from arc_tree_plan, but with a
+ * window a row's nodes count as the steps of one way down (a node's depth is the number of set bits below its own). */
+int arc_tree_attention(const arc_kv_pages *pages, const arc_paged_batch *batch, const arc_tree *tree, const void *q,
+                       uint32_t ldq, uint32_t hpk, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
+                       void *workspace, arc_stream_t stream);
+
+/* The step's end.  targets[n]: the target model's token after row n, read; or, with logits ([tokens][vocab] of
+ * logits_dtype ARC_F32, ARC_F16 or ARC_BF16, ldl elements from row to row), written: the largest logit's
+ * index, the lowest of equals (NaN is never the largest; 0 for a row without a number), of every row that belongs to a
+ * request.  Each tree is walked from node 0: to the first child whose token (drafts[]) is the target's token
+ * after the node, until there is none.  Of request b with k nodes on that way:
+ *   counts[b] = k, tokens_out at its first k rows = the target's tokens after them (what the request
+ *   goes on with: k - 1 accepted drafts and one more), ARC_NO_TOKEN at its other rows;
+ *   lens_out[b] = lens[b] - rows + k (lens_out may be lens);
+ *   in each of the layers' pools, node i-th on the way moves to place i behind the context, K and V;
+ *   pages that held only other nodes go onto the free list (a stack as arc_paged_plan's, of room for
+ *   num_pages; NULL: they stay with the request), requests in order, first page to last.  free_count_out may
+ *   be free_count.
+ * A chunk counts 1 (the target's token after its last row), keeps all its positions and moves nothing; a
+ * request without rows counts 0.  layers: 1 .. ARC_MAX_LAYERS pools of one shape (host array).  A position whose page
+ * is none of the pool does not move.  workspace: arc_tree_commit_workspace_bytes() bytes, 256-byte
+ * aligned, as arc_paged_attention's.  Of the batch, all but positions, slots and max_new is used. */
+size_t arc_tree_commit_workspace_bytes(const arc_paged_batch *batch);
+int arc_tree_commit(const arc_kv_pages *layers, uint32_t num_layers, const arc_paged_batch *batch, const arc_tree *tree,
+                    int logits_dtype, const void *logits, uint64_t ldl, uint32_t vocab, const uint32_t *drafts,
+                    uint32_t *targets, uint32_t *lens_out, uint32_t *counts, uint32_t *tokens_out, uint32_t *free_pages,
+                    uint32_t num_pages, const uint32_t *free_count, uint32_t *free_count_out, void *workspace,
+                    arc_stream_t stream);
+
+/* Products in 8-bit floating point: e4m3 values (OCP: largest 448, no infinities) with an fp32 scale
+ * for each block of 128: of a row of activations, or of 128 rows of weights (the last blocks may be
+ * shorter).  For steps of any number of rows, beside arc_gemv and arc_prefill_gemm.  No counterpart in the reference. */
+typedef struct arc_fp8_rows { /* rows of activations, device */
+    void *q;                  /* [rows][ldq] e4m3, 16-byte aligned */
+    float *scales;            /* [ceil(cols / 128)][lds]: block b of row m at b * lds + m */
+    uint32_t rows, cols;      /* cols: a multiple of 16, at most 2^22; rows below 2^24 */
+    uint32_t ldq;             /* bytes from row to row: a multiple of 16, >= cols, at most 2^22 */
+    uint32_t lds;             /* >= rows */
+} arc_fp8_rows;
+
+typedef struct arc_fp8_weights { /* device */
+    const void *w;               /* [rows][ldw] e4m3, 16-byte aligned: row n makes output n */
+    const float *scales;         /* [ceil(rows / 128)][lds] */
+    uint32_t rows, cols;         /* as arc_fp8_rows */
+    uint32_t ldw;
+    uint32_t lds;                /* >= ceil(cols / 128) */
+} arc_fp8_weights;
+
+/* Rows of x (x_dtype ARC_F32, ARC_F16 or ARC_BF16, ldx elements from row to row: a multiple of 8; 16-byte
+ * aligned) to e4m3: scale = max(largest magnitude of the block / 448, 2^-126), value = x / scale rounded to
+ * nearest even.  A block with an infinity or NaN gets scale and values NaN.  x and out share no memory. */
+int arc_fp8_quantize(int x_dtype, const void *x, uint32_t ldx, const arc_fp8_rows *out, arc_stream_t stream);
+
+/* y[m][n] = sum_k x[m][k] w[n][k] (+ residual[m][n]), x and w with their scales; y and residual of y_dtype
+ * (ARC_F32, ARC_F16, ARC_BF16), ldy and ldr elements from row to row (16-byte aligned rows are quickest); residual may be
+ * NULL, or y itself.  Products of scales that leave fp32's normal range do not keep their bits.
+ * workspace: arc_fp8_gemm_workspace_bytes(w->rows, w->cols, x->rows, 0) bytes, 256-byte
+ * aligned, any contents, for one call at a time.  No rows: nothing is done. */
+size_t arc_fp8_gemm_workspace_bytes(uint32_t n, uint32_t k, uint32_t rows, int gated);
+int arc_fp8_gemm(const arc_fp8_weights *w, const arc_fp8_rows *x, int y_dtype, void *y, uint32_t ldy, const void *residual,
+                 uint32_t ldr, void *workspace, arc_stream_t stream);
+/* y = silu(x gate^T) * (x up^T), silu(g) = g / (1 + exp(-g)), in fp32 and rounded once; gate and up of one shape;
+ * workspace as above with gated = 1. */
+int arc_fp8_gateup(const arc_fp8_weights *gate, const arc_fp8_weights *up, const arc_fp8_rows *x, int y_dtype, void *y,
+                   uint32_t ldy, void *workspace, arc_stream_t stream);
+
 /* Tuning hook: force the GEMV lane layout for later launches on this host
  * thread (bs = super-block quads per row: 1,2,4,8,16; rpl = rows per lane:
  * 1,2,4).  bs = 0 restores the automatic choice. */
@@ -480,7 +580,6 @@ int arc_synth_normal(uint64_t seed, uint64_t stream, size_t n, float mean, float
  * attn_v (Q4_K or Q6_K), q/k/v biases, attn_output (Q4_K), ffn_norm,
  * ffn_gate/up (Q4_K), ffn_down (Q4_K or Q6_K); token_embd (Q4_K),
  * output_norm, output (Q6_K).  Norm weights and biases are fp32. */
-#define ARC_MAX_LAYERS 64
 
 typedef struct arc_model_dims {
     uint32_t hidden, q_heads, kv_heads, head_dim, ffn, vocab, layers;
