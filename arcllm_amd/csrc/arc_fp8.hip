@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void k_fp8_quantize(Quantize a)
 {
     __shared__ float scales[4][kQuantRows];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t col = blockIdx.x * 512 + lane * 8, row0 = blockIdx.y * kQuantRows;
+    const uint32_t col = blockIdx.y * 512 + lane * 8, row0 = blockIdx.x * kQuantRows;
     const bool in = col < a.cols;
     for (uint32_t i = wave; i < kQuantRows && row0 + i < a.rows; i += 4) {
         float v[8];
@@ -86,8 +86,8 @@ __global__ __launch_bounds__(256) void k_fp8_quantize(Quantize a)
     }
     __syncthreads();
     const uint32_t b = threadIdx.x / kQuantRows, r = threadIdx.x % kQuantRows;
-    if (b < 4 && row0 + r < a.rows && (blockIdx.x * 4 + b) * kFpBlock < a.cols)
-        a.scales[uint64_t(blockIdx.x * 4 + b) * a.lds + row0 + r] = scales[b][r];
+    if (b < 4 && row0 + r < a.rows && (blockIdx.y * 4 + b) * kFpBlock < a.cols)
+        a.scales[uint64_t(blockIdx.y * 4 + b) * a.lds + row0 + r] = scales[b][r];
 }
 
 // ------------------------------------------------------------------- product
@@ -101,6 +101,8 @@ struct Gemm {
     uint32_t M, N, K, blocks;
     uint32_t ldw[2], ldws[2], ldx, ldxs, ldy, ldr;
     uint32_t wide;  // y and residual take 4 values at a time
+    float* part;    // sums of the parts of a tile's blocks, if there are several
+    uint32_t mtiles, ntiles, splits;
 };
 
 // 4 neighbouring outputs of a row: the activation or the residual, rounded once.
@@ -209,6 +211,238 @@ __global__ __launch_bounds__(512) void k_fp8_few(Gemm a)
     store_out<Y>(a, m0 + r, n0 + 4 * g, t[0]);
 }
 
+// Tiles.  A workgroup of GM x GN waves has BM rows of x and BN rows of w, a wave WM x WN tiles of 16 x 16.  A block of both
+// comes straight into LDS, S blocks deep; one barrier a block.  With the activation a wave's weights are half gate, half
+// up, at the same outputs.
+template <bool GATED_, bool FAST_, int WM_, int WN_, int GM_, int GN_, int S_>
+struct TileShape {
+    static constexpr bool GATED = GATED_, FAST = FAST_;
+    static constexpr int WM = WM_, WN = WN_, GM = GM_, GN = GN_, S = S_, NW = GM * GN, G = GATED ? 2 : 1;
+    static constexpr uint32_t BM = 16 * WM * GM, BN = 16 * WN * GN, OUT = BN / G;  // outputs of a row
+    static constexpr uint32_t CW = BN / 8 / NW, CX = BM / 8 / NW, COPIES = CW + CX + 2;  // a wave's, of a block
+    static constexpr uint32_t XS = BM < 64 ? 64 : BM;
+    static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0 && NW % 2 == 0);
+    struct Lds {
+        __align__(16) uint8_t w[S][BN * kFpBlock];
+        __align__(16) uint8_t x[S][BM * kFpBlock];
+        float xs[S][XS];
+        float ws[S][64];  // of the gate's or plain weights' blocks of 128 rows, from 32 on the up's
+    };
+};
+
+__device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+// 16 or 4 bytes per lane from memory straight into LDS, lane i's at lds + 16 i (4 i).  Assembly: the compiler would wait
+// for such a copy before any read of LDS; there is no register for a load in flight to write, and
+// nothing else here uses m0.
+__device__ __forceinline__ void copy16(uint32_t lds, const void* base, uint32_t off)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t lds, const void* from)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t lds, const void* base, uint32_t off)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
+__device__ __forceinline__ uint32_t lds_at(const void* p)
+{
+    typedef __attribute__((address_space(3))) const void lptr;
+    return uniform(uint32_t(reinterpret_cast<uintptr_t>((lptr*)(p))));
+}
+// A row's 8 blocks of 16 bytes lie at place c ^ swizzle(row): 16 lanes that read one block of 16 rows fall on all 64 banks.
+__device__ __forceinline__ uint32_t swizzle(uint32_t row) { return (row >> 1) & 7u; }
+
+// Where a workgroup works: neighbours (which go to the 8 XCDs in turn) are spread so that an XCD's have tiles next to each
+// other, 8 of x by some of w, which its L2 then holds.
+struct Place {
+    uint32_t m, n, split;  // tile of x, of w, part of the blocks
+};
+__device__ __forceinline__ Place place_of(const Gemm& a, uint32_t id)
+{
+    const uint32_t tiles = a.mtiles * a.ntiles, all = tiles * a.splits, q = all >> 3, rest = all & 7u, xcd = id & 7u;
+    id = xcd * q + min(xcd, rest) + (id >> 3);
+    Place p;
+    p.split = id / tiles;
+    const uint32_t t = id - p.split * tiles, group = t / (8 * a.ntiles), in = t - group * 8 * a.ntiles;
+    const uint32_t rows = min(8u, a.mtiles - group * 8);
+    p.n = in / rows;
+    p.m = group * 8 + in - p.n * rows;
+    return p;
+}
+
+template <typename Y, typename C>
+__device__ __forceinline__ void finish(const Gemm& a, const Place& at, uint32_t wave, int i, int j, uint32_t lane, f32x4 v, f32x4 up)
+{
+    const uint32_t wm = wave / C::GN, wn = wave % C::GN;
+    const uint32_t m = at.m * C::BM + (wm * C::WM + j) * 16 + (lane & 15u);
+    const uint32_t n = at.n * C::OUT + wn * (C::OUT / C::GN) + i * 16 + 4 * (lane >> 4);
+    if constexpr (C::GATED)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = silu(v[e]) * up[e];
+    store_out<Y>(a, m, n, v);
+}
+
+template <typename Y, typename C>
+__global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
+{
+    constexpr int WM = C::WM, WN = C::WN, S = C::S, G = C::G;
+    __shared__ typename C::Lds lds;
+    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4, wave = uniform(threadIdx.x >> 6);
+    const uint32_t wm = wave / C::GN, wn = wave % C::GN;
+    const Place at = place_of(a, blockIdx.x);
+    const uint32_t n0 = at.n * C::OUT, m0 = at.m * C::BM;
+    const uint32_t b0 = uint32_t(uint64_t(a.blocks) * at.split / a.splits), b1 = uint32_t(uint64_t(a.blocks) * (at.split + 1) / a.splits);
+
+    // what each copy of this wave reads: 8 rows, a lane 16 bytes of row 8 * (i * NW + wave) + lane / 8
+    const uint32_t row8 = lane >> 3, chunk = ((lane & 7u) ^ swizzle(8 * wave + row8)) * 16;
+    uint32_t woff[C::CW], xoff[C::CX];
+#pragma unroll
+    for (uint32_t i = 0; i < C::CW; ++i) {
+        const uint32_t R = 8 * (i * C::NW + wave) + row8, strip = R / (16 * WN), in = R % (16 * WN);
+        const uint32_t n = n0 + strip * (16 * WN / G) + in % (16 * WN / G), h = in / (16 * WN / G);
+        woff[i] = (min(n, a.N - 1) - n0) * a.ldw[h] + chunk;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < C::CX; ++i) xoff[i] = (min(m0 + 8 * (i * C::NW + wave) + row8, a.M - 1) - m0) * a.ldx + chunk;
+    const uint32_t xsoff = (min(m0 + 64 * (wave % (C::XS / 64)) + lane, a.M - 1) - m0) * 4;
+    const uint32_t nblock = n0 / kFpBlock, nblocks = (a.N + kFpBlock - 1) / kFpBlock;
+    const uint32_t wsoff = (min(nblock + (lane & 31u), nblocks - 1) - nblock) * a.ldws[lane >> 5 & (G - 1)] * 4;
+
+    auto copy_block = [&](uint32_t b, uint32_t buf) {
+        const uint32_t k = b * kFpBlock;
+        const bool whole = k + kFpBlock <= a.K;  // else blocks from column K on are zeros
+#pragma unroll
+        for (uint32_t i = 0; i < C::CW; ++i) {
+            const uint32_t rows = i * C::NW + wave, h = G == 1 ? 0 : (8 * rows) % (16 * WN) / (8 * WN);
+            const uint8_t* base = a.w[h] + uint64_t(n0) * a.ldw[h] + k;
+            const uint32_t to = lds_at(&lds.w[buf][rows * 1024]);
+            if (whole) copy16(to, base, woff[i]);
+            else copy16(to, k + chunk < a.K ? static_cast<const void*>(base + woff[i]) : kZeros);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < C::CX; ++i) {
+            const uint32_t rows = i * C::NW + wave;
+            const uint8_t* base = a.x + uint64_t(m0) * a.ldx + k;
+            const uint32_t to = lds_at(&lds.x[buf][rows * 1024]);
+            if (whole) copy16(to, base, xoff[i]);
+            else copy16(to, k + chunk < a.K ? static_cast<const void*>(base + xoff[i]) : kZeros);
+        }
+        copy4(lds_at(&lds.xs[buf][64 * (wave % (C::XS / 64))]), a.xs + uint64_t(b) * a.ldxs + m0, xsoff);
+        if constexpr (G == 1) {
+            copy4(lds_at(&lds.ws[buf][0]), a.ws[0] + uint64_t(nblock) * a.ldws[0] + b, wsoff);
+        } else {
+            const float* base = (lane < 32 ? a.ws[0] + uint64_t(nblock) * a.ldws[0] : a.ws[1] + uint64_t(nblock) * a.ldws[1]) + b;
+            const float* from = base + wsoff / 4;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_at(&lds.ws[buf][0])), "v"(from) : "memory");
+        }
+    };
+
+    f32x4 acc[WN][WM];
+#pragma unroll
+    for (int i = 0; i < WN; ++i)
+#pragma unroll
+        for (int j = 0; j < WM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+        if (b0 + i < b1) copy_block(b0 + i, i);
+    uint32_t buf = 0;
+    for (uint32_t b = b0; b < b1; ++b) {
+        // this block's copies have arrived; those of the S - 2 after it may be under way
+        if (S > 2 && b + S - 2 < b1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * C::COPIES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's; and the block before is read
+        const uint32_t ahead = buf == 0 ? S - 1 : buf - 1;
+        if (b + S - 1 < b1) copy_block(b + S - 1, ahead);
+
+        const uint8_t* xl = &lds.x[buf][(wm * WM * 16 + r) * kFpBlock];
+        const uint8_t* wl = &lds.w[buf][(wn * WN * 16 + r) * kFpBlock];
+        const uint32_t place = (g ^ swizzle(r)) * 16;
+        auto frag_at = [&](const uint8_t* p) {
+            return Frag{*reinterpret_cast<const u32x4*>(p + place), *reinterpret_cast<const u32x4*>(p + (place ^ 64u))};
+        };
+        float s[G][WM];
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            const uint32_t nw = n0 + wn * (C::OUT / C::GN);
+            const float w = lds.ws[buf][32 * h + nw / kFpBlock - nblock];
+#pragma unroll
+            for (int j = 0; j < WM; ++j) s[h][j] = w * lds.xs[buf][(wm * WM + j) * 16 + r];
+        }
+        if constexpr (C::FAST) {
+            i32x8 xf[WM];
+#pragma unroll
+            for (int j = 0; j < WM; ++j) xf[j] = __builtin_bit_cast(i32x8, frag_at(xl + j * 16 * kFpBlock));
+            f32x4 p[2][WM];
+#pragma unroll
+            for (int i = 0; i <= WN; ++i) {
+                if (i < WN) {
+                    const i32x8 wf = __builtin_bit_cast(i32x8, frag_at(wl + i * 16 * kFpBlock));
+#pragma unroll
+                    for (int j = 0; j < WM; ++j)
+                        p[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf[j], f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+                }
+                if (i > 0)
+#pragma unroll
+                    for (int j = 0; j < WM; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[i - 1][j][e] = __builtin_fmaf(p[(i - 1) & 1][j][e], s[(i - 1) / (WN / G)][j], acc[i - 1][j][e]);
+            }
+        } else {
+            Wide xf[WM];
+#pragma unroll
+            for (int j = 0; j < WM; ++j) xf[j] = widen(frag_at(xl + j * 16 * kFpBlock));
+#pragma unroll
+            for (int i = 0; i < WN; ++i) {
+                const Wide wf = widen(frag_at(wl + i * 16 * kFpBlock));
+#pragma unroll
+                for (int j = 0; j < WM; ++j) {
+                    const f32x4 p = block_sums(wf, xf[j]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(p[e], s[i / (WN / G)][j], acc[i][j][e]);
+                }
+            }
+        }
+        buf = buf + 1 == S ? 0 : buf + 1;
+    }
+    if (a.splits == 1) {
+#pragma unroll
+        for (int i = 0; i < WN / G; ++i)
+#pragma unroll
+            for (int j = 0; j < WM; ++j) finish<Y, C>(a, at, wave, i, j, lane, acc[i][j], acc[i + WN / G * (G - 1)][j]);
+        return;
+    }
+    f32x4* part = reinterpret_cast<f32x4*>(a.part) + ((uint64_t(at.m) * a.ntiles + at.n) * a.splits + at.split) * (C::BM * C::BN / 4);
+#pragma unroll
+    for (int i = 0; i < WN; ++i)
+#pragma unroll
+        for (int j = 0; j < WM; ++j) part[((wave * WN + i) * WM + j) * 64 + lane] = acc[i][j];
+}
+
+// Adds up the parts of a tile in order; a thread has 4 outputs, those of one lane above.
+template <typename Y, typename C>
+__global__ __launch_bounds__(256) void k_fp8_join(Gemm a)
+{
+    constexpr uint32_t kEach = C::BM * C::OUT / 4;  // threads to a tile
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, tile = id / kEach, e = id % kEach;
+    if (tile >= a.mtiles * a.ntiles) return;
+    const uint32_t lane = e % 64, q = e / 64, j = q % C::WM, i = q / C::WM % (C::WN / C::G), wave = q / (C::WM * C::WN / C::G);
+    const Place at{tile / a.ntiles, tile % a.ntiles, 0};
+    const f32x4* part = reinterpret_cast<const f32x4*>(a.part) + uint64_t(tile) * a.splits * (C::BM * C::BN / 4);
+    f32x4 v = {0, 0, 0, 0}, up = {0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t s = 0; s < a.splits; ++s, part += C::BM * C::BN / 4) {
+        v += part[((wave * C::WN + i) * C::WM + j) * 64 + lane];
+        if constexpr (C::GATED) up += part[((wave * C::WN + i + C::WN / 2) * C::WM + j) * 64 + lane];
+    }
+    finish<Y, C>(a, at, wave, int(i), int(j), lane, v, up);
+}
+
 // ---------------------------------------------------------------------- host
 constexpr uint32_t kMaxLd = 1u << 22;     // bytes from row to row of w and x
 constexpr uint32_t kMaxRows = 1u << 24;
@@ -243,16 +477,56 @@ int check_weights(const arc_fp8_weights* w, const arc_fp8_rows* x)
 }
 uint32_t bytes_of(int dtype) { return dtype == ARC_F32 ? 4 : dtype == ARC_F16 || dtype == ARC_BF16 ? 2 : 0; }
 
-template <typename Y, bool GATED>
-hipError_t launch_few(const Gemm& a, hipStream_t st)
+// Which kernel takes a product, and its tiles.
+enum class Form { few, rows32, rows64, rows128, rows256 };
+struct Plan {
+    Form form;
+    uint32_t mtiles, ntiles, splits;
+    size_t bytes;  // of workspace
+};
+Plan plan_of(uint32_t N, uint32_t blocks, uint32_t M, bool gated, bool fast)
 {
-    hipLaunchKernelGGL((k_fp8_few<Y, GATED>), dim3((a.N + 15) / 16, (a.M + 15) / 16), dim3(64 * kFewWaves8), 0, st, a);
+    auto tiles = [](uint32_t n, uint32_t each) { return (n + each - 1) / each; };
+    Plan p{Form::few, 0, 0, 1, 256};
+    if (M <= 16) return p;
+    uint32_t bm, bn;
+    if (M <= 32) p.form = Form::rows32, bm = 32, bn = 128;
+    else if (M <= 64) p.form = Form::rows64, bm = 64, bn = 128;
+    else p.form = Form::rows128, bm = 128, bn = 128;
+    if (fast && M > 64 && uint64_t(tiles(M, 256)) * tiles(N, gated ? 128 : 256) >= 192) p.form = Form::rows256, bm = bn = 256;
+    p.mtiles = tiles(M, bm);
+    p.ntiles = tiles(N, gated ? bn / 2 : bn);
+    const uint64_t all = uint64_t(p.mtiles) * p.ntiles;
+    while (p.splits < 32 && all * (p.splits * 2) <= 512 && blocks / (p.splits * 2) >= 4) p.splits *= 2;
+    if (p.splits > 1) p.bytes = size_t(all) * p.splits * bm * bn * sizeof(float);
+    return p;
+}
+
+template <typename Y, typename C>
+hipError_t launch_tile(const Gemm& a, hipStream_t st)
+{
+    hipLaunchKernelGGL((k_fp8_tile<Y, C>), dim3(a.mtiles * a.ntiles * a.splits), dim3(C::NW * 64), 0, st, a);
+    if (a.splits > 1) {
+        if (hipError_t e = hipGetLastError()) return e;
+        hipLaunchKernelGGL((k_fp8_join<Y, C>), dim3(a.mtiles * a.ntiles * (C::BM * C::OUT / 1024)), dim3(256), 0, st, a);
+    }
+    return hipGetLastError();
+}
+template <typename Y, bool GATED>
+hipError_t launch_form(const Gemm& a, Form form, hipStream_t st)
+{
+    constexpr bool FAST = sizeof(Y) == 2;
+    if (form == Form::few) hipLaunchKernelGGL((k_fp8_few<Y, GATED>), dim3((a.N + 15) / 16, (a.M + 15) / 16), dim3(64 * kFewWaves8), 0, st, a);
+    else if (form == Form::rows32) return launch_tile<Y, TileShape<GATED, FAST, 2, 2, 1, 4, 3>>(a, st);
+    else if (form == Form::rows64) return launch_tile<Y, TileShape<GATED, FAST, 4, 2, 1, 4, 3>>(a, st);
+    else if (form == Form::rows128) return launch_tile<Y, TileShape<GATED, FAST, 4, 4, 2, 2, 2>>(a, st);
+    else if constexpr (FAST) return launch_tile<Y, TileShape<GATED, FAST, 4, 8, 4, 2, 2>>(a, st);
     return hipGetLastError();
 }
 template <typename Y>
-hipError_t launch(const Gemm& a, bool gated, hipStream_t st)
+hipError_t launch(const Gemm& a, Form form, bool gated, hipStream_t st)
 {
-    return gated ? launch_few<Y, true>(a, st) : launch_few<Y, false>(a, st);
+    return gated ? launch_form<Y, true>(a, form, st) : launch_form<Y, false>(a, form, st);
 }
 
 int product(const arc_fp8_weights* w, const arc_fp8_weights* up, bool gated, const arc_fp8_rows* x, int y_dtype, void* y, uint32_t ldy,
@@ -300,9 +574,16 @@ int product(const arc_fp8_weights* w, const arc_fp8_weights* up, bool gated, con
     a.ldy = ldy;
     a.ldr = ldr;
     a.wide = aligned(y, 4 * size) && ldy % 4 == 0 && (!residual || (aligned(residual, 4 * size) && ldr % 4 == 0));
-    const hipError_t e = y_dtype == ARC_F32   ? launch<float>(a, gated, st)
-                         : y_dtype == ARC_F16 ? launch<_Float16>(a, gated, st)
-                                              : launch<bf16>(a, gated, st);
+    const Plan p = plan_of(N, a.blocks, a.M, gated, size == 2);
+    if (uint64_t(p.mtiles) * p.ntiles * p.splits >= (1u << 22))
+        return set_error(ARC_ERR_UNSUPPORTED, "%u rows by %u outputs: more tiles than one call takes", a.M, N);
+    a.part = static_cast<float*>(workspace);
+    a.mtiles = p.mtiles;
+    a.ntiles = p.ntiles;
+    a.splits = p.splits;
+    const hipError_t e = y_dtype == ARC_F32   ? launch<float>(a, p.form, gated, st)
+                         : y_dtype == ARC_F16 ? launch<_Float16>(a, p.form, gated, st)
+                                              : launch<bf16>(a, p.form, gated, st);
     return check_hip(e, "fp8 product");
 }
 
@@ -324,7 +605,7 @@ int arc_fp8_quantize(int x_dtype, const void* x, uint32_t ldx, const arc_fp8_row
         return set_error(ARC_ERR_INVALID_ARGUMENT, "x and the rows share memory");
     if (out->rows == 0) return ARC_OK;
     const Quantize a{x, static_cast<uint8_t*>(out->q), out->scales, out->rows, out->cols, ldx, out->ldq, out->lds};
-    const dim3 grid((out->cols + 511) / 512, (out->rows + kQuantRows - 1) / kQuantRows);
+    const dim3 grid((out->rows + kQuantRows - 1) / kQuantRows, (out->cols + 511) / 512);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (x_dtype == ARC_F32) hipLaunchKernelGGL(k_fp8_quantize<float>, grid, dim3(256), 0, st, a);
     else if (x_dtype == ARC_F16) hipLaunchKernelGGL(k_fp8_quantize<_Float16>, grid, dim3(256), 0, st, a);
@@ -334,8 +615,10 @@ int arc_fp8_quantize(int x_dtype, const void* x, uint32_t ldx, const arc_fp8_row
 
 size_t arc_fp8_gemm_workspace_bytes(uint32_t N, uint32_t K, uint32_t M, int gated)
 {
-    (void)gated;
-    return N == 0 || N > kMaxRows || M > kMaxRows || K == 0 || K % 16 || K > kMaxLd ? 0 : 256;
+    if (N == 0 || N > kMaxRows || M > kMaxRows || K == 0 || K % 16 || K > kMaxLd) return 0;
+    const uint32_t blocks = (K + kFpBlock - 1) / kFpBlock;
+    const size_t fast = plan_of(N, blocks, M, gated != 0, true).bytes, wide = plan_of(N, blocks, M, gated != 0, false).bytes;
+    return fast > wide ? fast : wide;
 }
 
 int arc_fp8_gemm(const arc_fp8_weights* w, const arc_fp8_rows* x, int y_dtype, void* y, uint32_t ldy, const void* residual, uint32_t ldr,
