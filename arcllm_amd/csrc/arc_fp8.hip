@@ -7,6 +7,8 @@
 // multiply-adds in fp32.
 #include "arc_paged.hpp"
 
+#include <type_traits>
+
 namespace arc {
 namespace {
 
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(512) void k_fp8_few(Gemm a)
 // up, at the same outputs.
 template <bool GATED_, bool FAST_, int WM_, int WN_, int GM_, int GN_, int S_>
 struct TileShape {
-    static constexpr bool GATED = GATED_, FAST = FAST_;
+    static constexpr bool GATED = GATED_, FAST = FAST_, DEEP = FAST && WN_ >= 4;
     static constexpr int WM = WM_, WN = WN_, GM = GM_, GN = GN_, S = S_, NW = GM * GN, G = GATED ? 2 : 1;
     static constexpr uint32_t BM = 16 * WM * GM, BN = 16 * WN * GN, OUT = BN / G;  // outputs of a row
     static constexpr uint32_t CW = BN / 8 / NW, CX = BM / 8 / NW, COPIES = CW + CX + 2;  // a wave's, of a block
@@ -230,8 +232,6 @@ struct TileShape {
     };
 };
 
-__device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
-
 // 16 or 4 bytes per lane from memory straight into LDS, lane i's at lds + 16 i (4 i).  Assembly: the compiler would wait
 // for such a copy before any read of LDS; there is no register for a load in flight to write, and
 // nothing else here uses m0.
@@ -239,13 +239,23 @@ __device__ __forceinline__ void copy16(uint32_t lds, const void* base, uint32_t 
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
-__device__ __forceinline__ void copy16(uint32_t lds, const void* from)
+// x's values from column K on become zeros, c the lane's first column: against what stands there in w's place, finite
+// unless w's row has a NaN before K, which then is its output anyway.
+__device__ __forceinline__ void only_to(Frag& f, uint32_t c, uint32_t K)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f.lo[i] = c < K ? f.lo[i] : 0u;
+        f.hi[i] = c + 64 < K ? f.hi[i] : 0u;
+    }
 }
 __device__ __forceinline__ void copy4(uint32_t lds, const void* base, uint32_t off)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t lds, const void* from)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory");
 }
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
 __device__ __forceinline__ uint32_t lds_at(const void* p)
@@ -274,6 +284,53 @@ __device__ __forceinline__ Place place_of(const Gemm& a, uint32_t id)
     return p;
 }
 
+// A wave's copies of a block: CW of weights, CX of x, 8 rows each (a lane 16 bytes of row 8 * (i * NW + wave) + lane / 8),
+// and two of scales.  Rows past the last are the last again; from column K on a row's last 16 values, see only_to.
+template <typename C>
+struct Copies {
+    uint32_t wave, n0, m0, row8, chunk, xsoff, nblock;
+    const float* ws;
+    __device__ __forceinline__ Copies(const Gemm& a, const Place& at, uint32_t wave_, uint32_t lane)
+    {
+        wave = wave_;
+        n0 = at.n * C::OUT;
+        m0 = at.m * C::BM;
+        row8 = lane >> 3;
+        chunk = ((lane & 7u) ^ swizzle(8 * wave + row8)) * 16;  // the same for all copies, as NW is even
+        xsoff = (min(m0 + 64 * (wave % (C::XS / 64)) + lane, a.M - 1) - m0) * 4;
+        nblock = n0 / kFpBlock;
+        const uint32_t h = C::GATED ? lane >> 5 : 0;
+        ws = (C::GATED && h ? a.ws[1] : a.ws[0]) + uint64_t(min(nblock + (lane & 31u), (a.N - 1) / kFpBlock)) * (C::GATED && h ? a.ldws[1] : a.ldws[0]);
+    }
+    __device__ __forceinline__ void rows(const Gemm& a, uint32_t to, const uint8_t* base, uint32_t last, uint32_t ld, uint32_t k) const
+    {
+        copy16(to, base + k, __umul24(min(row8, last), ld) + min(chunk, a.K - 16 - k));
+    }
+    // Copy i of block b: one of weights, then of x, then the scales.
+    __device__ __forceinline__ void one(const Gemm& a, typename C::Lds& lds, uint32_t b, uint32_t buf, uint32_t i) const
+    {
+        const uint32_t k = b * kFpBlock;
+        if (i < C::CW) {
+            constexpr uint32_t kStrip = 16 * C::WN, kHalf = kStrip / C::G;
+            const uint32_t R = 8 * (i * C::NW + wave), strip = R / kStrip, in = R % kStrip, h = C::GATED ? in / kHalf : 0;
+            const uint32_t n = min(n0 + strip * kHalf + in % kHalf, a.N - 1), ld = h ? a.ldw[1] : a.ldw[0];
+            rows(a, lds_at(&lds.w[buf][R * kFpBlock]), (h ? a.w[1] : a.w[0]) + uint64_t(n) * ld, a.N - 1 - n, ld, k);
+        } else if (i < C::CW + C::CX) {
+            const uint32_t R = 8 * ((i - C::CW) * C::NW + wave), m = min(m0 + R, a.M - 1);
+            rows(a, lds_at(&lds.x[buf][R * kFpBlock]), a.x + uint64_t(m) * a.ldx, a.M - 1 - m, a.ldx, k);
+        } else if (i == C::CW + C::CX) {
+            copy4(lds_at(&lds.xs[buf][64 * (wave % (C::XS / 64))]), a.xs + uint64_t(b) * a.ldxs + m0, xsoff);
+        } else {
+            copy4(lds_at(&lds.ws[buf][0]), ws + b);
+        }
+    }
+    __device__ __forceinline__ void block(const Gemm& a, typename C::Lds& lds, uint32_t b, uint32_t buf) const
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < C::COPIES; ++i) one(a, lds, b, buf, i);
+    }
+};
+
 template <typename Y, typename C>
 __device__ __forceinline__ void finish(const Gemm& a, const Place& at, uint32_t wave, int i, int j, uint32_t lane, f32x4 v, f32x4 up)
 {
@@ -286,6 +343,25 @@ __device__ __forceinline__ void finish(const Gemm& a, const Place& at, uint32_t 
     store_out<Y>(a, m, n, v);
 }
 
+// The tile's outputs, or its sums for k_fp8_join.
+template <typename Y, typename C>
+__device__ __forceinline__ void put_tile(const Gemm& a, const Place& at, uint32_t wave, uint32_t lane, const f32x4 (&acc)[C::WN][C::WM])
+{
+    constexpr int WM = C::WM, WN = C::WN, G = C::G;
+    if (a.splits == 1) {
+#pragma unroll
+        for (int i = 0; i < WN / G; ++i)
+#pragma unroll
+            for (int j = 0; j < WM; ++j) finish<Y, C>(a, at, wave, i, j, lane, acc[i][j], acc[i + WN / G * (G - 1)][j]);
+        return;
+    }
+    f32x4* part = reinterpret_cast<f32x4*>(a.part) + ((uint64_t(at.m) * a.ntiles + at.n) * a.splits + at.split) * (C::BM * C::BN / 4);
+#pragma unroll
+    for (int i = 0; i < WN; ++i)
+#pragma unroll
+        for (int j = 0; j < WM; ++j) part[((wave * WN + i) * WM + j) * 64 + lane] = acc[i][j];
+}
+
 template <typename Y, typename C>
 __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
 {
@@ -294,53 +370,10 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4, wave = uniform(threadIdx.x >> 6);
     const uint32_t wm = wave / C::GN, wn = wave % C::GN;
     const Place at = place_of(a, blockIdx.x);
-    const uint32_t n0 = at.n * C::OUT, m0 = at.m * C::BM;
+    const uint32_t n0 = at.n * C::OUT, nblock = n0 / kFpBlock;
     const uint32_t b0 = uint32_t(uint64_t(a.blocks) * at.split / a.splits), b1 = uint32_t(uint64_t(a.blocks) * (at.split + 1) / a.splits);
 
-    // what each copy of this wave reads: 8 rows, a lane 16 bytes of row 8 * (i * NW + wave) + lane / 8
-    const uint32_t row8 = lane >> 3, chunk = ((lane & 7u) ^ swizzle(8 * wave + row8)) * 16;
-    uint32_t woff[C::CW], xoff[C::CX];
-#pragma unroll
-    for (uint32_t i = 0; i < C::CW; ++i) {
-        const uint32_t R = 8 * (i * C::NW + wave) + row8, strip = R / (16 * WN), in = R % (16 * WN);
-        const uint32_t n = n0 + strip * (16 * WN / G) + in % (16 * WN / G), h = in / (16 * WN / G);
-        woff[i] = (min(n, a.N - 1) - n0) * a.ldw[h] + chunk;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < C::CX; ++i) xoff[i] = (min(m0 + 8 * (i * C::NW + wave) + row8, a.M - 1) - m0) * a.ldx + chunk;
-    const uint32_t xsoff = (min(m0 + 64 * (wave % (C::XS / 64)) + lane, a.M - 1) - m0) * 4;
-    const uint32_t nblock = n0 / kFpBlock, nblocks = (a.N + kFpBlock - 1) / kFpBlock;
-    const uint32_t wsoff = (min(nblock + (lane & 31u), nblocks - 1) - nblock) * a.ldws[lane >> 5 & (G - 1)] * 4;
-
-    auto copy_block = [&](uint32_t b, uint32_t buf) {
-        const uint32_t k = b * kFpBlock;
-        const bool whole = k + kFpBlock <= a.K;  // else blocks from column K on are zeros
-#pragma unroll
-        for (uint32_t i = 0; i < C::CW; ++i) {
-            const uint32_t rows = i * C::NW + wave, h = G == 1 ? 0 : (8 * rows) % (16 * WN) / (8 * WN);
-            const uint8_t* base = a.w[h] + uint64_t(n0) * a.ldw[h] + k;
-            const uint32_t to = lds_at(&lds.w[buf][rows * 1024]);
-            if (whole) copy16(to, base, woff[i]);
-            else copy16(to, k + chunk < a.K ? static_cast<const void*>(base + woff[i]) : kZeros);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < C::CX; ++i) {
-            const uint32_t rows = i * C::NW + wave;
-            const uint8_t* base = a.x + uint64_t(m0) * a.ldx + k;
-            const uint32_t to = lds_at(&lds.x[buf][rows * 1024]);
-            if (whole) copy16(to, base, xoff[i]);
-            else copy16(to, k + chunk < a.K ? static_cast<const void*>(base + xoff[i]) : kZeros);
-        }
-        copy4(lds_at(&lds.xs[buf][64 * (wave % (C::XS / 64))]), a.xs + uint64_t(b) * a.ldxs + m0, xsoff);
-        if constexpr (G == 1) {
-            copy4(lds_at(&lds.ws[buf][0]), a.ws[0] + uint64_t(nblock) * a.ldws[0] + b, wsoff);
-        } else {
-            const float* base = (lane < 32 ? a.ws[0] + uint64_t(nblock) * a.ldws[0] : a.ws[1] + uint64_t(nblock) * a.ldws[1]) + b;
-            const float* from = base + wsoff / 4;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_at(&lds.ws[buf][0])), "v"(from) : "memory");
-        }
-    };
-
+    const Copies<C> copies(a, at, wave, lane);
     f32x4 acc[WN][WM];
 #pragma unroll
     for (int i = 0; i < WN; ++i)
@@ -349,7 +382,7 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
 
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
-        if (b0 + i < b1) copy_block(b0 + i, i);
+        if (b0 + i < b1) copies.block(a, lds, b0 + i, i);
     uint32_t buf = 0;
     for (uint32_t b = b0; b < b1; ++b) {
         // this block's copies have arrived; those of the S - 2 after it may be under way
@@ -357,7 +390,7 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's; and the block before is read
         const uint32_t ahead = buf == 0 ? S - 1 : buf - 1;
-        if (b + S - 1 < b1) copy_block(b + S - 1, ahead);
+        if (b + S - 1 < b1) copies.block(a, lds, b + S - 1, ahead);
 
         const uint8_t* xl = &lds.x[buf][(wm * WM * 16 + r) * kFpBlock];
         const uint8_t* wl = &lds.w[buf][(wn * WN * 16 + r) * kFpBlock];
@@ -373,10 +406,16 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
 #pragma unroll
             for (int j = 0; j < WM; ++j) s[h][j] = w * lds.xs[buf][(wm * WM + j) * 16 + r];
         }
+        Frag xb[WM];
+#pragma unroll
+        for (int j = 0; j < WM; ++j) xb[j] = frag_at(xl + j * 16 * kFpBlock);
+        if ((b + 1) * kFpBlock > a.K)
+#pragma unroll
+            for (int j = 0; j < WM; ++j) only_to(xb[j], b * kFpBlock + g * 16, a.K);
         if constexpr (C::FAST) {
             i32x8 xf[WM];
 #pragma unroll
-            for (int j = 0; j < WM; ++j) xf[j] = __builtin_bit_cast(i32x8, frag_at(xl + j * 16 * kFpBlock));
+            for (int j = 0; j < WM; ++j) xf[j] = __builtin_bit_cast(i32x8, xb[j]);
             f32x4 p[2][WM];
 #pragma unroll
             for (int i = 0; i <= WN; ++i) {
@@ -396,7 +435,7 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
         } else {
             Wide xf[WM];
 #pragma unroll
-            for (int j = 0; j < WM; ++j) xf[j] = widen(frag_at(xl + j * 16 * kFpBlock));
+            for (int j = 0; j < WM; ++j) xf[j] = widen(xb[j]);
 #pragma unroll
             for (int i = 0; i < WN; ++i) {
                 const Wide wf = widen(frag_at(wl + i * 16 * kFpBlock));
@@ -410,18 +449,143 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
         }
         buf = buf + 1 == S ? 0 : buf + 1;
     }
-    if (a.splits == 1) {
-#pragma unroll
-        for (int i = 0; i < WN / G; ++i)
-#pragma unroll
-            for (int j = 0; j < WM; ++j) finish<Y, C>(a, at, wave, i, j, lane, acc[i][j], acc[i + WN / G * (G - 1)][j]);
-        return;
-    }
-    f32x4* part = reinterpret_cast<f32x4*>(a.part) + ((uint64_t(at.m) * a.ntiles + at.n) * a.splits + at.split) * (C::BM * C::BN / 4);
+    put_tile<Y, C>(a, at, wave, lane, acc);
+}
+
+// Large tiles.  Bound by the matrix cores if everything else keeps out of their way: per block and wave 32 (16) products of 32
+// cycles, 4 fused multiply-adds for each, 24 (16) LDS reads.  So the order is fixed by hand: products in pairs of
+// w's tiles, each followed by the multiply-adds of the product three before it and by LDS reads of what the next pair
+// needs.  The one barrier of a block stands before its last pair, when all of the block is in registers: behind it the
+// next block but one is copied over it, and the next one's first operands are read while the last pair is multiplied, x's
+// into the registers that the pair has just left.
+template <typename Y, typename C>
+__global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm a)
+{
+    constexpr int WM = C::WM, WN = C::WN, G = C::G, NP = WN / 2, PAIR = 2 * WM, SLOTS = WN * WM, LAG = 3;
+    static_assert(C::FAST && C::S == 2 && WM == 4 && NP % 2 == 0 && C::CW + C::CX == 8);
+    __shared__ typename C::Lds lds;
+    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4, wave = uniform(threadIdx.x >> 6);
+    const uint32_t wm = wave / C::GN, wn = wave % C::GN;
+    const Place at = place_of(a, blockIdx.x);
+    const uint32_t b0 = uint32_t(uint64_t(a.blocks) * at.split / a.splits), b1 = uint32_t(uint64_t(a.blocks) * (at.split + 1) / a.splits);
+    const Copies<C> copies(a, at, wave, lane);
+
+    const uint32_t place = (g ^ swizzle(r)) * 16, wrow = (wn * WN * 16 + r) * kFpBlock, xrow = (wm * WM * 16 + r) * kFpBlock;
+    const uint32_t wsat = (at.n * C::OUT + wn * (C::OUT / C::GN)) / kFpBlock - copies.nblock;
+    Frag wf[2][2], xf[WM];
+    float s[G][WM], sn[G][WM], xs[WM];
+    f32x4 acc[WN][WM], p[LAG + 1];
 #pragma unroll
     for (int i = 0; i < WN; ++i)
 #pragma unroll
-        for (int j = 0; j < WM; ++j) part[((wave * WN + i) * WM + j) * 64 + lane] = acc[i][j];
+        for (int j = 0; j < WM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i <= LAG; ++i) p[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int j = 0; j < WM; ++j) s[h][j] = 0.0f;
+    auto half = [&](const uint8_t* rows, int tile, uint32_t at_) { return *reinterpret_cast<const u32x4*>(rows + tile * 16 * kFpBlock + at_); };
+    auto read_w = [&](uint32_t buf, int tile, Frag& f, int which) {
+        if (which == 0) f.lo = half(&lds.w[buf][wrow], tile, place);
+        else f.hi = half(&lds.w[buf][wrow], tile, place ^ 64u);
+    };
+    auto read_x = [&](uint32_t buf, int tile) {
+        xf[tile].lo = half(&lds.x[buf][xrow], tile, place);
+        xf[tile].hi = half(&lds.x[buf][xrow], tile, place ^ 64u);
+    };
+    auto read_xs = [&](uint32_t buf, int j) { xs[j] = lds.xs[buf][(wm * WM + j) * 16 + r]; };
+    auto read_scales = [&](uint32_t buf) {
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            const float w = lds.ws[buf][32 * h + wsat];
+#pragma unroll
+            for (int j = 0; j < WM; ++j) sn[h][j] = xs[j] * w;
+        }
+    };
+
+    copies.block(a, lds, b0, 0);
+    if (b0 + 1 < b1) {
+        copies.block(a, lds, b0 + 1, 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::COPIES) : "memory");
+    } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < WM; ++j) {
+        read_x(0, j);
+        only_to(xf[j], b0 * kFpBlock + g * 16, a.K);
+        read_xs(0, j);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) read_w(0, e >> 1, wf[0][e >> 1], e & 1);
+    read_scales(0);
+
+    // Block b from buffer buf.  AHEAD: the next block but one is copied; else it is not, and the next is the last, which K may
+    // end; LAST: there is no next.  One basic block, else the compiler takes the multiply-adds out of their places.
+    auto step = [&](auto ahead, auto last, uint32_t b, uint32_t buf) {
+        constexpr bool AHEAD = decltype(ahead)::value, LAST = decltype(last)::value;
+#pragma unroll
+        for (int q = 0; q < SLOTS; ++q) {
+            const int P = q / PAIR, e = q % PAIR, j = e >> 1;
+            if (!LAST && P == NP - 1 && e == 0) {
+                // the next block's copies have arrived, everyone's; this one is read
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            p[q % (LAG + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, wf[P & 1][e & 1]),
+                                                                               __builtin_bit_cast(i32x8, xf[j]), f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+            if (P < NP - 1) {
+                if (e < 4) read_w(buf, 2 * (P + 1) + (e >> 1), wf[(P + 1) & 1][e >> 1], e & 1);
+            } else if constexpr (!LAST) {
+                if (e & 1) {
+                    read_x(buf ^ 1u, j);
+                    read_xs(buf ^ 1u, j);
+                } else if (e < 4) {
+                    read_w(buf ^ 1u, j, wf[0][j], 0);
+                    read_w(buf ^ 1u, j, wf[0][j], 1);
+                }
+                if constexpr (AHEAD) {
+                    copies.one(a, lds, b + 2, buf, uint32_t(e));
+                    if (e == 1) copies.one(a, lds, b + 2, buf, C::CW + C::CX);
+                    if (e == 3) copies.one(a, lds, b + 2, buf, C::CW + C::CX + 1);
+                }
+            }
+            if (q == LAG)
+#pragma unroll
+                for (int h = 0; h < G; ++h)
+#pragma unroll
+                    for (int jj = 0; jj < WM; ++jj) s[h][jj] = sn[h][jj];
+            const int k = (q + SLOTS - LAG) % SLOTS, ki = 2 * (k / PAIR) + (k % PAIR & 1), kj = k % PAIR >> 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                acc[ki][kj][i] = __builtin_fmaf(p[k % (LAG + 1)][i], s[ki / (WN / G)][kj], acc[ki][kj][i]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (!LAST) {
+            read_scales(buf ^ 1u);
+            if constexpr (!AHEAD)
+#pragma unroll
+                for (int j = 0; j < WM; ++j) only_to(xf[j], (b + 1) * kFpBlock + g * 16, a.K);
+        }
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    uint32_t b = b0, buf = 0;
+    for (; b + 2 < b1; ++b, buf ^= 1u) step(yes, no, b, buf);
+    if (b + 1 < b1) {
+        step(no, no, b, buf);
+        ++b;
+        buf ^= 1u;
+    }
+    step(no, yes, b, buf);
+#pragma unroll
+    for (int k = SLOTS - LAG; k < SLOTS; ++k) {
+        const int ki = 2 * (k / PAIR) + (k % PAIR & 1), kj = k % PAIR >> 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[ki][kj][i] = __builtin_fmaf(p[k % (LAG + 1)][i], s[ki / (WN / G)][kj], acc[ki][kj][i]);
+    }
+    put_tile<Y, C>(a, at, wave, lane, acc);
 }
 
 // Adds up the parts of a tile in order; a thread has 4 outputs, those of one lane above.
@@ -505,7 +669,8 @@ Plan plan_of(uint32_t N, uint32_t blocks, uint32_t M, bool gated, bool fast)
 template <typename Y, typename C>
 hipError_t launch_tile(const Gemm& a, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_fp8_tile<Y, C>), dim3(a.mtiles * a.ntiles * a.splits), dim3(C::NW * 64), 0, st, a);
+    if constexpr (C::DEEP) hipLaunchKernelGGL((k_fp8_deep<Y, C>), dim3(a.mtiles * a.ntiles * a.splits), dim3(C::NW * 64), 0, st, a);
+    else hipLaunchKernelGGL((k_fp8_tile<Y, C>), dim3(a.mtiles * a.ntiles * a.splits), dim3(C::NW * 64), 0, st, a);
     if (a.splits > 1) {
         if (hipError_t e = hipGetLastError()) return e;
         hipLaunchKernelGGL((k_fp8_join<Y, C>), dim3(a.mtiles * a.ntiles * (C::BM * C::OUT / 1024)), dim3(256), 0, st, a);
