@@ -107,8 +107,24 @@ struct Gemm {
     uint32_t mtiles, ntiles, splits;
 };
 
+// The kernel's arguments (its one parameter, a Gemm), read again: a phase that takes its own copy keeps none of it in
+// scalar registers for the phases after it.
+__device__ __forceinline__ const Gemm& arguments()
+{
+    typedef __attribute__((address_space(4))) const Gemm Arg;
+    Arg* p = (Arg*)(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(p));
+    return *(const Gemm*)(p);
+}
+
 // 4 neighbouring outputs of a row: the activation or the residual, rounded once.
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+// silu, off by some 2^-20 with the hardware's exponential and reciprocal, which is enough for 16 bits.
+template <typename Y>
+__device__ __forceinline__ float silu(float g)
+{
+    if constexpr (sizeof(Y) == 2) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f));
+    else return g / (1.0f + expf(-g));
+}
 template <typename Y>
 __device__ __forceinline__ void store_out(const Gemm& a, uint32_t m, uint32_t n, f32x4 v)
 {
@@ -209,20 +225,21 @@ __global__ __launch_bounds__(512) void k_fp8_few(Gemm a)
     }
     if constexpr (GATED)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[0][i] = silu(t[0][i]) * t[1][i];
+        for (int i = 0; i < 4; ++i) t[0][i] = silu<Y>(t[0][i]) * t[1][i];
     store_out<Y>(a, m0 + r, n0 + 4 * g, t[0]);
 }
 
 // Tiles.  A workgroup of GM x GN waves has BM rows of x and BN rows of w, a wave WM x WN tiles of 16 x 16.  A block of both
 // comes straight into LDS, S blocks deep; one barrier a block.  With the activation a wave's weights are half gate, half
 // up, at the same outputs.
-template <bool GATED_, bool FAST_, int WM_, int WN_, int GM_, int GN_, int S_>
+template <bool GATED_, bool FAST_, bool DEEP_, int WM_, int WN_, int GM_, int GN_, int S_>
 struct TileShape {
-    static constexpr bool GATED = GATED_, FAST = FAST_, DEEP = FAST && WN_ >= 4;
+    static constexpr bool GATED = GATED_, FAST = FAST_, DEEP = DEEP_;
     static constexpr int WM = WM_, WN = WN_, GM = GM_, GN = GN_, S = S_, NW = GM * GN, G = GATED ? 2 : 1;
     static constexpr uint32_t BM = 16 * WM * GM, BN = 16 * WN * GN, OUT = BN / G;  // outputs of a row
     static constexpr uint32_t CW = BN / 8 / NW, CX = BM / 8 / NW, COPIES = CW + CX + 2;  // a wave's, of a block
     static constexpr uint32_t XS = BM < 64 ? 64 : BM;
+    static constexpr uint32_t WGS = NW == 8 ? 256 : 512;  // that fill the card
     static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0 && NW % 2 == 0);
     struct Lds {
         __align__(16) uint8_t w[S][BN * kFpBlock];
@@ -306,18 +323,32 @@ struct Copies {
     {
         copy16(to, base + k, __umul24(min(row8, last), ld) + min(chunk, a.K - 16 - k));
     }
+    // Whether copy i is of the gate or the up weights.
+    __device__ __forceinline__ uint32_t half(uint32_t i) const { return 8 * (i * C::NW + wave) % (16 * C::WN) / (8 * C::WN); }
+    // Where copy i's 8 rows begin, and the last that there is, counted from there.
+    __device__ __forceinline__ const uint8_t* group(const Gemm& a, uint32_t i, uint32_t& last) const
+    {
+        if (i < C::CW) {
+            constexpr uint32_t kStrip = 16 * C::WN, kHalf = kStrip / C::G;
+            const uint32_t R = 8 * (i * C::NW + wave), h = C::GATED ? half(i) : 0;
+            const uint32_t n = min(n0 + R / kStrip * kHalf + R % kHalf, a.N - 1);
+            last = a.N - 1 - n;
+            return a.w[h] + uint64_t(n) * a.ldw[h];
+        }
+        const uint32_t m = min(m0 + 8 * ((i - C::CW) * C::NW + wave), a.M - 1);
+        last = a.M - 1 - m;
+        return a.x + uint64_t(m) * a.ldx;
+    }
     // Copy i of block b: one of weights, then of x, then the scales.
     __device__ __forceinline__ void one(const Gemm& a, typename C::Lds& lds, uint32_t b, uint32_t buf, uint32_t i) const
     {
         const uint32_t k = b * kFpBlock;
-        if (i < C::CW) {
-            constexpr uint32_t kStrip = 16 * C::WN, kHalf = kStrip / C::G;
-            const uint32_t R = 8 * (i * C::NW + wave), strip = R / kStrip, in = R % kStrip, h = C::GATED ? in / kHalf : 0;
-            const uint32_t n = min(n0 + strip * kHalf + in % kHalf, a.N - 1), ld = h ? a.ldw[1] : a.ldw[0];
-            rows(a, lds_at(&lds.w[buf][R * kFpBlock]), (h ? a.w[1] : a.w[0]) + uint64_t(n) * ld, a.N - 1 - n, ld, k);
-        } else if (i < C::CW + C::CX) {
-            const uint32_t R = 8 * ((i - C::CW) * C::NW + wave), m = min(m0 + R, a.M - 1);
-            rows(a, lds_at(&lds.x[buf][R * kFpBlock]), a.x + uint64_t(m) * a.ldx, a.M - 1 - m, a.ldx, k);
+        if (i < C::CW + C::CX) {
+            uint32_t last;
+            const uint8_t* base = group(a, i, last);
+            const bool is_w = i < C::CW;
+            rows(a, lds_at(is_w ? &lds.w[buf][8 * (i * C::NW + wave) * kFpBlock] : &lds.x[buf][8 * ((i - C::CW) * C::NW + wave) * kFpBlock]),
+                 base, last, is_w ? a.ldw[C::GATED ? half(i) : 0] : a.ldx, k);
         } else if (i == C::CW + C::CX) {
             copy4(lds_at(&lds.xs[buf][64 * (wave % (C::XS / 64))]), a.xs + uint64_t(b) * a.ldxs + m0, xsoff);
         } else {
@@ -331,6 +362,55 @@ struct Copies {
     }
 };
 
+// The same copies of whole blocks, one after the other, with what does not change kept in scalar registers: a copy is
+// then 4 scalar and 2 vector instructions beside its own.
+template <typename C>
+struct Stream {
+    const uint8_t* from[C::CW + C::CX];  // of the next block
+    uint32_t last[C::CW + C::CX];        // of its 8 rows, the last that there is
+    const float *xs, *ws;
+    uint32_t row8, chunk, xsoff, ldx, ldxs, ldw[C::G], w, x, xsat, wsat;
+    __device__ __forceinline__ Stream(const Gemm& a, const Place& at, uint32_t wave, uint32_t lane, typename C::Lds& lds, uint32_t b)
+    {
+        const Copies<C> c(a, at, wave, lane);
+        row8 = c.row8;
+        chunk = c.chunk;
+        xsoff = c.xsoff;
+        ldx = a.ldx;
+        ldxs = a.ldxs;
+#pragma unroll
+        for (int h = 0; h < C::G; ++h) ldw[h] = a.ldw[h];
+#pragma unroll
+        for (uint32_t i = 0; i < C::CW + C::CX; ++i) {
+            const uint8_t* p = c.group(a, i, last[i]) + uint64_t(b) * kFpBlock;
+            asm("" : "+s"(p), "+s"(last[i]));  // kept, not computed again
+            from[i] = p;
+        }
+        xs = a.xs + uint64_t(b) * ldxs + c.m0;
+        ws = c.ws + b;
+        w = lds_at(&lds.w[0][8 * c.wave * kFpBlock]);
+        x = lds_at(&lds.x[0][8 * c.wave * kFpBlock]);
+        xsat = lds_at(&lds.xs[0][64 * (c.wave % (C::XS / 64))]);
+        wsat = lds_at(&lds.ws[0][0]);
+    }
+    __device__ __forceinline__ void one(uint32_t i, uint32_t buf)
+    {
+        if (i < C::CW + C::CX) {
+            const bool is_w = i < C::CW;
+            const uint32_t ld = is_w ? ldw[C::GATED ? i % 2 : 0] : ldx;  // NW = WN: a half's rows are one copy of each wave
+            const uint32_t to = is_w ? w + buf * C::BN * kFpBlock + i * C::NW * 1024 : x + buf * C::BM * kFpBlock + (i - C::CW) * C::NW * 1024;
+            copy16(to, from[i], __umul24(min(row8, last[i]), ld) + chunk);
+            from[i] += kFpBlock;
+        } else if (i == C::CW + C::CX) {
+            copy4(xsat + buf * C::XS * 4, xs, xsoff);
+            xs += ldxs;
+        } else {
+            copy4(wsat + buf * 256, ws);
+            ++ws;
+        }
+    }
+};
+
 template <typename Y, typename C>
 __device__ __forceinline__ void finish(const Gemm& a, const Place& at, uint32_t wave, int i, int j, uint32_t lane, f32x4 v, f32x4 up)
 {
@@ -339,7 +419,7 @@ __device__ __forceinline__ void finish(const Gemm& a, const Place& at, uint32_t 
     const uint32_t n = at.n * C::OUT + wn * (C::OUT / C::GN) + i * 16 + 4 * (lane >> 4);
     if constexpr (C::GATED)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = silu(v[e]) * up[e];
+        for (int e = 0; e < 4; ++e) v[e] = silu<Y>(v[e]) * up[e];
     store_out<Y>(a, m, n, v);
 }
 
@@ -453,139 +533,147 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
 }
 
 // Large tiles.  Bound by the matrix cores if everything else keeps out of their way: per block and wave 32 (16) products of 32
-// cycles, 4 fused multiply-adds for each, 24 (16) LDS reads.  So the order is fixed by hand: products in pairs of
-// w's tiles, each followed by the multiply-adds of the product three before it and by LDS reads of what the next pair
-// needs.  The one barrier of a block stands before its last pair, when all of the block is in registers: behind it the
-// next block but one is copied over it, and the next one's first operands are read while the last pair is multiplied, x's
-// into the registers that the pair has just left.
+// cycles, 4 fused multiply-adds for each, 24 (16) LDS reads.  So the order is fixed by hand, each product with its part of the rest:
+// the multiply-adds of the product three before it, and LDS reads some 6 (3) products ahead of their use.  For that, a block's
+// products come in quarters: the lower half of w's tiles by x's first two, then by x's other two, the upper half by the
+// first two, by the others; half of w's and all of x's operands are in registers at once, and each is replaced when its
+// last product has begun.  In the third quarter all of the block is in registers: there stands its one barrier, behind which
+// the next block but one is copied over it and the next one's first operands are read.  All blocks are whole (K a multiple of 128).
 template <typename Y, typename C>
-__global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm a)
+__global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
 {
-    constexpr int WM = C::WM, WN = C::WN, G = C::G, NP = WN / 2, PAIR = 2 * WM, SLOTS = WN * WM, LAG = 3;
-    static_assert(C::FAST && C::S == 2 && WM == 4 && NP % 2 == 0 && C::CW + C::CX == 8);
+    constexpr int WM = C::WM, WN = C::WN, G = C::G, H = WN / 2, SLOTS = WN * WM, LAG = 3;
+    static_assert(C::FAST && C::S == 2 && WM == 4 && H % 2 == 0 && C::CW + C::CX == 8 && C::NW == WN);
     __shared__ typename C::Lds lds;
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4, wave = uniform(threadIdx.x >> 6);
     const uint32_t wm = wave / C::GN, wn = wave % C::GN;
-    const Place at = place_of(a, blockIdx.x);
-    const uint32_t b0 = uint32_t(uint64_t(a.blocks) * at.split / a.splits), b1 = uint32_t(uint64_t(a.blocks) * (at.split + 1) / a.splits);
-    const Copies<C> copies(a, at, wave, lane);
-
     const uint32_t place = (g ^ swizzle(r)) * 16, wrow = (wn * WN * 16 + r) * kFpBlock, xrow = (wm * WM * 16 + r) * kFpBlock;
-    const uint32_t wsat = (at.n * C::OUT + wn * (C::OUT / C::GN)) / kFpBlock - copies.nblock;
-    Frag wf[2][2], xf[WM];
-    float s[G][WM], sn[G][WM], xs[WM];
+    Frag wf[H], xf[WM];
+    float s[G][WM], xs[WM], ws[G];
     f32x4 acc[WN][WM], p[LAG + 1];
-#pragma unroll
-    for (int i = 0; i < WN; ++i)
-#pragma unroll
-        for (int j = 0; j < WM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i <= LAG; ++i) p[i] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int h = 0; h < G; ++h)
-#pragma unroll
-        for (int j = 0; j < WM; ++j) s[h][j] = 0.0f;
-    auto half = [&](const uint8_t* rows, int tile, uint32_t at_) { return *reinterpret_cast<const u32x4*>(rows + tile * 16 * kFpBlock + at_); };
-    auto read_w = [&](uint32_t buf, int tile, Frag& f, int which) {
-        if (which == 0) f.lo = half(&lds.w[buf][wrow], tile, place);
-        else f.hi = half(&lds.w[buf][wrow], tile, place ^ 64u);
+    // the wave's scale of w in a block's: a strip lies in one block of 128
+    auto scale_at = [&](uint32_t tile) { return (tile * C::OUT + wn * (C::OUT / C::GN)) / kFpBlock - tile * C::OUT / kFpBlock; };
+    uint32_t wsat = 0;
+    auto frag = [&](const uint8_t* rows, int tile) {
+        const uint8_t* at_ = rows + tile * 16 * kFpBlock;
+        return Frag{*reinterpret_cast<const u32x4*>(at_ + place), *reinterpret_cast<const u32x4*>(at_ + (place ^ 64u))};
     };
-    auto read_x = [&](uint32_t buf, int tile) {
-        xf[tile].lo = half(&lds.x[buf][xrow], tile, place);
-        xf[tile].hi = half(&lds.x[buf][xrow], tile, place ^ 64u);
+    auto read_w = [&](uint32_t buf, int tile) { wf[tile % H] = frag(&lds.w[buf][wrow], tile); };
+    auto read_x = [&](uint32_t buf, int tile) { xf[tile] = frag(&lds.x[buf][xrow], tile); };
+    auto read_scale = [&](uint32_t buf, int j) {
+        if (j < WM) xs[j] = lds.xs[buf][(wm * WM + j) * 16 + r];
+        else if (j - WM < G) ws[j - WM] = lds.ws[buf][32 * (j - WM) + wsat];
     };
-    auto read_xs = [&](uint32_t buf, int j) { xs[j] = lds.xs[buf][(wm * WM + j) * 16 + r]; };
-    auto read_scales = [&](uint32_t buf) {
+    auto set_scales = [&]() {
 #pragma unroll
-        for (int h = 0; h < G; ++h) {
-            const float w = lds.ws[buf][32 * h + wsat];
+        for (int h = 0; h < G; ++h)
 #pragma unroll
-            for (int j = 0; j < WM; ++j) sn[h][j] = xs[j] * w;
-        }
+            for (int j = 0; j < WM; ++j) s[h][j] = xs[j] * ws[h];
+    };
+    // the tiles of product q of a block
+    auto w_tile = [](int q) {
+        const int quarter = q / (2 * H), e = q % (2 * H);
+        return quarter == 0 || quarter == 1 ? e / 2 : quarter == 2 ? H + e / 4 * 2 + e % 2 : H + e / 2;
+    };
+    auto x_tile = [](int q) {
+        const int quarter = q / (2 * H), e = q % (2 * H);
+        return quarter == 2 ? e / 2 % 2 : 2 * (quarter % 2) + e % 2;
+    };
+    auto multiply = [&](int q) {
+        p[q % (LAG + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            __builtin_bit_cast(i32x8, wf[w_tile(q) % H]), __builtin_bit_cast(i32x8, xf[x_tile(q)]), f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+    };
+    auto add = [&](int q) {  // product q's multiply-adds
+        const int i = w_tile(q), j = x_tile(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(p[q % (LAG + 1)][e], s[i / (WN / G)][j], acc[i][j][e]);
     };
 
-    copies.block(a, lds, b0, 0);
-    if (b0 + 1 < b1) {
-        copies.block(a, lds, b0 + 1, 1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::COPIES) : "memory");
-    } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    asm volatile("s_barrier" ::: "memory");
-#pragma unroll
-    for (int j = 0; j < WM; ++j) {
-        read_x(0, j);
-        only_to(xf[j], b0 * kFpBlock + g * 16, a.K);
-        read_xs(0, j);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) read_w(0, e >> 1, wf[0][e >> 1], e & 1);
-    read_scales(0);
-
-    // Block b from buffer buf.  AHEAD: the next block but one is copied; else it is not, and the next is the last, which K may
-    // end; LAST: there is no next.  One basic block, else the compiler takes the multiply-adds out of their places.
-    auto step = [&](auto ahead, auto last, uint32_t b, uint32_t buf) {
-        constexpr bool AHEAD = decltype(ahead)::value, LAST = decltype(last)::value;
+    // A block from buffer buf.  AHEAD: the next block but one is copied.  One basic block, else the compiler takes the
+    // multiply-adds out of their places; so what there is no next block for is read all the same, from LDS as it is.
+    auto step = [&](auto ahead, Stream<C>& stream, uint32_t buf) {
+        constexpr int kRead = 6 * H - 2;  // from here on the block's LDS is read no more
 #pragma unroll
         for (int q = 0; q < SLOTS; ++q) {
-            const int P = q / PAIR, e = q % PAIR, j = e >> 1;
-            if (!LAST && P == NP - 1 && e == 0) {
-                // the next block's copies have arrived, everyone's; this one is read
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            // the next block's copies have arrived, everyone's; this one is read
+            if (q == kRead) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            multiply(q);
+            if (q == 0) read_w(buf, H - 1);
+            if (q == 1 || q == 2) read_x(buf, q + 1);
+            if (q >= 2 * H && q < 4 * H && q % 2) read_w(buf, H + (q - 2 * H) / 2);
+            if (q == kRead || q == kRead + 1) read_x(buf ^ 1u, q - kRead);
+            if (q > 6 * H && q % 2 && q < SLOTS - 1) read_w(buf ^ 1u, (q - 6 * H) / 2);
+            if (q >= SLOTS - WM - G) read_scale(buf ^ 1u, q - (SLOTS - WM - G));
+            if constexpr (decltype(ahead)::value) {
+                if (q >= kRead) stream.one(uint32_t(q - kRead), buf);
+                if (q == SLOTS - 1)
+#pragma unroll
+                    for (uint32_t i = SLOTS - kRead; i < C::COPIES; ++i) stream.one(i, buf);  // fewer products than copies
             }
-            p[q % (LAG + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, wf[P & 1][e & 1]),
-                                                                               __builtin_bit_cast(i32x8, xf[j]), f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-            if (P < NP - 1) {
-                if (e < 4) read_w(buf, 2 * (P + 1) + (e >> 1), wf[(P + 1) & 1][e >> 1], e & 1);
-            } else if constexpr (!LAST) {
-                if (e & 1) {
-                    read_x(buf ^ 1u, j);
-                    read_xs(buf ^ 1u, j);
-                } else if (e < 4) {
-                    read_w(buf ^ 1u, j, wf[0][j], 0);
-                    read_w(buf ^ 1u, j, wf[0][j], 1);
-                }
-                if constexpr (AHEAD) {
-                    copies.one(a, lds, b + 2, buf, uint32_t(e));
-                    if (e == 1) copies.one(a, lds, b + 2, buf, C::CW + C::CX);
-                    if (e == 3) copies.one(a, lds, b + 2, buf, C::CW + C::CX + 1);
-                }
-            }
-            if (q == LAG)
-#pragma unroll
-                for (int h = 0; h < G; ++h)
-#pragma unroll
-                    for (int jj = 0; jj < WM; ++jj) s[h][jj] = sn[h][jj];
-            const int k = (q + SLOTS - LAG) % SLOTS, ki = 2 * (k / PAIR) + (k % PAIR & 1), kj = k % PAIR >> 1;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                acc[ki][kj][i] = __builtin_fmaf(p[k % (LAG + 1)][i], s[ki / (WN / G)][kj], acc[ki][kj][i]);
+            if (q == LAG) set_scales();
+            add((q + SLOTS - LAG) % SLOTS);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (!LAST) {
-            read_scales(buf ^ 1u);
-            if constexpr (!AHEAD)
-#pragma unroll
-                for (int j = 0; j < WM; ++j) only_to(xf[j], (b + 1) * kFpBlock + g * 16, a.K);
-        }
     };
-    constexpr std::true_type yes{};
-    constexpr std::false_type no{};
-    uint32_t b = b0, buf = 0;
-    for (; b + 2 < b1; ++b, buf ^= 1u) step(yes, no, b, buf);
-    if (b + 1 < b1) {
-        step(no, no, b, buf);
-        ++b;
-        buf ^= 1u;
-    }
-    step(no, yes, b, buf);
+    // A workgroup goes on to its next tile by itself, so that its first copies are under way while this one's outputs are
+    // stored, and those while the next one is computed.
+    struct Part {
+        Place at;
+        uint32_t b0, b1;  // blocks
+    };
+    auto part_of = [&](uint32_t id) {
+        const Gemm& a = arguments();
+        Part d;
+        d.at = place_of(a, id);
+        d.b0 = uint32_t(uint64_t(a.blocks) * d.at.split / a.splits);
+        d.b1 = uint32_t(uint64_t(a.blocks) * (d.at.split + 1) / a.splits);
+        return d;
+    };
+    auto first_copies = [&](const Part& d) {
+        const Gemm& a = arguments();
+        const Copies<C> copies(a, d.at, wave, lane);
+        copies.block(a, lds, d.b0, 0);
+        if (d.b0 + 1 < d.b1) copies.block(a, lds, d.b0 + 1, 1);
+    };
+    const uint32_t parts = arguments().mtiles * arguments().ntiles * arguments().splits;
+    Part d = part_of(blockIdx.x);
+    first_copies(d);
+    constexpr int kStores = 0;
+    for (uint32_t id = blockIdx.x; id < parts; id += gridDim.x) {
+        wsat = scale_at(d.at.n);
 #pragma unroll
-    for (int k = SLOTS - LAG; k < SLOTS; ++k) {
-        const int ki = 2 * (k / PAIR) + (k % PAIR & 1), kj = k % PAIR >> 1;
+        for (int i = 0; i < WN; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[ki][kj][i] = __builtin_fmaf(p[k % (LAG + 1)][i], s[ki / (WN / G)][kj], acc[ki][kj][i]);
+            for (int j = 0; j < WM; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i <= LAG; ++i) p[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+            for (int j = 0; j < WM; ++j) s[h][j] = 0.0f;
+        // the first block's copies have arrived; the second's and the stores of the tile before are behind them
+        if (d.b0 + 1 < d.b1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::COPIES + kStores) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < WM + G; ++j) read_scale(0, j);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) read_x(0, j);
+#pragma unroll
+        for (int i = 0; i < H - 1; ++i) read_w(0, i);
+        Stream<C> stream(arguments(), d.at, wave, lane, lds, d.b0 + 2);
+        uint32_t b = d.b0, buf = 0;
+        for (; b + 2 < d.b1; ++b, buf ^= 1u) step(std::true_type{}, stream, buf);
+        for (; b < d.b1; ++b, buf ^= 1u) step(std::false_type{}, stream, buf);
+#pragma unroll
+        for (int q = SLOTS - LAG; q < SLOTS; ++q) add(q);
+        const Place done = d.at;
+        if (id + gridDim.x < parts) {
+            d = part_of(id + gridDim.x);
+            first_copies(d);
+        }
+        put_tile<Y, C>(arguments(), done, wave, lane, acc);
     }
-    put_tile<Y, C>(a, at, wave, lane, acc);
 }
 
 // Adds up the parts of a tile in order; a thread has 4 outputs, those of one lane above.
@@ -642,22 +730,24 @@ int check_weights(const arc_fp8_weights* w, const arc_fp8_rows* x)
 uint32_t bytes_of(int dtype) { return dtype == ARC_F32 ? 4 : dtype == ARC_F16 || dtype == ARC_BF16 ? 2 : 0; }
 
 // Which kernel takes a product, and its tiles.
-enum class Form { few, rows32, rows64, rows128, rows256 };
+enum class Form { few, rows32, rows64, rows128, deep128, deep256 };
 struct Plan {
     Form form;
     uint32_t mtiles, ntiles, splits;
     size_t bytes;  // of workspace
 };
-Plan plan_of(uint32_t N, uint32_t blocks, uint32_t M, bool gated, bool fast)
+Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
 {
     auto tiles = [](uint32_t n, uint32_t each) { return (n + each - 1) / each; };
+    const uint32_t blocks = tiles(K, kFpBlock);
+    const bool deep = fast && K % kFpBlock == 0;
     Plan p{Form::few, 0, 0, 1, 256};
     if (M <= 16) return p;
     uint32_t bm, bn;
     if (M <= 32) p.form = Form::rows32, bm = 32, bn = 128;
     else if (M <= 64) p.form = Form::rows64, bm = 64, bn = 128;
-    else p.form = Form::rows128, bm = 128, bn = 128;
-    if (fast && M > 64 && uint64_t(tiles(M, 256)) * tiles(N, gated ? 128 : 256) >= 192) p.form = Form::rows256, bm = bn = 256;
+    else if (deep && uint64_t(tiles(M, 256)) * tiles(N, gated ? 128 : 256) >= 192) p.form = Form::deep256, bm = bn = 256;
+    else p.form = deep ? Form::deep128 : Form::rows128, bm = 128, bn = 128;
     p.mtiles = tiles(M, bm);
     p.ntiles = tiles(N, gated ? bn / 2 : bn);
     const uint64_t all = uint64_t(p.mtiles) * p.ntiles;
@@ -669,8 +759,9 @@ Plan plan_of(uint32_t N, uint32_t blocks, uint32_t M, bool gated, bool fast)
 template <typename Y, typename C>
 hipError_t launch_tile(const Gemm& a, hipStream_t st)
 {
-    if constexpr (C::DEEP) hipLaunchKernelGGL((k_fp8_deep<Y, C>), dim3(a.mtiles * a.ntiles * a.splits), dim3(C::NW * 64), 0, st, a);
-    else hipLaunchKernelGGL((k_fp8_tile<Y, C>), dim3(a.mtiles * a.ntiles * a.splits), dim3(C::NW * 64), 0, st, a);
+    const uint32_t parts = a.mtiles * a.ntiles * a.splits;
+    if constexpr (C::DEEP) hipLaunchKernelGGL((k_fp8_deep<Y, C>), dim3(parts < C::WGS ? parts : C::WGS), dim3(C::NW * 64), 0, st, a);
+    else hipLaunchKernelGGL((k_fp8_tile<Y, C>), dim3(parts), dim3(C::NW * 64), 0, st, a);
     if (a.splits > 1) {
         if (hipError_t e = hipGetLastError()) return e;
         hipLaunchKernelGGL((k_fp8_join<Y, C>), dim3(a.mtiles * a.ntiles * (C::BM * C::OUT / 1024)), dim3(256), 0, st, a);
@@ -682,10 +773,11 @@ hipError_t launch_form(const Gemm& a, Form form, hipStream_t st)
 {
     constexpr bool FAST = sizeof(Y) == 2;
     if (form == Form::few) hipLaunchKernelGGL((k_fp8_few<Y, GATED>), dim3((a.N + 15) / 16, (a.M + 15) / 16), dim3(64 * kFewWaves8), 0, st, a);
-    else if (form == Form::rows32) return launch_tile<Y, TileShape<GATED, FAST, 2, 2, 1, 4, 3>>(a, st);
-    else if (form == Form::rows64) return launch_tile<Y, TileShape<GATED, FAST, 4, 2, 1, 4, 3>>(a, st);
-    else if (form == Form::rows128) return launch_tile<Y, TileShape<GATED, FAST, 4, 4, 2, 2, 2>>(a, st);
-    else if constexpr (FAST) return launch_tile<Y, TileShape<GATED, FAST, 4, 8, 4, 2, 2>>(a, st);
+    else if (form == Form::rows32) return launch_tile<Y, TileShape<GATED, FAST, false, 2, 2, 1, 4, 3>>(a, st);
+    else if (form == Form::rows64) return launch_tile<Y, TileShape<GATED, FAST, false, 4, 2, 1, 4, 3>>(a, st);
+    else if (form == Form::rows128) return launch_tile<Y, TileShape<GATED, FAST, false, 4, 4, 2, 2, 2>>(a, st);
+    else if constexpr (FAST) return form == Form::deep128 ? launch_tile<Y, TileShape<GATED, FAST, true, 4, 4, 2, 2, 2>>(a, st)
+                                                          : launch_tile<Y, TileShape<GATED, FAST, true, 4, 8, 4, 2, 2>>(a, st);
     return hipGetLastError();
 }
 template <typename Y>
@@ -739,7 +831,7 @@ int product(const arc_fp8_weights* w, const arc_fp8_weights* up, bool gated, con
     a.ldy = ldy;
     a.ldr = ldr;
     a.wide = aligned(y, 4 * size) && ldy % 4 == 0 && (!residual || (aligned(residual, 4 * size) && ldr % 4 == 0));
-    const Plan p = plan_of(N, a.blocks, a.M, gated, size == 2);
+    const Plan p = plan_of(N, a.K, a.M, gated, size == 2);
     if (uint64_t(p.mtiles) * p.ntiles * p.splits >= (1u << 22))
         return set_error(ARC_ERR_UNSUPPORTED, "%u rows by %u outputs: more tiles than one call takes", a.M, N);
     a.part = static_cast<float*>(workspace);
@@ -781,8 +873,7 @@ int arc_fp8_quantize(int x_dtype, const void* x, uint32_t ldx, const arc_fp8_row
 size_t arc_fp8_gemm_workspace_bytes(uint32_t N, uint32_t K, uint32_t M, int gated)
 {
     if (N == 0 || N > kMaxRows || M > kMaxRows || K == 0 || K % 16 || K > kMaxLd) return 0;
-    const uint32_t blocks = (K + kFpBlock - 1) / kFpBlock;
-    const size_t fast = plan_of(N, blocks, M, gated != 0, true).bytes, wide = plan_of(N, blocks, M, gated != 0, false).bytes;
+    const size_t fast = plan_of(N, K, M, gated != 0, true).bytes, wide = plan_of(N, K, M, gated != 0, false).bytes;
     return fast > wide ? fast : wide;
 }
 
