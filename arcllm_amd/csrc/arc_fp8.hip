@@ -7,8 +7,6 @@
 // multiply-adds in fp32.
 #include "arc_paged.hpp"
 
-#include <type_traits>
-
 namespace arc {
 namespace {
 
@@ -239,6 +237,7 @@ struct TileShape {
     static constexpr uint32_t BM = 16 * WM * GM, BN = 16 * WN * GN, OUT = BN / G;  // outputs of a row
     static constexpr uint32_t CW = BN / 8 / NW, CX = BM / 8 / NW, COPIES = CW + CX + 2;  // a wave's, of a block
     static constexpr uint32_t XS = BM < 64 ? 64 : BM;
+    static constexpr uint32_t kFirst = COPIES / 2;  // see Stream
     static constexpr uint32_t WGS = NW == 8 ? 256 : 512;  // that fill the card
     static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0 && NW % 2 == 0);
     struct Lds {
@@ -270,11 +269,31 @@ __device__ __forceinline__ void copy4(uint32_t lds, const void* base, uint32_t o
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
+// The same where `lanes` is all ones, nothing where it is 0: no branch, which would end a basic block.  All lanes of a wave
+// are active in these kernels.
+__device__ __forceinline__ void copy16_if(uint64_t lanes, uint32_t lds, const void* base, uint32_t off)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1" ::"s"(lds), "v"(off), "s"(base), "s"(lanes) : "memory");
+}
+__device__ __forceinline__ void copy4_if(uint64_t lanes, uint32_t lds, const void* base, uint32_t off)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1" ::"s"(lds), "v"(off), "s"(base), "s"(lanes) : "memory");
+}
+__device__ __forceinline__ void copy4_if(uint64_t lanes, uint32_t lds, const void* from)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %2\n\tglobal_load_lds_dword %1, off\n\ts_mov_b64 exec, -1" ::"s"(lds), "v"(from), "s"(lanes) : "memory");
+}
 __device__ __forceinline__ void copy4(uint32_t lds, const void* from)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory");
 }
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
+// All of a wave's lanes, or none; a scalar.
+__device__ __forceinline__ uint64_t lanes_if(bool yes)
+{
+    const uint32_t half = uniform(yes ? ~0u : 0u);
+    return uint64_t(half) << 32 | half;
+}
 __device__ __forceinline__ uint32_t lds_at(const void* p)
 {
     typedef __attribute__((address_space(3))) const void lptr;
@@ -370,6 +389,7 @@ struct Stream {
     uint32_t last[C::CW + C::CX];        // of its 8 rows, the last that there is
     const float *xs, *ws;
     uint32_t row8, chunk, xsoff, ldx, ldxs, ldw[C::G], w, x, xsat, wsat;
+    // Copies 0 .. kFirst - 1 begin with block b + 1, the others with b.
     __device__ __forceinline__ Stream(const Gemm& a, const Place& at, uint32_t wave, uint32_t lane, typename C::Lds& lds, uint32_t b)
     {
         const Copies<C> c(a, at, wave, lane);
@@ -382,7 +402,7 @@ struct Stream {
         for (int h = 0; h < C::G; ++h) ldw[h] = a.ldw[h];
 #pragma unroll
         for (uint32_t i = 0; i < C::CW + C::CX; ++i) {
-            const uint8_t* p = c.group(a, i, last[i]) + uint64_t(b) * kFpBlock;
+            const uint8_t* p = c.group(a, i, last[i]) + uint64_t(b + (i < C::kFirst)) * kFpBlock;
             asm("" : "+s"(p), "+s"(last[i]));  // kept, not computed again
             from[i] = p;
         }
@@ -393,19 +413,19 @@ struct Stream {
         xsat = lds_at(&lds.xs[0][64 * (c.wave % (C::XS / 64))]);
         wsat = lds_at(&lds.ws[0][0]);
     }
-    __device__ __forceinline__ void one(uint32_t i, uint32_t buf)
+    __device__ __forceinline__ void one(uint64_t lanes, uint32_t i, uint32_t buf)
     {
         if (i < C::CW + C::CX) {
             const bool is_w = i < C::CW;
             const uint32_t ld = is_w ? ldw[C::GATED ? i % 2 : 0] : ldx;  // NW = WN: a half's rows are one copy of each wave
             const uint32_t to = is_w ? w + buf * C::BN * kFpBlock + i * C::NW * 1024 : x + buf * C::BM * kFpBlock + (i - C::CW) * C::NW * 1024;
-            copy16(to, from[i], __umul24(min(row8, last[i]), ld) + chunk);
+            copy16_if(lanes, to, from[i], __umul24(min(row8, last[i]), ld) + chunk);
             from[i] += kFpBlock;
         } else if (i == C::CW + C::CX) {
-            copy4(xsat + buf * C::XS * 4, xs, xsoff);
+            copy4_if(lanes, xsat + buf * C::XS * 4, xs, xsoff);
             xs += ldxs;
         } else {
-            copy4(wsat + buf * 256, ws);
+            copy4_if(lanes, wsat + buf * 256, ws);
             ++ws;
         }
     }
@@ -423,23 +443,39 @@ __device__ __forceinline__ void finish(const Gemm& a, const Place& at, uint32_t 
     store_out<Y>(a, m, n, v);
 }
 
-// The tile's outputs, or its sums for k_fp8_join.
+// The tile's outputs, or its sums for k_fp8_join.  Whether it took WM * WN / G stores: a whole tile's outputs.
 template <typename Y, typename C>
-__device__ __forceinline__ void put_tile(const Gemm& a, const Place& at, uint32_t wave, uint32_t lane, const f32x4 (&acc)[C::WN][C::WM])
+__device__ __forceinline__ bool put_tile(const Gemm& a, const Place& at, uint32_t wave, uint32_t lane, const f32x4 (&acc)[C::WN][C::WM])
 {
     constexpr int WM = C::WM, WN = C::WN, G = C::G;
-    if (a.splits == 1) {
+    if (a.splits > 1) {
+        f32x4* part = reinterpret_cast<f32x4*>(a.part) + ((uint64_t(at.m) * a.ntiles + at.n) * a.splits + at.split) * (C::BM * C::BN / 4);
 #pragma unroll
-        for (int i = 0; i < WN / G; ++i)
+        for (int i = 0; i < WN; ++i)
 #pragma unroll
-            for (int j = 0; j < WM; ++j) finish<Y, C>(a, at, wave, i, j, lane, acc[i][j], acc[i + WN / G * (G - 1)][j]);
-        return;
+            for (int j = 0; j < WM; ++j) part[((wave * WN + i) * WM + j) * 64 + lane] = acc[i][j];
+        return false;
     }
-    f32x4* part = reinterpret_cast<f32x4*>(a.part) + ((uint64_t(at.m) * a.ntiles + at.n) * a.splits + at.split) * (C::BM * C::BN / 4);
+    if (a.wide && !a.res && (at.m + 1) * C::BM <= a.M && (at.n + 1) * C::OUT <= a.N) {
+        const uint32_t m = at.m * C::BM + wave / C::GN * (WM * 16) + (lane & 15u), n = at.n * C::OUT + wave % C::GN * (C::OUT / C::GN) + 4 * (lane >> 4);
 #pragma unroll
-    for (int i = 0; i < WN; ++i)
+        for (int j = 0; j < WM; ++j) {
+            Y* row = static_cast<Y*>(a.y) + uint64_t(m + 16 * j) * a.ldy + n;
 #pragma unroll
-        for (int j = 0; j < WM; ++j) part[((wave * WN + i) * WM + j) * 64 + lane] = acc[i][j];
+            for (int i = 0; i < WN / G; ++i) {
+                vec4<Y> o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = static_cast<Y>(C::GATED ? silu<Y>(acc[i][j][e]) * acc[i + WN / G * (G - 1)][j][e] : acc[i][j][e]);
+                *reinterpret_cast<vec4<Y>*>(row + 16 * i) = o;
+            }
+        }
+        return true;
+    }
+#pragma unroll
+    for (int i = 0; i < WN / G; ++i)
+#pragma unroll
+        for (int j = 0; j < WM; ++j) finish<Y, C>(a, at, wave, i, j, lane, acc[i][j], acc[i + WN / G * (G - 1)][j]);
+    return false;
 }
 
 template <typename Y, typename C>
@@ -589,9 +625,11 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
         for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(p[q % (LAG + 1)][e], s[i / (WN / G)][j], acc[i][j][e]);
     };
 
-    // A block from buffer buf.  AHEAD: the next block but one is copied.  One basic block, else the compiler takes the
-    // multiply-adds out of their places; so what there is no next block for is read all the same, from LDS as it is.
-    auto step = [&](auto ahead, Stream<C>& stream, uint32_t buf) {
+    // A block from buffer buf.  Where there is a next one (`next`), the second half of its copies; where there is one behind
+    // that, the first half of its.  Spread out like that they do not hold up the waves, as 64 copies at once do.  One
+    // basic block, else the compiler takes the multiply-adds out of their places; so what there is no next block for is read all the
+    // same, from LDS as it is.
+    auto step = [&](Stream<C>& stream, uint64_t next, uint64_t behind, uint32_t buf) {
         constexpr int kRead = 6 * H - 2;  // from here on the block's LDS is read no more
 #pragma unroll
         for (int q = 0; q < SLOTS; ++q) {
@@ -604,12 +642,9 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
             if (q == kRead || q == kRead + 1) read_x(buf ^ 1u, q - kRead);
             if (q > 6 * H && q % 2 && q < SLOTS - 1) read_w(buf ^ 1u, (q - 6 * H) / 2);
             if (q >= SLOTS - WM - G) read_scale(buf ^ 1u, q - (SLOTS - WM - G));
-            if constexpr (decltype(ahead)::value) {
-                if (q >= kRead) stream.one(uint32_t(q - kRead), buf);
-                if (q == SLOTS - 1)
-#pragma unroll
-                    for (uint32_t i = SLOTS - kRead; i < C::COPIES; ++i) stream.one(i, buf);  // fewer products than copies
-            }
+            constexpr int kEvery = SLOTS >= 32 ? 2 : 1;
+            if (q % kEvery == 0 && q / kEvery < int(C::COPIES - C::kFirst)) stream.one(next, C::kFirst + q / kEvery, buf ^ 1u);
+            if (q >= kRead && (q - kRead) % kEvery == 0 && (q - kRead) / kEvery < int(C::kFirst)) stream.one(behind, (q - kRead) / kEvery, buf);
             if (q == LAG) set_scales();
             add((q + SLOTS - LAG) % SLOTS);
             __builtin_amdgcn_sched_barrier(0);
@@ -633,12 +668,14 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
         const Gemm& a = arguments();
         const Copies<C> copies(a, d.at, wave, lane);
         copies.block(a, lds, d.b0, 0);
-        if (d.b0 + 1 < d.b1) copies.block(a, lds, d.b0 + 1, 1);
+        if (d.b0 + 1 < d.b1)
+#pragma unroll
+            for (uint32_t i = 0; i < C::kFirst; ++i) copies.one(a, lds, d.b0 + 1, 1, i);
     };
     const uint32_t parts = arguments().mtiles * arguments().ntiles * arguments().splits;
     Part d = part_of(blockIdx.x);
     first_copies(d);
-    constexpr int kStores = 0;
+    bool stored = false;  // WM * WN / G stores, no more and no less
     for (uint32_t id = blockIdx.x; id < parts; id += gridDim.x) {
         wsat = scale_at(d.at.n);
 #pragma unroll
@@ -651,9 +688,10 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
         for (int h = 0; h < G; ++h)
 #pragma unroll
             for (int j = 0; j < WM; ++j) s[h][j] = 0.0f;
-        // the first block's copies have arrived; the second's and the stores of the tile before are behind them
-        if (d.b0 + 1 < d.b1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::COPIES + kStores) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // the first block's copies have arrived; what of the second's has begun and the stores of the tile before are behind them
+        if (d.b0 + 1 == d.b1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else if (stored) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::kFirst + WM * WN / G) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::kFirst) : "memory");
         asm volatile("s_barrier" ::: "memory");
 #pragma unroll
         for (int j = 0; j < WM + G; ++j) read_scale(0, j);
@@ -661,10 +699,9 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
         for (int j = 0; j < 2; ++j) read_x(0, j);
 #pragma unroll
         for (int i = 0; i < H - 1; ++i) read_w(0, i);
-        Stream<C> stream(arguments(), d.at, wave, lane, lds, d.b0 + 2);
-        uint32_t b = d.b0, buf = 0;
-        for (; b + 2 < d.b1; ++b, buf ^= 1u) step(std::true_type{}, stream, buf);
-        for (; b < d.b1; ++b, buf ^= 1u) step(std::false_type{}, stream, buf);
+        Stream<C> stream(arguments(), d.at, wave, lane, lds, d.b0 + 1);
+        uint32_t buf = 0;
+        for (uint32_t b = d.b0; b < d.b1; ++b, buf ^= 1u) step(stream, lanes_if(b + 1 < d.b1), lanes_if(b + 2 < d.b1), buf);
 #pragma unroll
         for (int q = SLOTS - LAG; q < SLOTS; ++q) add(q);
         const Place done = d.at;
@@ -672,7 +709,7 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
             d = part_of(id + gridDim.x);
             first_copies(d);
         }
-        put_tile<Y, C>(arguments(), done, wave, lane, acc);
+        stored = put_tile<Y, C>(arguments(), done, wave, lane, acc);
     }
 }
 
