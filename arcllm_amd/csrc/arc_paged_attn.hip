@@ -20,6 +20,7 @@
 // tile runs over the same units as a causal one, and only those that reach behind the context look at masks.
 #include "arc_paged.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace arc {
@@ -1110,6 +1111,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
             for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
         Running run;
 
+        // trees are rarely a multiple of a tile's rows: waves without any only copy
+        const bool rows_here = wave * 32 < s.x.rows;
+
         // the page of the lane's position in unit u
         auto page_of = [&](uint32_t u) {
             const int32_t kp = int32_t(unit_start(s.x, u, kManyKeys) + lane);
@@ -1147,67 +1151,69 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
                     __syncthreads();
                 }
 
-                f32x16 sc[2];
+                if (!TREE || rows_here) {
+                    f32x16 sc[2];
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
+                    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[kt][i] = 0.0f;
-                // K's operands 4 steps ahead of their products: LDS answers in some 200 cycles
+                        for (int i = 0; i < 16; ++i) sc[kt][i] = 0.0f;
+                    // K's operands 4 steps ahead of their products: LDS answers in some 200 cycles
 #pragma unroll
-                for (int st = 0; st < D / 16; ++st)
+                    for (int st = 0; st < D / 16; ++st)
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) {
-                        const uint32_t rr = 32u * kt + l32;
-                        const vec8<T> kf =
-                            *reinterpret_cast<const vec8<T>*>(&ks[cur][rr * D + (((2u * st + h2) ^ k_swizzle<D>(rr)) << 3)]);
-                        sc[kt] = mfma<T>(kf, q[st], sc[kt]);
+                        for (int kt = 0; kt < 2; ++kt) {
+                            const uint32_t rr = 32u * kt + l32;
+                            const vec8<T> kf =
+                                *reinterpret_cast<const vec8<T>*>(&ks[cur][rr * D + (((2u * st + h2) ^ k_swizzle<D>(rr)) << 3)]);
+                            sc[kt] = mfma<T>(kf, q[st], sc[kt]);
+                        }
+                    __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+#pragma unroll
+                    for (int i = 0; i < D / 8 - kAhead; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
                     }
-                __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
-#pragma unroll
-                for (int i = 0; i < D / 8 - kAhead; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                // V's operands a step ahead of theirs
-                vec8<T> vt[2][D / 32];
-#pragma unroll
-                for (int t = 0; t < D / 32; ++t) vt[0][t] = load_vt<T, D>(vs[cur], 0, t);
-                if (!whole) {
-                    hide(sc[0], uint32_t(valid) & sight.bits(k0, p.window, p.sinks));
-                    hide(sc[1], uint32_t(valid >> 32) & sight.bits(k0 + 32, p.window, p.sinks));
-                }
-                float mx = sc[0][0];
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
-                rescale<T>(xor_max<32>(mx), p.scale, run, o);
-                float k = p.scale, c;
-                exponents(run, k, c, sc[0], sc[1]);
-                float sum = 0.0f;  // as in the few-rows kernel
-                auto weights = [&](int st) {  // the 16 positions of step st: their weights, rounded; sum adds the unrounded
-                    f32x16& x = sc[st >> 1];
-#pragma unroll
-                    for (int i = 8 * (st & 1); i < 8 * (st & 1) + 8; ++i) {
-                        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], k, c));
-                        sum += x[i];
-                    }
-                    return narrow<T>(x, 8 * (st & 1));
-                };
-                vec8<T> w = weights(0);
-#pragma unroll
-                for (int st = 0; st < 4; ++st) {
+                    __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
                     __builtin_amdgcn_sched_barrier(0);
-                    if (st < 3)
+                    // V's operands a step ahead of theirs
+                    vec8<T> vt[2][D / 32];
 #pragma unroll
-                        for (int t = 0; t < D / 32; ++t) vt[(st + 1) & 1][t] = load_vt<T, D>(vs[cur], st + 1, t);
+                    for (int t = 0; t < D / 32; ++t) vt[0][t] = load_vt<T, D>(vs[cur], 0, t);
+                    if (!whole) {
+                        hide(sc[0], uint32_t(valid) & sight.bits(k0, p.window, p.sinks));
+                        hide(sc[1], uint32_t(valid >> 32) & sight.bits(k0 + 32, p.window, p.sinks));
+                    }
+                    float mx = sc[0][0];
 #pragma unroll
-                    for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(vt[st & 1][t], w, o[t]);
-                    if (st < 3) w = weights(st + 1);
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
+                    rescale<T>(xor_max<32>(mx), p.scale, run, o);
+                    float k = p.scale, c;
+                    exponents(run, k, c, sc[0], sc[1]);
+                    float sum = 0.0f;  // as in the few-rows kernel
+                    auto weights = [&](int st) {  // the 16 positions of step st: their weights, rounded; sum adds the unrounded
+                        f32x16& x = sc[st >> 1];
+#pragma unroll
+                        for (int i = 8 * (st & 1); i < 8 * (st & 1) + 8; ++i) {
+                            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], k, c));
+                            sum += x[i];
+                        }
+                        return narrow<T>(x, 8 * (st & 1));
+                    };
+                    vec8<T> w = weights(0);
+#pragma unroll
+                    for (int st = 0; st < 4; ++st) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (st < 3)
+#pragma unroll
+                            for (int t = 0; t < D / 32; ++t) vt[(st + 1) & 1][t] = load_vt<T, D>(vs[cur], st + 1, t);
+#pragma unroll
+                        for (int t = 0; t < D / 32; ++t) o[t] = mfma<T>(vt[st & 1][t], w, o[t]);
+                        if (st < 3) w = weights(st + 1);
+                    }
+                    run.l += sum;
                 }
-                run.l += sum;
                 cur ^= 1;
                 page = npage;
                 npage = far;
@@ -1492,6 +1498,15 @@ int attention(const arc_kv_pages* pages, const arc_paged_batch* batch, const arc
     a.few_rows = !many ? ~0u : few ? kFewRows : 0u;
     a.few_wgs = few ? kFewWgs : 0;
     a.many_wgs = many ? many_wgs(pages->head_dim) : 0;
+    if (tree && many) {
+        // one launch where the rows say that trees are the rule: the many-rows kernel has the time for few rows too, as its
+        // waves without rows only copy
+        if (batch->tokens * uint64_t(hpk) >= kFewRows / 2 * uint64_t(batch->requests)) a.few_rows = a.few_wgs = 0;
+        // no more workgroups than there can be units
+        const uint64_t tiles = uint64_t(batch->tokens) * hpk / (32u * many_waves(pages->head_dim)) + batch->requests;
+        const uint64_t units = (uint64_t(batch->max_pages) * pages->page_size + kManyKeys - 1) / kManyKeys;
+        a.many_wgs = uint32_t(std::min<uint64_t>(a.many_wgs, tiles * pages->kv_heads * units));
+    }
     const hipError_t e = tree ? launch_type<true>(a, pages, st) : launch_type<false>(a, pages, st);
     return check_hip(e, tree ? "tree attention" : "paged attention");
 }
