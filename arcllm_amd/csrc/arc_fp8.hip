@@ -27,6 +27,26 @@ __device__ __forceinline__ float scale_of(uint32_t most)
     return fmaxf(__builtin_bit_cast(float, most) / kE4m3Max, 0x1p-126f);
 }
 
+// x / s rounded to nearest for a block's values, |x| <= 448 s: q = x r with r = 1 / s, corrected by r times the remainder
+// x - q s, which a fused multiply-add gives exactly (P. Markstein, IBM J. Res. Dev. 34, 1990).  The compiler's division takes 11
+// instructions a value, this one 5; the remainder of tiny values would be lost below fp32's range, so they are scaled up.
+struct Divider {
+    float s, r, up;
+    __device__ __forceinline__ explicit Divider(float scale)
+    {
+        up = scale < 0x1p-60f ? 0x1p64f : 1.0f;
+        s = scale * up;
+        r = __builtin_amdgcn_rcpf(s);
+        r = __builtin_fmaf(__builtin_fmaf(-s, r, 1.0f), r, r);
+    }
+    __device__ __forceinline__ float operator()(float x) const
+    {
+        x *= up;
+        const float q = x * r;
+        return __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-q, s, x), r, q), x);  // of zeros too
+    }
+};
+
 // The largest of 16 lanes (a DPP row), as bits of magnitudes.
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_u(uint32_t v)
@@ -55,33 +75,42 @@ constexpr uint32_t kQuantRows = 32;
 template <typename X>
 __global__ __launch_bounds__(256) void k_fp8_quantize(Quantize a)
 {
+    constexpr uint32_t kAhead = sizeof(X) == 4 ? 4 : 8;
     __shared__ float scales[4][kQuantRows];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t col = blockIdx.y * 512 + lane * 8, row0 = blockIdx.x * kQuantRows;
     const bool in = col < a.cols;
-    for (uint32_t i = wave; i < kQuantRows && row0 + i < a.rows; i += 4) {
-        float v[8];
+    const X* p = static_cast<const X*>(a.x) + min(col, a.cols - 8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        if (in) {
-            const X* p = static_cast<const X*>(a.x) + uint64_t(row0 + i) * a.ldx + col;
-            const vec8<X> r = *reinterpret_cast<const vec8<X>*>(p);
+    for (uint32_t at = 0; at < kQuantRows; at += 4 * kAhead) {
+        vec8<X> r[kAhead];  // so many rows on their way at once
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(r[j]);
-        }
-        uint32_t most = 0;
+        for (uint32_t j = 0; j < kAhead; ++j)
+            r[j] = __builtin_nontemporal_load(reinterpret_cast<const vec8<X>*>(p + uint64_t(min(row0 + at + 4 * j + wave, a.rows - 1)) * a.ldx));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
-        const float s = scale_of(row_max(most));
-        if ((lane & 15u) == 0) scales[lane >> 4][i] = s;
-        if (in) {
-            uint32_t w[2] = {0, 0};
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            const uint32_t i = at + 4 * j + wave;
+            float v[8];
+            uint32_t most = 0;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                w[j] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j] / s, v[4 * j + 1] / s, 0, false));
-                w[j] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2] / s, v[4 * j + 3] / s, int(w[j]), true));
+            for (int e = 0; e < 8; ++e) {
+                v[e] = in ? static_cast<float>(r[j][e]) : 0.0f;
+                most = max(most, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
             }
-            *reinterpret_cast<uint2*>(a.q + uint64_t(row0 + i) * a.ldq + col) = make_uint2(w[0], w[1]);
+            const float s = scale_of(row_max(most));
+            if ((lane & 15u) == 0) scales[lane >> 4][i] = s;
+            if (in && row0 + i < a.rows) {
+                const Divider by(s);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = by(v[e]);
+                uint32_t w[2] = {0, 0};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    w[e] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * e], v[4 * e + 1], 0, false));
+                    w[e] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * e + 2], v[4 * e + 3], int(w[e]), true));
+                }
+                *reinterpret_cast<uint2*>(a.q + uint64_t(row0 + i) * a.ldq + col) = make_uint2(w[0], w[1]);
+            }
         }
     }
     __syncthreads();

@@ -92,18 +92,34 @@ struct Argmax {
     uint64_t ldl;
     uint32_t requests, tokens, vocab, splits;
 };
-// A workgroup to a part of a row; rows behind the last request are not read.
+// A workgroup to a part of a row; rows behind the last request are not read.  Bound by reading the logits: 16 bytes a lane
+// from the first 16-byte border on, four at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void k_tree_argmax(Argmax a)
 {
+    constexpr uint32_t V = 16 / sizeof(T), kAhead = 4;
+    typedef T wide __attribute__((ext_vector_type(16 / sizeof(T))));
     __shared__ Best waves[4];
     const uint32_t row = blockIdx.x / a.splits, split = blockIdx.x % a.splits, tid = threadIdx.x;
     if (row >= a.starts[a.requests]) return;
-    const uint32_t each = ((a.vocab + a.splits - 1) / a.splits + 7) & ~7u;
-    const uint32_t c0 = min(split * each, a.vocab), c1 = min(c0 + each, a.vocab);
     const T* p = static_cast<const T*>(a.logits) + uint64_t(row) * a.ldl;
+    // the row's values before its first border, its wide ones, those behind: the parts share the wide ones
+    const uint32_t head = min(uint32_t(-reinterpret_cast<uintptr_t>(p) & 15u) / uint32_t(sizeof(T)), a.vocab);
+    const uint32_t n = (a.vocab - head) / V, each = (n + a.splits - 1) / a.splits;
+    const uint32_t v0 = min(split * each, n), v1 = min(v0 + each, n);
+    const wide* w = reinterpret_cast<const wide*>(p + head);
     Best best{-INFINITY, kNoToken};
-    for (uint32_t c = c0 + tid; c < c1; c += 256) take(best, p[c], c);
+    if (split == 0 && tid < head) take(best, p[tid], tid);
+    for (uint32_t v = v0 + tid; v < v1; v += kAhead * 256) {
+        wide x[kAhead];
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) x[i] = __builtin_nontemporal_load(w + min(v + i * 256, v1 - 1));
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (uint32_t e = 0; e < V; ++e) take(best, x[i][e], head + min(v + i * 256, v1 - 1) * V + e);
+    }
+    if (split + 1 == a.splits && tid < a.vocab - head - n * V) take(best, p[head + n * V + tid], head + n * V + tid);
     for (int d = 32; d; d >>= 1) best = better(best, Best{__shfl_xor(best.val, d), uint32_t(__shfl_xor(int(best.idx), d))});
     if ((tid & 63u) == 0) waves[tid >> 6] = best;
     __syncthreads();
@@ -207,25 +223,41 @@ __device__ __forceinline__ bool place_of(const Move& a, uint32_t b, uint32_t pos
     return page < a.num_pages;
 }
 
-// A workgroup to a request and layer: row path[i] of the walk to place i, each thread the same 16 bytes of every row, so
-// that a row is read before its place is written (path[i] >= i, in rising order).  The workgroups of one more layer
-// number return the pages.
+// A workgroup to a request and layer: row path[i] of the walk to place i.  A few rows of some KB: a chain of round trips to
+// memory (rows, walk, pages, values), so each is made for all rows at once.  Each thread has the same 16 bytes of
+// every row and reads 8 rows before it writes any: a row is then read before its place is written, as path[i] >= i and both rise.
+// The workgroup of one more layer number returns the pages.
 __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
 {
+    constexpr uint32_t kBatch = 8;
     const uint32_t tid = threadIdx.x, layer = blockIdx.y;
     if (layer < a.layers) {
+        __shared__ uint64_t from[kMaxNodes], to[kMaxNodes];  // byte offsets; kNowhere: the row stays
+        constexpr uint64_t kNowhere = ~0ull;
         const uint32_t b = blockIdx.x;
         if (b >= a.requests) return;
         const Rows r = rows_of(a.starts, a.tokens, b);
-        if (r.n == 0 || r.n > 32 * a.words || a.held[b] < r.all) return;
-        const uint32_t base = a.held[b] - r.all, kept = a.counts[b], width = a.row_bytes / 16;
+        const uint32_t held = a.held[b], kept = a.counts[b];
+        if (r.n == 0 || r.n > 32 * a.words || held < r.all || kept < 2) return;
+        const uint32_t base = held - r.all, width = a.row_bytes / 16;
+        for (uint32_t i = tid; i < kept; i += 256) {
+            const uint32_t node = a.path[r.first + i];
+            uint64_t to_at, from_at;
+            const bool moves = node != i && place_of(a, b, base + i, to_at) && place_of(a, b, base + node, from_at);
+            from[i] = moves ? from_at : kNowhere;
+            to[i] = to_at;
+        }
+        __syncthreads();
         for (uint32_t c = tid; c < 2 * width; c += 256) {
             uint8_t* pool = static_cast<uint8_t*>(c < width ? layers.k[layer] : layers.v[layer]) + (c < width ? c : c - width) * 16;
-            for (uint32_t i = 1; i < kept; ++i) {
-                const uint32_t from = a.path[r.first + i];
-                uint64_t to_at, from_at;
-                if (from == i || !place_of(a, b, base + i, to_at) || !place_of(a, b, base + from, from_at)) continue;
-                *reinterpret_cast<uint4*>(pool + to_at) = *reinterpret_cast<const uint4*>(pool + from_at);
+            for (uint32_t i0 = 1; i0 < kept; i0 += kBatch) {
+                uint4 v[kBatch];
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i)
+                    if (i0 + i < kept && from[i0 + i] != kNowhere) v[i] = *reinterpret_cast<const uint4*>(pool + from[i0 + i]);
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i)
+                    if (i0 + i < kept && from[i0 + i] != kNowhere) *reinterpret_cast<uint4*>(pool + to[i0 + i]) = v[i];
             }
         }
         return;
