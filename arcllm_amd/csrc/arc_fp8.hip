@@ -7,6 +7,8 @@
 // multiply-adds in fp32.
 #include "arc_paged.hpp"
 
+#include <cmath>
+
 namespace arc {
 namespace {
 
@@ -182,9 +184,13 @@ struct Frag {
 __device__ __forceinline__ Frag load_frag(const uint8_t* row, uint32_t c, uint32_t K)
 {
     Frag f;
-    f.lo = f.hi = u32x4{0, 0, 0, 0};
-    if (c < K) f.lo = *reinterpret_cast<const u32x4*>(row + c);
-    if (c + 64 < K) f.hi = *reinterpret_cast<const u32x4*>(row + c + 64);
+    f.lo = *reinterpret_cast<const u32x4*>(row + min(c, K - 16));
+    f.hi = *reinterpret_cast<const u32x4*>(row + min(c + 64, K - 16));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f.lo[i] = c < K ? f.lo[i] : 0u;
+        f.hi[i] = c + 64 < K ? f.hi[i] : 0u;
+    }
     return f;
 }
 // 8 e4m3 values as fp16, which holds them all.
@@ -218,6 +224,7 @@ template <typename Y, bool GATED>
 __global__ __launch_bounds__(512) void k_fp8_few(Gemm a)
 {
     constexpr int G = GATED ? 2 : 1;
+    constexpr uint32_t kAhead = 4;
     __shared__ f32x4 sums[kFewWaves8][G][64];
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
     const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
@@ -227,17 +234,38 @@ __global__ __launch_bounds__(512) void k_fp8_few(Gemm a)
     f32x4 acc[G];
 #pragma unroll
     for (int h = 0; h < G; ++h) acc[h] = f32x4{0, 0, 0, 0};
-    for (uint32_t b = wave; b < a.blocks; b += kFewWaves8) {
-        const uint32_t c = b * kFpBlock + g * 16;
-        const Wide xf = widen(load_frag(x, c, a.K));
-        const float xs = a.xs[uint64_t(b) * a.ldxs + m];
+    const uint8_t* w[G];
+    const float* ws[G];
 #pragma unroll
-        for (int h = 0; h < G; ++h) {
-            const Wide wf = widen(load_frag(a.w[h] + uint64_t(n) * a.ldw[h], c, a.K));
-            const float s = xs * a.ws[h][uint64_t(n0 / kFpBlock) * a.ldws[h] + b];
-            const f32x4 p = block_sums(wf, xf);
+    for (int h = 0; h < G; ++h) {
+        w[h] = a.w[h] + uint64_t(n) * a.ldw[h];
+        ws[h] = a.ws[h] + uint64_t(n0 / kFpBlock) * a.ldws[h];
+    }
+    for (uint32_t b0 = wave; b0 < a.blocks; b0 += kAhead * kFewWaves8) {
+        Frag xf[kAhead], wf[kAhead][G];  // so many blocks on their way at once
+        float xs[kAhead], sw[kAhead][G];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[h][i] = __builtin_fmaf(p[i], s, acc[h][i]);
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t b = min(b0 + i * kFewWaves8, a.blocks - 1), c = b * kFpBlock + g * 16;
+            xf[i] = load_frag(x, c, a.K);
+            xs[i] = a.xs[uint64_t(b) * a.ldxs + m];
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                wf[i][h] = load_frag(w[h], c, a.K);
+                sw[i][h] = ws[h][b];
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            if (b0 + i * kFewWaves8 >= a.blocks) break;
+            const Wide xw = widen(xf[i]);
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                const f32x4 p = block_sums(widen(wf[i][h]), xw);
+                const float s = xs[i] * sw[i][h];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[h][e] = __builtin_fmaf(p[e], s, acc[h][e]);
+            }
         }
     }
 #pragma unroll
@@ -795,31 +823,50 @@ int check_weights(const arc_fp8_weights* w, const arc_fp8_rows* x)
 }
 uint32_t bytes_of(int dtype) { return dtype == ARC_F32 ? 4 : dtype == ARC_F16 || dtype == ARC_BF16 ? 2 : 0; }
 
-// Which kernel takes a product, and its tiles.
+// Which kernel takes a product, its tiles, and into how many parts their blocks are cut: what is expected to be quickest.
+// A block costs a workgroup `one` us where it has a compute unit to itself, `two` where two share one; the last round may be
+// short; beginning and end of a tile cost about 4 blocks; k_fp8_join 3 us and the sums' way there and back at 8 TB/s.  The
+// times are those of 28 and 148 blocks at 24 to 4096 rows, which this meets within 15 %: of 3584 x 18944 in bf16, 2048 rows,
+// tiles of 128, 185 us, of 256 in two parts 170; 1024 rows 135, and of 256 in four parts 104; of 4608 x 3584, 4096 rows, 93 and 109.
 enum class Form { few, rows32, rows64, rows128, deep128, deep256 };
 struct Plan {
     Form form;
     uint32_t mtiles, ntiles, splits;
     size_t bytes;  // of workspace
 };
+struct Shape {
+    Form form;
+    uint32_t bm, bn;
+    float one, two;  // deep256: alone on its compute unit; of few workgroups, of a full card
+};
 Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
 {
+    Plan best{Form::few, 0, 0, 1, 256};
+    if (M <= 16) return best;
     auto tiles = [](uint32_t n, uint32_t each) { return (n + each - 1) / each; };
     const uint32_t blocks = tiles(K, kFpBlock);
+    const Shape rows32{Form::rows32, 32, 128, fast ? 0.60f : 0.80f, fast ? 0.90f : 1.10f};
+    const Shape rows64{Form::rows64, 64, 128, fast ? 0.63f : 0.92f, fast ? 0.97f : 1.25f};
+    const Shape rows128{Form::rows128, 128, 128, fast ? 1.0f : 1.25f, fast ? 1.6f : 2.1f};
+    const Shape deep128{Form::deep128, 128, 128, 0.75f, 1.25f}, deep256{Form::deep256, 256, 256, 1.35f, 1.90f};
     const bool deep = fast && K % kFpBlock == 0;
-    Plan p{Form::few, 0, 0, 1, 256};
-    if (M <= 16) return p;
-    uint32_t bm, bn;
-    if (M <= 32) p.form = Form::rows32, bm = 32, bn = 128;
-    else if (M <= 64) p.form = Form::rows64, bm = 64, bn = 128;
-    else if (deep && uint64_t(tiles(M, 256)) * tiles(N, gated ? 128 : 256) >= 192) p.form = Form::deep256, bm = bn = 256;
-    else p.form = deep ? Form::deep128 : Form::rows128, bm = 128, bn = 128;
-    p.mtiles = tiles(M, bm);
-    p.ntiles = tiles(N, gated ? bn / 2 : bn);
-    const uint64_t all = uint64_t(p.mtiles) * p.ntiles;
-    while (p.splits < 32 && all * (p.splits * 2) <= 512 && blocks / (p.splits * 2) >= 4) p.splits *= 2;
-    if (p.splits > 1) p.bytes = size_t(all) * p.splits * bm * bn * sizeof(float);
-    return p;
+    const Shape of[2] = {M <= 32 ? rows32 : M <= 64 ? rows64 : deep ? deep128 : rows128, deep256};
+    float least = INFINITY;
+    for (const Shape& s : of) {
+        if (s.form == Form::deep256 && (!deep || M <= 64)) continue;
+        const uint32_t mtiles = tiles(M, s.bm), ntiles = tiles(N, gated ? s.bn / 2 : s.bn);
+        for (uint32_t splits = 1; splits <= 16 && (splits == 1 || blocks / splits >= 4); splits *= 2) {
+            const double parts = double(mtiles) * ntiles * splits, share = s.form == Form::deep256 ? 256 : 512;
+            const double full = std::floor(parts / share), rest = parts - full * share;
+            const double last = rest == 0 ? 0 : share == 256 ? s.one + (s.two - s.one) * rest / 256 : rest <= 256 ? s.one : s.two;
+            const size_t sums = splits > 1 ? size_t(parts) * s.bm * s.bn * sizeof(float) : 0;
+            const float time = float((full * s.two + last) * (tiles(blocks, splits) + 4) + (splits > 1 ? 3 + sums / 4e6 : 0));
+            if (time >= least) continue;
+            least = time;
+            best = Plan{s.form, mtiles, ntiles, splits, sums ? sums : 256};
+        }
+    }
+    return best;
 }
 
 template <typename Y, typename C>
