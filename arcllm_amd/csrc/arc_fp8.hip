@@ -825,7 +825,7 @@ uint32_t bytes_of(int dtype) { return dtype == ARC_F32 ? 4 : dtype == ARC_F16 ||
 
 // Which kernel takes a product, its tiles, and into how many parts their blocks are cut: what is expected to be quickest.
 // A block costs a workgroup `one` us where it has a compute unit to itself, `two` where two share one; the last round may be
-// short; beginning and end of a tile cost about 4 blocks; k_fp8_join 3 us and the sums' way there and back at 8 TB/s.  The
+// short; beginning and end of a tile cost about 4 blocks; k_fp8_join 3 us and the sums' way there and back at 6 TB/s.  The
 // times are those of 28 and 148 blocks at 24 to 4096 rows, which this meets within 15 %: of 3584 x 18944 in bf16, 2048 rows,
 // tiles of 128, 185 us, of 256 in two parts 170; 1024 rows 135, and of 256 in four parts 104; of 4608 x 3584, 4096 rows, 93 and 109.
 enum class Form { few, rows32, rows64, rows128, deep128, deep256 };
@@ -848,7 +848,7 @@ Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
     const Shape rows32{Form::rows32, 32, 128, fast ? 0.60f : 0.80f, fast ? 0.90f : 1.10f};
     const Shape rows64{Form::rows64, 64, 128, fast ? 0.63f : 0.92f, fast ? 0.97f : 1.25f};
     const Shape rows128{Form::rows128, 128, 128, fast ? 1.0f : 1.25f, fast ? 1.6f : 2.1f};
-    const Shape deep128{Form::deep128, 128, 128, 0.75f, 1.25f}, deep256{Form::deep256, 256, 256, 1.35f, 1.90f};
+    const Shape deep128{Form::deep128, 128, 128, 0.75f, 1.25f}, deep256{Form::deep256, 256, 256, 1.45f, 1.95f};
     const bool deep = fast && K % kFpBlock == 0;
     const Shape of[2] = {M <= 32 ? rows32 : M <= 64 ? rows64 : deep ? deep128 : rows128, deep256};
     float least = INFINITY;
@@ -860,7 +860,7 @@ Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
             const double full = std::floor(parts / share), rest = parts - full * share;
             const double last = rest == 0 ? 0 : share == 256 ? s.one + (s.two - s.one) * rest / 256 : rest <= 256 ? s.one : s.two;
             const size_t sums = splits > 1 ? size_t(parts) * s.bm * s.bn * sizeof(float) : 0;
-            const float time = float((full * s.two + last) * (tiles(blocks, splits) + 4) + (splits > 1 ? 3 + sums / 4e6 : 0));
+            const float time = float((full * s.two + last) * (tiles(blocks, splits) + 4) + (splits > 1 ? 3 + sums / 3e6 : 0));
             if (time >= least) continue;
             least = time;
             best = Plan{s.form, mtiles, ntiles, splits, sums ? sums : 256};
