@@ -345,6 +345,12 @@ __device__ __forceinline__ void copy4(uint32_t lds, const void* from)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory");
 }
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
+template <typename T>
+__device__ __forceinline__ T* uniform(T* p)
+{
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<T*>(uint64_t(uniform(uint32_t(v >> 32))) << 32 | uniform(uint32_t(v)));
+}
 // All of a wave's lanes, or none; a scalar.
 __device__ __forceinline__ uint64_t lanes_if(bool yes)
 {
@@ -446,8 +452,8 @@ struct Stream {
     uint32_t last[C::CW + C::CX];        // of its 8 rows, the last that there is
     const float *xs, *ws;
     uint32_t row8, chunk, xsoff, ldx, ldxs, ldw[C::G], w, x, xsat, wsat;
-    // Copies 0 .. kFirst - 1 begin with block b + 1, the others with b.
-    __device__ __forceinline__ Stream(const Gemm& a, const Place& at, uint32_t wave, uint32_t lane, typename C::Lds& lds, uint32_t b)
+    // Copies 0 .. kFirst - 1 begin with block `first`, the others with b.
+    __device__ __forceinline__ Stream(const Gemm& a, const Place& at, uint32_t wave, uint32_t lane, typename C::Lds& lds, uint32_t first, uint32_t b)
     {
         const Copies<C> c(a, at, wave, lane);
         row8 = c.row8;
@@ -455,11 +461,13 @@ struct Stream {
         xsoff = c.xsoff;
         ldx = a.ldx;
         ldxs = a.ldxs;
+        // which half a copy's rows are of goes by the copy, or by the wave
+        static_assert(C::NW == C::WN || 8 * C::NW % (16 * C::WN) == 0);
 #pragma unroll
-        for (int h = 0; h < C::G; ++h) ldw[h] = a.ldw[h];
+        for (int h = 0; h < C::G; ++h) ldw[h] = C::NW == C::WN ? a.ldw[h] : a.ldw[C::GATED ? c.half(0) : 0];
 #pragma unroll
         for (uint32_t i = 0; i < C::CW + C::CX; ++i) {
-            const uint8_t* p = c.group(a, i, last[i]) + uint64_t(b + (i < C::kFirst)) * kFpBlock;
+            const uint8_t* p = c.group(a, i, last[i]) + uint64_t(i < C::kFirst ? first : b) * kFpBlock;
             asm("" : "+s"(p), "+s"(last[i]));  // kept, not computed again
             from[i] = p;
         }
@@ -470,21 +478,31 @@ struct Stream {
         xsat = lds_at(&lds.xs[0][64 * (c.wave % (C::XS / 64))]);
         wsat = lds_at(&lds.ws[0][0]);
     }
+    template <bool IF = true>
     __device__ __forceinline__ void one(uint64_t lanes, uint32_t i, uint32_t buf)
     {
         if (i < C::CW + C::CX) {
             const bool is_w = i < C::CW;
-            const uint32_t ld = is_w ? ldw[C::GATED ? i % 2 : 0] : ldx;  // NW = WN: a half's rows are one copy of each wave
+            const uint32_t ld = is_w ? ldw[C::GATED ? i % 2 : 0] : ldx;
             const uint32_t to = is_w ? w + buf * C::BN * kFpBlock + i * C::NW * 1024 : x + buf * C::BM * kFpBlock + (i - C::CW) * C::NW * 1024;
-            copy16_if(lanes, to, from[i], __umul24(min(row8, last[i]), ld) + chunk);
-            from[i] += kFpBlock;
+            const uint32_t off = __umul24(min(row8, last[i]), ld) + chunk;
+            if (IF) copy16_if(lanes, to, from[i], off);
+            else copy16(to, from[i], off);
+            from[i] = uniform(from[i] + kFpBlock);
         } else if (i == C::CW + C::CX) {
-            copy4_if(lanes, xsat + buf * C::XS * 4, xs, xsoff);
-            xs += ldxs;
+            if (IF) copy4_if(lanes, xsat + buf * C::XS * 4, xs, xsoff);
+            else copy4(xsat + buf * C::XS * 4, xs, xsoff);
+            xs = uniform(xs + ldxs);
         } else {
-            copy4_if(lanes, wsat + buf * 256, ws);
+            if (IF) copy4_if(lanes, wsat + buf * 256, ws);
+            else copy4(wsat + buf * 256, ws);
             ++ws;
         }
+    }
+    __device__ __forceinline__ void block(uint32_t buf)
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < C::COPIES; ++i) one<false>(0, i, buf);
     }
 };
 
@@ -556,6 +574,7 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
         if (b0 + i < b1) copies.block(a, lds, b0 + i, i);
+    Stream<C> stream(a, at, wave, lane, lds, b0 + S - 1, b0 + S - 1);
     uint32_t buf = 0;
     for (uint32_t b = b0; b < b1; ++b) {
         // this block's copies have arrived; those of the S - 2 after it may be under way
@@ -563,7 +582,10 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's; and the block before is read
         const uint32_t ahead = buf == 0 ? S - 1 : buf - 1;
-        if (b + S - 1 < b1) copies.block(a, lds, b + S - 1, ahead);
+        if (b + S - 1 < b1) {
+            if ((b + S) * kFpBlock <= a.K) stream.block(ahead);
+            else copies.block(a, lds, b + S - 1, ahead);
+        }
 
         const uint8_t* xl = &lds.x[buf][(wm * WM * 16 + r) * kFpBlock];
         const uint8_t* wl = &lds.w[buf][(wn * WN * 16 + r) * kFpBlock];
@@ -756,7 +778,7 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
         for (int j = 0; j < 2; ++j) read_x(0, j);
 #pragma unroll
         for (int i = 0; i < H - 1; ++i) read_w(0, i);
-        Stream<C> stream(arguments(), d.at, wave, lane, lds, d.b0 + 1);
+        Stream<C> stream(arguments(), d.at, wave, lane, lds, d.b0 + 2, d.b0 + 1);
         uint32_t buf = 0;
         for (uint32_t b = d.b0; b < d.b1; ++b, buf ^= 1u) step(stream, lanes_if(b + 1 < d.b1), lanes_if(b + 2 < d.b1), buf);
 #pragma unroll
