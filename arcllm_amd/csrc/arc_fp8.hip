@@ -7,6 +7,7 @@
 // multiply-adds in fp32.
 #include "arc_paged.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace arc {
@@ -647,6 +648,123 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
     put_tile<Y, C>(a, at, wave, lane, acc);
 }
 
+// 17 to 64 rows of x and few outputs.  Bound by reading the weights once; larger tiles would leave much of the card idle, or their
+// parts' sums to a second launch, 5 us.  A workgroup has 16 outputs (GATED: with the activation, 16 rows of gate and of up);
+// its waves take the blocks in turn, each with its own place in LDS for two of them and no barrier, and add up in wave order.
+// The price is that x goes to every workgroup, from the L2: 3 times the weights' bytes at 48 rows.  45 rows, 3584 x 18944, in
+// fp32: 20 us, tiles in 16 parts 24; 32 rows, 512 x 3584: 4.4 and 8.4.  Operands straight into registers, without LDS, took
+// 41: 16 rows of 64 bytes are as many requests as 16 of 128.
+template <bool GATED, int WM>
+struct OwnShape {
+    static constexpr int G = GATED ? 2 : 1, NW = 2 * G + 2 * WM <= 8 ? 8 : 6;
+    static constexpr uint32_t GROUPS = 2 * G + 2 * WM;  // copies of 8 rows to a block, besides the scales'
+    struct Lds {
+        __align__(16) uint8_t rows[NW][2][GROUPS * 1024];
+        float xs[NW][2][64];
+    };
+};
+template <typename Y, bool GATED, int WM>
+__global__ __launch_bounds__(512, 2) void k_fp8_own(Gemm a)
+{
+    typedef OwnShape<GATED, WM> C;
+    constexpr int G = C::G, NW = C::NW;
+    constexpr bool FAST = sizeof(Y) == 2;
+    __shared__ union {
+        typename C::Lds copied;
+        f32x4 sums[NW][G][WM][64];
+    } lds;
+    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4, wave = uniform(threadIdx.x >> 6);
+    const uint32_t n0 = blockIdx.x * 16;
+    const uint32_t row8 = lane >> 3, chunk = ((lane & 7u) ^ swizzle(row8)) * 16;  // of a group's rows 8 .. 15: ^ 64
+    const uint8_t* from[C::GROUPS];
+    uint32_t last[C::GROUPS];
+#pragma unroll
+    for (uint32_t i = 0; i < C::GROUPS; ++i) {
+        const bool is_w = i < 2 * G;
+        const uint32_t row = is_w ? min(n0 + 8 * (i & 1u), a.N - 1) : min(8 * (i - 2 * G), a.M - 1);
+        last[i] = (is_w ? a.N : a.M) - 1 - row;
+        from[i] = uniform((is_w ? a.w[i / 2 % G] : a.x) + uint64_t(row) * (is_w ? a.ldw[i / 2 % G] : a.ldx) + wave * kFpBlock);
+    }
+    const uint32_t xsoff = min(lane, a.M - 1) * 4;
+    auto copy_block = [&](uint32_t b, uint32_t buf) {  // the blocks in the wave's order
+        const uint32_t left = a.K - 16 - b * kFpBlock, to = lds_at(&lds.copied.rows[wave][buf][0]);
+#pragma unroll
+        for (uint32_t i = 0; i < C::GROUPS; ++i) {
+            const uint32_t ld = i < 2 * G ? a.ldw[i / 2 % G] : a.ldx;
+            copy16(to + i * 1024, from[i], __umul24(min(row8, last[i]), ld) + min(chunk ^ (i % 2 * 64), left));
+            from[i] = uniform(from[i] + NW * kFpBlock);
+        }
+        copy4(lds_at(&lds.copied.xs[wave][buf][0]), uniform(a.xs + uint64_t(b) * a.ldxs), xsoff);
+    };
+    f32x4 acc[G][WM];
+#pragma unroll
+    for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int j = 0; j < WM; ++j) acc[h][j] = f32x4{0, 0, 0, 0};
+    const uint32_t place = (g ^ swizzle(r)) * 16;
+    if (wave < NW && wave < a.blocks) copy_block(wave, 0);
+    uint32_t buf = 0;
+    for (uint32_t b = wave; b < a.blocks; b += NW, buf ^= 1u) {
+        if (b + NW < a.blocks) {
+            copy_block(b + NW, buf ^ 1u);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::GROUPS + 1) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const uint8_t* rows = lds.copied.rows[wave][buf];
+        auto frag = [&](uint32_t tile) {
+            const uint8_t* p = rows + (tile * 16 + r) * kFpBlock;
+            return Frag{*reinterpret_cast<const u32x4*>(p + place), *reinterpret_cast<const u32x4*>(p + (place ^ 64u))};
+        };
+        Frag wf[G];
+        float ws[G];
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            wf[h] = frag(h);
+            ws[h] = a.ws[h][uint64_t(n0 / kFpBlock) * a.ldws[h] + b];
+        }
+#pragma unroll
+        for (int j = 0; j < WM; ++j) {
+            Frag xf = frag(G + j);
+            const float xs = lds.copied.xs[wave][buf][j * 16 + r];
+            if ((b + 1) * kFpBlock > a.K) only_to(xf, b * kFpBlock + g * 16, a.K);
+            Wide xw;
+            if constexpr (!FAST) xw = widen(xf);
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                f32x4 p;
+                if constexpr (FAST)
+                    p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, wf[h]), __builtin_bit_cast(i32x8, xf),
+                                                                         f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+                else p = block_sums(widen(wf[h]), xw);
+                const float s = xs * ws[h];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[h][j][e] = __builtin_fmaf(p[e], s, acc[h][j][e]);
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read, before the next copy but one
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int j = 0; j < WM; ++j) lds.sums[wave][h][j][lane] = acc[h][j];
+    __syncthreads();
+    for (uint32_t j = wave; j < uint32_t(WM); j += NW) {
+        f32x4 t[G];
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            t[h] = lds.sums[0][h][j][lane];
+#pragma unroll
+            for (int i = 1; i < NW; ++i) t[h] += lds.sums[i][h][j][lane];
+        }
+        if constexpr (GATED)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[0][e] = silu<Y>(t[0][e]) * t[1][e];
+        store_out<Y>(a, j * 16 + r, n0 + 4 * g, t[0]);
+    }
+}
+
 // Large tiles.  Bound by the matrix cores if everything else keeps out of their way: per block and wave 32 (16) products of 32
 // cycles, 4 fused multiply-adds for each, 24 (16) LDS reads.  So the order is fixed by hand, each product with its part of the rest:
 // the multiply-adds of the product three before it, and LDS reads some 6 (3) products ahead of their use.  For that, a block's
@@ -850,7 +968,7 @@ uint32_t bytes_of(int dtype) { return dtype == ARC_F32 ? 4 : dtype == ARC_F16 ||
 // short; beginning and end of a tile cost about 4 blocks; k_fp8_join 3 us and the sums' way there and back at 6 TB/s.  The
 // times are those of 28 and 148 blocks at 24 to 4096 rows, which this meets within 15 %: of 3584 x 18944 in bf16, 2048 rows,
 // tiles of 128, 185 us, of 256 in two parts 170; 1024 rows 135, and of 256 in four parts 104; of 4608 x 3584, 4096 rows, 93 and 109.
-enum class Form { few, rows32, rows64, rows128, deep128, deep256 };
+enum class Form { few, own, rows32, rows64, rows128, deep128, deep256 };
 struct Plan {
     Form form;
     uint32_t mtiles, ntiles, splits;
@@ -865,6 +983,7 @@ Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
 {
     Plan best{Form::few, 0, 0, 1, 256};
     if (M <= 16) return best;
+    float least = INFINITY;
     auto tiles = [](uint32_t n, uint32_t each) { return (n + each - 1) / each; };
     const uint32_t blocks = tiles(K, kFpBlock);
     const Shape rows32{Form::rows32, 32, 128, fast ? 0.60f : 0.80f, fast ? 0.90f : 1.10f};
@@ -872,8 +991,15 @@ Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
     const Shape rows128{Form::rows128, 128, 128, fast ? 1.0f : 1.25f, fast ? 1.6f : 2.1f};
     const Shape deep128{Form::deep128, 128, 128, 0.75f, 1.25f}, deep256{Form::deep256, 256, 256, 1.45f, 1.95f};
     const bool deep = fast && K % kFpBlock == 0;
+    if (M <= 64) {
+        // k_fp8_own, one workgroup to a compute unit: 2.5 us to begin and end, between them its copies, 1 KB each, or the weights
+        // that all of them read at 5.2 TB/s
+        const uint32_t copies = 2 * tiles(M, 16) + (gated ? 4 : 2);
+        const float each = (fast ? 0.0105f : 0.0125f) * (copies <= 8 ? 1.0f : 1.25f);
+        least = tiles(tiles(N, 16), 256) * (2.5f + std::max(blocks * copies * each, float(K) * (gated ? 8192 : 4096) / 5.2e6f));
+        best.form = Form::own;
+    }
     const Shape of[2] = {M <= 32 ? rows32 : M <= 64 ? rows64 : deep ? deep128 : rows128, deep256};
-    float least = INFINITY;
     for (const Shape& s : of) {
         if (s.form == Form::deep256 && (!deep || M <= 64)) continue;
         const uint32_t mtiles = tiles(M, s.bm), ntiles = tiles(N, gated ? s.bn / 2 : s.bn);
@@ -908,7 +1034,12 @@ hipError_t launch_form(const Gemm& a, Form form, hipStream_t st)
 {
     constexpr bool FAST = sizeof(Y) == 2;
     if (form == Form::few) hipLaunchKernelGGL((k_fp8_few<Y, GATED>), dim3((a.N + 15) / 16, (a.M + 15) / 16), dim3(64 * kFewWaves8), 0, st, a);
-    else if (form == Form::rows32) return launch_tile<Y, TileShape<GATED, FAST, false, 2, 2, 1, 4, 3>>(a, st);
+    else if (form == Form::own) {
+        auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3((a.N + 15) / 16), dim3(64 * waves), 0, st, a); };
+        if (a.M <= 32) launch(k_fp8_own<Y, GATED, 2>, OwnShape<GATED, 2>::NW);
+        else if (a.M <= 48) launch(k_fp8_own<Y, GATED, 3>, OwnShape<GATED, 3>::NW);
+        else launch(k_fp8_own<Y, GATED, 4>, OwnShape<GATED, 4>::NW);
+    } else if (form == Form::rows32) return launch_tile<Y, TileShape<GATED, FAST, false, 2, 2, 1, 4, 3>>(a, st);
     else if (form == Form::rows64) return launch_tile<Y, TileShape<GATED, FAST, false, 4, 2, 1, 4, 3>>(a, st);
     else if (form == Form::rows128) return launch_tile<Y, TileShape<GATED, FAST, false, 4, 4, 2, 2, 2>>(a, st);
     else if constexpr (FAST) return form == Form::deep128 ? launch_tile<Y, TileShape<GATED, FAST, true, 4, 4, 2, 2, 2>>(a, st)
