@@ -218,8 +218,9 @@ __device__ __forceinline__ f32x4 block_sums(const Wide& w, const Wide& x)
     return p;
 }
 
-// 16 rows of w and 16 of x to a workgroup; its 8 waves take the blocks in turn, straight from memory, and add up in
-// wave order through LDS.
+// Up to 16 rows of x.  16 rows of w to a workgroup; its 8 waves take the blocks in turn, straight from memory, four on their way at
+// once, and add up in wave order through LDS.  Bound by reading the weights: 1 row of 152064 outputs of 3584, 545 MB, 88 us,
+// 6.2 TB/s; of 4608, 6.7 us, of which the launch is half.
 constexpr uint32_t kFewWaves8 = 8;
 template <typename Y, bool GATED>
 __global__ __launch_bounds__(512) void k_fp8_few(Gemm a)
@@ -648,9 +649,9 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
     put_tile<Y, C>(a, at, wave, lane, acc);
 }
 
-// 17 to 64 rows of x and few outputs.  Bound by reading the weights once; larger tiles would leave much of the card idle, or their
+// Up to 64 rows of x and few outputs.  Bound by reading the weights once; larger tiles would leave much of the card idle, or their
 // parts' sums to a second launch, 5 us.  A workgroup has 16 outputs (GATED: with the activation, 16 rows of gate and of up);
-// its waves take the blocks in turn, each with its own place in LDS for two of them and no barrier, and add up in wave order.
+// its waves take the blocks in turn, each with its own place in LDS for two or more of them and no barrier, and add up in wave order.
 // The price is that x goes to every workgroup, from the L2: 3 times the weights' bytes at 48 rows.  45 rows, 3584 x 18944, in
 // fp32: 20 us, tiles in 16 parts 24; 32 rows, 512 x 3584: 4.4 and 8.4.  Operands straight into registers, without LDS, took
 // 41: 16 rows of 64 bytes are as many requests as 16 of 128.
@@ -658,9 +659,10 @@ template <bool GATED, int WM>
 struct OwnShape {
     static constexpr int G = GATED ? 2 : 1, NW = 2 * G + 2 * WM <= 8 ? 8 : 6;
     static constexpr uint32_t GROUPS = 2 * G + 2 * WM;  // copies of 8 rows to a block, besides the scales'
+    static constexpr uint32_t S = GROUPS <= 4 ? 4 : GROUPS <= 6 ? 3 : 2;  // blocks of a wave in LDS
     struct Lds {
-        __align__(16) uint8_t rows[NW][2][GROUPS * 1024];
-        float xs[NW][2][64];
+        __align__(16) uint8_t rows[NW][S][GROUPS * 1024];
+        float xs[NW][S][64];
     };
 };
 template <typename Y, bool GATED, int WM>
@@ -702,11 +704,18 @@ __global__ __launch_bounds__(512, 2) void k_fp8_own(Gemm a)
 #pragma unroll
         for (int j = 0; j < WM; ++j) acc[h][j] = f32x4{0, 0, 0, 0};
     const uint32_t place = (g ^ swizzle(r)) * 16;
-    if (wave < NW && wave < a.blocks) copy_block(wave, 0);
+    constexpr uint32_t S = C::S;
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < S; ++i)
+        if (wave + i * NW < a.blocks) copy_block(wave + i * NW, i);
     uint32_t buf = 0;
-    for (uint32_t b = wave; b < a.blocks; b += NW, buf ^= 1u) {
-        if (b + NW < a.blocks) {
-            copy_block(b + NW, buf ^ 1u);
+    for (uint32_t b = wave; b < a.blocks; b += NW, buf = buf + 1 == S ? 0 : buf + 1) {
+        if (b + (S - 1) * NW < a.blocks) {
+            copy_block(b + (S - 1) * NW, buf == 0 ? S - 1 : buf - 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * (C::GROUPS + 1)) : "memory");
+        } else if (S > 3 && b + 2 * NW < a.blocks) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (C::GROUPS + 1)) : "memory");
+        } else if (S > 2 && b + NW < a.blocks) {
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::GROUPS + 1) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -982,7 +991,12 @@ struct Shape {
 Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
 {
     Plan best{Form::few, 0, 0, 1, 256};
-    if (M <= 16) return best;
+    // few rows: from about 6 on k_fp8_own reads them more cheaply (16 rows, 3584 x 18944, 14.3 us and 19.6; 8 rows 14.4 and 17.2; 2 rows of
+    // 4608 x 3584 8.2 and 6.9), unless its workgroups come in many turns (152064 outputs, 8 rows, 143 and 117)
+    if (M <= 16) {
+        if (M >= 6 && N <= 32768) best.form = Form::own;
+        return best;
+    }
     float least = INFINITY;
     auto tiles = [](uint32_t n, uint32_t each) { return (n + each - 1) / each; };
     const uint32_t blocks = tiles(K, kFpBlock);
@@ -1036,7 +1050,8 @@ hipError_t launch_form(const Gemm& a, Form form, hipStream_t st)
     if (form == Form::few) hipLaunchKernelGGL((k_fp8_few<Y, GATED>), dim3((a.N + 15) / 16, (a.M + 15) / 16), dim3(64 * kFewWaves8), 0, st, a);
     else if (form == Form::own) {
         auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3((a.N + 15) / 16), dim3(64 * waves), 0, st, a); };
-        if (a.M <= 32) launch(k_fp8_own<Y, GATED, 2>, OwnShape<GATED, 2>::NW);
+        if (a.M <= 16) launch(k_fp8_own<Y, GATED, 1>, OwnShape<GATED, 1>::NW);
+        else if (a.M <= 32) launch(k_fp8_own<Y, GATED, 2>, OwnShape<GATED, 2>::NW);
         else if (a.M <= 48) launch(k_fp8_own<Y, GATED, 3>, OwnShape<GATED, 3>::NW);
         else launch(k_fp8_own<Y, GATED, 4>, OwnShape<GATED, 4>::NW);
     } else if (form == Form::rows32) return launch_tile<Y, TileShape<GATED, FAST, false, 2, 2, 1, 4, 3>>(a, st);
