@@ -6,6 +6,8 @@
 // chunk.  Node i's parent is a node before it.
 #include "arc_paged.hpp"
 
+#include <algorithm>
+
 namespace arc {
 namespace {
 
@@ -305,6 +307,30 @@ int check_tree(const arc_tree* t)
     return ARC_OK;
 }
 
+// Arrays of a call: what it writes must not share memory with what it reads or else writes; `same`: this array may be
+// the input at the same address.
+struct Array {
+    const void* p;
+    uint64_t bytes;
+    const void* same;
+};
+bool share(const Array& a, const Array& b)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes && !(a.same == b.p && a.p == b.p);
+}
+template <size_t W, size_t R>
+bool shared(const Array (&written)[W], const Array (&read)[R])
+{
+    for (size_t i = 0; i < W; ++i) {
+        for (size_t j = i + 1; j < W; ++j)
+            if (share(written[i], written[j])) return true;
+        for (size_t j = 0; j < R; ++j)
+            if (share(written[i], read[j])) return true;
+    }
+    return false;
+}
+
 // Parts of a row of logits: enough workgroups to fill the card.
 uint32_t splits_of(uint32_t tokens)
 {
@@ -342,6 +368,10 @@ int arc_tree_plan(const arc_paged_batch* batch, const arc_tree* tree, arc_stream
     if (!batch->lens || !batch->starts || !batch->positions || !tree->masks)
         return set_error(ARC_ERR_INVALID_ARGUMENT, "null lens, starts, positions or masks");
     if (batch->requests == 0 || batch->tokens == 0) return ARC_OK;
+    const uint64_t tokens = batch->tokens * 4ull, requests = batch->requests * 4ull;
+    const Array written[] = {{tree->masks, tokens * tree->mask_words, nullptr}, {batch->positions, tokens, nullptr}};
+    const Array read[] = {{tree->parents, tokens, nullptr}, {batch->lens, requests, nullptr}, {batch->starts, requests + 4, nullptr}};
+    if (shared(written, read)) return set_error(ARC_ERR_INVALID_ARGUMENT, "masks and positions share memory with each other or with what is read");
     const TreePlan a{batch->lens, batch->starts, tree->parents, tree->masks, batch->positions, batch->requests, batch->tokens, tree->mask_words};
     hipLaunchKernelGGL(k_tree_plan, dim3(batch->requests), dim3(256), 0, static_cast<hipStream_t>(stream), a);
     return check_hip(hipGetLastError(), "tree plan");
@@ -384,9 +414,25 @@ int arc_tree_commit(const arc_kv_pages* layers, uint32_t num_layers, const arc_p
         if (!aligned(logits, size)) return set_error(ARC_ERR_INVALID_ARGUMENT, "logits must be aligned to their type");
         if (batch->tokens > kMaxLogitRows) return set_error(ARC_ERR_UNSUPPORTED, "%u rows of logits: at most 2^20", batch->tokens);
     }
+    const void* pools[2 * ARC_MAX_LAYERS];
+    for (uint32_t i = 0; i < num_layers; ++i) {
+        pools[2 * i] = layers[i].k;
+        pools[2 * i + 1] = layers[i].v;
+    }
+    std::sort(pools, pools + 2 * num_layers);
+    if (std::adjacent_find(pools, pools + 2 * num_layers) != pools + 2 * num_layers)
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "the same pages twice among the layers' k and v");
+    const Space sp = space_of(batch);
+    const uint64_t tokens = batch->tokens * 4ull, requests = batch->requests * 4ull;
+    const Array written[] = {{workspace, sp.bytes, nullptr}, {tokens_out, tokens, nullptr}, {counts, requests, nullptr},
+                             {lens_out, requests, batch->lens}, {free_pages, num_pages * 4ull, nullptr},
+                             {free_pages ? free_count_out : nullptr, 4, free_count}, {logits ? targets : nullptr, tokens, nullptr}};
+    const Array read[] = {{logits ? nullptr : targets, tokens, nullptr}, {drafts, tokens, nullptr}, {tree->parents, tokens, nullptr},
+                          {batch->lens, requests, nullptr}, {batch->starts, requests + 4, nullptr},
+                          {batch->tables, requests * batch->max_pages, nullptr}, {free_pages ? free_count : nullptr, 4, nullptr}};
+    if (shared(written, read)) return set_error(ARC_ERR_INVALID_ARGUMENT, "an array that is written shares memory with another of the call");
     hipStream_t st = static_cast<hipStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    const Space sp = space_of(batch);
     uint32_t *path = reinterpret_cast<uint32_t*>(ws), *held = reinterpret_cast<uint32_t*>(ws + sp.held);
     Best* parts = reinterpret_cast<Best*>(ws + sp.parts);
     const uint32_t splits = logits ? splits_of(batch->tokens) : 0;

@@ -436,7 +436,7 @@ typedef struct arc_tree { /* device arrays, in the order of the step's rows */
  * row its place, with no mask.  After arc_paged_plan, whose positions of trees count
  * rows and not depths (its slots stay: node i lies in slot i behind the context).  Rows
  * behind the last request are left as they were.  Of the batch, requests, tokens, lens,
- * starts and positions (written) are used. */
+ * starts and positions (written) are used.  The arrays share no memory. */
 int arc_tree_plan(const arc_paged_batch *batch, const arc_tree *tree, arc_stream_t stream);
 
 /* Bytes of device workspace arc_tree_attention needs, as arc_paged_attention_workspace_bytes. */
@@ -465,7 +465,8 @@ int arc_tree_attention(const arc_kv_pages *pages, const arc_paged_batch *batch, 
  *   num_pages; NULL: they stay with the request), requests in order, first page to last.  free_count_out may
  *   be free_count.
  * A chunk counts 1 (the target's token after its last row), keeps all its positions and moves nothing; a
- * request without rows counts 0.  layers: 1 .. ARC_MAX_LAYERS pools of one shape (host array).  A position whose page
+ * request without rows counts 0.  layers: 1 .. ARC_MAX_LAYERS pools of one shape (host array), none of them
+ * twice; what is written shares no memory with another array but where it may be one of them.  A position whose page
  * is none of the pool does not move.  workspace: arc_tree_commit_workspace_bytes() bytes, 256-byte
  * aligned, as arc_paged_attention's.  Of the batch, all but positions, slots and max_new is used. */
 size_t arc_tree_commit_workspace_bytes(const arc_paged_batch *batch);

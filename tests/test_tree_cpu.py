@@ -99,6 +99,33 @@ def test_commit_refusals(call):
     refused(call)
 
 
+def apart(**over):
+    """A commit whose arrays lie apart, but for `over`; none of them is followed."""
+    kw = dict(layers=[pages(k=(40 + 2 * i) * A, v=(41 + 2 * i) * A) for i in range(3)],
+              b=batch(tables=A, lens=2 * A, starts=3 * A), t=tree(parents=4 * A), drafts=5 * A, targets=6 * A, lens_out=7 * A, counts=8 * A,
+              tokens=9 * A, ws=10 * A, free_pages=11 * A, num_pages=8, free_count=12 * A, free_count_out=13 * A)
+    commit(**{**kw, **over})
+
+
+@pytest.mark.parametrize("over", [
+    dict(layers=[pages(), pages(k=3 * A, v=4 * A), pages()]), dict(layers=[pages(k=A, v=A)]), dict(layers=[pages(), pages(k=2 * A, v=3 * A)]),
+    dict(tokens=6 * A), dict(tokens=5 * A + 4), dict(tokens=8 * A), dict(counts=7 * A), dict(counts=2 * A), dict(lens_out=2 * A + 4),
+    dict(lens_out=3 * A), dict(lens_out=4 * A + 12), dict(free_pages=A), dict(free_count_out=12 * A - 2), dict(free_count_out=11 * A + 28),
+    dict(ws=9 * A), dict(free_pages=10 * A + 256), dict(targets=5 * A, **LOGITS), dict(targets=9 * A, **LOGITS),
+], ids=str)
+def test_commit_of_shared_memory_is_refused(over):
+    with pytest.raises(arc.ArcError, match="twice|shares memory"):
+        apart(**over)
+
+
+def test_plan_of_shared_memory_is_refused():
+    b = batch(lens=2 * A, starts=3 * A, positions=4 * A)
+    for t in (tree(parents=5 * A, masks=4 * A), tree(parents=5 * A, masks=5 * A + 12), tree(parents=4 * A, masks=6 * A),
+              tree(parents=5 * A, masks=2 * A), tree(parents=5 * A, masks=3 * A - 4, mask_words=1)):
+        with pytest.raises(arc.ArcError, match="share memory"):
+            arc.tree_plan(b, t)
+
+
 def test_commit_takes_pages_only():
     with pytest.raises(TypeError):
         commit(layers=[pages(), 5])
