@@ -33,7 +33,8 @@ struct TreePlan {
 };
 
 // A workgroup to a request, a lane to a node: it climbs from its node to the root, in LDS, and writes each word of its
-// mask when it has left it behind.  A climb is a chain of LDS reads (some 60 ns each): the tree's depth bounds it.
+// mask when it has left it behind.  A climb is a chain of LDS reads (some 60 ns each): the tree's depth bounds it.  One
+// tree of 26 nodes 3.5 us, 500 of up to 60 nodes 3.8: the launch.
 __global__ __launch_bounds__(256) void k_tree_plan(TreePlan a)
 {
     __shared__ uint32_t parent[kMaxNodes];
@@ -95,7 +96,8 @@ struct Argmax {
     uint32_t requests, tokens, vocab, splits;
 };
 // A workgroup to a part of a row; rows behind the last request are not read.  Bound by reading the logits: 16 bytes a lane
-// from the first 16-byte border on, four at a time.
+// from the first 16-byte border on, four at a time.  A step's end of 24 trees of up to 40 nodes with logits of 152064 in fp32: 73 us
+// in all, of which the logits, 365 MB, at 6.2 TB/s, would be 59.
 template <typename T>
 __global__ __launch_bounds__(256) void k_tree_argmax(Argmax a)
 {
@@ -141,7 +143,8 @@ struct Walk {
 };
 
 // A workgroup to a request: the target's token of each row, from the parts of its logits if there are any, then wave 0
-// walks from node 0 to the first child that holds the target's token, as long as there is one.
+// walks from node 0 to the first child that holds the target's token, as long as there is one: 64 nodes a look.  Bound by
+// its launch and a chain of three round trips to memory, about 4 us.
 __global__ __launch_bounds__(256) void k_tree_walk(Walk a)
 {
     __shared__ uint32_t parent[kMaxNodes], draft[kMaxNodes], said[kMaxNodes], path[kMaxNodes];
@@ -228,7 +231,7 @@ __device__ __forceinline__ bool place_of(const Move& a, uint32_t b, uint32_t pos
 // A workgroup to a request and layer: row path[i] of the walk to place i.  A few rows of some KB: a chain of round trips to
 // memory (rows, walk, pages, values), so each is made for all rows at once.  Each thread has the same 16 bytes of
 // every row and reads 8 rows before it writes any: a row is then read before its place is written, as path[i] >= i and both rise.
-// The workgroup of one more layer number returns the pages.
+// The workgroup of one more layer number returns the pages.  28 layers after one tree of 26 nodes: 9.3 us with the walk's launch.
 __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
 {
     constexpr uint32_t kBatch = 8;

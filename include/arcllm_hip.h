@@ -467,8 +467,8 @@ int arc_tree_attention(const arc_kv_pages *pages, const arc_paged_batch *batch, 
  * A chunk counts 1 (the target's token after its last row), keeps all its positions and moves nothing; a
  * request without rows counts 0.  layers: 1 .. ARC_MAX_LAYERS pools of one shape (host array), none of them
  * twice; what is written shares no memory with another array but where it may be one of them.  A position whose page
- * is none of the pool does not move.  workspace: arc_tree_commit_workspace_bytes() bytes, 256-byte
- * aligned, as arc_paged_attention's.  Of the batch, all but positions, slots and max_new is used. */
+ * is none of the pool does not move.  workspace: arc_tree_commit_workspace_bytes() bytes (fewer rows may need
+ * more), 256-byte aligned, as arc_paged_attention's.  Of the batch, all but positions, slots and max_new is used. */
 size_t arc_tree_commit_workspace_bytes(const arc_paged_batch *batch);
 int arc_tree_commit(const arc_kv_pages *layers, uint32_t num_layers, const arc_paged_batch *batch, const arc_tree *tree,
                     int logits_dtype, const void *logits, uint64_t ldl, uint32_t vocab, const uint32_t *drafts,
@@ -482,7 +482,7 @@ int arc_tree_commit(const arc_kv_pages *layers, uint32_t num_layers, const arc_p
 typedef struct arc_fp8_rows { /* rows of activations, device */
     void *q;                  /* [rows][ldq] e4m3, 16-byte aligned */
     float *scales;            /* [ceil(cols / 128)][lds]: block b of row m at b * lds + m */
-    uint32_t rows, cols;      /* cols: a multiple of 16, at most 2^22; rows below 2^24 */
+    uint32_t rows, cols;      /* cols: a multiple of 16, at most 2^22; rows at most 2^24 */
     uint32_t ldq;             /* bytes from row to row: a multiple of 16, >= cols, at most 2^22 */
     uint32_t lds;             /* >= rows */
 } arc_fp8_rows;
@@ -502,9 +502,11 @@ int arc_fp8_quantize(int x_dtype, const void *x, uint32_t ldx, const arc_fp8_row
 
 /* y[m][n] = sum_k x[m][k] w[n][k] (+ residual[m][n]), x and w with their scales; y and residual of y_dtype
  * (ARC_F32, ARC_F16, ARC_BF16), ldy and ldr elements from row to row (16-byte aligned rows are quickest); residual may be
- * NULL, or y itself.  Products of scales that leave fp32's normal range do not keep their bits.
- * workspace: arc_fp8_gemm_workspace_bytes(w->rows, w->cols, x->rows, 0) bytes, 256-byte
- * aligned, any contents, for one call at a time.  No rows: nothing is done. */
+ * NULL, or y itself; otherwise y shares no memory with what is read.  Sums are fp32, rounded once.  A y of 16 bits may lose of each 8
+ * neighbouring products what lies below 2^-13 of their largest (1.3e-5 of y for normal data), an fp32 one
+ * does not.  Products of scales that leave fp32's normal range do not keep their bits.
+ * workspace: arc_fp8_gemm_workspace_bytes(w->rows, w->cols, x->rows, 0) bytes (fewer rows may need more),
+ * 256-byte aligned, any contents, for one call at a time.  No rows: nothing is done. */
 size_t arc_fp8_gemm_workspace_bytes(uint32_t n, uint32_t k, uint32_t rows, int gated);
 int arc_fp8_gemm(const arc_fp8_weights *w, const arc_fp8_rows *x, int y_dtype, void *y, uint32_t ldy, const void *residual,
                  uint32_t ldr, void *workspace, arc_stream_t stream);

@@ -96,6 +96,23 @@ def test_quantize_many_rows():
     run_quantize(rng_of(4).standard_normal((70000, 16)), arc.F16)
 
 
+@pytest.mark.parametrize("dtype", ALL)
+def test_quantize_rows_at_any_16_bytes(dtype):
+    """x at an odd multiple of 16 bytes, q and the scales too; rows 8 columns from the next."""
+    rows, cols = 35, 272
+    x = rng_of(5).standard_normal((rows, cols))
+    bits = fl.to_device_bits(x, dtype)
+    lead, size = 16 // bits.itemsize, (cols + 8) * rows
+    flat = np.zeros(lead + size, bits.dtype)
+    flat[lead:].reshape(rows, cols + 8)[:, :cols] = bits
+    dx, q, s = D(flat), D(np.full(16 + rows * cols, 0xA5, np.uint8)), D(np.full(1 + 3 * rows, -3.0, np.float32))
+    arc.fp8_quantize(dtype, dx.ptr + 16, cols + 8, arc.Fp8Rows(q.ptr + 16, s.ptr + 4, rows, cols))
+    want_q, want_s = fl.quantize(fl.from_device_bits(bits, dtype).astype(np.float32))
+    got_q, got_s = q.download(np.uint8), s.download(np.float32)
+    assert np.all(got_q[:16] == 0xA5) and np.array_equal(got_q[16:].reshape(rows, cols), want_q)
+    assert got_s[0] == -3.0 and np.array_equal(got_s[1:].reshape(3, rows), want_s)
+
+
 # ------------------------------------------------------------------ product
 class Product:
     def __init__(self, M, N, K, seed=0, mats=1, ldq_pad=0, lds_pad=0, ldw_pad=0, ldws_pad=0):
