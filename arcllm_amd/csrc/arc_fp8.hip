@@ -661,8 +661,9 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
 // parts' sums to a second launch, 5 us.  A workgroup has 16 outputs (GATED: with the activation, 16 rows of gate and of up);
 // its waves take the blocks in turn, each with its own place in LDS for two or more of them and no barrier, and add up in wave order.
 // The price is that x goes to every workgroup, from the L2: 3 times the weights' bytes at 48 rows.  45 rows, 3584 x 18944, in
-// fp32: 20 us, tiles in 16 parts 24; 32 rows, 512 x 3584: 4.4 and 8.4.  Operands straight into registers, without LDS, took
-// 41: 16 rows of 64 bytes are as many requests as 16 of 128.
+// fp32: 18.6 us where the last cache still holds the weights, 25.8 from HBM; tiles in 16 parts 24 and 29; 32 rows, 512 x 3584: 4 and
+// 8.4.  Operands straight into registers, without LDS, took 41: 16 rows of 64 bytes are as many requests as 16 of 128.  Weights
+// a block further ahead than x gained nothing.
 template <bool GATED, int WM>
 struct OwnShape {
     static constexpr int G = GATED ? 2 : 1, NW = 2 * G + 2 * WM <= 8 ? 8 : 6;
@@ -717,7 +718,19 @@ __global__ __launch_bounds__(512, 2) void k_fp8_own(Gemm a)
     for (uint32_t i = 0; i + 1 < S; ++i)
         if (wave + i * NW < a.blocks) copy_block(wave + i * NW, i);
     uint32_t buf = 0;
+    const float* scales[G];  // a block's is read a turn ahead of its use
+    float ws[G], next_ws[G];
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+        scales[h] = a.ws[h] + uint64_t(n0 / kFpBlock) * a.ldws[h];
+        next_ws[h] = scales[h][min(wave, a.blocks - 1)];
+    }
     for (uint32_t b = wave; b < a.blocks; b += NW, buf = buf + 1 == S ? 0 : buf + 1) {
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            ws[h] = next_ws[h];
+            next_ws[h] = scales[h][min(b + NW, a.blocks - 1)];
+        }
         if (b + (S - 1) * NW < a.blocks) {
             copy_block(b + (S - 1) * NW, buf == 0 ? S - 1 : buf - 1);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * (C::GROUPS + 1)) : "memory");
@@ -734,12 +747,8 @@ __global__ __launch_bounds__(512, 2) void k_fp8_own(Gemm a)
             return Frag{*reinterpret_cast<const u32x4*>(p + place), *reinterpret_cast<const u32x4*>(p + (place ^ 64u))};
         };
         Frag wf[G];
-        float ws[G];
 #pragma unroll
-        for (int h = 0; h < G; ++h) {
-            wf[h] = frag(h);
-            ws[h] = a.ws[h][uint64_t(n0 / kFpBlock) * a.ldws[h] + b];
-        }
+        for (int h = 0; h < G; ++h) wf[h] = frag(h);
 #pragma unroll
         for (int j = 0; j < WM; ++j) {
             Frag xf = frag(G + j);
