@@ -660,7 +660,7 @@ def tree_commit(layers, batch: PagedBatch, tree: Tree, drafts, targets, lens_out
                 logits_dtype: int = F32, ldl: int = 0, vocab: int = 0, stream: Optional[Stream] = None) -> None:
     """The walk down each tree, the accepted rows' move in the pages of every layer (`layers`: KvPages), lengths
     and the pages that go back (arc_tree_commit).  With logits, `targets` is written, else read."""
-    if not all(type(p) is KvPages for p in layers):
+    if set(map(type, layers)) - {KvPages}:
         raise TypeError("layers: KvPages, one for each layer")
     pools = b"".join(layers)  # the structs side by side; (KvPages * n)(*layers) takes 15 us for 28
     check(lib().arc_tree_commit(pools, len(layers), C.byref(batch), C.byref(tree), logits_dtype, _ptr(logits), ldl, vocab,

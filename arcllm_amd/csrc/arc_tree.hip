@@ -142,49 +142,54 @@ struct Walk {
     uint32_t requests, tokens, words, splits;
 };
 
-// A workgroup to a request: the target's token of each row, from the parts of its logits if there are any, then wave 0
-// walks from node 0 to the first child that holds the target's token, as long as there is one: 64 nodes a look.  Bound by
-// its launch and a chain of three round trips to memory, about 4 us.
-__global__ __launch_bounds__(256) void k_tree_walk(Walk a)
+// Request b's target tokens, from the parts of its rows' logits if there are any, then wave 0's way from node 0 to the
+// first child that holds the target's token, as long as there is one: 64 nodes a look.  The nodes on a tree's way, 0 for
+// what is no tree; what the call gives is written where `writes`.
+struct WalkSpace {
+    uint32_t parent[kMaxNodes], draft[kMaxNodes], said[kMaxNodes], path[kMaxNodes];
+    uint32_t kept;
+};
+__device__ __forceinline__ uint32_t walk(const Walk& a, uint32_t b, const Rows& r, uint32_t len, bool writes, WalkSpace& l)
 {
-    __shared__ uint32_t parent[kMaxNodes], draft[kMaxNodes], said[kMaxNodes], path[kMaxNodes];
-    __shared__ uint32_t kept;
-    const uint32_t b = blockIdx.x, tid = threadIdx.x;
-    const Rows r = rows_of(a.starts, a.tokens, b);
-    const uint32_t len = a.lens[b];
-    if (a.splits)
+    const uint32_t tid = threadIdx.x;
+    auto said_after = [&](uint32_t i) {
+        if (!a.splits) return a.targets[r.first + i];
+        Best best{-INFINITY, kNoToken};
+        for (uint32_t s = 0; s < a.splits; ++s) best = better(best, a.parts[uint64_t(r.first + i) * a.splits + s]);
+        const uint32_t token = best.idx == kNoToken ? 0u : best.idx;
+        if (writes) a.targets[r.first + i] = token;
+        return token;
+    };
+    if (r.n == 0 || r.n > 32 * a.words) {
+        __syncthreads();  // everyone has read lens
+        if (!writes) return 0;
         for (uint32_t i = tid; i < r.n; i += 256) {
-            Best best{-INFINITY, kNoToken};
-            for (uint32_t s = 0; s < a.splits; ++s) best = better(best, a.parts[uint64_t(r.first + i) * a.splits + s]);
-            a.targets[r.first + i] = best.idx == kNoToken ? 0u : best.idx;
+            const uint32_t token = said_after(i);
+            if (i) a.tokens_out[r.first + i] = kNoToken;
+            if (i + 1 == r.n) a.tokens_out[r.first] = token;
         }
-    __syncthreads();
-    const bool tree = r.n <= 32 * a.words;
-    if (!tree || r.n == 0) {
-        for (uint32_t i = tid; i < r.n; i += 256) a.tokens_out[r.first + i] = i ? kNoToken : a.targets[r.first + r.n - 1];
         if (tid == 0) {
             a.counts[b] = r.n ? 1 : 0;
-            a.held[b] = len;
             a.lens_out[b] = len;
         }
-        return;
+        return 0;
     }
     for (uint32_t i = tid; i < r.n; i += 256) {
-        parent[i] = a.parents[r.first + i];
-        draft[i] = a.drafts[r.first + i];
-        said[i] = a.targets[r.first + i];
+        l.parent[i] = a.parents[r.first + i];
+        l.draft[i] = a.drafts[r.first + i];
+        l.said[i] = said_after(i);
     }
     __syncthreads();
     if (tid < 64) {
         uint32_t node = 0, n = 0;
         for (;;) {
-            if (tid == 0) path[n] = node;
+            if (tid == 0) l.path[n] = node;
             ++n;
-            const uint32_t want = said[node];
+            const uint32_t want = l.said[node];
             uint32_t next = kNoToken;
             for (uint32_t i = (node + 1) & ~63u; i < r.n; i += 64) {
                 const uint32_t c = i + tid;
-                const uint64_t fits = __ballot(c > node && c < r.n && parent[c] == node && draft[c] == want);
+                const uint64_t fits = __ballot(c > node && c < r.n && l.parent[c] == node && l.draft[c] == want);
                 if (fits) {
                     next = i + uint32_t(__builtin_ctzll(fits));
                     break;
@@ -193,18 +198,29 @@ __global__ __launch_bounds__(256) void k_tree_walk(Walk a)
             if (next == kNoToken) break;
             node = next;
         }
-        if (tid == 0) kept = n;
+        if (tid == 0) l.kept = n;
     }
     __syncthreads();
-    for (uint32_t i = tid; i < r.n; i += 256) {
-        a.tokens_out[r.first + i] = i < kept ? said[path[i]] : kNoToken;
-        if (i < kept) a.path[r.first + i] = path[i];
+    const uint32_t kept = l.kept;
+    if (writes) {
+        for (uint32_t i = tid; i < r.n; i += 256) a.tokens_out[r.first + i] = i < kept ? l.said[l.path[i]] : kNoToken;
+        if (tid == 0) {
+            a.counts[b] = kept;
+            a.lens_out[b] = base_of(len, r) + kept;
+        }
     }
-    if (tid == 0) {
-        a.counts[b] = kept;
-        a.held[b] = len;
-        a.lens_out[b] = base_of(len, r) + kept;
-    }
+    return kept;
+}
+
+// A workgroup to a request.  Bound by its launch and a chain of three round trips to memory, about 4 us.
+__global__ __launch_bounds__(256) void k_tree_walk(Walk a)
+{
+    __shared__ WalkSpace l;
+    const uint32_t b = blockIdx.x;
+    const Rows r = rows_of(a.starts, a.tokens, b);
+    const uint32_t len = a.lens[b], kept = walk(a, b, r, len, true, l);
+    for (uint32_t i = threadIdx.x; i < kept; i += 256) a.path[r.first + i] = l.path[i];
+    if (threadIdx.x == 0) a.held[b] = len;
 }
 
 // --------------------------------------------------------------------- move
@@ -228,43 +244,65 @@ __device__ __forceinline__ bool place_of(const Move& a, uint32_t b, uint32_t pos
     return page < a.num_pages;
 }
 
-// A workgroup to a request and layer: row path[i] of the walk to place i.  A few rows of some KB: a chain of round trips to
-// memory (rows, walk, pages, values), so each is made for all rows at once.  Each thread has the same 16 bytes of
-// every row and reads 8 rows before it writes any: a row is then read before its place is written, as path[i] >= i and both rise.
-// The workgroup of one more layer number returns the pages.  28 layers after one tree of 26 nodes: 9.3 us with the walk's launch.
-__global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
+// A layer's move: row node(i) of the way, `kept` long, to place i behind base.  A few rows of some KB: a chain of round
+// trips to memory (rows, walk, pages, values), so each is made for all rows at once.  Each thread has the same 16 bytes of
+// every row and reads 8 rows before it writes any: a row is then read before its place is written, as node(i) >= i and both rise.
+struct MoveSpace {
+    uint64_t from[kMaxNodes], to[kMaxNodes];  // byte offsets; kNowhere: the row stays
+};
+template <typename Node>
+__device__ __forceinline__ void move_rows(const Move& a, const Layers& layers, uint32_t layer, uint32_t b, uint32_t base, uint32_t kept,
+                                          MoveSpace& l, Node node)
 {
     constexpr uint32_t kBatch = 8;
+    constexpr uint64_t kNowhere = ~0ull;
+    const uint32_t tid = threadIdx.x, width = a.row_bytes / 16;
+    for (uint32_t i = tid; i < kept; i += 256) {
+        const uint32_t n = node(i);
+        uint64_t to_at, from_at;
+        const bool moves = n != i && place_of(a, b, base + i, to_at) && place_of(a, b, base + n, from_at);
+        l.from[i] = moves ? from_at : kNowhere;
+        l.to[i] = to_at;
+    }
+    __syncthreads();
+    for (uint32_t c = tid; c < 2 * width; c += 256) {
+        uint8_t* pool = static_cast<uint8_t*>(c < width ? layers.k[layer] : layers.v[layer]) + (c < width ? c : c - width) * 16;
+        for (uint32_t i0 = 1; i0 < kept; i0 += kBatch) {
+            uint4 v[kBatch];
+#pragma unroll
+            for (uint32_t i = 0; i < kBatch; ++i)
+                if (i0 + i < kept && l.from[i0 + i] != kNowhere) v[i] = *reinterpret_cast<const uint4*>(pool + l.from[i0 + i]);
+#pragma unroll
+            for (uint32_t i = 0; i < kBatch; ++i)
+                if (i0 + i < kept && l.from[i0 + i] != kNowhere) *reinterpret_cast<uint4*>(pool + l.to[i0 + i]) = v[i];
+        }
+    }
+}
+// Pages of a request, of len positions, that its accepted ones do not reach: the first, how many.
+struct Spare {
+    uint32_t low, n;
+};
+__device__ __forceinline__ Spare spare_of(const Move& a, const Rows& r, uint32_t len, uint32_t kept)
+{
+    if (r.n == 0 || r.n > 32 * a.words || len < r.all) return Spare{0, 0};
+    const uint32_t size = 1u << a.shift;
+    const uint32_t low = uint32_t((uint64_t(len - r.all + kept) + size - 1) >> a.shift);
+    const uint32_t end = min(uint32_t((uint64_t(len) + size - 1) >> a.shift), a.max_pages);
+    return Spare{low, end > low ? end - low : 0};
+}
+
+// A workgroup to a request and layer; that of one more layer number returns the pages.
+__global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
+{
     const uint32_t tid = threadIdx.x, layer = blockIdx.y;
     if (layer < a.layers) {
-        __shared__ uint64_t from[kMaxNodes], to[kMaxNodes];  // byte offsets; kNowhere: the row stays
-        constexpr uint64_t kNowhere = ~0ull;
+        __shared__ MoveSpace l;
         const uint32_t b = blockIdx.x;
         if (b >= a.requests) return;
         const Rows r = rows_of(a.starts, a.tokens, b);
         const uint32_t held = a.held[b], kept = a.counts[b];
         if (r.n == 0 || r.n > 32 * a.words || held < r.all || kept < 2) return;
-        const uint32_t base = held - r.all, width = a.row_bytes / 16;
-        for (uint32_t i = tid; i < kept; i += 256) {
-            const uint32_t node = a.path[r.first + i];
-            uint64_t to_at, from_at;
-            const bool moves = node != i && place_of(a, b, base + i, to_at) && place_of(a, b, base + node, from_at);
-            from[i] = moves ? from_at : kNowhere;
-            to[i] = to_at;
-        }
-        __syncthreads();
-        for (uint32_t c = tid; c < 2 * width; c += 256) {
-            uint8_t* pool = static_cast<uint8_t*>(c < width ? layers.k[layer] : layers.v[layer]) + (c < width ? c : c - width) * 16;
-            for (uint32_t i0 = 1; i0 < kept; i0 += kBatch) {
-                uint4 v[kBatch];
-#pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i)
-                    if (i0 + i < kept && from[i0 + i] != kNowhere) v[i] = *reinterpret_cast<const uint4*>(pool + from[i0 + i]);
-#pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i)
-                    if (i0 + i < kept && from[i0 + i] != kNowhere) *reinterpret_cast<uint4*>(pool + to[i0 + i]) = v[i];
-            }
-        }
+        move_rows(a, layers, layer, b, held - r.all, kept, l, [&](uint32_t i) { return a.path[r.first + i]; });
         return;
     }
     if (blockIdx.x || !a.free_pages) return;
@@ -272,16 +310,9 @@ __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
     uint32_t count = *a.free_count;
     for (uint32_t b0 = 0; b0 < a.requests; b0 += 256) {
         const uint32_t b = b0 + tid;
-        uint32_t low = 0, back = 0;
-        if (b < a.requests) {
-            const Rows r = rows_of(a.starts, a.tokens, b);
-            const uint32_t len = a.held[b], size = 1u << a.shift;
-            if (r.n && r.n <= 32 * a.words && len >= r.all) {
-                low = uint32_t((uint64_t(len - r.all + a.counts[b]) + size - 1) >> a.shift);
-                back = min(uint32_t((uint64_t(len) + size - 1) >> a.shift), a.max_pages);
-                back = back > low ? back - low : 0;
-            }
-        }
+        Spare spare{0, 0};
+        if (b < a.requests) spare = spare_of(a, rows_of(a.starts, a.tokens, b), a.held[b], a.counts[b]);
+        const uint32_t low = spare.low, back = spare.n;
         uint32_t inc = back;  // sums of the requests up to this one
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t v = uint32_t(__shfl_up(int(inc), d));
@@ -299,6 +330,28 @@ __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
         __syncthreads();
     }
     if (tid == 0) *a.free_count_out = min(count, a.list_pages);
+}
+
+// The step's end of one request where lens_out is not lens, in one launch: each layer's workgroup walks for itself, the last one
+// writes what the call gives and returns the pages.  28 layers after a tree of 26 nodes: 6.7 us, 9.3 in two launches.
+__global__ __launch_bounds__(256) void k_tree_one(Walk w, Move a, Layers layers)
+{
+    __shared__ WalkSpace l;
+    __shared__ MoveSpace at;
+    const uint32_t tid = threadIdx.x, layer = blockIdx.x;
+    const bool writes = layer == a.layers;
+    const Rows r = rows_of(w.starts, w.tokens, 0);
+    const uint32_t len = w.lens[0], count = writes && a.free_pages ? *a.free_count : 0;
+    const uint32_t kept = walk(w, 0, r, len, writes, l);  // a barrier in it: all have read the count
+    if (!writes) {
+        if (kept > 1 && len >= r.all) move_rows(a, layers, layer, 0, len - r.all, kept, at, [&](uint32_t i) { return l.path[i]; });
+        return;
+    }
+    if (!a.free_pages) return;
+    const Spare spare = spare_of(a, r, len, kept);
+    for (uint32_t i = tid; i < spare.n; i += 256)
+        if (count + i < a.list_pages) a.free_pages[count + i] = a.tables[spare.low + i];
+    if (tid == 0) *a.free_count_out = min(count + spare.n, a.list_pages);
 }
 
 // ---------------------------------------------------------------------- host
@@ -449,7 +502,8 @@ int arc_tree_commit(const arc_kv_pages* layers, uint32_t num_layers, const arc_p
     }
     const Walk w{batch->lens, batch->starts, tree->parents, drafts, targets, lens_out, counts, tokens_out, path, held, parts,
                  batch->requests, batch->tokens, tree->mask_words, splits};
-    if (batch->requests) hipLaunchKernelGGL(k_tree_walk, dim3(batch->requests), dim3(256), 0, st, w);
+    const bool one = batch->requests == 1 && lens_out != batch->lens;
+    if (batch->requests && !one) hipLaunchKernelGGL(k_tree_walk, dim3(batch->requests), dim3(256), 0, st, w);
     if (hipError_t e = hipGetLastError()) return check_hip(e, "tree commit");
     const uint32_t row_bytes = layers->kv_heads * layers->head_dim * 2;
     const Move m{batch->tables, held, batch->starts, counts, path, free_pages, free_count_out, free_count,
@@ -460,7 +514,8 @@ int arc_tree_commit(const arc_kv_pages* layers, uint32_t num_layers, const arc_p
         l.k[i] = layers[i].k;
         l.v[i] = layers[i].v;
     }
-    hipLaunchKernelGGL(k_tree_move, dim3(batch->requests ? batch->requests : 1, num_layers + (free_pages ? 1 : 0)), dim3(256), 0, st, m, l);
+    if (one) hipLaunchKernelGGL(k_tree_one, dim3(num_layers + 1), dim3(256), 0, st, w, m, l);
+    else hipLaunchKernelGGL(k_tree_move, dim3(batch->requests ? batch->requests : 1, num_layers + (free_pages ? 1 : 0)), dim3(256), 0, st, m, l);
     return check_hip(hipGetLastError(), "tree commit");
 }
 

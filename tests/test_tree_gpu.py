@@ -407,6 +407,32 @@ def test_commit(name, in_place):
     run.check(run.run(in_place=in_place))
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("name", ["chunk", "empty", "single row", "chain", "page 1", "wide heads", "layers", "strides", "rows behind", "without room", "no list"])
+def test_commit_of_one_request(name, in_place):
+    rng = rng_of(30)
+    kw = dict(chunk=dict(words=1), chain=dict(agree=0.97), layers=dict(layers=64), strides=dict(stride_pad=24, page=32), empty=dict(rows=3))
+    kw["page 1"], kw["wide heads"], kw["rows behind"] = dict(page=1), dict(kv_heads=40, dim=128, layers=3, dtype=arc.BF16), dict(rows=9)
+    kw["without room"] = kw["no list"] = dict(agree=0.1, page=4)
+    shape = dict(chunk=70, empty=[], chain=tl.chain(200)).get(name, tl.chain(1) if name == "single row" else tl.random_tree(rng, 60))
+    run = CommitRun([37], [shape], seed=31, **kw.get(name, {}))
+    if name == "no list":
+        run.check(run.run(in_place=in_place, free_list=False), free_list=False)
+    elif name == "without room":
+        run.check(run.run(in_place=in_place, num_pages=run.count + 5), num_pages=run.count + 5)
+    else:
+        run.check(run.run(in_place=in_place))
+
+
+def test_commit_of_one_request_from_logits():
+    run = CommitRun([37], [tl.random_tree(rng_of(32), 60)], seed=32, vocab=1003, agree=0.8)
+    logits = rng_of(33).standard_normal((run.rows, 1003)).astype(np.float32)
+    logits[np.arange(run.rows), run.targets[: run.rows]] = 50.0
+    got = run.run(logits=logits, ldl=1003)
+    assert np.array_equal(got["targets"][: run.rows], run.targets[: run.rows])
+    run.check(got)
+
+
 def test_commit_without_a_free_list():
     run = CommitRun([20, 9], trees(rng_of(22), [30, 12]), seed=22)
     got = run.run(free_list=False)
