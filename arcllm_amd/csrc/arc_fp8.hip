@@ -798,10 +798,11 @@ __global__ __launch_bounds__(512, 2) void k_fp8_own(Gemm a)
 // first two, by the others; half of w's and all of x's operands are in registers at once, and each is replaced when its
 // last product has begun.  In the third quarter all of the block is in registers: there stands its one barrier, behind which
 // the next block but one is copied over it and the next one's first operands are read.  All blocks are whole (K a multiple of 128).
-// Tiles of 256: 4096 rows of 18944 x 3584 with the activation 530 us, 2.1 PFLOP/s; 8192 x 8192 x 8192 2.3.  Next to the products, which busy
-// the cores for 2048 cycles a block, LDS serves 192 KB of operands and 64 KB of copies, 2048 cycles too: 16 KB of w and 8 of x to a
-// wave of 64 x 128 outputs.  Wider waves would read less, but the sums' 128 registers cannot grow: multiply-adds
-// take no operand from the other half of the register file.
+// Tiles of 256: 4096 rows of 18944 x 3584 with the activation 530 us, 2.1 PFLOP/s; 8192 x 8192 x 8192 2.3.  Products and their
+// multiply-adds alone reach 3.4 in a loop, at the clock that their power leaves.  Here the cores are busy for 51 % of the
+// cycles, at 1.8 GHz, LDS for 22 %, without conflicts; without the copies it would take 20 % less time, without the reads of
+// LDS 15 %.  A third place for blocks does not fit in LDS; copies begun earlier or all at once were slower (535 to 569 us), and so
+// was a last round of tiles cut in parts (536, and 95 instead of 87 for 4608 x 3584).
 template <typename Y, typename C>
 __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
 {
@@ -858,6 +859,8 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
     // same, from LDS as it is.
     auto step = [&](Stream<C>& stream, uint64_t next, uint64_t behind, uint32_t buf) {
         constexpr int kRead = 6 * H - 2;  // from here on the block's LDS is read no more
+        constexpr int kEvery = SLOTS >= 32 ? 2 : 1;
+        static_assert(C::kFirst * kEvery <= SLOTS - kRead && (C::COPIES - C::kFirst) * kEvery <= kRead, "each copy has its place");
 #pragma unroll
         for (int q = 0; q < SLOTS; ++q) {
             // the next block's copies have arrived, everyone's; this one is read
@@ -869,7 +872,6 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
             if (q == kRead || q == kRead + 1) read_x(buf ^ 1u, q - kRead);
             if (q > 6 * H && q % 2 && q < SLOTS - 1) read_w(buf ^ 1u, (q - 6 * H) / 2);
             if (q >= SLOTS - WM - G) read_scale(buf ^ 1u, q - (SLOTS - WM - G));
-            constexpr int kEvery = SLOTS >= 32 ? 2 : 1;
             if (q % kEvery == 0 && q / kEvery < int(C::COPIES - C::kFirst)) stream.one(next, C::kFirst + q / kEvery, buf ^ 1u);
             if (q >= kRead && (q - kRead) % kEvery == 0 && (q - kRead) / kEvery < int(C::kFirst)) stream.one(behind, (q - kRead) / kEvery, buf);
             if (q == LAG) set_scales();
