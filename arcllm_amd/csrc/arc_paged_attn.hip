@@ -131,19 +131,25 @@ __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, u
     r.rows = rows;
     r.base = int32_t(max(base, -(int64_t(1) << 25)));
     r.tiles = (rows + bm - 1) / bm;
-    r.first = double(ends + uint32_t(max(r.base, 0))) * a.hpk + bm;
-    const uint32_t nodes = TREE && is_tree(a, r) ? rows : 0;  // the tree lies behind the first node's window
+    const bool tree = TREE && is_tree(a, r);  // a step of chunks alone is cut as paged attention cuts it
+    // Trees over contexts that a workgroup takes in one turn cost the same, and a part (see below) is no less than one of their
+    // tiles: parts then begin where tiles do.  64 of 3 nodes at 30 positions, 28 heads, 11.5 us; else in pieces, 38.
+    constexpr uint32_t kTurn = FEW ? kFewWaves * kFewKeys : kManyKeys;
+    const uint32_t old = uint32_t(max(r.base, 0));
+    r.first = double(ends + (tree ? max(old, kTurn) : old)) * a.hpk + bm;
+    const uint32_t nodes = tree ? rows : 0;  // the tree lies behind the first node's window
     r.cap = a.window ? (double(ends) + a.window + a.sinks) * a.hpk + nodes + 2 * bm : 0x1p60;
     r.total = r.tiles == 1 ? fmin(r.first, r.cap) : cost_before(r, r.tiles, bm);
     const float spans = float(r.tiles) * ceilf(float(len) * (1.0f / keys));
     r.units = a.window ? fminf(spans, float(r.tiles) * (ceilf((float(a.window) + float(a.sinks) + float(nodes / a.hpk)) * (1.0f / keys)) + 2.0f)) : spans;
-    if (TREE && !FEW) {
+    if (tree && !FEW) {
         // up to 8 pieces of a tile are joined in the quicker way, worth some 3 units: 26 nodes at 501 positions, 28 heads on 4,
         // 15.2 us (a part to each unit 18.5); 60 nodes 19.6 (27.4); at 1700 18.4 (21.0); 32 heads of 64 on 8 at 1000 13.4 (18.1);
         // from 33 units on a unit a part is as quick or quicker
         const float each = r.units * __builtin_amdgcn_rcpf(float(r.tiles));
         if (each > 8.0f && each < 32.5f) r.units = float(r.tiles) * fmaxf(6.0f, ceilf(each * 0.25f - 0.01f));
     }
+    if (tree && FEW) r.units = fmaxf(r.units, float(kFewWaves) * float(r.tiles));
     r.units = fmaxf(r.units, 1.0f);
     return r;
 }

@@ -262,6 +262,13 @@ def test_many_trees(dtype):
     check(old, [tl.random_tree(rng, int(n)) for n in rng.integers(1, 12, 300)], kv_heads=1, hpk=7, dtype=dtype)
 
 
+@pytest.mark.parametrize("kv_heads,hpk", [(1, 4), (4, 7)])
+@pytest.mark.parametrize("most", [0, 3, 130])
+def test_many_short_contexts(most, kv_heads, hpk):
+    rng = rng_of(11, most)
+    check(rng.integers(0, most + 1, 41).tolist(), [tl.random_tree(rng, int(n)) for n in rng.integers(1, 5, 41)], kv_heads=kv_heads, hpk=hpk)
+
+
 def test_many_requests_of_one_row_and_few_trees():
     rng = rng_of(16)
     shapes = [tl.chain(1)] * 150
