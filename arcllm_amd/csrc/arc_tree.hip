@@ -152,22 +152,30 @@ struct WalkSpace {
 __device__ __forceinline__ uint32_t walk(const Walk& a, uint32_t b, const Rows& r, uint32_t len, bool writes, WalkSpace& l)
 {
     const uint32_t tid = threadIdx.x;
-    auto said_after = [&](uint32_t i) {
-        if (!a.splits) return a.targets[r.first + i];
-        Best best{-INFINITY, kNoToken};
-        for (uint32_t s = 0; s < a.splits; ++s) best = better(best, a.parts[uint64_t(r.first + i) * a.splits + s]);
-        const uint32_t token = best.idx == kNoToken ? 0u : best.idx;
-        if (writes) a.targets[r.first + i] = token;
-        return token;
+    // f(i, the target's token after row i), by one lane for each row: from targets, or as many lanes as a row's logits have
+    // parts take one of them each
+    auto said_after = [&](auto f) {
+        if (!a.splits) {
+            for (uint32_t i = tid; i < r.n; i += 256) f(i, a.targets[r.first + i]);
+            return;
+        }
+        const uint32_t part = tid & (a.splits - 1);
+        for (uint32_t i = tid / a.splits; i < r.n; i += 256 / a.splits) {
+            Best best = a.parts[uint64_t(r.first + i) * a.splits + part];
+            for (uint32_t d = a.splits >> 1; d; d >>= 1) best = better(best, Best{__shfl_xor(best.val, int(d)), uint32_t(__shfl_xor(int(best.idx), int(d)))});
+            if (part) continue;
+            const uint32_t token = best.idx == kNoToken ? 0u : best.idx;
+            if (writes) a.targets[r.first + i] = token;
+            f(i, token);
+        }
     };
     if (r.n == 0 || r.n > 32 * a.words) {
         __syncthreads();  // everyone has read lens
         if (!writes) return 0;
-        for (uint32_t i = tid; i < r.n; i += 256) {
-            const uint32_t token = said_after(i);
+        said_after([&](uint32_t i, uint32_t token) {
             if (i) a.tokens_out[r.first + i] = kNoToken;
             if (i + 1 == r.n) a.tokens_out[r.first] = token;
-        }
+        });
         if (tid == 0) {
             a.counts[b] = r.n ? 1 : 0;
             a.lens_out[b] = len;
@@ -177,8 +185,8 @@ __device__ __forceinline__ uint32_t walk(const Walk& a, uint32_t b, const Rows& 
     for (uint32_t i = tid; i < r.n; i += 256) {
         l.parent[i] = a.parents[r.first + i];
         l.draft[i] = a.drafts[r.first + i];
-        l.said[i] = said_after(i);
     }
+    said_after([&](uint32_t i, uint32_t token) { l.said[i] = token; });
     __syncthreads();
     if (tid < 64) {
         uint32_t node = 0, n = 0;
@@ -259,7 +267,7 @@ __device__ __forceinline__ void move_rows(const Move& a, const Layers& layers, u
     const uint32_t tid = threadIdx.x, width = a.row_bytes / 16;
     for (uint32_t i = tid; i < kept; i += 256) {
         const uint32_t n = node(i);
-        uint64_t to_at, from_at;
+        uint64_t to_at = 0, from_at = 0;
         const bool moves = n != i && place_of(a, b, base + i, to_at) && place_of(a, b, base + n, from_at);
         l.from[i] = moves ? from_at : kNowhere;
         l.to[i] = to_at;
@@ -387,7 +395,7 @@ bool shared(const Array (&written)[W], const Array (&read)[R])
     return false;
 }
 
-// Parts of a row of logits: enough workgroups to fill the card.
+// Parts of a row of logits, a power of two: enough workgroups to fill the card, and a few KB or more to each.
 uint32_t splits_of(uint32_t tokens)
 {
     uint32_t s = 1;
@@ -491,7 +499,8 @@ int arc_tree_commit(const arc_kv_pages* layers, uint32_t num_layers, const arc_p
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint32_t *path = reinterpret_cast<uint32_t*>(ws), *held = reinterpret_cast<uint32_t*>(ws + sp.held);
     Best* parts = reinterpret_cast<Best*>(ws + sp.parts);
-    const uint32_t splits = logits ? splits_of(batch->tokens) : 0;
+    uint32_t splits = logits ? splits_of(batch->tokens) : 0;
+    while (splits > 1 && vocab / splits < 4096) splits /= 2;
     if (splits && batch->requests && batch->tokens) {
         const Argmax a{logits, batch->starts, parts, ldl, batch->requests, batch->tokens, vocab, splits};
         const dim3 grid(batch->tokens * splits), block(256);
