@@ -78,8 +78,8 @@ struct Quantize {
 };
 
 // 16 lanes to a block, 8 values a lane; a wave has 4 blocks of a row, a workgroup those 4 of 32 rows, whose scales go
-// out through LDS so that they are written in whole lines.  Bound by HBM: 4096 rows of 18944 in bf16, 42 us, 5.6 TB/s of reads and
-// writes (a copy of 1 GB: 5.15); one row of 3584, 3.6 us, the launch.
+// out through LDS so that they are written in whole lines.  Bound by HBM: 4096 rows of 18944 in bf16, 48 us, 4.9 TB/s of reads and
+// writes (42 with inputs of which the last cache holds a part; a copy of 1 GB: 5.15 TB/s); one row of 3584, 3.6 us, the launch.
 constexpr uint32_t kQuantRows = 32;
 template <typename X>
 __global__ __launch_bounds__(256) void k_fp8_quantize(Quantize a)

@@ -1088,11 +1088,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 // clock under the matrix cores' power is what is left.  3 x 2000 tokens in a window of 1024, heads of 64: 137 to
 // 146 us, 0.5 PFLOP/s, bound by the softmax's vector instructions, as many per score as heads of 128 have for twice the
 // products.
-// Trees: 48 of up to 60 nodes at up to 8000, 28 heads of 128 on 4, 129 us; of up to 9 nodes 59.  A unit takes a wave 1.5 us
+// Trees: 48 of up to 60 nodes at up to 8000, 28 heads of 128 on 4, 124 us; of up to 9 nodes 58.  A unit takes a wave 1.5 us
 // however many of the waves have rows, so what bounds it is the units of tiles that are not full; waves without rows
 // only copy.  Not quicker: tiles of 128 rows, two workgroups to a compute unit (133 us: each unit copied more often);
 // two waves to 32 rows of a tile that is half empty, each with half a unit's positions (182 us: 59 registers too
-// many).  One tree of 26 nodes at 501: 15.2 us, of which the join is 4.
+// many).  One tree of 26 nodes at 501: 15.2 us, of which the join is 3.
 template <typename T, int D, int NW, bool WIDE, bool TREE>
 __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAttn)
 {
