@@ -309,6 +309,62 @@ def test_two_captured_steps_side_by_side():
             assert torch.equal(getattr(s, name), getattr(c, name)), name
 
 
+@pytest.mark.parametrize("logits", [False, True])
+def test_captured_commit_of_one_request(logits):
+    """One request's step end with lens_out apart from lens, captured once and replayed with other drafts, trees and
+    lengths: each replay equals the eager call on a second set of buffers."""
+    rng = np.random.default_rng(SEED + 4)
+    n, layers, vocab = 40, 5, 50
+
+    class Side:
+        def __init__(self):
+            self.kv = [[torch.arange(20 * PAGE * KV * DIM, device="cuda").remainder(2000 + 7 * i + j).half().view(20, PAGE, KV, DIM) for j in range(2)]
+                       for i in range(layers)]
+            self.tables = torch.randperm(20, generator=torch.Generator().manual_seed(1)).int().cuda().view(1, 20)
+            self.lens, self.starts = i32(1), i32(2)
+            self.parents, self.drafts, self.targets, self.tokens = i32(n), i32(n), i32(n), i32(n)
+            self.lens_out, self.counts, self.stack, self.count, self.count_out = i32(1), i32(1), i32(20), i32(1, fill=2), i32(1)
+            self.logits = torch.zeros(n, vocab, device="cuda")
+            self.pages = [arc.KvPages(p(k), p(v), 20, PAGE, KV, DIM, arc.F16) for k, v in self.kv]
+            self.batch = arc.PagedBatch(1, n, 20, n, p(self.tables), p(self.lens), p(self.starts))
+            self.ws = torch.full((arc.tree_commit_workspace_bytes(self.batch),), 255, dtype=torch.uint8, device="cuda")
+
+        def commit(self):
+            more = dict(logits=p(self.logits), ldl=vocab, vocab=vocab) if logits else {}
+            arc.tree_commit(self.pages, self.batch, arc.Tree(p(self.parents), None, 2), p(self.drafts), p(self.targets), p(self.lens_out),
+                            p(self.counts), p(self.tokens), p(self.ws), free_pages=p(self.stack), num_pages=20, free_count=p(self.count),
+                            free_count_out=p(self.count_out), stream=TorchStream(), **more)
+
+    a, b = Side(), Side()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a.commit()
+    torch.cuda.synchronize()
+    moved = 0
+    for rows in (40, 33, 1, 40):
+        parents = tl.random_tree(rng, rows) + [tl.NONE] * (n - rows)
+        said = rng.integers(0, vocab, n)
+        drafts = [int(said[q]) if q < i and rng.random() < 0.9 else 3 for i, q in enumerate(parents)]
+        x = rng.standard_normal((n, vocab)).astype(np.float32)
+        x[np.arange(n), said] = 9.0
+        length = int(rng.integers(0, 20 * PAGE - n)) + rows
+        for s in (a, b):
+            for dst, src in ((s.parents, np.array(parents, np.uint32).view(np.int32)), (s.drafts, np.array(drafts, np.int32)),
+                             (s.targets, said.astype(np.int32)), (s.lens, np.array([length], np.int32)), (s.starts, np.array([0, rows], np.int32)),
+                             (s.logits, x)):
+                dst.copy_(torch.from_numpy(src))
+        b.commit()
+        g.replay()
+        torch.cuda.synchronize()
+        for name in ("lens_out", "counts", "tokens", "targets", "stack", "count_out"):
+            assert torch.equal(getattr(a, name), getattr(b, name)), name
+        assert all(torch.equal(x, y) for u, v in zip(a.kv, b.kv) for x, y in zip(u, v))
+        assert 1 <= int(a.counts) <= rows and int(a.lens_out) == length - rows + int(a.counts)
+        moved += int(a.counts) - 1
+    assert moved > 0
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_a_chain_is_a_chunk(dim):
     """A tree that is a chain sees what a causal chunk sees: tree attention of both, and paged attention, on the same rows."""
