@@ -299,7 +299,7 @@ __device__ __forceinline__ Spare spare_of(const Move& a, const Rows& r, uint32_t
     return Spare{low, end > low ? end - low : 0};
 }
 
-// A workgroup to a request and layer; that of one more layer number returns the pages.
+// A workgroup to a request and layer; that of one more layer number returns the pages, table entries that are none left out.
 __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
 {
     const uint32_t tid = threadIdx.x, layer = blockIdx.y;
@@ -320,7 +320,9 @@ __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
         const uint32_t b = b0 + tid;
         Spare spare{0, 0};
         if (b < a.requests) spare = spare_of(a, rows_of(a.starts, a.tokens, b), a.held[b], a.counts[b]);
-        const uint32_t low = spare.low, back = spare.n;
+        const uint32_t* pages = a.tables + uint64_t(b) * a.max_pages + spare.low;
+        uint32_t back = 0;
+        for (uint32_t i = 0; i < spare.n; ++i) back += pages[i] < a.num_pages;
         uint32_t inc = back;  // sums of the requests up to this one
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t v = uint32_t(__shfl_up(int(inc), d));
@@ -328,13 +330,17 @@ __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
         }
         if ((tid & 63u) == 63) sums[tid >> 6] = inc;
         __syncthreads();
-        uint32_t before = count + inc - back;
+        uint32_t at = count + inc - back;
         for (uint32_t w = 0; w < 4; ++w) {
-            if (w < (tid >> 6)) before += sums[w];
+            if (w < (tid >> 6)) at += sums[w];
             count += sums[w];
         }
-        for (uint32_t i = 0; i < back; ++i)
-            if (before + i < a.list_pages) a.free_pages[before + i] = a.tables[uint64_t(b) * a.max_pages + low + i];
+        for (uint32_t i = 0; i < spare.n; ++i) {
+            const uint32_t page = pages[i];
+            if (page >= a.num_pages) continue;
+            if (at < a.list_pages) a.free_pages[at] = page;
+            ++at;
+        }
         __syncthreads();
     }
     if (tid == 0) *a.free_count_out = min(count, a.list_pages);
@@ -349,17 +355,31 @@ __global__ __launch_bounds__(256) void k_tree_one(Walk w, Move a, Layers layers)
     const uint32_t tid = threadIdx.x, layer = blockIdx.x;
     const bool writes = layer == a.layers;
     const Rows r = rows_of(w.starts, w.tokens, 0);
-    const uint32_t len = w.lens[0], count = writes && a.free_pages ? *a.free_count : 0;
+    const uint32_t len = w.lens[0];
+    uint32_t count = writes && a.free_pages ? *a.free_count : 0;
     const uint32_t kept = walk(w, 0, r, len, writes, l);  // a barrier in it: all have read the count
     if (!writes) {
         if (kept > 1 && len >= r.all) move_rows(a, layers, layer, 0, len - r.all, kept, at, [&](uint32_t i) { return l.path[i]; });
         return;
     }
     if (!a.free_pages) return;
+    __shared__ uint32_t sums[4];
     const Spare spare = spare_of(a, r, len, kept);
-    for (uint32_t i = tid; i < spare.n; i += 256)
-        if (count + i < a.list_pages) a.free_pages[count + i] = a.tables[spare.low + i];
-    if (tid == 0) *a.free_count_out = min(count + spare.n, a.list_pages);
+    const uint32_t lane = tid & 63u, wave = tid >> 6;
+    for (uint32_t i = 0; i < spare.n; i += 256) {
+        const uint32_t page = i + tid < spare.n ? a.tables[spare.low + i + tid] : kNoToken;
+        const uint64_t back = __ballot(page < a.num_pages);
+        if (lane == 0) sums[wave] = uint32_t(__builtin_popcountll(back));
+        __syncthreads();
+        uint32_t place = count + uint32_t(__builtin_popcountll(back & ((1ull << lane) - 1u)));
+        for (uint32_t w = 0; w < 4; ++w) {
+            if (w < wave) place += sums[w];
+            count += sums[w];
+        }
+        if (page < a.num_pages && place < a.list_pages) a.free_pages[place] = page;
+        __syncthreads();
+    }
+    if (tid == 0) *a.free_count_out = min(count, a.list_pages);
 }
 
 // ---------------------------------------------------------------------- host

@@ -462,8 +462,8 @@ int arc_tree_attention(const arc_kv_pages *pages, const arc_paged_batch *batch, 
  *   lens_out[b] = lens[b] - rows + k (lens_out may be lens);
  *   in each of the layers' pools, node i-th on the way moves to place i behind the context, K and V;
  *   pages that held only other nodes go onto the free list (a stack as arc_paged_plan's, of room for
- *   num_pages; NULL: they stay with the request), requests in order, first page to last.  free_count_out may
- *   be free_count.
+ *   num_pages; NULL: they stay with the request), requests in order, first page to last; table entries that are no
+ *   page of the pool do not, and what finds no room on the list is on none.  free_count_out may be free_count.
  * A chunk counts 1 (the target's token after its last row), keeps all its positions and moves nothing; a
  * request without rows counts 0.  layers: 1 .. ARC_MAX_LAYERS pools of one shape (host array), none of them
  * twice; what is written shares no memory with another array but where it may be one of them.  A position whose page
