@@ -1055,6 +1055,19 @@ Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
     return best;
 }
 
+// The most workspace that products of up to M rows take.  Up to 64 rows a plan depends on the number of 16 rows, beyond on that of
+// 128, so one of each is asked.  Of a product cut in parts the sums' way alone, bytes / 3e6 us, is less than what cutting can
+// save, the tiles' last round: two * (blocks + 4) us at most (`two` <= 2.1, with some room 7e6 for 3e6 * 2.1); in two parts
+// or more, so beyond these many rows none is cut.
+size_t most_bytes(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
+{
+    const uint64_t sums = 7000000ull * ((K + kFpBlock - 1) / kFpBlock + 4);
+    const uint32_t end = uint32_t(std::min<uint64_t>(M, sums / (8ull * N * (gated ? 2 : 1)) + 256));
+    size_t most = plan_of(N, K, M, gated, fast).bytes;
+    for (uint32_t m = 16; m < end; m += m < 64 ? 16 : m < 128 ? 64 : 128) most = std::max(most, plan_of(N, K, m, gated, fast).bytes);
+    return most;
+}
+
 template <typename Y, typename C>
 hipError_t launch_tile(const Gemm& a, hipStream_t st)
 {
@@ -1178,8 +1191,7 @@ int arc_fp8_quantize(int x_dtype, const void* x, uint32_t ldx, const arc_fp8_row
 size_t arc_fp8_gemm_workspace_bytes(uint32_t N, uint32_t K, uint32_t M, int gated)
 {
     if (N == 0 || N > kMaxRows || M > kMaxRows || K == 0 || K % 16 || K > kMaxLd) return 0;
-    const size_t fast = plan_of(N, K, M, gated != 0, true).bytes, wide = plan_of(N, K, M, gated != 0, false).bytes;
-    return fast > wide ? fast : wide;
+    return std::max(most_bytes(N, K, M, gated != 0, true), most_bytes(N, K, M, gated != 0, false));
 }
 
 int arc_fp8_gemm(const arc_fp8_weights* w, const arc_fp8_rows* x, int y_dtype, void* y, uint32_t ldy, const void* residual, uint32_t ldr,

@@ -505,8 +505,9 @@ int arc_fp8_quantize(int x_dtype, const void *x, uint32_t ldx, const arc_fp8_row
  * NULL, or y itself; otherwise y shares no memory with what is read.  Sums are fp32, rounded once.  A y of 16 bits may lose of each 8
  * neighbouring products what lies below 2^-13 of their largest (1.3e-5 of y for normal data), an fp32 one
  * does not.  Products of scales that leave fp32's normal range do not keep their bits.
- * workspace: arc_fp8_gemm_workspace_bytes(w->rows, w->cols, x->rows, 0) bytes (fewer rows may need more),
- * 256-byte aligned, any contents, for one call at a time.  No rows: nothing is done. */
+ * workspace: arc_fp8_gemm_workspace_bytes(w->rows, w->cols, rows, 0) bytes for some rows >= x->rows (what it
+ * gives serves any call of these weights and up to so many rows), 256-byte aligned, any contents, for one call at a
+ * time.  No rows: nothing is done. */
 size_t arc_fp8_gemm_workspace_bytes(uint32_t n, uint32_t k, uint32_t rows, int gated);
 int arc_fp8_gemm(const arc_fp8_weights *w, const arc_fp8_rows *x, int y_dtype, void *y, uint32_t ldy, const void *residual,
                  uint32_t ldr, void *workspace, arc_stream_t stream);
