@@ -423,9 +423,21 @@ uint32_t splits_of(uint32_t tokens)
     return s;
 }
 
-// Where a commit's workspace holds what.
+// The most parts that logits of up to `tokens` rows are read in: rows of one number of parts end where 2048 are
+// reached with half of it.
+size_t most_parts(uint32_t tokens)
+{
+    size_t most = size_t(tokens) * splits_of(tokens);
+    for (uint32_t s = 64; s > 1; s /= 2) {
+        const uint32_t n = 4096 / s - 1;
+        if (n <= tokens) most = std::max(most, size_t(n) * splits_of(n));
+    }
+    return most;
+}
+
+// Where a commit's workspace holds what: `bytes` of a step of these rows, `most` of any of fewer too.
 struct Space {
-    size_t held, parts, bytes;
+    size_t held, parts, bytes, most;
 };
 Space space_of(const arc_paged_batch* b)
 {
@@ -434,6 +446,7 @@ Space space_of(const arc_paged_batch* b)
     s.held = up(b->tokens * sizeof(uint32_t));
     s.parts = s.held + up(b->requests * sizeof(uint32_t));
     s.bytes = s.parts + up((size_t(b->tokens) * splits_of(b->tokens) + 1) * sizeof(Best));
+    s.most = s.parts + up((most_parts(b->tokens) + 1) * sizeof(Best));
     return s;
 }
 
@@ -463,7 +476,7 @@ int arc_tree_plan(const arc_paged_batch* batch, const arc_tree* tree, arc_stream
 
 size_t arc_tree_commit_workspace_bytes(const arc_paged_batch* batch)
 {
-    return check_batch_sizes(batch) ? 0 : space_of(batch).bytes;
+    return check_batch_sizes(batch) ? 0 : space_of(batch).most;
 }
 
 int arc_tree_commit(const arc_kv_pages* layers, uint32_t num_layers, const arc_paged_batch* batch, const arc_tree* tree, int logits_dtype,

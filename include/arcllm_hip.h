@@ -467,8 +467,8 @@ int arc_tree_attention(const arc_kv_pages *pages, const arc_paged_batch *batch, 
  * A chunk counts 1 (the target's token after its last row), keeps all its positions and moves nothing; a
  * request without rows counts 0.  layers: 1 .. ARC_MAX_LAYERS pools of one shape (host array), none of them
  * twice; what is written shares no memory with another array but where it may be one of them.  A position whose page
- * is none of the pool does not move.  workspace: arc_tree_commit_workspace_bytes() bytes (fewer rows may need
- * more), 256-byte aligned, as arc_paged_attention's.  Of the batch, all but positions, slots and max_new is used. */
+ * is none of the pool does not move.  workspace: arc_tree_commit_workspace_bytes() bytes of a batch of no fewer requests
+ * and rows, 256-byte aligned, as arc_paged_attention's.  Of the batch, all but positions, slots and max_new is used. */
 size_t arc_tree_commit_workspace_bytes(const arc_paged_batch *batch);
 int arc_tree_commit(const arc_kv_pages *layers, uint32_t num_layers, const arc_paged_batch *batch, const arc_tree *tree,
                     int logits_dtype, const void *logits, uint64_t ldl, uint32_t vocab, const uint32_t *drafts,
