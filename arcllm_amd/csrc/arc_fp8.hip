@@ -994,6 +994,15 @@ int check_weights(const arc_fp8_weights* w, const arc_fp8_rows* x)
         return set_error(ARC_ERR_INVALID_ARGUMENT, "weights: lds %u is less than the blocks of %u columns", w->lds, w->cols);
     return ARC_OK;
 }
+Rows2d values_of(const void* p, uint32_t rows, uint32_t cols, uint32_t ld) { return Rows2d{p, rows, cols, ld}; }
+Rows2d weight_scales_of(const arc_fp8_weights& w)
+{
+    return Rows2d{w.scales, (w.rows + kFpBlock - 1) / kFpBlock, (w.cols + kFpBlock - 1) / kFpBlock * sizeof(float), w.lds * sizeof(float)};
+}
+Rows2d row_scales_of(const arc_fp8_rows& x)
+{
+    return Rows2d{x.scales, (x.cols + kFpBlock - 1) / kFpBlock, x.rows * sizeof(float), x.lds * sizeof(float)};
+}
 uint32_t bytes_of(int dtype) { return dtype == ARC_F32 ? 4 : dtype == ARC_F16 || dtype == ARC_BF16 ? 2 : 0; }
 
 // Which kernel takes a product, its tiles, and into how many parts their blocks are cut: what is expected to be quickest.
@@ -1125,6 +1134,16 @@ int product(const arc_fp8_weights* w, const arc_fp8_weights* up, bool gated, con
     if (rows_overlap(y, row, uint64_t(ldy) * size, x->q, x->cols, x->ldq, x->rows))
         return set_error(ARC_ERR_INVALID_ARGUMENT, "y and the rows share memory");
     if (x->rows == 0) return ARC_OK;
+    const Plan p = plan_of(N, x->cols, x->rows, gated, size == 2);
+    const Rows2d out{y, x->rows, row, uint64_t(ldy) * size}, sums = bytes_at(workspace, p.splits > 1 ? p.bytes : 0);
+    const Rows2d read[] = {values_of(w->w, N, w->cols, w->ldw), weight_scales_of(*w), gated ? values_of(up->w, N, up->cols, up->ldw) : Rows2d{},
+                           gated ? weight_scales_of(*up) : Rows2d{}, row_scales_of(*x)};
+    for (const Rows2d& r : read)
+        if (overlap(out, r) || overlap(sums, r))
+            return set_error(ARC_ERR_INVALID_ARGUMENT, "y or the workspace and the weights or scales share memory");
+    if (overlap(sums, out) || overlap(sums, Rows2d{residual, x->rows, row, uint64_t(ldr) * size}) ||
+        overlap(sums, values_of(x->q, x->rows, x->cols, x->ldq)))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "the workspace and y, the residual or the rows share memory");
     Gemm a{};
     a.w[0] = static_cast<const uint8_t*>(w->w);
     a.ws[0] = w->scales;
@@ -1149,7 +1168,6 @@ int product(const arc_fp8_weights* w, const arc_fp8_weights* up, bool gated, con
     a.ldy = ldy;
     a.ldr = ldr;
     a.wide = aligned(y, 4 * size) && ldy % 4 == 0 && (!residual || (aligned(residual, 4 * size) && ldr % 4 == 0));
-    const Plan p = plan_of(N, a.K, a.M, gated, size == 2);
     if (uint64_t(p.mtiles) * p.ntiles * p.splits >= (1u << 22))
         return set_error(ARC_ERR_UNSUPPORTED, "%u rows by %u outputs: more tiles than one call takes", a.M, N);
     a.part = static_cast<float*>(workspace);
@@ -1179,6 +1197,10 @@ int arc_fp8_quantize(int x_dtype, const void* x, uint32_t ldx, const arc_fp8_row
     if (rows_overlap(x, uint64_t(out->cols) * size, uint64_t(ldx) * size, out->q, out->cols, out->ldq, out->rows))
         return set_error(ARC_ERR_INVALID_ARGUMENT, "x and the rows share memory");
     if (out->rows == 0) return ARC_OK;
+    const Rows2d scales = row_scales_of(*out);
+    if (overlap(scales, Rows2d{x, out->rows, uint64_t(out->cols) * size, uint64_t(ldx) * size}) ||
+        overlap(scales, values_of(out->q, out->rows, out->cols, out->ldq)))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "the scales and x or the rows share memory");
     const Quantize a{x, static_cast<uint8_t*>(out->q), out->scales, out->rows, out->cols, ldx, out->ldq, out->lds};
     const dim3 grid((out->rows + kQuantRows - 1) / kQuantRows, (out->cols + 511) / 512);
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -5,6 +5,8 @@
 #include "arc_device.hpp"
 #include "../../include/arcllm_hip.h"
 
+#include <utility>
+
 namespace arc {
 
 constexpr uint32_t kMaxRequests = 1u << 20;
@@ -51,6 +53,34 @@ inline bool rows_overlap(const void* a, uint64_t wa, uint64_t sa, const void* b,
     const uint64_t d = (x > y ? x - y : y - x) % sa;  // b's columns behind a's, or a's behind b's
     const uint64_t first = x > y ? wb : wa, second = x > y ? wa : wb;
     return d < first || d + second > sa;
+}
+
+// `rows` rows of `width` bytes, `stride` apart.
+struct Rows2d {
+    const void* p;
+    uint64_t rows, width, stride;
+};
+inline Rows2d bytes_at(const void* p, uint64_t bytes) { return Rows2d{p, bytes ? 1u : 0u, bytes, bytes}; }
+
+// Whether two such arrays share memory, gaps between their rows left out: where both have gaps, the one of fewer rows is
+// looked at row by row (of more than 2^15 rows each, by their spans).
+inline bool overlap(Rows2d a, Rows2d b)
+{
+    if (!a.p || !b.p || !a.rows || !b.rows || !a.width || !b.width) return false;
+    auto begin = [](const Rows2d& r) { return reinterpret_cast<uintptr_t>(r.p); };
+    auto end = [&](const Rows2d& r) { return begin(r) + (r.rows - 1) * r.stride + r.width; };
+    if (end(a) <= begin(b) || end(b) <= begin(a)) return false;
+    if (a.rows > b.rows) std::swap(a, b);
+    if (a.rows > 1 && a.width == a.stride) a = bytes_at(a.p, a.rows * a.stride);
+    if (b.width >= b.stride) b = bytes_at(b.p, end(b) - begin(b));
+    if (a.rows > 1u << 15) return true;
+    for (uint64_t i = 0; i < a.rows; ++i) {
+        const uintptr_t x0 = begin(a) + i * a.stride, x1 = x0 + a.width;
+        // the first row of b that ends behind x0
+        const uint64_t first = x0 < begin(b) + b.width ? 0 : (x0 - begin(b) - b.width) / b.stride + 1;
+        if (first < b.rows && begin(b) + first * b.stride < x1) return true;
+    }
+    return false;
 }
 
 inline uint32_t log2_of(uint32_t pow2) { return uint32_t(__builtin_ctz(pow2)); }

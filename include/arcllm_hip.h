@@ -497,14 +497,16 @@ typedef struct arc_fp8_weights { /* device */
 
 /* Rows of x (x_dtype ARC_F32, ARC_F16 or ARC_BF16, ldx elements from row to row: a multiple of 8; 16-byte
  * aligned) to e4m3: scale = max(largest magnitude of the block / 448, 2^-126), value = x / scale rounded to
- * nearest even.  A block with an infinity or NaN gets scale and values NaN.  x and out share no memory. */
+ * nearest even.  A block with an infinity or NaN gets scale and values NaN.  x and out's arrays share no memory
+ * (refused). */
 int arc_fp8_quantize(int x_dtype, const void *x, uint32_t ldx, const arc_fp8_rows *out, arc_stream_t stream);
 
 /* y[m][n] = sum_k x[m][k] w[n][k] (+ residual[m][n]), x and w with their scales; y and residual of y_dtype
- * (ARC_F32, ARC_F16, ARC_BF16), ldy and ldr elements from row to row (16-byte aligned rows are quickest); residual may be
- * NULL, or y itself; otherwise y shares no memory with what is read.  Sums are fp32, rounded once.  A y of 16 bits may lose of each 8
- * neighbouring products what lies below 2^-13 of their largest (1.3e-5 of y for normal data), an fp32 one
- * does not.  Products of scales that leave fp32's normal range do not keep their bits.
+ * (ARC_F32, ARC_F16, ARC_BF16), ldy and ldr elements from row to row (16-byte aligned rows are quickest); residual
+ * may be NULL, or y itself; otherwise y and the workspace share no memory with what is read or each other
+ * (refused).  Sums are fp32, rounded once.  A y of 16 bits may lose of each 8 neighbouring products what lies
+ * below 2^-13 of their largest (1.3e-5 of y for normal data), an fp32 one does not.  Products of scales that leave
+ * fp32's normal range do not keep their bits.
  * workspace: arc_fp8_gemm_workspace_bytes(w->rows, w->cols, rows, 0) bytes for some rows >= x->rows (what it
  * gives serves any call of these weights and up to so many rows), 256-byte aligned, any contents, for one call at a
  * time.  No rows: nothing is done. */
