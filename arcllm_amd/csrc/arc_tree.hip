@@ -7,6 +7,7 @@
 #include "arc_paged.hpp"
 
 #include <algorithm>
+#include <iterator>
 
 namespace arc {
 namespace {
@@ -394,15 +395,12 @@ int check_tree(const arc_tree* t)
 // Arrays of a call: what it writes must not share memory with what it reads or else writes; `same`: this array may be
 // the input at the same address.
 struct Array {
-    const void* p;
-    uint64_t bytes;
+    Rows2d at;
     const void* same;
+    Array(const void* p, uint64_t bytes, const void* same_ = nullptr) : at(bytes_at(p, bytes)), same(same_) {}
+    explicit Array(const Rows2d& rows) : at(rows), same(nullptr) {}
 };
-bool share(const Array& a, const Array& b)
-{
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-    return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes && !(a.same == b.p && a.p == b.p);
-}
+bool share(const Array& a, const Array& b) { return !(a.same && a.same == b.at.p && a.at.p == b.at.p) && overlap(a.at, b.at); }
 template <size_t W, size_t R>
 bool shared(const Array (&written)[W], const Array (&read)[R])
 {
@@ -414,6 +412,58 @@ bool shared(const Array (&written)[W], const Array (&read)[R])
     }
     return false;
 }
+
+// The K and V of all layers: pools of one shape, whose pages may lie in turns.
+class Pools {
+public:
+    Pools(const arc_kv_pages* layers, uint32_t num_layers)
+        : n_(2 * num_layers), pages_(layers->num_pages), page_(uint64_t(layers->page_size) * layers->kv_heads * layers->head_dim * 2),
+          stride_(layers->page_stride * 2), span_((pages_ - 1) * stride_ + page_)
+    {
+        for (uint32_t i = 0; i < num_layers; ++i) {
+            at_[2 * i] = reinterpret_cast<uintptr_t>(layers[i].k);
+            at_[2 * i + 1] = reinterpret_cast<uintptr_t>(layers[i].v);
+        }
+        std::sort(at_, at_ + n_);
+        for (uint32_t i = 1; i < n_; ++i) apart_ &= at_[i] - at_[i - 1] >= span_;
+    }
+    bool twice() const { return std::adjacent_find(at_, at_ + n_) != at_ + n_; }
+    // Whether two of them share memory.  Those whose ranges meet are told apart by their places in a stride, in one pass
+    // over the sorted places; pairs are only looked at where that leaves a doubt.
+    bool overlap() const
+    {
+        if (apart_) return false;
+        uint64_t place[2 * ARC_MAX_LAYERS + 1];
+        for (uint32_t i = 0; i < n_; ++i) place[i] = at_[i] % stride_;
+        std::sort(place, place + n_);
+        place[n_] = place[0] + stride_;
+        bool clear = true;
+        for (uint32_t i = 0; i < n_; ++i) clear &= place[i + 1] - place[i] >= page_;
+        if (clear) return false;
+        for (uint32_t i = 0; i < n_; ++i)
+            for (uint32_t j = i + 1; j < n_ && at_[j] - at_[i] < span_; ++j)
+                if (rows_overlap(pool(i), page_, stride_, pool(j), page_, stride_, pages_)) return true;
+        return false;
+    }
+    // Whether rows share memory with one of them.
+    bool hold(const Rows2d& rows) const
+    {
+        if (!rows.p || !rows.rows) return false;
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(rows.p), hi = lo + (rows.rows - 1) * rows.stride + rows.width;
+        for (const uintptr_t* p = std::lower_bound(at_, at_ + n_, hi); p != at_; --p) {
+            if (p[-1] + span_ <= lo) break;  // as those before it
+            if (arc::overlap(rows, Rows2d{reinterpret_cast<const void*>(p[-1]), pages_, page_, stride_})) return true;
+        }
+        return false;
+    }
+
+private:
+    const void* pool(uint32_t i) const { return reinterpret_cast<const void*>(at_[i]); }
+    uintptr_t at_[2 * ARC_MAX_LAYERS];
+    uint32_t n_;
+    uint64_t pages_, page_, stride_, span_;  // bytes of a page, from page to page, of all
+    bool apart_ = true;                      // their ranges do not meet
+};
 
 // Parts of a row of logits, a power of two: enough workgroups to fill the card, and a few KB or more to each.
 uint32_t splits_of(uint32_t tokens)
@@ -466,8 +516,8 @@ int arc_tree_plan(const arc_paged_batch* batch, const arc_tree* tree, arc_stream
         return set_error(ARC_ERR_INVALID_ARGUMENT, "null lens, starts, positions or masks");
     if (batch->requests == 0 || batch->tokens == 0) return ARC_OK;
     const uint64_t tokens = batch->tokens * 4ull, requests = batch->requests * 4ull;
-    const Array written[] = {{tree->masks, tokens * tree->mask_words, nullptr}, {batch->positions, tokens, nullptr}};
-    const Array read[] = {{tree->parents, tokens, nullptr}, {batch->lens, requests, nullptr}, {batch->starts, requests + 4, nullptr}};
+    const Array written[] = {{tree->masks, tokens * tree->mask_words}, {batch->positions, tokens}};
+    const Array read[] = {{tree->parents, tokens}, {batch->lens, requests}, {batch->starts, requests + 4}};
     if (shared(written, read)) return set_error(ARC_ERR_INVALID_ARGUMENT, "masks and positions share memory with each other or with what is read");
     const TreePlan a{batch->lens, batch->starts, tree->parents, tree->masks, batch->positions, batch->requests, batch->tokens, tree->mask_words};
     hipLaunchKernelGGL(k_tree_plan, dim3(batch->requests), dim3(256), 0, static_cast<hipStream_t>(stream), a);
@@ -511,23 +561,23 @@ int arc_tree_commit(const arc_kv_pages* layers, uint32_t num_layers, const arc_p
         if (!aligned(logits, size)) return set_error(ARC_ERR_INVALID_ARGUMENT, "logits must be aligned to their type");
         if (batch->tokens > kMaxLogitRows) return set_error(ARC_ERR_UNSUPPORTED, "%u rows of logits: at most 2^20", batch->tokens);
     }
-    const void* pools[2 * ARC_MAX_LAYERS];
-    for (uint32_t i = 0; i < num_layers; ++i) {
-        pools[2 * i] = layers[i].k;
-        pools[2 * i + 1] = layers[i].v;
-    }
-    std::sort(pools, pools + 2 * num_layers);
-    if (std::adjacent_find(pools, pools + 2 * num_layers) != pools + 2 * num_layers)
-        return set_error(ARC_ERR_INVALID_ARGUMENT, "the same pages twice among the layers' k and v");
+    const Pools pools(layers, num_layers);
+    if (pools.twice()) return set_error(ARC_ERR_INVALID_ARGUMENT, "the same pages twice among the layers' k and v");
+    if (pools.overlap()) return set_error(ARC_ERR_INVALID_ARGUMENT, "pages of two of the layers' k and v share memory");
     const Space sp = space_of(batch);
     const uint64_t tokens = batch->tokens * 4ull, requests = batch->requests * 4ull;
-    const Array written[] = {{workspace, sp.bytes, nullptr}, {tokens_out, tokens, nullptr}, {counts, requests, nullptr},
-                             {lens_out, requests, batch->lens}, {free_pages, num_pages * 4ull, nullptr},
-                             {free_pages ? free_count_out : nullptr, 4, free_count}, {logits ? targets : nullptr, tokens, nullptr}};
-    const Array read[] = {{logits ? nullptr : targets, tokens, nullptr}, {drafts, tokens, nullptr}, {tree->parents, tokens, nullptr},
-                          {batch->lens, requests, nullptr}, {batch->starts, requests + 4, nullptr},
-                          {batch->tables, requests * batch->max_pages, nullptr}, {free_pages ? free_count : nullptr, 4, nullptr}};
+    const uint32_t logit_bytes = logits_dtype == ARC_F32 ? 4 : 2;
+    const Array written[] = {{workspace, sp.bytes}, {tokens_out, tokens}, {counts, requests}, {lens_out, requests, batch->lens},
+                             {free_pages, num_pages * 4ull}, {free_pages ? free_count_out : nullptr, 4, free_count},
+                             {logits ? targets : nullptr, tokens}};
+    const Array read[] = {{logits ? nullptr : targets, tokens}, {drafts, tokens}, {tree->parents, tokens}, {batch->lens, requests},
+                          {batch->starts, requests + 4}, {batch->tables, requests * batch->max_pages},
+                          {free_pages ? free_count : nullptr, 4},
+                          Array(Rows2d{logits, batch->tokens, uint64_t(vocab) * logit_bytes, ldl * logit_bytes})};
     if (shared(written, read)) return set_error(ARC_ERR_INVALID_ARGUMENT, "an array that is written shares memory with another of the call");
+    auto in_pools = [&](const Array& a) { return pools.hold(a.at); };
+    if (std::any_of(std::begin(written), std::end(written), in_pools) || std::any_of(std::begin(read), std::end(read), in_pools))
+        return set_error(ARC_ERR_INVALID_ARGUMENT, "an array of the call shares memory with the pages");
     hipStream_t st = static_cast<hipStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint32_t *path = reinterpret_cast<uint32_t*>(ws), *held = reinterpret_cast<uint32_t*>(ws + sp.held);

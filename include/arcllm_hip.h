@@ -465,10 +465,11 @@ int arc_tree_attention(const arc_kv_pages *pages, const arc_paged_batch *batch, 
  *   num_pages; NULL: they stay with the request), requests in order, first page to last; table entries that are no
  *   page of the pool do not, and what finds no room on the list is on none.  free_count_out may be free_count.
  * A chunk counts 1 (the target's token after its last row), keeps all its positions and moves nothing; a
- * request without rows counts 0.  layers: 1 .. ARC_MAX_LAYERS pools of one shape (host array), none of them
- * twice; what is written shares no memory with another array but where it may be one of them.  A position whose page
- * is none of the pool does not move.  workspace: arc_tree_commit_workspace_bytes() bytes of a batch of no fewer requests
- * and rows, 256-byte aligned, as arc_paged_attention's.  Of the batch, all but positions, slots and max_new is used. */
+ * request without rows counts 0.  layers: 1 .. ARC_MAX_LAYERS pools of one shape (host array), which share no memory
+ * (their pages may lie in turns); nor does what is written with another array, but where it may be one of them, or any
+ * array with the pages (all of this refused).  A position whose page is none of the pool does not move.
+ * workspace: arc_tree_commit_workspace_bytes() bytes of a batch of no fewer requests and rows, 256-byte aligned, as
+ * arc_paged_attention's.  Of the batch, all but positions, slots and max_new is used. */
 size_t arc_tree_commit_workspace_bytes(const arc_paged_batch *batch);
 int arc_tree_commit(const arc_kv_pages *layers, uint32_t num_layers, const arc_paged_batch *batch, const arc_tree *tree,
                     int logits_dtype, const void *logits, uint64_t ldl, uint32_t vocab, const uint32_t *drafts,
