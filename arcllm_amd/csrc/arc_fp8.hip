@@ -10,15 +10,14 @@
 // so (but in k_fp8_few, which memory bounds).  For outputs of 32 bits the values are converted
 // to fp16, which holds them, and whose products the cores add in fp32: half the rate
 // (4096 rows of 18944 x 3584 with the activation, 1040 us and 530).
+#include "arc_fp8_plan.hpp"
 #include "arc_paged.hpp"
 
 #include <algorithm>
-#include <cmath>
 
 namespace arc {
 namespace {
 
-constexpr uint32_t kFpBlock = 128;
 constexpr float kE4m3Max = 448.0f;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -1005,78 +1004,6 @@ Rows2d row_scales_of(const arc_fp8_rows& x)
 }
 uint32_t bytes_of(int dtype) { return dtype == ARC_F32 ? 4 : dtype == ARC_F16 || dtype == ARC_BF16 ? 2 : 0; }
 
-// Which kernel takes a product, its tiles, and into how many parts their blocks are cut: what is expected to be quickest.
-// A block costs a workgroup `one` us where it has a compute unit to itself, `two` where two share one; the last round may be
-// short; beginning and end of a tile cost about 4 blocks; k_fp8_join 3 us and the sums' way there and back at 6 TB/s.  The
-// times are those of 28 and 148 blocks at 24 to 4096 rows, which this meets within 15 %: of 3584 x 18944 in bf16, 2048 rows,
-// tiles of 128, 185 us, of 256 in two parts 170; 1024 rows 135, and of 256 in four parts 104; of 4608 x 3584, 4096 rows, 93 and 109.
-enum class Form { few, own, rows32, rows64, rows128, deep128, deep256 };
-struct Plan {
-    Form form;
-    uint32_t mtiles, ntiles, splits;
-    size_t bytes;  // of workspace
-};
-struct Shape {
-    Form form;
-    uint32_t bm, bn;
-    float one, two;  // deep256: alone on its compute unit; of few workgroups, of a full card
-};
-Plan plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
-{
-    Plan best{Form::few, 0, 0, 1, 256};
-    // few rows: from about 6 on k_fp8_own reads them more cheaply (16 rows, 3584 x 18944, 14.3 us and 19.6; 8 rows 14.4 and 17.2; 2 rows of
-    // 4608 x 3584 8.2 and 6.9), unless its workgroups come in many turns (152064 outputs, 8 rows, 143 and 117)
-    if (M <= 16) {
-        if (M >= 6 && N <= 32768) best.form = Form::own;
-        return best;
-    }
-    float least = INFINITY;
-    auto tiles = [](uint32_t n, uint32_t each) { return (n + each - 1) / each; };
-    const uint32_t blocks = tiles(K, kFpBlock);
-    const Shape rows32{Form::rows32, 32, 128, fast ? 0.60f : 0.80f, fast ? 0.90f : 1.10f};
-    const Shape rows64{Form::rows64, 64, 128, fast ? 0.63f : 0.92f, fast ? 0.97f : 1.25f};
-    const Shape rows128{Form::rows128, 128, 128, fast ? 1.0f : 1.25f, fast ? 1.6f : 2.1f};
-    const Shape deep128{Form::deep128, 128, 128, 0.75f, 1.25f}, deep256{Form::deep256, 256, 256, 1.45f, 1.95f};
-    const bool deep = fast && K % kFpBlock == 0;
-    if (M <= 64) {
-        // k_fp8_own, one workgroup to a compute unit: 2.5 us to begin and end, between them its copies, 1 KB each, or the weights
-        // that all of them read at 5.2 TB/s
-        const uint32_t copies = 2 * tiles(M, 16) + (gated ? 4 : 2);
-        const float each = (fast ? 0.0105f : 0.0125f) * (copies <= 8 ? 1.0f : 1.25f);
-        least = tiles(tiles(N, 16), 256) * (2.5f + std::max(blocks * copies * each, float(K) * (gated ? 8192 : 4096) / 5.2e6f));
-        best.form = Form::own;
-    }
-    const Shape of[2] = {M <= 32 ? rows32 : M <= 64 ? rows64 : deep ? deep128 : rows128, deep256};
-    for (const Shape& s : of) {
-        if (s.form == Form::deep256 && (!deep || M <= 64)) continue;
-        const uint32_t mtiles = tiles(M, s.bm), ntiles = tiles(N, gated ? s.bn / 2 : s.bn);
-        for (uint32_t splits = 1; splits <= 16 && (splits == 1 || blocks / splits >= 4); splits *= 2) {
-            const double parts = double(mtiles) * ntiles * splits, share = s.form == Form::deep256 ? 256 : 512;
-            const double full = std::floor(parts / share), rest = parts - full * share;
-            const double last = rest == 0 ? 0 : share == 256 ? s.one + (s.two - s.one) * rest / 256 : rest <= 256 ? s.one : s.two;
-            const size_t sums = splits > 1 ? size_t(parts) * s.bm * s.bn * sizeof(float) : 0;
-            const float time = float((full * s.two + last) * (tiles(blocks, splits) + 4) + (splits > 1 ? 3 + sums / 3e6 : 0));
-            if (time >= least) continue;
-            least = time;
-            best = Plan{s.form, mtiles, ntiles, splits, sums ? sums : 256};
-        }
-    }
-    return best;
-}
-
-// The most workspace that products of up to M rows take.  Up to 64 rows a plan depends on the number of 16 rows, beyond on that of
-// 128, so one of each is asked.  Of a product cut in parts the sums' way alone, bytes / 3e6 us, is less than what cutting can
-// save, the tiles' last round: two * (blocks + 4) us at most (`two` <= 2.1, with some room 7e6 for 3e6 * 2.1); in two parts
-// or more, so beyond these many rows none is cut.
-size_t most_bytes(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
-{
-    const uint64_t sums = 7000000ull * ((K + kFpBlock - 1) / kFpBlock + 4);
-    const uint32_t end = uint32_t(std::min<uint64_t>(M, sums / (8ull * N * (gated ? 2 : 1)) + 256));
-    size_t most = plan_of(N, K, M, gated, fast).bytes;
-    for (uint32_t m = 16; m < end; m += m < 64 ? 16 : m < 128 ? 64 : 128) most = std::max(most, plan_of(N, K, m, gated, fast).bytes);
-    return most;
-}
-
 template <typename Y, typename C>
 hipError_t launch_tile(const Gemm& a, hipStream_t st)
 {
@@ -1090,25 +1017,25 @@ hipError_t launch_tile(const Gemm& a, hipStream_t st)
     return hipGetLastError();
 }
 template <typename Y, bool GATED>
-hipError_t launch_form(const Gemm& a, Form form, hipStream_t st)
+hipError_t launch_form(const Gemm& a, Fp8Form form, hipStream_t st)
 {
     constexpr bool FAST = sizeof(Y) == 2;
-    if (form == Form::few) hipLaunchKernelGGL((k_fp8_few<Y, GATED>), dim3((a.N + 15) / 16), dim3(64 * kFewWaves), 0, st, a);
-    else if (form == Form::own) {
+    if (form == Fp8Form::few) hipLaunchKernelGGL((k_fp8_few<Y, GATED>), dim3((a.N + 15) / 16), dim3(64 * kFewWaves), 0, st, a);
+    else if (form == Fp8Form::own) {
         auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3((a.N + 15) / 16), dim3(64 * waves), 0, st, a); };
         if (a.M <= 16) launch(k_fp8_own<Y, GATED, 1>, OwnShape<GATED, 1>::NW);
         else if (a.M <= 32) launch(k_fp8_own<Y, GATED, 2>, OwnShape<GATED, 2>::NW);
         else if (a.M <= 48) launch(k_fp8_own<Y, GATED, 3>, OwnShape<GATED, 3>::NW);
         else launch(k_fp8_own<Y, GATED, 4>, OwnShape<GATED, 4>::NW);
-    } else if (form == Form::rows32) return launch_tile<Y, TileShape<GATED, FAST, false, 2, 2, 1, 4, 3>>(a, st);
-    else if (form == Form::rows64) return launch_tile<Y, TileShape<GATED, FAST, false, 4, 2, 1, 4, 3>>(a, st);
-    else if (form == Form::rows128) return launch_tile<Y, TileShape<GATED, FAST, false, 4, 4, 2, 2, 2>>(a, st);
-    else if constexpr (FAST) return form == Form::deep128 ? launch_tile<Y, TileShape<GATED, FAST, true, 4, 4, 2, 2, 2>>(a, st)
+    } else if (form == Fp8Form::rows32) return launch_tile<Y, TileShape<GATED, FAST, false, 2, 2, 1, 4, 3>>(a, st);
+    else if (form == Fp8Form::rows64) return launch_tile<Y, TileShape<GATED, FAST, false, 4, 2, 1, 4, 3>>(a, st);
+    else if (form == Fp8Form::rows128) return launch_tile<Y, TileShape<GATED, FAST, false, 4, 4, 2, 2, 2>>(a, st);
+    else if constexpr (FAST) return form == Fp8Form::deep128 ? launch_tile<Y, TileShape<GATED, FAST, true, 4, 4, 2, 2, 2>>(a, st)
                                                           : launch_tile<Y, TileShape<GATED, FAST, true, 4, 8, 4, 2, 2>>(a, st);
     return hipGetLastError();
 }
 template <typename Y>
-hipError_t launch(const Gemm& a, Form form, bool gated, hipStream_t st)
+hipError_t launch(const Gemm& a, Fp8Form form, bool gated, hipStream_t st)
 {
     return gated ? launch_form<Y, true>(a, form, st) : launch_form<Y, false>(a, form, st);
 }
@@ -1134,7 +1061,7 @@ int product(const arc_fp8_weights* w, const arc_fp8_weights* up, bool gated, con
     if (rows_overlap(y, row, uint64_t(ldy) * size, x->q, x->cols, x->ldq, x->rows))
         return set_error(ARC_ERR_INVALID_ARGUMENT, "y and the rows share memory");
     if (x->rows == 0) return ARC_OK;
-    const Plan p = plan_of(N, x->cols, x->rows, gated, size == 2);
+    const Fp8Plan p = fp8_plan_of(N, x->cols, x->rows, gated, size == 2);
     const Rows2d out{y, x->rows, row, uint64_t(ldy) * size}, sums = bytes_at(workspace, p.splits > 1 ? p.bytes : 0);
     const Rows2d read[] = {values_of(w->w, N, w->cols, w->ldw), weight_scales_of(*w), gated ? values_of(up->w, N, up->cols, up->ldw) : Rows2d{},
                            gated ? weight_scales_of(*up) : Rows2d{}, row_scales_of(*x)};
@@ -1213,7 +1140,7 @@ int arc_fp8_quantize(int x_dtype, const void* x, uint32_t ldx, const arc_fp8_row
 size_t arc_fp8_gemm_workspace_bytes(uint32_t N, uint32_t K, uint32_t M, int gated)
 {
     if (N == 0 || N > kMaxRows || M > kMaxRows || K == 0 || K % 16 || K > kMaxLd) return 0;
-    return std::max(most_bytes(N, K, M, gated != 0, true), most_bytes(N, K, M, gated != 0, false));
+    return std::max(fp8_most_bytes(N, K, M, gated != 0, true), fp8_most_bytes(N, K, M, gated != 0, false));
 }
 
 int arc_fp8_gemm(const arc_fp8_weights* w, const arc_fp8_rows* x, int y_dtype, void* y, uint32_t ldy, const void* residual, uint32_t ldr,
