@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace arc {
 namespace {
@@ -76,12 +77,18 @@ struct PagedAttn {
     Piece *few_p, *many_p;
     uint32_t few_slot, many_slot;  // rows of a slot
     uint32_t few_wgs, many_wgs;    // workgroups of this call's launches (0: not launched)
-    const uint32_t *masks, *positions;  // of trees
+};
+// Of the TREE kernels.  The others' arguments are 24 bytes and a cache line shorter: one request at 501 positions 11.1 us, not 11.2.
+struct TreeAttn : PagedAttn {
+    const uint32_t *masks, *positions;
     uint32_t words;
     uint32_t once;  // every tree is one tile: nothing of K and V is read twice
 };
+template <bool TREE>
+using Attn = std::conditional_t<TREE, TreeAttn, PagedAttn>;
+__device__ __forceinline__ const TreeAttn& of_tree(const PagedAttn& a) { return static_cast<const TreeAttn&>(a); }
 
-// The kernel's arguments (its one parameter, a PagedAttn), read again: a phase that takes its own copy keeps
+// The kernel's arguments (its one parameter, a PagedAttn or a TreeAttn), read again: a phase that takes its own copy keeps
 // none of it in scalar registers for the phases after it.
 __device__ __forceinline__ const PagedAttn& arguments()
 {
@@ -115,7 +122,7 @@ __device__ __forceinline__ double cost_before(const Request& r, uint32_t t, doub
 }
 
 // Whether a request's rows are a tree, not a chunk.
-__device__ __forceinline__ bool is_tree(const PagedAttn& a, const Request& r) { return r.rows <= 32 * a.words * a.hpk; }
+__device__ __forceinline__ bool is_tree(const PagedAttn& a, const Request& r) { return r.rows <= 32 * of_tree(a).words * a.hpk; }
 
 template <bool TREE, bool FEW, uint32_t bm>
 __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, uint32_t s1, uint32_t held)
@@ -137,11 +144,15 @@ __device__ __forceinline__ Request request_of(const PagedAttn& a, uint32_t s0, u
     constexpr uint32_t kTurn = FEW ? kFewWaves * kFewKeys : kManyKeys;
     const uint32_t old = uint32_t(max(r.base, 0));
     r.first = double(ends + (tree ? max(old, kTurn) : old)) * a.hpk + bm;
-    const uint32_t nodes = tree ? rows : 0;  // the tree lies behind the first node's window
-    r.cap = a.window ? (double(ends) + a.window + a.sinks) * a.hpk + nodes + 2 * bm : 0x1p60;
+    r.cap = a.window ? (double(ends) + a.window + a.sinks) * a.hpk + 2 * bm : 0x1p60;
+    if (tree && a.window) r.cap += rows;  // the tree lies behind the first node's window
+    auto seen = [&] {
+        const float all = float(a.window) + float(a.sinks);
+        return tree ? all + float(rows / a.hpk) : all;
+    };
     r.total = r.tiles == 1 ? fmin(r.first, r.cap) : cost_before(r, r.tiles, bm);
     const float spans = float(r.tiles) * ceilf(float(len) * (1.0f / keys));
-    r.units = a.window ? fminf(spans, float(r.tiles) * (ceilf((float(a.window) + float(a.sinks) + float(nodes / a.hpk)) * (1.0f / keys)) + 2.0f)) : spans;
+    r.units = a.window ? fminf(spans, float(r.tiles) * (ceilf(seen() * (1.0f / keys)) + 2.0f)) : spans;
     if (tree && !FEW) {
         // up to 8 pieces of a tile are joined in the quicker way, worth some 3 units: 26 nodes at 501 positions, 28 heads on 4,
         // 15.2 us (a part to each unit 18.5); 60 nodes 19.6 (27.4); at 1700 18.4 (21.0); 32 heads of 64 on 8 at 1000 13.4 (18.1);
@@ -720,9 +731,10 @@ __device__ __forceinline__ Sight<TREE> sight_of(const PagedAttn& a, const Segmen
     v.qpos = s.base + int32_t(i);
     if constexpr (TREE) {
         v.base = s.base;
-        v.words = s.x.pos0 < s.base ? a.words : 0u;  // see tile_at
-        v.mask = a.masks + uint64_t(s.token + i) * a.words;
-        v.depth = a.window && v.words ? int32_t(a.positions[s.token + i]) - s.base : 0;
+        const TreeAttn& t = of_tree(a);
+        v.words = s.x.pos0 < s.base ? t.words : 0u;  // see tile_at
+        v.mask = t.masks + uint64_t(s.token + i) * t.words;
+        v.depth = a.window && v.words ? int32_t(t.positions[s.token + i]) - s.base : 0;
     }
     return v;
 }
@@ -927,7 +939,7 @@ __device__ __forceinline__ void wave_fence()  // this wave's LDS accesses before
 // requests of up to 8000, 28 heads on 4 (271 MB) 57 us, 4.8 TB/s, of which 3 are the walk and 4 the join; 2 of
 // 131071, 64 on 8 (732 MB) 123 us, 5.9 TB/s; plain reads of as much reach 6.2.  Pages of 1 to 8 positions: as long.
 template <typename T, int D, bool WIDE, bool TREE>
-__global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
+__global__ __launch_bounds__(256, 2) void k_paged_few(Attn<TREE>)
 {
     __shared__ struct {  // rows first: m0, which says where a copy goes, is used below 2^16 only
         __align__(16) float joined[4 * 32 * D];  // K and V rows of each wave, then the waves' outputs
@@ -1094,7 +1106,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn)
 // two waves to 32 rows of a tile that is half empty, each with half a unit's positions (182 us: 59 registers too
 // many).  One tree of 26 nodes at 501: 15.2 us, of which the join is 3.
 template <typename T, int D, int NW, bool WIDE, bool TREE>
-__global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAttn)
+__global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(Attn<TREE>)
 {
     constexpr int NT = NW * 64;
     constexpr uint32_t kBm = NW * 32, kOwn = kManyKeys / NW;  // rows of K and V that a wave copies
@@ -1142,7 +1154,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void k_paged_many(PagedAt
             const uint32_t at = wave * kOwn, pos = unit_start(s.x, u, kManyKeys) + at;
             // past the caches' keeping where no other tile reads it: 48 trees of up to 9 tokens at up to 8000, 28 heads, 58 us
             // instead of 66; with several tiles to a tree (16 of up to 250 at 4000) 3 % slower
-            if (TREE && arguments().once) copy_rows<true, true, TREE, kOwn, WIDE, D>(p, &ks[buf][at * D], &vs[buf][at * D], page, at, pos);
+            if (TREE && of_tree(arguments()).once) copy_rows<true, true, TREE, kOwn, WIDE, D>(p, &ks[buf][at * D], &vs[buf][at * D], page, at, pos);
             else copy_rows<true, true, false, kOwn, WIDE, D>(p, &ks[buf][at * D], &vs[buf][at * D], page, at, pos);
         };
         if (s.u0 < s.u1) {
@@ -1412,7 +1424,7 @@ Space space_of(uint32_t dim, uint32_t hpk, uint32_t tokens)
 }
 
 template <typename T, int D, bool WIDE, bool TREE>
-void launch_tiles(const PagedAttn& a, hipStream_t st)
+void launch_tiles(const TreeAttn& a, hipStream_t st)
 {
     if (a.few_wgs) hipLaunchKernelGGL((k_paged_few<T, D, WIDE, TREE>), dim3(a.few_wgs), dim3(256), 0, st, a);
     if (a.many_wgs)
@@ -1420,7 +1432,7 @@ void launch_tiles(const PagedAttn& a, hipStream_t st)
 }
 
 template <typename T, int D, bool TREE>
-hipError_t launch_paged(const PagedAttn& a, hipStream_t st)
+hipError_t launch_paged(const TreeAttn& a, hipStream_t st)
 {
     if (a.shift >= 4) launch_tiles<T, D, true, TREE>(a, st);
     else launch_tiles<T, D, false, TREE>(a, st);
@@ -1439,7 +1451,7 @@ int check_sizes(const arc_kv_pages* pages, const arc_paged_batch* batch, uint32_
 }
 
 template <bool TREE>
-hipError_t launch_type(const PagedAttn& a, const arc_kv_pages* pages, hipStream_t st)
+hipError_t launch_type(const TreeAttn& a, const arc_kv_pages* pages, hipStream_t st)
 {
     const bool f16 = pages->dtype == ARC_F16;
     if (pages->head_dim == 64) return f16 ? launch_paged<_Float16, 64, TREE>(a, st) : launch_paged<bf16, 64, TREE>(a, st);
@@ -1475,7 +1487,7 @@ int attention(const arc_kv_pages* pages, const arc_paged_batch* batch, const arc
     if (batch->tokens == 0 || batch->requests == 0) return ARC_OK;
     const Space sp = space_of(pages->head_dim, hpk, batch->tokens);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    PagedAttn a{};
+    TreeAttn a{};
     a.q = q;
     a.k = pages->k;
     a.v = pages->v;
