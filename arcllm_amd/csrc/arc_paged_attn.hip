@@ -109,7 +109,10 @@ struct Request {
     uint32_t tiles;   // per kv head
     double first, cap;  // cost of tile 0; no tile costs more than cap
     double total;       // of a kv head's tiles
-    float units;        // no fewer than its tiles have for a kv head, about as many
+    // how many units its tiles count for, of a kv head, when a step is cut into parts of a unit (few rows: one for each wave):
+    // about as many as they have and no fewer, but of trees fewer in the many-rows kernel (9 to 32 units a tile: a part
+    // to several) and in the few-rows kernel as many as a workgroup takes in one turn, or more
+    float units;
 };
 
 // Cost of tiles 0 .. t-1: tile t costs min(first + t * bm, cap), in positions times
@@ -231,7 +234,8 @@ struct Walk {
     Tile x;
 };
 
-// Boundary of part w, the same number wherever it is computed; a part has a unit's cost or more, so none is empty.
+// Boundary of part w, the same number wherever it is computed.  A tile costs 64 and more for each of its units (so do short
+// trees' whose units count as a turn's), so a part is never empty, though it may hold no whole unit.
 __device__ __forceinline__ double part_at(const Walk& l, uint32_t w)
 {
     return w >= l.parts ? l.total : floor(l.step * double(w));
