@@ -234,8 +234,8 @@ struct Walk {
     Tile x;
 };
 
-// Boundary of part w, the same number wherever it is computed.  A tile costs 64 and more for each of its units (so do short
-// trees' whose units count as a turn's), so a part is never empty, though it may hold no whole unit.
+// Boundary of part w, the same number wherever it is computed.  A tile costs far more than one for each unit that it counts
+// for, so a part is never empty, though it may hold no whole unit.
 __device__ __forceinline__ double part_at(const Walk& l, uint32_t w)
 {
     return w >= l.parts ? l.total : floor(l.step * double(w));
