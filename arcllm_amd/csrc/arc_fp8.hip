@@ -303,9 +303,9 @@ __global__ __launch_bounds__(512) void k_fp8_few(Gemm a)
 // Tiles.  A workgroup of GM x GN waves has BM rows of x and BN rows of w, a wave WM x WN tiles of 16 x 16.  A block of both
 // comes straight into LDS, S blocks deep; one barrier a block.  With the activation a wave's weights are half gate, half
 // up, at the same outputs.  32 and 64 rows: bound by the weights' way into LDS (48 rows of 152064 x 3584, 109 us, 5.1 TB/s;
-// fp32 128); 3 blocks deep, as more take a workgroup from the compute unit for no gain.  128 rows: for fp32 by
-// the conversions (4096 rows of 4608 x 3584, 147 us, 0.92 PFLOP/s); with e4m3 products only for a last block that is
-// not whole (K 3600, 105 us, where 3584 take k_fp8_deep 87).
+// fp32 126); 3 blocks deep, as more take a workgroup from the compute unit for no gain.  128 rows: for fp32 by
+// the conversions (4096 rows of 4608 x 3584, 138 us, 0.98 PFLOP/s); with e4m3 products only for a last block that is
+// not whole (K 3600, 105 us with weights in the last cache, where 3584 take k_fp8_deep 87).
 template <bool GATED_, bool FAST_, bool DEEP_, int WM_, int WN_, int GM_, int GN_, int S_>
 struct TileShape {
     static constexpr bool GATED = GATED_, FAST = FAST_, DEEP = DEEP_;
@@ -660,9 +660,10 @@ __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_tile(Gemm a)
 // parts' sums to a second launch, 5 us.  A workgroup has 16 outputs (GATED: with the activation, 16 rows of gate and of up);
 // its waves take the blocks in turn, each with its own place in LDS for two or more of them and no barrier, and add up in wave order.
 // The price is that x goes to every workgroup, from the L2: 3 times the weights' bytes at 48 rows.  45 rows, 3584 x 18944, in
-// fp32: 18.6 us where the last cache still holds the weights, 25.8 from HBM; tiles in 16 parts 24 and 29; 32 rows, 512 x 3584: 4 and
-// 8.4.  Operands straight into registers, without LDS, took 41: 16 rows of 64 bytes are as many requests as 16 of 128.  Weights
-// a block further ahead than x gained nothing.
+// fp32: 17.8 us where the last cache still holds the weights, 25.6 from HBM, 2.8 TB/s, as a wave has at most one block of
+// weights under way beside the one that it works on; tiles in 16 parts 24 and 29; 32 rows, 512 x 3584: 4 and 8.4.
+// Operands straight into registers, without LDS, took 41: 16 rows of 64 bytes are as many requests as 16 of 128.  Weights
+// a block further ahead than x gained nothing while the last cache held them; from HBM it was not measured.
 template <bool GATED, int WM>
 struct OwnShape {
     static constexpr int G = GATED ? 2 : 1, NW = 2 * G + 2 * WM <= 8 ? 8 : 6;
@@ -801,7 +802,7 @@ __global__ __launch_bounds__(512, 2) void k_fp8_own(Gemm a)
 // multiply-adds alone reach 3.4 in a loop, at the clock that their power leaves.  Here the cores are busy for 51 % of the
 // cycles, at 1.8 GHz, LDS for 22 %, without conflicts; without the copies it would take 20 % less time, without the reads of
 // LDS 15 %.  A third place for blocks does not fit in LDS; copies begun earlier or all at once were slower (535 to 569 us), and so
-// was a last round of tiles cut in parts (536, and 95 instead of 87 for 4608 x 3584).
+// was a last round of tiles cut in parts (536, and 95 instead of 87 for 4608 x 3584 with weights in the last cache, 105 from HBM).
 template <typename Y, typename C>
 __global__ __launch_bounds__(C::NW * 64, 2) void k_fp8_deep(Gemm)
 {

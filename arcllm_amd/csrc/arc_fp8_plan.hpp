@@ -14,8 +14,11 @@ constexpr uint32_t kFpBlock = 128;  // columns, and rows of weights, to a scale
 // Which kernel takes a product, its tiles, and into how many parts their blocks are cut: what is expected to be quickest.
 // A block costs a workgroup `one` us where it has a compute unit to itself, `two` where two share one; the last round may be
 // short; beginning and end of a tile cost about 4 blocks; k_fp8_join 3 us and the sums' way there and back at 6 TB/s.  The
-// times are those of 28 and 148 blocks at 24 to 4096 rows, which this meets within 15 %: of 3584 x 18944 in bf16, 2048 rows,
-// tiles of 128, 185 us, of 256 in two parts 170; 1024 rows 135, and of 256 in four parts 104; of 4608 x 3584, 4096 rows, 93 and 109.
+// constants come from products of 28 and 148 blocks, 24 to 4096 rows.  Expected times are from a third below those measured with weights
+// from memory (8 blocks; 45 rows of 3584 x 18944) to a sixth or, in fp32, a quarter above (4096 rows).  What the choice has
+// to tell apart, so measured, bf16: 3584 x 18944, 2048 rows, tiles of 128 183 us, of 256 in two parts 165; 1024 rows,
+// tiles of 128 in one and two parts 145 and 113, of 256 in four 101; 4608 x 3584, 4096 rows, tiles of 128 105, of 256 108; 2048
+// rows 71 and 64.
 enum class Fp8Form { few, own, rows32, rows64, rows128, deep128, deep256 };
 struct Fp8Plan {
     Fp8Form form;
@@ -30,8 +33,11 @@ struct Fp8Tiles {
 inline Fp8Plan fp8_plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
 {
     Fp8Plan best{Fp8Form::few, 0, 0, 1, 256};
-    // few rows: from about 6 on k_fp8_own reads them more cheaply (16 rows, 3584 x 18944, 14.3 us and 19.6; 8 rows 14.4 and 17.2; 2 rows of
-    // 4608 x 3584 8.2 and 6.9), unless its workgroups come in many turns (152064 outputs, 8 rows, 143 and 117)
+    // few rows: from about 6 on k_fp8_own reads them more cheaply where its workgroups come in one turn, and where they come in
+    // many does not.  6, 8 and 16 rows with weights from memory, k_fp8_own and k_fp8_few, us: 3584 x 18944 18.0 and 19.1, 18.1 and
+    // 19.3, 18.7 and 20.5; 4608 x 3584 8.3 and 7.9, 8.5 and 8.3, 9.1 and 9.9; 152064 x 3584 135 and 108, 139 and 117, 152
+    // and 142.  The border stands high: at 18944 outputs 20.1 and 17.0, 20.5 and 18.0, 22.1 and 21.7, at 32768 31.7 and
+    // 26.6, 32.4 and 28.2, 35.2 and 34.1
     if (M <= 16) {
         if (M >= 6 && N <= 32768) best.form = Fp8Form::own;
         return best;
@@ -70,16 +76,17 @@ inline Fp8Plan fp8_plan_of(uint32_t N, uint32_t K, uint32_t M, bool gated, bool 
     return best;
 }
 
-// The most workspace that products of up to M rows take.  Up to 64 rows a plan depends on the number of 16 rows, beyond on that of
-// 128, so one of each is asked.  Of a product cut in parts the sums' way alone, bytes / 3e6 us, is less than what cutting can
-// save, the tiles' last round: two * (blocks + 4) us at most (`two` <= 2.1, with some room 7e6 for 3e6 * 2.1); in two parts
-// or more, so beyond these many rows none is cut.
+// The most workspace that products of up to M rows take.  Up to 64 rows a plan depends on the number of 16 rows, beyond on
+// that of 128, so one of each is asked.  Of a product cut in parts the sums' way alone, bytes / 3e6 us, is less than what
+// cutting can save, the tiles' last round: two * (blocks + 4) us at most (`two` <= 2.1; with some room 7e6 for
+// 3e6 * 2.1).  The sums of two parts or more are 8 bytes an output, so beyond `end` rows nothing is cut.
 inline size_t fp8_most_bytes(uint32_t N, uint32_t K, uint32_t M, bool gated, bool fast)
 {
     const uint64_t sums = 7000000ull * ((K + kFpBlock - 1) / kFpBlock + 4);
     const uint32_t end = uint32_t(std::min<uint64_t>(M, sums / (8ull * N * (gated ? 2 : 1)) + 256));
     size_t most = fp8_plan_of(N, K, M, gated, fast).bytes;
-    for (uint32_t m = 16; m < end; m += m < 64 ? 16 : m < 128 ? 64 : 128) most = std::max(most, fp8_plan_of(N, K, m, gated, fast).bytes);
+    for (uint32_t m = 16; m < end; m += m < 64 ? 16 : m < 128 ? 64 : 128)
+        most = std::max(most, fp8_plan_of(N, K, m, gated, fast).bytes);
     return most;
 }
 

@@ -97,8 +97,8 @@ struct Argmax {
     uint32_t requests, tokens, vocab, splits;
 };
 // A workgroup to a part of a row; rows behind the last request are not read.  Bound by reading the logits: 16 bytes a lane
-// from the first 16-byte border on, four at a time.  A step's end of 24 trees of up to 40 nodes with logits of 152064 in fp32: 73 us
-// in all, of which the logits, 365 MB, at 6.2 TB/s, would be 59.
+// from the first 16-byte border on, four at a time.  A step's end of 24 trees of up to 40 nodes with logits of 152064 in fp32: 70
+// to 76 us in all, of which the logits, 365 MB, at 6.2 TB/s, would be 59.
 template <typename T>
 __global__ __launch_bounds__(256) void k_tree_argmax(Argmax a)
 {
@@ -300,7 +300,7 @@ __device__ __forceinline__ Spare spare_of(const Move& a, const Rows& r, uint32_t
     return Spare{low, end > low ? end - low : 0};
 }
 
-// A workgroup to a request and layer; that of one more layer number returns the pages, table entries that are none left out.
+// A workgroup to a request and layer; that of one more layer number returns the pages, without table entries that are none.
 __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
 {
     const uint32_t tid = threadIdx.x, layer = blockIdx.y;
@@ -348,7 +348,8 @@ __global__ __launch_bounds__(256) void k_tree_move(Move a, Layers layers)
 }
 
 // The step's end of one request where lens_out is not lens, in one launch: each layer's workgroup walks for itself, the last one
-// writes what the call gives and returns the pages.  28 layers after a tree of 26 nodes: 6.7 us, 9.3 in two launches.
+// writes what the call gives and returns the pages.  28 layers after a tree of 26 nodes: 6.8 us, in two launches 9.8; in a
+// graph 3.8 and 5.2.
 __global__ __launch_bounds__(256) void k_tree_one(Walk w, Move a, Layers layers)
 {
     __shared__ WalkSpace l;

@@ -506,8 +506,10 @@ int arc_fp8_quantize(int x_dtype, const void *x, uint32_t ldx, const arc_fp8_row
  * (ARC_F32, ARC_F16, ARC_BF16), ldy and ldr elements from row to row (16-byte aligned rows are quickest); residual
  * may be NULL, or y itself; otherwise y and the workspace share no memory with what is read or each other
  * (refused).  Sums are fp32, rounded once.  A y of 16 bits may lose of each 8 neighbouring products what lies
- * below 2^-13 of their largest (1.3e-5 of y for normal data), an fp32 one does not.  Products of scales that leave
- * fp32's normal range do not keep their bits.
+ * below 2^-13 of their largest (1.3e-5 of y for normal data), an fp32 one does not.  Which kernel takes a call, and so
+ * the order of its sums and whether a y of 16 bits loses that, goes by rows, n, k and the type: a row's last bits may
+ * depend on how many rows share its call, never on what the others hold.  Products of scales that leave fp32's
+ * normal range do not keep their bits.
  * workspace: arc_fp8_gemm_workspace_bytes(w->rows, w->cols, rows, 0) bytes for some rows >= x->rows (what it
  * gives serves any call of these weights and up to so many rows), 256-byte aligned, any contents, for one call at a
  * time.  No rows: nothing is done. */
